@@ -269,6 +269,91 @@ QTTS_API int qtts_q4_quantize_dev(const float* data_dev, int k, int n, uint8_t* 
 /* Same with host buffers (copies in, runs, copies out). */
 QTTS_API int qtts_q4_quantize(const float* data, int k, int n, uint8_t* packed, uint16_t* scales);
 
+/* ---- 8-bit paged K/V cache on device pointers ------------------------------
+ * No counterpart in the reference (its caches are f32, gemv.rs:77-86).  A
+ * page holds 16 positions of every K/V head:
+ *   codes  int8 [page][K|V][kv_head][16][head_dim]   value = code * scale
+ *   scales f32  [page][K|V][kv_head]
+ * page_stride (bytes, a multiple of 16) and scale_stride (floats) lead from
+ * one page to the next, so that `codes` and `scales` may point at one layer
+ * of a pool that holds several.  page_table[seq][pages_per_seq] maps position
+ * p of a sequence to page page_table[seq][p / 16].  All buffers lie on one
+ * device (the current one or another); calls are asynchronous on `stream`, a
+ * stream of that device, use no workspace, allocate nothing and can be
+ * captured.  Tables and rows are device data that the host does not see:
+ * what is out of range there is skipped, and a bit of *flags (an int of the
+ * device, null = none, never cleared here) says so. */
+#define QTTS_F32 0
+#define QTTS_F16 1
+#define QTTS_BF16 2
+#define QTTS_KV8_BAD_ROW 1    /* seq past n_seqs, or a position outside the sequence's pages */
+#define QTTS_KV8_BAD_PAGE 2   /* a page table entry outside [0, n_pages) */
+#define QTTS_KV8_ROPE_RANGE 4 /* a position outside the rotation tables (left unrotated) */
+typedef struct {
+  int8_t* codes;
+  float* scales;
+  const int32_t* page_table;
+  int n_pages, n_seqs, pages_per_seq;
+  int kv_heads, head_dim; /* head_dim 64 or 128 */
+  int64_t page_stride, scale_stride;
+} qtts_kv8_cache;
+/* Appends row r's K and V ([n_rows][kv_heads * head_dim] of `dtype`, row
+ * strides in elements, multiples of 4) at position pos[r] of sequence seq[r]
+ * (seq < 0: a padding row, skipped).  On the way, each step rounded in f32:
+ * k_norm / q_norm (f16 [head_dim], nullable): RMS norm of each head, eps
+ * 1e-6 (talker.rs:89-99 apply_qk_norm); rope_cos / rope_sin (f32
+ * [rope_rows][head_dim / 2], nullable): rotation of the two halves by the
+ * angles of rope_pos[r] (null: pos[r]).  q (nullable) takes the same way to
+ * q_out, which may be q.
+ * The rows of one sequence stand together in the order of consecutive
+ * positions, and no position occurs twice.  An append ends the sequence at
+ * its last row: later positions of that page are dropped.
+ * A block is a page's K or V of one head.  Its scale is the largest finite
+ * new value / 127 when its first position is appended; later it stays while
+ * the new values fit, and grows to max(need, 1.25 * scale) when they do not,
+ * the earlier codes being rounded again (all such roundings together at most
+ * 2.5 steps of the final scale).  NaN is stored as 0, infinities as +-127. */
+QTTS_API int qtts_kv8_append_dev(const qtts_kv8_cache* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                 const void* q, int64_t ldq, void* q_out, int64_t ldqo, int heads, int dtype,
+                                 const uint16_t* q_norm, const uint16_t* k_norm, const float* rope_cos,
+                                 const float* rope_sin, int rope_rows, const int32_t* seq, const int32_t* pos,
+                                 const int32_t* rope_pos, int n_rows, int32_t* flags, void* stream);
+/* GQA attention over that cache: row r ([heads * head_dim] of `dtype`,
+ * `heads` a multiple of kv_heads) attends positions [0, pos[r]] of sequence
+ * seq[r], or the last `window` of them (0: all); out = softmax(scale * q.k) v
+ * and lse[n_rows][heads] (nullable, f32) its log-sum-exp.  pos < 0: nothing is
+ * attended, out is 0 and lse -inf.  seq < 0: a padding row, left as it was.
+ * Sums are held in f32; q and the softmax weights keep about 22 bits with f32
+ * q, so that f32 results agree with f32 arithmetic to ~1e-6.  max_rows (the
+ * rows that one sequence has next to each other; 0 = 1) and max_len (the
+ * longest sequence; 0 = the whole table) choose how the work is split; results
+ * are right whatever they say. */
+QTTS_API int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t ldq, int heads, int dtype,
+                                    float scale, int window, const int32_t* seq, const int32_t* pos, int n_rows,
+                                    int max_rows, int max_len, void* out, int64_t ldo, float* lse, int32_t* flags,
+                                    void* stream);
+
+/* ---- sampling rows of logits on device pointers ----------------------------
+ * qtts_sample with nucleus and min-p filters, for rows of up to 262144 logits
+ * and uniform numbers that the caller gives.  Per row (stride ld elements):
+ * tokens are ordered by logit, equal ones by index; NaN counts as -inf, and
+ * -inf is never drawn.  temperature[r] (null: 1) divides the logits; not above
+ * 0: the first token of the order is taken.  w = exp((logit - largest) /
+ * temperature).  Kept are the first top_k[r] (null or < 1: all); of these the
+ * shortest beginning that holds top_p[r] of their weight (null or not below
+ * 1: all; at least one token); of these w >= min_p[r] (null or not above 0:
+ * all, above 1 counts as 1).  token[r] = the first index, in index order, at
+ * which the kept weights' running sum passes u[r] (in [0, 1), clamped) of
+ * their total.  Weights are whole multiples of 2^-45, so sums do not depend on
+ * their order.  kept[r] (nullable) counts the kept tokens, logprob[r]
+ * (nullable) = log(w / total).  A row of nothing but -inf and NaN: token -1,
+ * kept 0, logprob -inf.  An infinite largest logit: the infinite ones share. */
+#define QTTS_SAMPLE_ROWS_MAX_V 262144
+QTTS_API int qtts_sample_rows_dev(const void* logits, int64_t ld, int dtype, int n_rows, int V,
+                                  const float* temperature, const int32_t* top_k, const float* top_p,
+                                  const float* min_p, const float* u, int32_t* token, int32_t* kept, float* logprob,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,773 @@
+// kv8.cu -- the paged K/V cache held in 8 bits (sm_100a): appending to it with
+// QK-norm and position rotation on the way, and attention over it.
+//
+// A page holds 16 positions of every K/V head: codes int8
+// [page][K|V][kv_head][16][head_dim], one f32 scale per [page][K|V][kv_head];
+// an element's value is code * scale.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <float.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "engine.h"
+#include "kv8.h"
+
+namespace cg = cooperative_groups;
+
+namespace qtts {
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// ---- four consecutive elements of a row --------------------------------------
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __half* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(__half* p, float4 v) {
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(half2_bits(__floats2half2_rn(v.x, v.y)), half2_bits(__floats2half2_rn(v.z, v.w)));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+__device__ __forceinline__ void raise(int* flags, int bit) {
+  if (flags) atomicOr(flags, bit);
+}
+
+// codes and scale of (page, K = 0 / V = 1, kv head)
+__device__ __forceinline__ int8_t* block_codes(const qtts_kv8_cache& c, int page, int which, int h) {
+  return c.codes + (size_t)page * c.page_stride + (size_t)(which * c.kv_heads + h) * kKv8Page * c.head_dim;
+}
+__device__ __forceinline__ float* block_scale(const qtts_kv8_cache& c, int page, int which, int h) {
+  return c.scales + (size_t)page * c.scale_stride + which * c.kv_heads + h;
+}
+
+// ---- append --------------------------------------------------------------------
+// A head's row of HD values lies on HD / 4 lanes, four consecutive values each,
+// so that loads and the 4-byte code stores are whole lines and the rotation's
+// partner (half a head away) is one lane shuffle away.
+
+// RMS norm over the head (the formula of the q/k/v epilogue): the mean of
+// squares is summed in f64 (order-free to f32, so that a code does not depend
+// on the reduction tree), everything after it is one f32 rounding per step.
+template <int HD>
+__device__ __forceinline__ float4 head_norm(float4 x, float4 g) {
+  double ss = (double)x.x * x.x + (double)x.y * x.y + (double)x.z * x.z + (double)x.w * x.w;
+#pragma unroll
+  for (int o = HD / 8; o; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
+  const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn((float)(ss / HD), 1e-6f)));
+  return make_float4(__fmul_rn(__fmul_rn(x.x, inv), g.x), __fmul_rn(__fmul_rn(x.y, inv), g.y),
+                     __fmul_rn(__fmul_rn(x.z, inv), g.z), __fmul_rn(__fmul_rn(x.w, inv), g.w));
+}
+// (a, b) -> (a cos - b sin, b cos + a sin) of the two halves, products and sum
+// rounded one by one (no contraction)
+template <int HD>
+__device__ __forceinline__ float4 rotate(float4 x, float4 c, float4 s, bool upper) {
+  float4 y;
+  y.x = __shfl_xor_sync(kFull, x.x, HD / 8);
+  y.y = __shfl_xor_sync(kFull, x.y, HD / 8);
+  y.z = __shfl_xor_sync(kFull, x.z, HD / 8);
+  y.w = __shfl_xor_sync(kFull, x.w, HD / 8);
+  const float sg = upper ? 1.0f : -1.0f;  // a product's sign change is exact
+  return make_float4(__fadd_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x) * sg),
+                     __fadd_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y) * sg),
+                     __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z) * sg),
+                     __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w) * sg));
+}
+__device__ __forceinline__ float4 norm_weight(const __half* w, int d0) {
+  return w ? load4(w + d0) : make_float4(1.f, 1.f, 1.f, 1.f);
+}
+
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= FLT_MAX ? a : 0.0f;  // NaN and infinities set no scale
+}
+// nearest code, ties to even; NaN -> 0, infinities -> +-127
+__device__ __forceinline__ uint32_t code_of(float v, float inv) {
+  const int q = __float2int_rn(__fmul_rn(v, inv));
+  return (uint32_t)max(-127, min(127, q)) & 0xffu;
+}
+__device__ __forceinline__ uint32_t codes4(float4 v, float inv) {
+  return code_of(v.x, inv) | (code_of(v.y, inv) << 8) | (code_of(v.z, inv) << 16) | (code_of(v.w, inv) << 24);
+}
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
+  const float4 v = make_float4((float)(int8_t)(w & 0xff), (float)(int8_t)((w >> 8) & 0xff),
+                               (float)(int8_t)((w >> 16) & 0xff), (float)(int8_t)(w >> 24));
+  return codes4(v, ratio);
+}
+
+// Rows [chunk * d.chunk, + d.chunk): every block (run of rows of one sequence,
+// consecutive positions, one page) that starts there, for one K or V head.
+template <typename T, int HD>
+__device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int h) {
+  constexpr int LPT = HD / 4, TPW = 32 / LPT, STEPS = kKv8Page / TPW;  // lanes per token, tokens per step
+  const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
+  const bool upper = (lane % LPT) >= LPT / 2;
+  const qtts_kv8_cache& c = d.c;
+  // lane i holds row first + i; a block that starts in the chunk ends before lane 32
+  const int first = chunk * d.chunk - 1, row = first + lane;
+  int seq = -1, pos = -1;
+  if (row >= 0 && row < d.n_rows) {
+    seq = d.seq[row];
+    pos = d.pos[row];
+  }
+  const bool ok = seq >= 0 && seq < c.n_seqs && pos >= 0 && pos < c.pages_per_seq * kKv8Page;
+  if (seq >= 0 && !ok && lane >= 1 && lane <= d.chunk) raise(d.flags, QTTS_KV8_BAD_ROW);
+  const int pseq = __shfl_up_sync(kFull, seq, 1), ppos = __shfl_up_sync(kFull, pos, 1);
+  const bool cont = ok && lane > 0 && pseq == seq && ppos == pos - 1 && pos % kKv8Page != 0;
+  const unsigned conts = __ballot_sync(kFull, cont);
+  unsigned starts = __ballot_sync(kFull, ok && !cont && lane >= 1 && lane <= d.chunk);
+  const T* src = static_cast<const T*>(which ? d.v : d.k);
+  const long ld = which ? d.ldv : d.ldk;
+  const float4 g = norm_weight(which ? nullptr : d.k_norm, d0);
+  while (starts) {
+    const int i = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const int n = i == 31 ? 1 : __ffs(~(conts >> (i + 1)));  // 1 + the rows that continue it
+    const int bseq = __shfl_sync(kFull, seq, i), bpos = __shfl_sync(kFull, pos, i);
+    const int slot0 = bpos % kKv8Page;
+    const int page = c.page_table[(size_t)bseq * c.pages_per_seq + bpos / kKv8Page];
+    if (page < 0 || page >= c.n_pages) {
+      if (lane == 0) raise(d.flags, QTTS_KV8_BAD_PAGE);
+      continue;
+    }
+    float* sp = block_scale(c, page, which, h);
+    int8_t* codes = block_codes(c, page, which, h);
+    const float had = slot0 ? *sp : 0.0f;
+    float4 x[STEPS];
+    float big = 0.0f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s * TPW >= n) break;
+      const int t = s * TPW + sub;
+      if (t < n) x[s] = load4(src + (size_t)(first + i + t) * ld + (size_t)h * HD + d0);
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (s * TPW >= n) break;
+      const int t = s * TPW + sub;
+      if (which == 0) {
+        if (d.k_norm) x[s] = head_norm<HD>(x[s], g);
+        if (d.rope_cos) {
+          float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (t < n) {
+            const int rp = d.rope_pos ? d.rope_pos[first + i + t] : bpos + t;
+            if (rp >= 0 && rp < d.rope_rows) {
+              cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+              sn = load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+            } else {
+              raise(d.flags, QTTS_KV8_ROPE_RANGE);
+            }
+          }
+          x[s] = rotate<HD>(x[s], cs, sn, upper);
+        }
+      }
+      if (t < n)
+        big = fmaxf(big, fmaxf(fmaxf(finite_abs(x[s].x), finite_abs(x[s].y)),
+                               fmaxf(finite_abs(x[s].z), finite_abs(x[s].w))));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, o));
+    // 127 steps to the largest value; the floor keeps 1 / scale finite
+    const float need = big > 0.0f ? fmaxf(__fmul_rn(big, (float)(1.0 / 127.0)), FLT_MIN) : 0.0f;
+    float scale = need;
+    if (slot0) {
+      // A block that grows does so by a quarter at least: its earlier codes
+      // are rounded again, and with steps of 1.25 those roundings add up to
+      // at most 1/2 (1 + 1/1.25 + ...) = 2.5 of the final steps.
+      scale = need <= had ? had : fmaxf(need, __fmul_rn(1.25f, had));
+      if (scale != had) {
+        const float ratio = scale > 0.0f ? __fdiv_rn(had, scale) : 0.0f;
+        for (int t = sub; t < slot0; t += TPW) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(codes + t * HD + d0);
+          *w = requant4(*w, ratio);
+        }
+      }
+    }
+    const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (s * TPW >= n) break;
+      const int t = s * TPW + sub;
+      if (t < n) *reinterpret_cast<uint32_t*>(codes + (slot0 + t) * HD + d0) = codes4(x[s], inv);
+    }
+    if (lane == 0) *sp = scale;
+  }
+}
+
+constexpr int kQHeads = 4;  // query heads of one warp
+
+template <typename T, int HD>
+__device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
+  constexpr int LPT = HD / 4, TPW = 32 / LPT;
+  const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
+  const bool upper = (lane % LPT) >= LPT / 2;
+  const int seq = d.seq[row], pos = d.pos[row];
+  if (seq < 0 || seq >= d.c.n_seqs || pos < 0 || pos >= d.c.pages_per_seq * kKv8Page) return;  // flagged with K and V
+  const float4 g = norm_weight(d.q_norm, d0);
+  float4 cs, sn;
+  bool turn = d.rope_cos != nullptr;
+  if (turn) {
+    const int rp = d.rope_pos ? d.rope_pos[row] : pos;
+    turn = rp >= 0 && rp < d.rope_rows;
+    if (turn) {
+      cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+      sn = load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+    } else {
+      raise(d.flags, QTTS_KV8_ROPE_RANGE);
+    }
+  }
+  const T* src = static_cast<const T*>(d.q) + (size_t)row * d.ldq;
+  T* dst = static_cast<T*>(d.q_out) + (size_t)row * d.ldqo;
+  constexpr int N = kQHeads / TPW;
+  float4 x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int h = h0 + i * TPW + sub;
+    x[i] = h < d.heads ? load4(src + (size_t)h * HD + d0) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int h = h0 + i * TPW + sub;
+    if (d.q_norm) x[i] = head_norm<HD>(x[i], g);
+    if (turn) x[i] = rotate<HD>(x[i], cs, sn, upper);
+    if (h < d.heads) store4(dst + (size_t)h * HD + d0, x[i]);
+  }
+}
+
+// A warp takes the blocks that start in a chunk of rows, for one K or V head
+// (they are its alone: the block's scale needs all of its new tokens, which
+// stay in registers between the maximum and the codes), or kQHeads query heads
+// of one row.  HBM-bound: every input is read once, every output written once,
+// and a block that grows has its earlier codes read and written again.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (w < d.kv_warps) {
+    const int per = 2 * d.c.kv_heads, j = (int)(w % per);
+    append_blocks<T, HD>(d, (int)(w / per), j & 1, j >> 1);
+  } else if (w < d.n_warps) {
+    const int per = (d.heads + kQHeads - 1) / kQHeads;
+    const long i = w - d.kv_warps;
+    rotate_queries<T, HD>(d, (int)(i / per), (int)(i % per) * kQHeads);
+  }
+}
+
+// ---- attention -------------------------------------------------------------------
+// Scores and products run on the matrix units in f16 with f32 sums.  A code is
+// exact in f16; a query (scaled by a power of two to at most 2) and a weight
+// (at most 2) are split into f16 hi + lo, lo scaled by 2^11, about 22 bits.
+// One m16n8k16 product takes up to 8 slots (a slot is a query head of a row)
+// with hi in row s and lo in row s + 8 of its 16-row operand, so the split
+// costs nothing, and hi + lo of a slot meet in one thread.
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two bytes of w ^ 0x80808080 (a code + 128) become the f16 pair 1024 + (code +
+// 128) by a byte permute onto 0x64; subtracting 1152 is exact.
+__device__ __forceinline__ uint32_t half2_of(uint32_t biased, uint32_t sel) {
+  uint32_t r = __byte_perm(biased, 0x64646464u, sel);
+  const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+  return half2_bits(h);
+}
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) { split_pair(a, b, hi, lo); }
+
+constexpr int kSlots = 8;
+constexpr int kAttnWarps = 4;
+
+// One sequence's rows of a unit: what its slots see.
+struct Segment {
+  int row0, rows;  // rows [row0, row0 + rows)
+  int seq;
+  int lo, hi;      // positions [lo, hi) that any of them sees
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_constant__ Kv8AttnDesc d) {
+  constexpr int NT = HD / 8;   // dims a thread's V chunk holds, and n-tiles of the output
+  constexpr int KJ = HD / 64;  // 64-dim halves of a row
+  __shared__ float s_o[kAttnWarps][kSlots][HD];
+  __shared__ float s_m[kAttnWarps][kSlots], s_l[kAttnWarps][kSlots];
+  __shared__ float s_po[kSlots][HD];
+  __shared__ float s_pm[kSlots], s_pl[kSlots];
+  pdl_launch_dependents();
+  pdl_wait();
+  const qtts_kv8_cache& c = d.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int nsplit = gridDim.y, split = blockIdx.y;
+  const int per = c.kv_heads * d.head_chunks;
+  const int unit = blockIdx.x / per, rest = blockIdx.x % per;
+  const int kvh = rest / d.head_chunks, hc = rest % d.head_chunks;
+  const int group = d.heads / c.kv_heads;
+  const int h0 = kvh * group + hc * d.unit_heads;                        // first query head of the unit
+  const int nh = min(d.unit_heads, group - hc * d.unit_heads);           // its heads
+  const int row_end = min(d.n_rows, (unit + 1) * d.group_rows);
+  const int cap = c.pages_per_seq * kKv8Page;
+  cg::cluster_group cluster = cg::this_cluster();
+
+  for (int row = unit * d.group_rows; row < row_end;) {
+    // the next run of rows of one sequence
+    Segment sg;
+    sg.row0 = row;
+    sg.seq = d.seq[row];
+    sg.lo = 0x7fffffff;
+    sg.hi = 0;
+    for (; row < row_end && d.seq[row] == sg.seq; ++row) {
+      int p = d.pos[row];
+      if (p >= cap) {
+        if (tid == 0 && sg.seq >= 0) raise(d.flags, QTTS_KV8_BAD_ROW);
+        p = cap - 1;
+      }
+      if (p < 0) continue;
+      sg.hi = max(sg.hi, p + 1);
+      sg.lo = min(sg.lo, d.window > 0 ? max(0, p + 1 - d.window) : 0);
+    }
+    sg.rows = row - sg.row0;
+    if (sg.seq < 0) continue;  // padding
+    if (sg.seq >= c.n_seqs) {
+      if (tid == 0) raise(d.flags, QTTS_KV8_BAD_ROW);
+      continue;
+    }
+    const int nslots = sg.rows * nh;
+    // this thread's slot: query fragments, scale, and the positions it sees
+    uint32_t qa[KJ * 4][4];
+    float qscale = 0.0f;
+    int see_lo = 0, see_hi = 0;
+    {
+      float4 x[KJ][4];
+      float big = 0.0f;
+      const bool on = g < nslots;
+      const T* qp = static_cast<const T*>(d.q) + (size_t)(sg.row0 + (on ? g / nh : 0)) * d.ldq +
+                    (size_t)(h0 + (on ? g % nh : 0)) * HD;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[j][i] = on ? load4(qp + 16 * (t + 4 * j) + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          big = fmaxf(big, fmaxf(fmaxf(fabsf(x[j][i].x), fabsf(x[j][i].y)), fmaxf(fabsf(x[j][i].z), fabsf(x[j][i].w))));
+        }
+      big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
+      const int ef = (__float_as_int(big) >> 23) & 255;
+      const int ex = ef == 0 || ef == 255 ? 0 : ef - 127;
+      const float dn = ldexpf(1.0f, -ex);
+      qscale = ldexpf(d.scale * 1.4426950408889634f, ex);  // scores in units of log 2
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          split_f16(x[j][i].x * dn, x[j][i].y * dn, qa[j * 4 + i][0], qa[j * 4 + i][1]);
+          split_f16(x[j][i].z * dn, x[j][i].w * dn, qa[j * 4 + i][2], qa[j * 4 + i][3]);
+        }
+      if (on) {
+        see_hi = min(d.pos[sg.row0 + g / nh], cap - 1) + 1;
+        see_lo = d.window > 0 ? max(0, see_hi - d.window) : 0;
+      }
+    }
+    float o[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+    float m = -INFINITY, mo = -INFINITY, l = 0.0f;
+
+    // this split's pages, this warp's among them
+    const int p0 = sg.hi > 0 ? sg.lo / kKv8Page : 0, p1 = (sg.hi + kKv8Page - 1) / kKv8Page;
+    const int share = (p1 - p0 + nsplit - 1) / nsplit;
+    const int pb = p0 + split * share, pe = min(p1, pb + share);
+    const int* table = c.page_table + (size_t)sg.seq * c.pages_per_seq;
+    for (int pg = pb + warp; pg < pe; pg += kAttnWarps) {
+      const int page = table[pg];
+      if (page < 0 || page >= c.n_pages) {
+        if (lane == 0) raise(d.flags, QTTS_KV8_BAD_PAGE);
+        continue;
+      }
+      const int8_t* kb = block_codes(c, page, 0, kvh);
+      const int8_t* vb = block_codes(c, page, 1, kvh);
+      const float sk = *block_scale(c, page, 0, kvh), sv = *block_scale(c, page, 1, kvh);
+      uint4 kw[2][KJ];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+          kw[n][j] = *reinterpret_cast<const uint4*>(kb + (n * 8 + g) * HD + 16 * (t + 4 * j));
+      uint32_t vw[4][NT / 4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, dims NT * g ...
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int8_t* src = vb + (2 * t + (e & 1) + (e >> 1) * 8) * HD + NT * g;
+        if (NT == 16) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src);
+          vw[e][0] = u.x;
+          vw[e][1] = u.y;
+          vw[e][NT / 4 - 2] = u.z;
+          vw[e][NT / 4 - 1] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          vw[e][0] = u.x;
+          vw[e][1] = u.y;
+        }
+      }
+      // scores: positions 8n + 2t, + 1 of slot g in (acc[n][0] + 2^-11 acc[n][2], ...)
+      float acc[2][4] = {};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          const uint32_t w[4] = {kw[n][j].x, kw[n][j].y, kw[n][j].z, kw[n][j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t u = w[i] ^ 0x80808080u;
+            mma16816(acc[n], qa[j * 4 + i], half2_of(u, 0x4140), half2_of(u, 0x4342));
+          }
+        }
+      float s[2][2], pm = -INFINITY;
+      const float f = qscale * sk;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = pg * kKv8Page + n * 8 + 2 * t + e;
+          s[n][e] = at >= see_lo && at < see_hi ? (acc[n][e] + acc[n][e + 2] * (1.0f / kSplitLoScale)) * f : -INFINITY;
+          pm = fmaxf(pm, s[n][e]);
+        }
+      pm = fmaxf(pm, __shfl_xor_sync(kFull, pm, 1));
+      pm = fmaxf(pm, __shfl_xor_sync(kFull, pm, 2));
+      // sv = fr * 2^ev; the output's running exponent follows score + ev, so
+      // that the weights times sv stay within f16 whatever the scales are
+      const int svb = __float_as_int(sv), svx = (svb >> 23) & 255;
+      const float ev = svx == 0 ? -126.0f : svx == 255 ? 0.0f : (float)(svx - 127);
+      const float fr = svx == 0 ? sv * 0x1p126f
+                                : svx == 255 ? sv : __int_as_float((svb & 0x807fffff) | 0x3f800000);
+      const float mn = fmaxf(m, pm), mon = fmaxf(mo, pm + ev);
+      const float mz = mn == -INFINITY ? 0.0f : mn;
+      l *= ex2(m - mz);
+      const float beta = mo == mon ? 1.0f : ex2(mo - mon);
+      if (__any_sync(kFull, beta != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] *= beta;
+      }
+      m = mn;
+      mo = mon;
+      const float fac = mon == -INFINITY ? 0.0f : ex2(fminf(mz - mon + ev, 120.0f)) * fr;
+      uint32_t pa[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float a = ex2(s[n][0] - mz), b = ex2(s[n][1] - mz);
+        l += a + b;
+        split_f16(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
+      }
+#pragma unroll
+      for (int q = 0; q < NT / 4; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = vw[e][q] ^ 0x80808080u;
+        const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
+        const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
+        mma16816(o[q * 4 + 0], pa, half2_of(a01, 0x4140), half2_of(b01, 0x4140));
+        mma16816(o[q * 4 + 1], pa, half2_of(a01, 0x4342), half2_of(b01, 0x4342));
+        mma16816(o[q * 4 + 2], pa, half2_of(a23, 0x4140), half2_of(b23, 0x4140));
+        mma16816(o[q * 4 + 3], pa, half2_of(a23, 0x4342), half2_of(b23, 0x4342));
+      }
+    }
+    // join the warps, then the splits of the cluster, in their order
+    l += __shfl_xor_sync(kFull, l, 1);
+    l += __shfl_xor_sync(kFull, l, 2);
+    if (l != l) m = INFINITY;  // a NaN score: the joins below then give NaN
+    const float back = m == -INFINITY || mo == -INFINITY ? 0.0f : ex2(mo - m);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        s_o[warp][g][NT * (2 * t + e) + i] = (o[i][e] + o[i][e + 2] * (1.0f / kSplitLoScale)) * back;
+    if (t == 0) {
+      s_m[warp][g] = m;
+      s_l[warp][g] = l;
+    }
+    __syncthreads();
+    for (int i = tid; i < nslots * HD; i += kAttnWarps * 32) {
+      const int s = i / HD, e = i % HD;
+      float mx = s_m[0][s];
+      for (int w = 1; w < kAttnWarps; ++w) mx = fmaxf(mx, s_m[w][s]);
+      float sum = 0.0f, ll = 0.0f;
+      if (mx > -INFINITY)
+        for (int w = 0; w < kAttnWarps; ++w) {
+          const float k = ex2(s_m[w][s] - mx);
+          sum += s_o[w][s][e] * k;
+          ll += s_l[w][s] * k;
+        }
+      s_po[s][e] = sum;
+      if (e == 0) {
+        s_pm[s] = mx;
+        s_pl[s] = ll;
+      }
+    }
+    if (nsplit > 1) cluster.sync();
+    else __syncthreads();
+    for (int i = tid + split * kAttnWarps * 32; i < nslots * HD; i += nsplit * kAttnWarps * 32) {
+      const int s = i / HD, e = i % HD;
+      float mx = -INFINITY, sum = 0.0f, ll = 0.0f;
+      for (int r = 0; r < nsplit; ++r) mx = fmaxf(mx, nsplit > 1 ? *cluster.map_shared_rank(&s_pm[s], r) : s_pm[s]);
+      for (int r = 0; r < nsplit; ++r) {
+        const float rm = nsplit > 1 ? *cluster.map_shared_rank(&s_pm[s], r) : s_pm[s];
+        const float k = rm == -INFINITY ? 0.0f : ex2(rm - mx);
+        sum += (nsplit > 1 ? *cluster.map_shared_rank(&s_po[s][e], r) : s_po[s][e]) * k;
+        ll += (nsplit > 1 ? *cluster.map_shared_rank(&s_pl[s], r) : s_pl[s]) * k;
+      }
+      const int orow = sg.row0 + s / nh, head = h0 + s % nh;
+      const float v = mx == -INFINITY ? 0.0f : __fdiv_rn(sum, ll);
+      T* op = static_cast<T*>(d.out) + (size_t)orow * d.ldo + (size_t)head * HD + e;
+      if constexpr (sizeof(T) == 4) *op = v;
+      else *op = T(v);
+      if (e == 0 && d.lse)
+        d.lse[(size_t)orow * d.heads + head] = mx == -INFINITY ? -INFINITY : (mx + log2f(ll)) * 0.6931471805599453f;
+    }
+    if (nsplit > 1) cluster.sync();
+    else __syncthreads();
+  }
+}
+
+template <typename T, int HD>
+cudaError_t launch_append_t(const Kv8AppendDesc& d, cudaStream_t st) {
+  return launch_k(kv8_append_kernel<T, HD>, dim3((unsigned)((d.n_warps + 3) / 4)), dim3(128), 0, st,
+                  LaunchOpts{true, 1}, d);
+}
+template <typename T, int HD>
+cudaError_t launch_attn_t(const Kv8AttnDesc& d, unsigned units, unsigned nsplit, cudaStream_t st) {
+  return launch_k(kv8_attn_kernel<T, HD>, dim3(units, nsplit), dim3(kAttnWarps * 32), 0, st, LaunchOpts{true, nsplit},
+                  d);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_append(Kv8AppendDesc d, int dtype, int sms, cudaStream_t st) {
+  // A warp per row, head and K / V while that fits the device at once (64
+  // warps an SM); above that a warp looks at up to 16 rows, which hold one
+  // block of a long prompt or 16 of single tokens.
+  d.chunk = 1;
+  auto kv_warps = [&] { return ((long)d.n_rows + d.chunk - 1) / d.chunk * 2 * d.c.kv_heads; };
+  while (d.chunk < kKv8Page && kv_warps() > (long)sms * 64) d.chunk *= 2;
+  d.kv_warps = kv_warps();
+  d.n_warps = d.kv_warps + (d.q ? (long)d.n_rows * ((d.heads + kQHeads - 1) / kQHeads) : 0);
+  const bool w = d.c.head_dim == 128;
+  switch (dtype) {
+    case DT_F16: return w ? launch_append_t<__half, 128>(d, st) : launch_append_t<__half, 64>(d, st);
+    case DT_BF16: return w ? launch_append_t<__nv_bfloat16, 128>(d, st) : launch_append_t<__nv_bfloat16, 64>(d, st);
+    default: return w ? launch_append_t<float, 128>(d, st) : launch_append_t<float, 64>(d, st);
+  }
+}
+
+cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st) {
+  const int group = d.heads / d.c.kv_heads;
+  d.unit_heads = std::min(group, kSlots);
+  d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
+  d.group_rows = std::max(1, std::min(max_rows, kSlots / d.unit_heads));
+  const long units = ((long)d.n_rows + d.group_rows - 1) / d.group_rows * d.c.kv_heads * d.head_chunks;
+  // split a row's pages while the units leave SMs free and every warp has a page
+  const int pages = (max_len + kKv8Page - 1) / kKv8Page;
+  unsigned ns = 1;
+  while (ns < 8 && units * ns < 2l * sms && (int)ns * kAttnWarps < pages) ns *= 2;
+  const unsigned u = (unsigned)units;
+  const bool w = d.c.head_dim == 128;
+  switch (dtype) {
+    case DT_F16: return w ? launch_attn_t<__half, 128>(d, u, ns, st) : launch_attn_t<__half, 64>(d, u, ns, st);
+    case DT_BF16:
+      return w ? launch_attn_t<__nv_bfloat16, 128>(d, u, ns, st) : launch_attn_t<__nv_bfloat16, 64>(d, u, ns, st);
+    default: return w ? launch_attn_t<float, 128>(d, u, ns, st) : launch_attn_t<float, 64>(d, u, ns, st);
+  }
+}
+
+// ---- host side of the entry points ----------------------------------------------
+
+OnDeviceOf::OnDeviceOf(const void* p) {
+  cudaPointerAttributes a;
+  cudaError_t e = cudaPointerGetAttributes(&a, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    code = e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver ? QTTS_ERR_NODEV : QTTS_ERR_CUDA;
+    err = cudaGetErrorString(e);
+    return;
+  }
+  if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) {
+    code = QTTS_ERR_BADARG;
+    err = "not a device pointer";
+    return;
+  }
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || (cur != a.device && cudaSetDevice(a.device) != cudaSuccess)) {
+    cudaGetLastError();
+    code = QTTS_ERR_CUDA;
+    err = "the device of the buffers cannot be made current";
+    return;
+  }
+  if (cur != a.device) prev_ = cur;
+  static int sms[64] = {0};
+  int n = a.device >= 0 && a.device < 64 ? sms[a.device] : 0;
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, a.device) != cudaSuccess || n <= 0) n = 148;
+    if (a.device >= 0 && a.device < 64) sms[a.device] = n;
+  }
+  sm_count = n;
+}
+OnDeviceOf::~OnDeviceOf() {
+  if (prev_ >= 0) cudaSetDevice(prev_);
+}
+
+namespace {
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// nullptr, or what is wrong with the cache description
+const char* cache_fault(const qtts_kv8_cache* c) {
+  if (!c || !c->codes || !c->scales || !c->page_table) return "the cache has a null pointer";
+  if (c->head_dim != 64 && c->head_dim != 128) return "the cache's head_dim is not 64 or 128";
+  if (c->kv_heads <= 0 || c->kv_heads > 1024) return "the cache's kv_heads is not 1..1024";
+  if (c->n_pages <= 0 || c->n_seqs <= 0 || c->pages_per_seq <= 0) return "the cache has no pages or sequences";
+  if (c->pages_per_seq > INT32_MAX / kKv8Page) return "a sequence's positions pass 2^31";
+  if (c->page_stride < 2ll * c->kv_heads * kKv8Page * c->head_dim || c->page_stride % 16)
+    return "page_stride is less than a page or not a multiple of 16";
+  if (c->scale_stride < 2ll * c->kv_heads) return "scale_stride is less than a page's scales";
+  if (!aligned(c->codes, 16) || !aligned(c->scales, 4) || !aligned(c->page_table, 4)) return "the cache is misaligned";
+  return nullptr;
+}
+// rows of `cols` elements: four-element loads
+const char* rows_fault(const void* p, int64_t ld, int64_t cols, int dtype) {
+  if (!p) return "a null pointer";
+  if (ld < cols || ld % 4) return "a row stride that is less than a row or not a multiple of 4";
+  if (!aligned(p, 4 * dtype_bytes(dtype))) return "a misaligned pointer";
+  return nullptr;
+}
+int refuse(const char* what, const char* why) { return fail(QTTS_ERR_BADARG, std::string(what) + ": " + why); }
+int launched(cudaError_t e) {
+  if (e == cudaSuccess) return QTTS_OK;
+  cudaGetLastError();
+  return fail(QTTS_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace qtts
+
+using namespace qtts;
+
+extern "C" {
+
+int qtts_kv8_append_dev(const qtts_kv8_cache* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                        const void* q, int64_t ldq, void* q_out, int64_t ldqo, int heads, int dtype,
+                        const uint16_t* q_norm, const uint16_t* k_norm, const float* rope_cos, const float* rope_sin,
+                        int rope_rows, const int32_t* seq, const int32_t* pos, const int32_t* rope_pos, int n_rows,
+                        int32_t* flags, void* stream) try {
+  const char* f = cache_fault(cache);
+  if (f) return refuse("kv8 append", f);
+  if (dtype != QTTS_F32 && dtype != QTTS_F16 && dtype != QTTS_BF16) return refuse("kv8 append", "unknown dtype");
+  if (n_rows < 0 || (n_rows > 0 && (!seq || !pos))) return refuse("kv8 append", "bad rows");
+  const int64_t kv_cols = (int64_t)cache->kv_heads * cache->head_dim;
+  if (n_rows > 0) {
+    if ((f = rows_fault(k, ldk, kv_cols, dtype)) || (f = rows_fault(v, ldv, kv_cols, dtype))) return refuse("kv8 append, k or v", f);
+    if (!q != !q_out) return refuse("kv8 append", "q and q_out go together");
+    if (q) {
+      if (heads <= 0 || heads > 16384) return refuse("kv8 append", "bad heads");
+      const int64_t cols = (int64_t)heads * cache->head_dim;
+      if ((f = rows_fault(q, ldq, cols, dtype)) || (f = rows_fault(q_out, ldqo, cols, dtype))) return refuse("kv8 append, q", f);
+    }
+  }
+  if (!rope_cos != !rope_sin || (rope_cos && rope_rows <= 0)) return refuse("kv8 append", "bad rotation tables");
+  if (!aligned(rope_cos, 16) || !aligned(rope_sin, 16) || !aligned(q_norm, 8) || !aligned(k_norm, 8))
+    return refuse("kv8 append", "misaligned rotation tables or norm weights");
+  if (n_rows == 0) return QTTS_OK;
+  OnDeviceOf on(cache->codes);
+  if (on.err) return fail(on.code, std::string("kv8 append, the cache: ") + on.err);
+  Kv8AppendDesc d;
+  d.c = *cache;
+  d.q = q;
+  d.k = k;
+  d.v = v;
+  d.q_out = q_out;
+  d.ldq = ldq;
+  d.ldk = ldk;
+  d.ldv = ldv;
+  d.ldqo = ldqo;
+  d.heads = q ? heads : 0;
+  d.q_norm = reinterpret_cast<const __half*>(q_norm);
+  d.k_norm = reinterpret_cast<const __half*>(k_norm);
+  d.rope_cos = rope_cos;
+  d.rope_sin = rope_sin;
+  d.rope_rows = rope_rows;
+  d.seq = seq;
+  d.pos = pos;
+  d.rope_pos = rope_pos;
+  d.n_rows = n_rows;
+  d.flags = flags;
+  return launched(launch_kv8_append(d, dtype, on.sm_count, (cudaStream_t)stream));
+} catch (...) {
+  return QTTS_ERR_OOM;
+}
+
+int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t ldq, int heads, int dtype, float scale,
+                           int window, const int32_t* seq, const int32_t* pos, int n_rows, int max_rows, int max_len,
+                           void* out, int64_t ldo, float* lse, int32_t* flags, void* stream) try {
+  const char* f = cache_fault(cache);
+  if (f) return refuse("kv8 attention", f);
+  if (dtype != QTTS_F32 && dtype != QTTS_F16 && dtype != QTTS_BF16) return refuse("kv8 attention", "unknown dtype");
+  if (heads <= 0 || heads % cache->kv_heads || heads > 16384)
+    return refuse("kv8 attention", "heads is not a multiple of the cache's kv_heads (up to 16384)");
+  if (window < 0 || max_rows < 0 || max_len < 0) return refuse("kv8 attention", "negative window, max_rows or max_len");
+  if (n_rows < 0 || (n_rows > 0 && (!seq || !pos))) return refuse("kv8 attention", "bad rows");
+  if (n_rows == 0) return QTTS_OK;
+  const int64_t cols = (int64_t)heads * cache->head_dim;
+  if ((f = rows_fault(q, ldq, cols, dtype)) || (f = rows_fault(out, ldo, cols, dtype))) return refuse("kv8 attention, q or out", f);
+  if ((int64_t)n_rows * heads > INT32_MAX) return fail(QTTS_ERR_RANGE, "kv8 attention: n_rows * heads passes 2^31");
+  OnDeviceOf on(cache->codes);
+  if (on.err) return fail(on.code, std::string("kv8 attention, the cache: ") + on.err);
+  Kv8AttnDesc d;
+  d.c = *cache;
+  d.q = q;
+  d.out = out;
+  d.lse = lse;
+  d.ldq = ldq;
+  d.ldo = ldo;
+  d.heads = heads;
+  d.scale = scale;
+  d.window = window;
+  d.seq = seq;
+  d.pos = pos;
+  d.n_rows = n_rows;
+  d.flags = flags;
+  const int cap = cache->pages_per_seq * kKv8Page;
+  int len = max_len == 0 ? cap : std::min(max_len, cap);
+  if (window > 0) len = std::min(len, window + std::max(1, max_rows) - 1);
+  return launched(launch_kv8_attention(d, dtype, max_rows == 0 ? 1 : max_rows, len, on.sm_count, (cudaStream_t)stream));
+} catch (...) {
+  return QTTS_ERR_OOM;
+}
+
+}  // extern "C"

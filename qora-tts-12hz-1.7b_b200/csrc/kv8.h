@@ -1,0 +1,65 @@
+// kv8.h -- the 8-bit paged K/V cache: descriptors and launchers of its append
+// and attention kernels, and what the entry points on device pointers share.
+#pragma once
+#include "../../include/qtts.h"
+#include "kernels.h"
+
+namespace qtts {
+
+constexpr int kKv8Page = 16;  // positions per page, the block a scale belongs to
+
+enum DType : int { DT_F32 = QTTS_F32, DT_F16 = QTTS_F16, DT_BF16 = QTTS_BF16 };
+inline int dtype_bytes(int t) { return t == DT_F32 ? 4 : 2; }
+
+// Makes the device that holds `p` current while it lives, so that a caller's
+// buffers may lie on another device than its current one.  `err` says why not
+// (a host pointer, no device).
+class OnDeviceOf {
+ public:
+  explicit OnDeviceOf(const void* p);
+  ~OnDeviceOf();
+  const char* err = nullptr;
+  int code = 0;
+  int sm_count = 148;
+
+ private:
+  int prev_ = -1;
+};
+
+struct Kv8AppendDesc {
+  qtts_kv8_cache c;
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  void* q_out = nullptr;
+  long ldq = 0, ldk = 0, ldv = 0, ldqo = 0;
+  int heads = 0;
+  const __half *q_norm = nullptr, *k_norm = nullptr;
+  const float *rope_cos = nullptr, *rope_sin = nullptr;
+  int rope_rows = 0;
+  const int *seq = nullptr, *pos = nullptr, *rope_pos = nullptr;
+  int n_rows = 0;
+  int* flags = nullptr;
+  int chunk = 1;       // rows whose blocks one warp looks for (1, 2, 4, 8 or 16)
+  long kv_warps = 0;   // warps of K / V blocks; the q warps follow them
+  long n_warps = 0;
+};
+cudaError_t launch_kv8_append(Kv8AppendDesc d, int dtype, int sms, cudaStream_t st);
+
+struct Kv8AttnDesc {
+  qtts_kv8_cache c;
+  const void* q = nullptr;
+  void* out = nullptr;
+  float* lse = nullptr;
+  long ldq = 0, ldo = 0;
+  int heads = 0;
+  float scale = 1.0f;
+  int window = 0;
+  const int *seq = nullptr, *pos = nullptr;
+  int n_rows = 0;
+  int* flags = nullptr;
+  int group_rows = 1;   // rows of one unit
+  int head_chunks = 1;  // units along the query heads of one K/V head
+  int unit_heads = 1;   // query heads of a unit
+};
+cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st);
+
+}  // namespace qtts

@@ -60,6 +60,13 @@ class Utterance(C.Structure):
                 ("params", SampleParams)]
 
 
+class Kv8CacheDesc(C.Structure):
+    """qtts.h qtts_kv8_cache."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("page_table", C.c_void_p), ("n_pages", C.c_int),
+                ("n_seqs", C.c_int), ("pages_per_seq", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_stride", C.c_int64), ("scale_stride", C.c_int64)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built: run `make -C {PKG_DIR}` (the CUDA path has no fallback)")
@@ -115,6 +122,11 @@ def _load():
         "qtts_q4_dequant_dev": (C.c_int, [P, P, C.c_int, C.c_int, P, P]),
         "qtts_expf_dev": (C.c_int, [P, P, C.c_int, P]),
         "qtts_q4_quantize_dev": (C.c_int, [P, C.c_int, C.c_int, P, P, P]),
+        "qtts_kv8_append_dev": (C.c_int, [C.POINTER(Kv8CacheDesc), P, C.c_int64, P, C.c_int64, P, C.c_int64, P,
+                                          C.c_int64, C.c_int, C.c_int, P, P, P, P, C.c_int, P, P, P, C.c_int, P, P]),
+        "qtts_kv8_attention_dev": (C.c_int, [C.POINTER(Kv8CacheDesc), P, C.c_int64, C.c_int, C.c_int, C.c_float,
+                                             C.c_int, P, P, C.c_int, C.c_int, C.c_int, P, C.c_int64, P, P, P]),
+        "qtts_sample_rows_dev": (C.c_int, [P, C.c_int64, C.c_int, C.c_int, C.c_int, P, P, P, P, P, P, P, P, P]),
         "qtts_q4_quantize": (C.c_int, [fp, C.c_int, C.c_int, C.POINTER(C.c_uint8), C.POINTER(C.c_uint16)]),
     }
     for name, (res, args) in sig.items():
@@ -482,3 +494,67 @@ def q4_quantize_dev(data_ptr, k, n, packed_ptr, scales_ptr, stream=0):
 def expf_dev(x_ptr, y_ptr, n, stream=0):
     """The sampler's exp (bit-identical to glibc expf), for validation."""
     _check(lib.qtts_expf_dev(x_ptr, y_ptr, n, stream or None))
+
+
+# ---- 8-bit paged K/V cache and row sampling on device pointers (qtts.h) --------
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}  # qtts.h QTTS_F32 / QTTS_F16 / QTTS_BF16
+KV8_PAGE = 16  # positions per page
+KV8_BAD_ROW, KV8_BAD_PAGE, KV8_ROPE_RANGE = 1, 2, 4  # bits of the flags word
+SAMPLE_ROWS_MAX_V = 262144
+
+
+def _dtype(name: str) -> int:
+    if name not in DTYPES:
+        raise QttsError(ERR_BADARG, f"dtype must be one of {sorted(DTYPES)}, got {name!r}")
+    return DTYPES[name]
+
+
+class Kv8Cache:
+    """Describes a paged 8-bit K/V cache that lives in the caller's device
+    buffers (qtts.h qtts_kv8_cache): codes int8 [page][2][kv_heads][16][head_dim],
+    scales f32 [page][2][kv_heads], page_table i32 [n_seqs][pages_per_seq].
+    The strides (bytes of codes, floats of scales; 0 = pages stand close)
+    address one layer of a pool of several."""
+
+    def __init__(self, codes_ptr: int, scales_ptr: int, page_table_ptr: int, n_pages: int, n_seqs: int,
+                 pages_per_seq: int, kv_heads: int, head_dim: int, page_stride: int = 0, scale_stride: int = 0):
+        self.desc = Kv8CacheDesc(codes_ptr, scales_ptr, page_table_ptr, n_pages, n_seqs, pages_per_seq, kv_heads,
+                                 head_dim, page_stride or 2 * kv_heads * KV8_PAGE * head_dim,
+                                 scale_stride or 2 * kv_heads)
+        self.ref = C.byref(self.desc)
+        self.kv_cols = kv_heads * head_dim
+        self.head_dim = head_dim
+
+
+def kv8_append_dev(cache: Kv8Cache, k_ptr, v_ptr, seq_ptr, pos_ptr, n_rows, dtype="f32", q_ptr=0, q_out_ptr=0,
+                   heads=0, q_norm_ptr=0, k_norm_ptr=0, cos_ptr=0, sin_ptr=0, rope_rows=0, rope_pos_ptr=0, ldk=0,
+                   ldv=0, ldq=0, ldqo=0, flags_ptr=0, stream=0):
+    """Append K and V rows to the 8-bit cache, QK-norm and position rotation
+    on the way, the rotated queries to q_out (qtts.h qtts_kv8_append_dev).
+    Row strides of 0: the rows stand close."""
+    kv, qc = cache.kv_cols, heads * cache.head_dim
+    _check(lib.qtts_kv8_append_dev(cache.ref, k_ptr or None, ldk or kv, v_ptr or None, ldv or kv, q_ptr or None,
+                                   ldq or qc, q_out_ptr or None, ldqo or qc, heads, _dtype(dtype), q_norm_ptr or None,
+                                   k_norm_ptr or None, cos_ptr or None, sin_ptr or None, rope_rows, seq_ptr or None,
+                                   pos_ptr or None, rope_pos_ptr or None, n_rows, flags_ptr or None, stream or None))
+
+
+def kv8_attention_dev(cache: Kv8Cache, q_ptr, out_ptr, seq_ptr, pos_ptr, n_rows, heads, dtype="f32", scale=None,
+                      window=0, max_rows=0, max_len=0, lse_ptr=0, ldq=0, ldo=0, flags_ptr=0, stream=0):
+    """GQA attention of rows over the 8-bit cache (qtts.h
+    qtts_kv8_attention_dev); scale None is 1 / sqrt(head_dim)."""
+    cols = heads * cache.head_dim
+    _check(lib.qtts_kv8_attention_dev(cache.ref, q_ptr or None, ldq or cols, heads, _dtype(dtype),
+                                      cache.head_dim ** -0.5 if scale is None else scale, window, seq_ptr or None,
+                                      pos_ptr or None, n_rows, max_rows, max_len, out_ptr or None, ldo or cols,
+                                      lse_ptr or None, flags_ptr or None, stream or None))
+
+
+def sample_rows_dev(logits_ptr, n_rows, V, u_ptr, token_ptr, dtype="f32", temperature_ptr=0, top_k_ptr=0, top_p_ptr=0,
+                    min_p_ptr=0, kept_ptr=0, logprob_ptr=0, ld=0, stream=0):
+    """Temperature / top-k / top-p / min-p sampling of rows of logits from
+    given uniform numbers (qtts.h qtts_sample_rows_dev)."""
+    _check(lib.qtts_sample_rows_dev(logits_ptr or None, ld or V, _dtype(dtype), n_rows, V, temperature_ptr or None,
+                                    top_k_ptr or None, top_p_ptr or None, min_p_ptr or None, u_ptr or None,
+                                    token_ptr or None, kept_ptr or None, logprob_ptr or None, stream or None))

@@ -1,0 +1,490 @@
+"""The 8-bit paged K/V cache on the GPU: appended codes and scales bit for bit
+against the documented f32 steps, attention against a 64-bit restatement."""
+import numpy as np
+import pytest
+
+import serving_ref as R
+from conftest import has_gpu
+
+pytestmark = pytest.mark.gpu
+if has_gpu():
+    import torch
+
+    TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def dev(x, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    return t if dtype is None else t.to(TYPES[dtype])
+
+
+def host(t):
+    return t.float().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+class Pool:
+    """A cache of random blocks on the host and the device; `layers` > 1 makes
+    it one layer of a larger pool."""
+
+    def __init__(self, qtts, rng, n_seqs, per_seq, kvh, hd, spare=2, layers=1, layer=0):
+        n = n_seqs * per_seq + spare
+        self.codes = np.clip(np.rint(rng.standard_normal((n, 2, kvh, 16, hd)) * 36), -127, 127).astype(np.int8)
+        self.scales = (np.exp(0.5 * rng.standard_normal((n, 2, kvh))) / 36).astype(np.float32)
+        self.table = rng.permutation(n)[:n_seqs * per_seq].reshape(n_seqs, per_seq).astype(np.int32)
+        self.d_codes = torch.full((n, layers, 2, kvh, 16, hd), 77, dtype=torch.int8, device="cuda")
+        self.d_scales = torch.full((n, layers, 2, kvh), 3.0, device="cuda")
+        self.layer = layer
+        self.d_codes[:, layer] = dev(self.codes)
+        self.d_scales[:, layer] = dev(self.scales)
+        self.d_table = dev(self.table)
+        blk = 2 * kvh * 16 * hd
+        self.cache = qtts.Kv8Cache(self.d_codes.data_ptr() + layer * blk, self.d_scales.data_ptr() + layer * 2 * kvh * 4,
+                                   self.d_table.data_ptr(), n, n_seqs, per_seq, kvh, hd, layers * blk,
+                                   layers * 2 * kvh)
+        self.kvh, self.hd = kvh, hd
+
+    def got(self):
+        return host(self.d_codes[:, self.layer]), host(self.d_scales[:, self.layer])
+
+    def others_untouched(self):
+        keep = [i for i in range(self.d_codes.shape[1]) if i != self.layer]
+        return bool((self.d_codes[:, keep] == 77).all()) and bool((self.d_scales[:, keep] == 3.0).all())
+
+
+def tables(n, hd):
+    a = np.arange(n)[:, None] * 10000.0 ** (-np.arange(hd // 2) / (hd // 2))
+    return np.cos(a).astype(np.float32), np.sin(a).astype(np.float32)
+
+
+def rows_of(parts):
+    """[(seq, first position, rows)] -> seq, pos"""
+    seq = np.concatenate([np.full(n, s) for s, _, n in parts]).astype(np.int32)
+    pos = np.concatenate([p + np.arange(n) for _, p, n in parts]).astype(np.int32)
+    return seq, pos
+
+
+APPENDS = {
+    "one token at 0": [(0, 0, 1)],
+    "one token inside a page": [(1, 21, 1)],
+    "last slot": [(2, 47, 1)],
+    "a page and a bit": [(0, 0, 17)],
+    "chunks that start and end inside pages": [(0, 5, 30), (-1, 0, 2), (2, 31, 2), (1, 15, 3), (-1, 9, 5)],
+    "single tokens and padding": [(2, 3, 1), (-1, 0, 1), (0, 16, 1), (1, 40, 1), (-1, 5, 3)],
+    "a chunk boundary inside a block": [(0, 1, 14), (1, 0, 47), (2, 2, 20)],
+}
+
+
+@pytest.mark.parametrize("parts", APPENDS.values(), ids=APPENDS.keys())
+@pytest.mark.parametrize("hd,kvh,heads", [(128, 2, 4), (64, 3, 3), (128, 1, 7)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_append_bit_exact(qtts, parts, hd, kvh, heads, dtype):
+    rng = np.random.default_rng(hd + kvh + len(parts))
+    p = Pool(qtts, rng, 3, 3, kvh, hd, layers=3, layer=1)
+    seq, pos = rows_of(parts)
+    n = len(seq)
+    # strided rows of a fused projection; values on both sides of the blocks' scales
+    qkv = dev((rng.standard_normal((n, (heads + 2 * kvh) * hd + 8)) * 2).astype(np.float32), dtype)
+    q, k, v = (qkv[:, a * hd:b * hd] for a, b in ((0, heads), (heads, heads + kvh), (heads + kvh, heads + 2 * kvh)))
+    cos, sin = tables(48, hd)
+    gq, gk = (1 + 0.1 * rng.standard_normal((2, hd))).astype(np.float16)
+    out = torch.full((n, heads * hd), 9.0, dtype=TYPES[dtype], device="cuda")
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+    dc, ds, dgq, dgk, dseq, dpos = dev(cos), dev(sin), dev(gq), dev(gk), dev(seq), dev(pos)
+    ld = qkv.stride(0)
+    qtts.kv8_append_dev(p.cache, k.data_ptr(), v.data_ptr(), dseq.data_ptr(), dpos.data_ptr(), n, dtype=dtype,
+                        q_ptr=q.data_ptr(), q_out_ptr=out.data_ptr(), heads=heads, q_norm_ptr=dgq.data_ptr(),
+                        k_norm_ptr=dgk.data_ptr(), cos_ptr=dc.data_ptr(), sin_ptr=ds.data_ptr(), rope_rows=48,
+                        ldk=ld, ldv=ld, ldq=ld, flags_ptr=flags.data_ptr())
+    torch.cuda.synchronize()
+    R.append(p.codes, p.scales, p.table, host(k), host(v), seq, pos, gk, cos, sin)
+    codes, scales = p.got()
+    assert np.array_equal(scales, p.scales)
+    assert np.array_equal(codes, p.codes)
+    assert p.others_untouched() and flags.item() == 0
+    want = np.full((n, heads * hd), 9.0, np.float32)
+    for r in range(n):
+        if seq[r] >= 0:
+            want[r] = R.norm_rotate(host(q[r]).reshape(heads, hd), gq, cos[pos[r]], sin[pos[r]]).reshape(-1)
+    assert torch.equal(out, dev(want, dtype))
+
+
+def run_append(qtts, p, k, v, seq, pos, **kw):
+    t = [dev(x) for x in (k, v, seq.astype(np.int32), pos.astype(np.int32))]
+    qtts.kv8_append_dev(p.cache, *(x.data_ptr() for x in t), len(seq), **kw)
+    torch.cuda.synchronize()
+
+
+def test_append_token_by_token_and_special_values(qtts):
+    # 40 single-token appends (fresh pages, blocks that grow and blocks that
+    # do not), with zeros, NaN, infinities, subnormals and huge values among them
+    rng = np.random.default_rng(1)
+    p = Pool(qtts, rng, 1, 3, 2, 64)
+    k, v = rng.standard_normal((2, 40, 128)).astype(np.float32)
+    k *= 1.1 ** (np.arange(40) % 16)[:, None]
+    v[0:3] = 0.0
+    k[5, :3] = [np.nan, np.inf, -np.inf]
+    v[16] = np.nan
+    v[17] = 1e-42
+    v[33, 7] = 3e38
+    k[32], v[32] = -0.0, np.inf
+    for t in range(40):
+        a = slice(t, t + 1)
+        run_append(qtts, p, k[a], v[a], np.zeros(1, int), np.array([t]))
+        R.append(p.codes, p.scales, p.table, k[a], v[a], [0], [t])
+    codes, scales = p.got()
+    assert np.array_equal(scales, p.scales) and np.array_equal(codes, p.codes)
+    assert np.all(np.isfinite(scales)) and codes.min() >= -127
+
+
+def test_append_without_norm_rotation_or_queries_and_rope_positions(qtts):
+    rng = np.random.default_rng(2)
+    for kw in ("bare", "rope_pos"):
+        p = Pool(qtts, rng, 2, 2, 1, 128)
+        seq, pos = rows_of([(1, 3, 20), (0, 30, 2)])
+        k, v = rng.standard_normal((2, 22, 128)).astype(np.float32)
+        if kw == "bare":
+            run_append(qtts, p, k, v, seq, pos)
+            R.append(p.codes, p.scales, p.table, k, v, seq, pos)
+        else:  # angles of other positions; one of them outside the tables: unrotated, flagged
+            cos, sin = tables(64, 128)
+            rp = (pos + 17).astype(np.int32)
+            rp[3] = 64
+            dc, ds, drp = dev(cos), dev(sin), dev(rp)
+            flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+            run_append(qtts, p, k, v, seq, pos, cos_ptr=dc.data_ptr(), sin_ptr=ds.data_ptr(), rope_rows=64,
+                       rope_pos_ptr=drp.data_ptr(), flags_ptr=flags.data_ptr())
+            R.append(p.codes, p.scales, p.table, k, v, seq, pos, None, cos, sin, rp)
+            assert flags.item() == qtts.KV8_ROPE_RANGE
+        codes, scales = p.got()
+        assert np.array_equal(scales, p.scales) and np.array_equal(codes, p.codes)
+
+
+def test_append_many_rows(qtts):
+    # enough rows that a warp looks through chunks of them: single tokens of
+    # 700 sequences, then a long prompt
+    rng = np.random.default_rng(3)
+    p = Pool(qtts, rng, 700, 2, 8, 64)
+    seq, pos = np.arange(700), rng.integers(0, 32, 700)
+    k, v = rng.standard_normal((2, 700, 512)).astype(np.float32)
+    run_append(qtts, p, k, v, seq, pos)
+    R.append(p.codes, p.scales, p.table, k, v, seq, pos)
+    codes, scales = p.got()
+    assert np.array_equal(scales, p.scales) and np.array_equal(codes, p.codes)
+    p = Pool(qtts, rng, 3, 200, 8, 64)
+    seq, pos = rows_of([(0, 7, 2903), (1, 0, 1), (2, 100, 1501)])
+    k, v = rng.standard_normal((2, len(seq), 512)).astype(np.float32)
+    run_append(qtts, p, k, v, seq, pos)
+    R.append(p.codes, p.scales, p.table, k, v, seq, pos)
+    codes, scales = p.got()
+    assert np.array_equal(scales, p.scales) and np.array_equal(codes, p.codes)
+
+
+def test_rows_and_pages_out_of_range_are_skipped_and_flagged(qtts):
+    rng = np.random.default_rng(4)
+    for what, bit in (("row", qtts.KV8_BAD_ROW), ("position", qtts.KV8_BAD_ROW), ("page", qtts.KV8_BAD_PAGE),
+                      ("negative page", qtts.KV8_BAD_PAGE)):
+        p = Pool(qtts, rng, 2, 2, 1, 64)
+        seq, pos = rows_of([(0, 14, 4), (1, 3, 1)])
+        if what == "row":
+            seq[4] = 2
+        elif what == "position":
+            pos[4] = 32
+        else:
+            p.table[0, 1] = -1 if what == "negative page" else 2 ** 30
+            p.d_table.copy_(dev(p.table))
+        k, v = rng.standard_normal((2, 5, 64)).astype(np.float32)
+        flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+        run_append(qtts, p, k, v, seq, pos, flags_ptr=flags.data_ptr())
+        R.append(p.codes, p.scales, p.table, k, v, seq, pos)
+        codes, scales = p.got()
+        assert np.array_equal(scales, p.scales) and np.array_equal(codes, p.codes)
+        assert flags.item() == bit, what
+        flags.zero_()
+        check_attention(qtts, p, rng, seq, pos, 2, "f32", flags=flags, skip_bad=True)
+        assert flags.item() == bit, what
+
+
+# ---- attention -------------------------------------------------------------------
+
+
+def check_attention(qtts, p, rng, seq, pos, heads, dtype, window=0, scale=None, max_rows=0, max_len=0, flags=None,
+                    q=None, ldx=0, skip_bad=False, stream=None):
+    n, cols = len(seq), heads * p.hd
+    scale = p.hd ** -0.5 if scale is None else scale
+    big = dev((rng.standard_normal((n, cols + ldx)) if q is None else q).astype(np.float32), dtype)
+    out = torch.full((n, cols + ldx), 5.0, dtype=TYPES[dtype], device="cuda")
+    lse = torch.full((n, heads), 5.0, device="cuda")
+    dseq, dpos = dev(seq.astype(np.int32)), dev(pos.astype(np.int32))
+    torch.cuda.synchronize()
+    qtts.kv8_attention_dev(p.cache, big.data_ptr(), out.data_ptr(), dseq.data_ptr(), dpos.data_ptr(), n, heads,
+                           dtype=dtype, scale=scale, window=window, max_rows=max_rows, max_len=max_len,
+                           lse_ptr=lse.data_ptr(), ldq=cols + ldx, ldo=cols + ldx,
+                           flags_ptr=flags.data_ptr() if flags is not None else 0, stream=stream or 0)
+    torch.cuda.synchronize()
+    want, wlse = np.full((n, cols), 5.0), np.full((n, heads), 5.0)
+    most, vmax = R.attention(p.codes, p.scales, p.table, host(big)[:, :cols], heads, seq, pos, scale, window, want, wlse)
+    assert bool((out[:, cols:] == 5.0).all())
+    # Sums of products in f32, 2^-23 of the absolute sum per 16-term step: a
+    # score is off by d <= most * (hd/16 steps + 8 for the split, the scaling
+    # and the exponent) * 2^-23; weights by twice that and 2^-20 for exp2 and
+    # the f16 pair; the weighted sum by 2^-23 a step of 16 positions, joins
+    # included; and the result is rounded once to its type.
+    length = max(1, int(pos.max()) + 1)
+    d = most * (p.hd / 16 + 8) * 2.0 ** -23
+    tol = vmax * (2 * d + 2.0 ** -20 + (length / 16 + 32) * 2.0 ** -23) + HALF_STEP[dtype] * np.abs(want)
+    got, glse = host(out[:, :cols]).astype(np.float64), host(lse).astype(np.float64)
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) - tol)
+    assert np.array_equal(np.isinf(glse), np.isinf(wlse))
+    fin = ~np.isinf(wlse)
+    assert np.all(np.abs(glse - np.where(fin, wlse, 0))[fin] <= d + 2.0 ** -20 + 2.0 ** -22 * np.abs(wlse[fin]))
+    return out, lse
+
+
+LENGTHS = np.array([-1, 0, 1, 7, 8, 14, 15, 16, 17, 31, 32, 47, 63, 64, 65, 100, 150, 159])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,heads,kvh", [(128, 4, 2), (128, 16, 1), (64, 3, 3), (64, 12, 1), (128, 10, 2), (64, 8, 1)])
+def test_single_tokens(qtts, hd, heads, kvh, dtype):
+    rng = np.random.default_rng(hd * heads + kvh)
+    n = len(LENGTHS)
+    p = Pool(qtts, rng, n, 10, kvh, hd, layers=2, layer=1)
+    check_attention(qtts, p, rng, np.arange(n), LENGTHS, heads, dtype, ldx=8)
+
+
+@pytest.mark.parametrize("window", [1, 5, 16, 72])
+@pytest.mark.parametrize("hd,heads,kvh", [(64, 4, 4), (128, 4, 2)])
+def test_windows(qtts, window, hd, heads, kvh):
+    rng = np.random.default_rng(window)
+    p = Pool(qtts, rng, 3, 10, kvh, hd)
+    seq, pos = rows_of([(1, 0, 150), (-1, 0, 3), (0, 90, 2), (2, 8, 70)])
+    check_attention(qtts, p, rng, seq, pos, heads, "f32", window=window, max_rows=150)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 2, 128), (8, 1, 64), (16, 1, 128), (3, 3, 64)])
+@pytest.mark.parametrize("max_rows", [1, 3, 200])
+def test_chunks_of_rows(qtts, heads, kvh, hd, dtype, max_rows):
+    # causal rows of several sequences, padding among and behind them, whatever the hint says
+    rng = np.random.default_rng(heads * hd + max_rows)
+    p = Pool(qtts, rng, 5, 12, kvh, hd)
+    seq, pos = rows_of([(3, 0, 33), (-1, 4, 2), (0, 100, 5), (1, 191, 1), (2, -3, 9), (4, 0, 130), (-1, 0, 7)])
+    check_attention(qtts, p, rng, seq, pos, heads, dtype, max_rows=max_rows)
+
+
+def test_rows_in_any_order(qtts):
+    # attention, unlike the append, does not ask for an order: the same row
+    # twice, positions going down, sequences alternating
+    rng = np.random.default_rng(11)
+    p = Pool(qtts, rng, 2, 10, 2, 128)
+    seq = np.array([0, 0, 1, 0, 1, 1, 1, 1, 0, 0] * 9)
+    pos = rng.integers(-1, 160, 90)
+    pos[1] = pos[0]
+    for max_rows in (1, 4, 64):
+        check_attention(qtts, p, rng, seq, pos, 4, "f32", max_rows=max_rows)
+
+
+def test_padding_rows_are_left_alone(qtts):
+    rng = np.random.default_rng(12)
+    p = Pool(qtts, rng, 1, 2, 1, 64)
+    seq = np.array([-1] * 20)
+    for max_rows in (1, 20):
+        out, lse = check_attention(qtts, p, rng, seq, np.zeros(20, int), 2, "f32", max_rows=max_rows)
+        assert bool((out == 5.0).all()) and bool((lse == 5.0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_scales_far_apart(qtts, rows):
+    # blocks whose scales differ by many powers of two, zero blocks, and NaN in
+    # the scales of pages that no row sees
+    rng = np.random.default_rng(13)
+    p = Pool(qtts, rng, 2, 9, 1, 128)
+    p.scales[:, 1] *= (10.0 ** rng.integers(-9, 10, p.scales[:, 1].shape)).astype(np.float32)
+    p.scales[p.table[0, 2], 1] = 0.0
+    p.scales[p.table[0, 3], 0] = 0.0
+    p.scales[p.table[1, :6], 1] = 0.0
+    p.scales[p.table[:, 8]] = np.nan
+    p.d_scales[:, 0] = dev(p.scales)
+    seq, pos = rows_of([(0, 127 - rows + 1, rows), (1, 95 - rows + 1, rows)])
+    check_attention(qtts, p, rng, seq, pos, 2, "f32", max_rows=rows)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("size", [1e-20, 1e-3, 30.0])
+def test_queries_of_any_size(qtts, size, rows):
+    rng = np.random.default_rng(14)
+    p = Pool(qtts, rng, 1, 4, 1, 64)
+    seq, pos = rows_of([(0, 60 - rows, rows)])
+    q = rng.standard_normal((rows, 128)) * size
+    q[0, 5] *= 1000
+    check_attention(qtts, p, rng, seq, pos, 2, "f32", q=q, scale=0.01, max_rows=rows)
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_not_a_number_stays_in_its_row(qtts, rows):
+    rng = np.random.default_rng(15)
+    p = Pool(qtts, rng, 1, 4, 1, 64)
+    seq, pos = rows_of([(0, 60 - rows, rows)])
+    q = torch.randn(rows, 128, device="cuda")
+    q[0, 3] = float("nan")
+    q[1, 70] = float("inf")
+    out = torch.zeros_like(q)
+    t = dev(seq), dev(pos)
+    qtts.kv8_attention_dev(p.cache, q.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), rows, 2,
+                           max_rows=rows)
+    torch.cuda.synchronize()
+    assert bool(out[0, :64].isnan().all()) and not bool(out[0, 64:].isnan().any())
+    assert bool(out[1, 64:].isnan().all()) and not bool(out[1, :64].isnan().any())
+    assert not bool(out[2:].isnan().any())
+
+
+@pytest.mark.parametrize("length,rows", [(3000, 1), (9999, 1), (9999, 3), (2500, 100)])
+def test_long_caches(qtts, length, rows):
+    rng = np.random.default_rng(length)
+    p = Pool(qtts, rng, 2, (length + 15) // 16, 1, 128)
+    seq, pos = rows_of([(1, length - rows, rows)])
+    check_attention(qtts, p, rng, seq, pos, 2, "f32", max_rows=rows)
+
+
+def test_offsets_past_32_bits(qtts):
+    # pages 400 MB apart: the last one lies past 4 GB of codes
+    rng = np.random.default_rng(16)
+    kvh, hd, n = 1, 64, 12
+    blk, stride = 2 * kvh * 16 * hd, 400_000_000
+    codes = torch.zeros(stride * (n - 1) + blk, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(n, 2, kvh, device="cuda")
+    table = np.arange(n)[::-1].reshape(1, n).astype(np.int32).copy()
+    d_table = dev(table)
+    cache = qtts.Kv8Cache(codes.data_ptr(), scales.data_ptr(), d_table.data_ptr(), n, 1, n, kvh, hd, page_stride=stride)
+    seq, pos = rows_of([(0, 0, 190)])
+    k, v = rng.standard_normal((2, 190, hd)).astype(np.float32)
+    t = [dev(x) for x in (k, v, seq, pos)]
+    qtts.kv8_append_dev(cache, *(x.data_ptr() for x in t), 190)
+    small, s_scales = np.zeros((n, 2, kvh, 16, hd), np.int8), np.zeros((n, 2, kvh), np.float32)
+    R.append(small, s_scales, table, k, v, seq, pos)
+    got = torch.stack([codes[i * stride:i * stride + blk] for i in range(n)]).cpu().numpy().reshape(small.shape)
+    assert np.array_equal(got, small) and np.array_equal(host(scales), s_scales)
+
+    class P:
+        pass
+
+    p = P()
+    p.codes, p.scales, p.table, p.hd, p.cache = small, s_scales, table, hd, cache
+    for max_rows in (1, 190):
+        check_attention(qtts, p, rng, seq, pos, 1, "f32", max_rows=max_rows)
+
+
+def test_results_do_not_change_from_run_to_run(qtts):
+    rng = np.random.default_rng(17)
+    p = Pool(qtts, rng, 3, 40, 2, 128)
+    for parts, max_rows in (([(0, 600, 1), (1, 639, 1)], 1), ([(2, 300, 200)], 200)):
+        seq, pos = rows_of(parts)
+        q = rng.standard_normal((len(seq), 512))
+        a, la = check_attention(qtts, p, rng, seq, pos, 4, "f32", q=q, max_rows=max_rows)
+        b, lb = check_attention(qtts, p, rng, seq, pos, 4, "f32", q=q, max_rows=max_rows)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def test_host_buffers_are_refused(qtts):
+    t = torch.zeros(1 << 16, dtype=torch.uint8)
+    c = qtts.Kv8Cache(t.data_ptr() // 16 * 16 + 16, t.data_ptr(), t.data_ptr(), 1, 1, 1, 1, 64)
+    x = torch.zeros(64, device="cuda")
+    for f in (lambda: qtts.kv8_append_dev(c, x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr(), 1),
+              lambda: qtts.kv8_attention_dev(c, x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr(), 1, 1)):
+        with pytest.raises(qtts.QttsError) as e:
+            f()
+        assert e.value.code == qtts.ERR_BADARG
+    torch.cuda.synchronize()
+
+
+# ---- a decode run ------------------------------------------------------------------
+
+
+def test_decode_steps_in_a_graph_on_another_stream(qtts):
+    """Prefill, then single-token steps of append, attention, a Q4 head and
+    sampling captured once and replayed, every step against the restatements."""
+    rng = np.random.default_rng(18)
+    kvh, heads, hd, V, steps = 2, 4, 64, 96, 21
+    p = Pool(qtts, rng, 3, 4, kvh, hd)
+    cos, sin = tables(64, hd)
+    gq, gk = (1 + 0.1 * rng.standard_normal((2, hd))).astype(np.float16)
+    packed = rng.integers(0, 256, heads * hd * V // 2, dtype=np.uint8)
+    qs = np.abs(rng.standard_normal(heads * hd * V // 32) * 0.2).astype(np.float16)
+    d = {n: dev(x) for n, x in dict(cos=cos, sin=sin, gq=gq, gk=gk, packed=packed, qs=qs).items()}
+    cols = (heads + 2 * kvh) * hd
+
+    def append(stream, qkv, out, seq, pos, n):
+        b = qkv.data_ptr()
+        qtts.kv8_append_dev(p.cache, b + heads * hd * 4, b + (heads + kvh) * hd * 4, seq.data_ptr(), pos.data_ptr(), n,
+                            q_ptr=b, q_out_ptr=out.data_ptr(), heads=heads, q_norm_ptr=d["gq"].data_ptr(),
+                            k_norm_ptr=d["gk"].data_ptr(), cos_ptr=d["cos"].data_ptr(), sin_ptr=d["sin"].data_ptr(),
+                            rope_rows=64, ldk=cols, ldv=cols, ldq=cols, stream=stream)
+
+    def reference(x, seq, pos, q64):
+        q, k, v = x[:, :heads * hd], x[:, heads * hd:(heads + kvh) * hd], x[:, (heads + kvh) * hd:]
+        R.append(p.codes, p.scales, p.table, k, v, seq, pos, gk, cos, sin)
+        for r in range(len(seq)):
+            q64[r] = R.norm_rotate(q[r].reshape(heads, hd), gq, cos[pos[r]], sin[pos[r]]).reshape(-1)
+
+    # prefill of three prompts of unlike length
+    parts = [(0, 0, 30), (1, 0, 1), (2, 0, 17)]
+    seq, pos = rows_of(parts)
+    x = rng.standard_normal((len(seq), cols)).astype(np.float32)
+    dx, dq, dseq, dpos = dev(x), torch.zeros(len(seq), heads * hd, device="cuda"), dev(seq), dev(pos)
+    append(0, dx, dq, dseq, dpos, len(seq))
+    reference(x, seq, pos, np.zeros((len(seq), heads * hd)))
+
+    st = torch.cuda.Stream()
+    n = 3
+    qkv, q, att = (torch.zeros(n, c, device="cuda") for c in (cols, heads * hd, heads * hd))
+    logits, u = torch.zeros(n, V, device="cuda"), torch.zeros(n, device="cuda")
+    token, seq1, pos1 = torch.zeros(n, dtype=torch.int32, device="cuda"), dev(np.arange(3, dtype=np.int32)), torch.zeros(
+        n, dtype=torch.int32, device="cuda")
+    sb = qtts.q4_gemv_scratch_bytes(heads * hd, V, n)
+    scratch = torch.zeros(sb, dtype=torch.uint8, device="cuda")
+    tk, tp = torch.full((n,), 40, dtype=torch.int32, device="cuda"), torch.full((n,), 0.9, device="cuda")
+
+    def step():
+        s = st.cuda_stream
+        append(s, qkv, q, seq1, pos1, n)
+        qtts.kv8_attention_dev(p.cache, q.data_ptr(), att.data_ptr(), seq1.data_ptr(), pos1.data_ptr(), n, heads,
+                               max_len=64, stream=s)
+        qtts.q4_gemv_dev(d["packed"].data_ptr(), d["qs"].data_ptr(), heads * hd, V, att.data_ptr(), n,
+                         logits.data_ptr(), scratch.data_ptr(), sb, s)
+        qtts.sample_rows_dev(logits.data_ptr(), n, V, u.data_ptr(), token.data_ptr(), top_k_ptr=tk.data_ptr(),
+                             top_p_ptr=tp.data_ptr(), stream=s)
+
+    # once outside a capture, over positions that the first replay writes again
+    pos1.copy_(dev(np.array([30, 1, 17], np.int32)))
+    torch.cuda.synchronize()
+    saved = p.d_codes.clone(), p.d_scales.clone()
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.synchronize()
+    p.d_codes.copy_(saved[0])
+    p.d_scales.copy_(saved[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        step()
+    for i in range(steps):
+        x = rng.standard_normal((n, cols)).astype(np.float32)
+        at = np.array([30 + i, 1 + i, 17 + i], np.int32)
+        uu = rng.random(n).astype(np.float32)
+        qkv.copy_(dev(x))
+        pos1.copy_(dev(at))
+        u.copy_(dev(uu))
+        graph.replay()
+        torch.cuda.synchronize()
+        q64, want, wl = np.zeros((n, heads * hd), np.float32), np.zeros((n, heads * hd)), np.zeros((n, heads))
+        reference(x, np.arange(3), at, q64)
+        codes, scales = p.got()
+        assert np.array_equal(scales, p.scales) and np.array_equal(codes, p.codes), i
+        assert np.array_equal(host(q), q64)
+        R.attention(p.codes, p.scales, p.table, q64, heads, np.arange(3), at, hd ** -0.5, 0, want, wl)
+        # scores of at most ~30 in units of 2^-23 steps (see check_attention) and |v| < 6
+        assert np.max(np.abs(host(att) - want)) <= 6 * (60 * 16 * 2.0 ** -23 + 2.0 ** -19)
+        lg = host(logits)
+        for r in range(n):
+            tok, _, _, margin = R.sample(lg[r], 1.0, 40, 0.9, 0.0, uu[r])
+            assert int(token[r]) == tok or margin < 1e-9
