@@ -303,18 +303,48 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
 constexpr int kSlots = 8;
 constexpr int kAttnWarps = 4;
 
-// One sequence's rows of a unit: what its slots see.
-struct Segment {
-  int row0, rows;  // rows [row0, row0 + rows)
-  int seq;
-  int lo, hi;      // positions [lo, hi) that any of them sees
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared memory of the single-token kernel.  Each warp has a ring of kStages
+// pages; a page's K and V block is copied 16 bytes a lane, and the 16-byte
+// chunks of a row change places so that the fragment reads below (8 lanes of
+// 16 bytes at a time: K two rows x four chunks, V four rows x two chunks) hit
+// every bank once.
+constexpr int kStages = 4;
+template <int HD>
+struct Ring {
+  static constexpr int kBlock = kKv8Page * HD;  // bytes of one K or V block
+  static constexpr int kPer = kBlock / 512;     // copies of a lane per block
+  static constexpr int kWarp = kStages * 2 * kBlock;
+  static __device__ __forceinline__ int k_at(int row, int byte) {
+    return HD == 128 ? row * 128 + (byte ^ ((row & 1) << 6)) : row * 64 + byte;
+  }
+  static __device__ __forceinline__ int v_at(int row, int byte) {
+    if (HD == 128) return row * 128 + (byte ^ ((row & 6) << 4));
+    const int line = row >> 1;
+    return line * 128 + ((((row & 1) << 6) | byte) ^ ((line & 3) << 5));
+  }
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_constant__ Kv8AttnDesc d) {
+__global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __grid_constant__ Kv8AttnDesc d) {
   constexpr int NT = HD / 8;   // dims a thread's V chunk holds, and n-tiles of the output
   constexpr int KJ = HD / 64;  // 64-dim halves of a row
-  __shared__ float s_o[kAttnWarps][kSlots][HD];
+  using R = Ring<HD>;
+  extern __shared__ __align__(128) uint8_t ring[];
+  float(*s_o)[kSlots][HD] = reinterpret_cast<float(*)[kSlots][HD]>(ring);  // after the pages: each warp's sums
+  static_assert(R::kWarp >= kSlots * HD * 4, "the warps' sums lie over the ring");
+  __shared__ float s_scale[kAttnWarps][kStages][2];
   __shared__ float s_m[kAttnWarps][kSlots], s_l[kAttnWarps][kSlots];
   __shared__ float s_po[kSlots][HD];
   __shared__ float s_pm[kSlots], s_pl[kSlots];
@@ -327,36 +357,82 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
   const int unit = blockIdx.x / per, rest = blockIdx.x % per;
   const int kvh = rest / d.head_chunks, hc = rest % d.head_chunks;
   const int group = d.heads / c.kv_heads;
-  const int h0 = kvh * group + hc * d.unit_heads;                        // first query head of the unit
-  const int nh = min(d.unit_heads, group - hc * d.unit_heads);           // its heads
-  const int row_end = min(d.n_rows, (unit + 1) * d.group_rows);
+  const int h0 = kvh * group + hc * d.unit_heads;               // first query head of the unit
+  const int nh = min(d.unit_heads, group - hc * d.unit_heads);  // its heads
   const int cap = c.pages_per_seq * kKv8Page;
   cg::cluster_group cluster = cg::this_cluster();
+  uint8_t* my_ring = ring + warp * R::kWarp;
+  const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(my_ring);
+  const uint32_t scale_s = (uint32_t)__cvta_generic_to_shared(&s_scale[warp][0][0]);
 
-  for (int row = unit * d.group_rows; row < row_end;) {
-    // the next run of rows of one sequence
-    Segment sg;
-    sg.row0 = row;
-    sg.seq = d.seq[row];
-    sg.lo = 0x7fffffff;
-    sg.hi = 0;
-    for (; row < row_end && d.seq[row] == sg.seq; ++row) {
-      int p = d.pos[row];
-      if (p >= cap) {
-        if (tid == 0 && sg.seq >= 0) raise(d.flags, QTTS_KV8_BAD_ROW);
-        p = cap - 1;
+  // lane i: row i of the unit
+  const int unit_row0 = unit * d.group_rows, unit_rows = min(d.group_rows, d.n_rows - unit_row0);
+  int rseq = -1, rpos = -1;
+  if (lane < unit_rows) {
+    rseq = d.seq[unit_row0 + lane];
+    rpos = d.pos[unit_row0 + lane];
+    if (rseq >= 0 && (rseq >= c.n_seqs || rpos >= cap)) {
+      if (warp == 0) raise(d.flags, QTTS_KV8_BAD_ROW);
+      if (rseq >= c.n_seqs) rseq = -1;
+      rpos = min(rpos, cap - 1);
+    }
+  }
+  for (int i0 = 0; i0 < unit_rows;) {
+    // the next run of rows of one sequence: rows [i0, i0 + rows) of the unit
+    const int seq = __shfl_sync(kFull, rseq, i0);
+    const unsigned other = __ballot_sync(kFull, rseq != seq || lane >= unit_rows) & (kFull << i0);
+    const int rows = (other ? __ffs(other) - 1 : 32) - i0;
+    const bool mine = lane >= i0 && lane < i0 + rows && rpos >= 0;
+    const int hi = __reduce_max_sync(kFull, mine ? rpos + 1 : 0);
+    const int lo = __reduce_min_sync(kFull, mine ? (d.window > 0 ? max(0, rpos + 1 - d.window) : 0) : 0x7fffffff);
+    const int row0 = unit_row0 + i0;
+    const int slot_row = i0 + min(g / nh, rows - 1);
+    const int slot_pos = __shfl_sync(kFull, rpos, slot_row);
+    i0 += rows;
+    if (seq < 0) continue;  // padding
+    const int nslots = rows * nh;
+    const bool on = g < nslots;
+
+    // this split's pages [pb, pe); the warp takes every kAttnWarps-th of them
+    const int p0 = hi > 0 ? lo / kKv8Page : 0, p1 = (hi + kKv8Page - 1) / kKv8Page;
+    const int share = (p1 - p0 + nsplit - 1) / nsplit;
+    const int pb = p0 + split * share + warp, pe = min(p1, p0 + (split + 1) * share);
+    const int np = pb < pe ? (pe - pb + kAttnWarps - 1) / kAttnWarps : 0;
+    const int* table = c.page_table + (size_t)seq * c.pages_per_seq;
+    int entries = -1;        // lane i: the page of the 32 * k + i-th of them
+    unsigned skip = 0;       // bit s: stage s holds no page
+    auto issue = [&](int i) {
+      if (i < np) {
+        if ((i & 31) == 0) {
+          const int pg = pb + (i + lane) * kAttnWarps;
+          entries = pg < pe ? table[pg] : -1;
+          if (pg < pe && (entries < 0 || entries >= c.n_pages)) {
+            raise(d.flags, QTTS_KV8_BAD_PAGE);
+            entries = -1;
+          }
+        }
+        const int page = __shfl_sync(kFull, entries, i & 31), s = i % kStages;
+        skip &= ~(1u << s);
+        if (page < 0) {
+          skip |= 1u << s;
+        } else {
+          const int8_t* kb = block_codes(c, page, 0, kvh) + lane * 16;
+          const int8_t* vb = block_codes(c, page, 1, kvh) + lane * 16;
+          const uint32_t dst = ring_s + s * 2 * R::kBlock;
+#pragma unroll
+          for (int j = 0; j < R::kPer; ++j) {
+            const int row = (lane * 16 + j * 512) / HD, byte = lane * 16 % HD;
+            cp_async16(dst + R::k_at(row, byte), kb + j * 512);
+            cp_async16(dst + R::kBlock + R::v_at(row, byte), vb + j * 512);
+          }
+          if (lane < 2) cp_async4(scale_s + (s * 2 + lane) * 4, block_scale(c, page, lane, kvh));
+        }
       }
-      if (p < 0) continue;
-      sg.hi = max(sg.hi, p + 1);
-      sg.lo = min(sg.lo, d.window > 0 ? max(0, p + 1 - d.window) : 0);
-    }
-    sg.rows = row - sg.row0;
-    if (sg.seq < 0) continue;  // padding
-    if (sg.seq >= c.n_seqs) {
-      if (tid == 0) raise(d.flags, QTTS_KV8_BAD_ROW);
-      continue;
-    }
-    const int nslots = sg.rows * nh;
+      cp_async_commit();  // one group a step, empty or not
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+
     // this thread's slot: query fragments, scale, and the positions it sees
     uint32_t qa[KJ * 4][4];
     float qscale = 0.0f;
@@ -364,8 +440,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
     {
       float4 x[KJ][4];
       float big = 0.0f;
-      const bool on = g < nslots;
-      const T* qp = static_cast<const T*>(d.q) + (size_t)(sg.row0 + (on ? g / nh : 0)) * d.ldq +
+      const T* qp = static_cast<const T*>(d.q) + (size_t)(unit_row0 + slot_row) * d.ldq +
                     (size_t)(h0 + (on ? g % nh : 0)) * HD;
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
@@ -388,7 +463,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
           split_f16(x[j][i].z * dn, x[j][i].w * dn, qa[j * 4 + i][2], qa[j * 4 + i][3]);
         }
       if (on) {
-        see_hi = min(d.pos[sg.row0 + g / nh], cap - 1) + 1;
+        see_hi = slot_pos + 1;
         see_lo = d.window > 0 ? max(0, see_hi - d.window) : 0;
       }
     }
@@ -399,62 +474,39 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
       for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
     float m = -INFINITY, mo = -INFINITY, l = 0.0f;
 
-    // this split's pages, this warp's among them
-    const int p0 = sg.hi > 0 ? sg.lo / kKv8Page : 0, p1 = (sg.hi + kKv8Page - 1) / kKv8Page;
-    const int share = (p1 - p0 + nsplit - 1) / nsplit;
-    const int pb = p0 + split * share, pe = min(p1, pb + share);
-    const int* table = c.page_table + (size_t)sg.seq * c.pages_per_seq;
-    for (int pg = pb + warp; pg < pe; pg += kAttnWarps) {
-      const int page = table[pg];
-      if (page < 0 || page >= c.n_pages) {
-        if (lane == 0) raise(d.flags, QTTS_KV8_BAD_PAGE);
-        continue;
-      }
-      const int8_t* kb = block_codes(c, page, 0, kvh);
-      const int8_t* vb = block_codes(c, page, 1, kvh);
-      const float sk = *block_scale(c, page, 0, kvh), sv = *block_scale(c, page, 1, kvh);
-      uint4 kw[2][KJ];
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int j = 0; j < KJ; ++j)
-          kw[n][j] = *reinterpret_cast<const uint4*>(kb + (n * 8 + g) * HD + 16 * (t + 4 * j));
-      uint32_t vw[4][NT / 4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, dims NT * g ...
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int8_t* src = vb + (2 * t + (e & 1) + (e >> 1) * 8) * HD + NT * g;
-        if (NT == 16) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src);
-          vw[e][0] = u.x;
-          vw[e][1] = u.y;
-          vw[e][NT / 4 - 2] = u.z;
-          vw[e][NT / 4 - 1] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src);
-          vw[e][0] = u.x;
-          vw[e][1] = u.y;
-        }
-      }
+    for (int i = 0; i < np; ++i) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();  // every lane's copies of page i are there, and its reads of page i - 1 done
+      const int st = i % kStages;
+      const bool skipped = (skip >> st) & 1;
+      issue(i + kStages - 1);
+      if (skipped) continue;
+      const uint8_t* kb = my_ring + st * 2 * R::kBlock;
+      const uint8_t* vb = kb + R::kBlock;
+      const float sk = s_scale[warp][st][0], sv = s_scale[warp][st][1];
+      const int at0 = (pb + i * kAttnWarps) * kKv8Page + 2 * t;
       // scores: positions 8n + 2t, + 1 of slot g in (acc[n][0] + 2^-11 acc[n][2], ...)
       float acc[2][4] = {};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int j = 0; j < KJ; ++j) {
+        uint4 kw[2];
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) {
-          const uint32_t w[4] = {kw[n][j].x, kw[n][j].y, kw[n][j].z, kw[n][j].w};
+        for (int n = 0; n < 2; ++n) kw[n] = *reinterpret_cast<const uint4*>(kb + R::k_at(n * 8 + g, 16 * (t + 4 * j)));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t u = w[i] ^ 0x80808080u;
-            mma16816(acc[n], qa[j * 4 + i], half2_of(u, 0x4140), half2_of(u, 0x4342));
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t u = (e == 0 ? kw[n].x : e == 1 ? kw[n].y : e == 2 ? kw[n].z : kw[n].w) ^ 0x80808080u;
+            mma16816(acc[n], qa[j * 4 + e], half2_of(u, 0x4140), half2_of(u, 0x4342));
           }
-        }
+      }
       float s[2][2], pm = -INFINITY;
       const float f = qscale * sk;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int at = pg * kKv8Page + n * 8 + 2 * t + e;
+          const int at = at0 + n * 8 + e;
           s[n][e] = at >= see_lo && at < see_hi ? (acc[n][e] + acc[n][e + 2] * (1.0f / kSplitLoScale)) * f : -INFINITY;
           pm = fmaxf(pm, s[n][e]);
         }
@@ -472,9 +524,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
       const float beta = mo == mon ? 1.0f : ex2(mo - mon);
       if (__any_sync(kFull, beta != 1.0f)) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int k = 0; k < NT; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][e] *= beta;
+          for (int e = 0; e < 4; ++e) o[k][e] *= beta;
       }
       m = mn;
       mo = mon;
@@ -485,6 +537,22 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
         const float a = ex2(s[n][0] - mz), b = ex2(s[n][1] - mz);
         l += a + b;
         split_f16(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
+      }
+      uint32_t vw[4][NT / 4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, dims NT * g ...
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint8_t* src = vb + R::v_at(2 * t + (e & 1) + (e >> 1) * 8, NT * g);
+        if (NT == 16) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src);
+          vw[e][0] = u.x;
+          vw[e][1] = u.y;
+          vw[e][NT / 4 - 2] = u.z;
+          vw[e][NT / 4 - 1] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          vw[e][0] = u.x;
+          vw[e][1] = u.y;
+        }
       }
 #pragma unroll
       for (int q = 0; q < NT / 4; ++q) {
@@ -504,56 +572,82 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const __grid_
     l += __shfl_xor_sync(kFull, l, 2);
     if (l != l) m = INFINITY;  // a NaN score: the joins below then give NaN
     const float back = m == -INFINITY || mo == -INFINITY ? 0.0f : ex2(mo - m);
+    cp_async_wait<0>();
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
+    if (on) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        s_o[warp][g][NT * (2 * t + e) + i] = (o[i][e] + o[i][e + 2] * (1.0f / kSplitLoScale)) * back;
-    if (t == 0) {
-      s_m[warp][g] = m;
-      s_l[warp][g] = l;
+#pragma unroll
+        for (int k = 0; k < NT; k += 4) {
+          float4 v;
+          v.x = (o[k][e] + o[k][e + 2] * (1.0f / kSplitLoScale)) * back;
+          v.y = (o[k + 1][e] + o[k + 1][e + 2] * (1.0f / kSplitLoScale)) * back;
+          v.z = (o[k + 2][e] + o[k + 2][e + 2] * (1.0f / kSplitLoScale)) * back;
+          v.w = (o[k + 3][e] + o[k + 3][e + 2] * (1.0f / kSplitLoScale)) * back;
+          *reinterpret_cast<float4*>(&s_o[warp][g][NT * (2 * t + e) + k]) = v;
+        }
+      if (t == 0) {
+        s_m[warp][g] = m;
+        s_l[warp][g] = l;
+      }
     }
     __syncthreads();
+    auto write = [&](int s, int e, float mx, float ll, float sum) {
+      const size_t orow = row0 + s / nh;
+      const int head = h0 + s % nh;
+      const float v = mx == -INFINITY ? 0.0f : __fdiv_rn(sum, ll);
+      T* op = static_cast<T*>(d.out) + orow * d.ldo + (size_t)head * HD + e;
+      if constexpr (sizeof(T) == 4) *op = v;
+      else *op = T(v);
+      if (e == 0 && d.lse)
+        d.lse[orow * d.heads + head] = mx == -INFINITY ? -INFINITY : (mx + log2f(ll)) * 0.6931471805599453f;
+    };
     for (int i = tid; i < nslots * HD; i += kAttnWarps * 32) {
       const int s = i / HD, e = i % HD;
       float mx = s_m[0][s];
+#pragma unroll
       for (int w = 1; w < kAttnWarps; ++w) mx = fmaxf(mx, s_m[w][s]);
       float sum = 0.0f, ll = 0.0f;
-      if (mx > -INFINITY)
+      if (mx > -INFINITY) {
+#pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) {
           const float k = ex2(s_m[w][s] - mx);
           sum += s_o[w][s][e] * k;
           ll += s_l[w][s] * k;
         }
-      s_po[s][e] = sum;
-      if (e == 0) {
-        s_pm[s] = mx;
-        s_pl[s] = ll;
+      }
+      if (nsplit == 1) {
+        write(s, e, mx, ll, sum);
+      } else {
+        s_po[s][e] = sum;
+        if (e == 0) {
+          s_pm[s] = mx;
+          s_pl[s] = ll;
+        }
       }
     }
-    if (nsplit > 1) cluster.sync();
-    else __syncthreads();
+    if (nsplit == 1) {
+      __syncthreads();
+      continue;
+    }
+    cluster.sync();
     for (int i = tid + split * kAttnWarps * 32; i < nslots * HD; i += nsplit * kAttnWarps * 32) {
       const int s = i / HD, e = i % HD;
       float mx = -INFINITY, sum = 0.0f, ll = 0.0f;
-      for (int r = 0; r < nsplit; ++r) mx = fmaxf(mx, nsplit > 1 ? *cluster.map_shared_rank(&s_pm[s], r) : s_pm[s]);
       for (int r = 0; r < nsplit; ++r) {
-        const float rm = nsplit > 1 ? *cluster.map_shared_rank(&s_pm[s], r) : s_pm[s];
-        const float k = rm == -INFINITY ? 0.0f : ex2(rm - mx);
-        sum += (nsplit > 1 ? *cluster.map_shared_rank(&s_po[s][e], r) : s_po[s][e]) * k;
-        ll += (nsplit > 1 ? *cluster.map_shared_rank(&s_pl[s], r) : s_pl[s]) * k;
+        // one pass: the sums so far are scaled down when a larger maximum comes
+        const float rm = *cluster.map_shared_rank(&s_pm[s], r), ro = *cluster.map_shared_rank(&s_po[s][e], r),
+                    rl = *cluster.map_shared_rank(&s_pl[s], r);
+        const float mn = fmaxf(mx, rm);
+        if (mn == -INFINITY) continue;
+        const float a = ex2(mx - mn), b = ex2(rm - mn);
+        sum = sum * a + ro * b;
+        ll = ll * a + rl * b;
+        mx = mn;
       }
-      const int orow = sg.row0 + s / nh, head = h0 + s % nh;
-      const float v = mx == -INFINITY ? 0.0f : __fdiv_rn(sum, ll);
-      T* op = static_cast<T*>(d.out) + (size_t)orow * d.ldo + (size_t)head * HD + e;
-      if constexpr (sizeof(T) == 4) *op = v;
-      else *op = T(v);
-      if (e == 0 && d.lse)
-        d.lse[(size_t)orow * d.heads + head] = mx == -INFINITY ? -INFINITY : (mx + log2f(ll)) * 0.6931471805599453f;
+      write(s, e, mx, ll, sum);
     }
-    if (nsplit > 1) cluster.sync();
-    else __syncthreads();
+    cluster.sync();  // no CTA goes on while its sums are read
   }
 }
 
@@ -562,10 +656,22 @@ cudaError_t launch_append_t(const Kv8AppendDesc& d, cudaStream_t st) {
   return launch_k(kv8_append_kernel<T, HD>, dim3((unsigned)((d.n_warps + 3) / 4)), dim3(128), 0, st,
                   LaunchOpts{true, 1}, d);
 }
+// Splits of a unit's pages: doubled while the CTAs do not fill the device
+// (three an SM) and every warp keeps two pages.  Clusters of 16 need an opt-in.
 template <typename T, int HD>
-cudaError_t launch_attn_t(const Kv8AttnDesc& d, unsigned units, unsigned nsplit, cudaStream_t st) {
-  return launch_k(kv8_attn_kernel<T, HD>, dim3(units, nsplit), dim3(kAttnWarps * 32), 0, st, LaunchOpts{true, nsplit},
-                  d);
+cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, cudaStream_t st) {
+  constexpr int smem = kAttnWarps * Ring<HD>::kWarp;
+  static std::atomic<int> ready[kMaxDevices];
+  const cudaError_t set = once_per_device(ready, [] {
+    const cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(kv8_attn_kernel<T, HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  if (set != cudaSuccess) return set;
+  unsigned ns = 1;
+  while (ns < 16 && units * ns * 2 <= 3l * sms && pages >= (int)ns * 2 * kAttnWarps) ns *= 2;
+  return launch_k(kv8_attn_kernel<T, HD>, dim3((unsigned)units, ns), dim3(kAttnWarps * 32), smem, st,
+                  LaunchOpts{true, ns}, d);
 }
 
 }  // namespace
@@ -593,17 +699,16 @@ cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max
   d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
   d.group_rows = std::max(1, std::min(max_rows, kSlots / d.unit_heads));
   const long units = ((long)d.n_rows + d.group_rows - 1) / d.group_rows * d.c.kv_heads * d.head_chunks;
-  // split a row's pages while the units leave SMs free and every warp has a page
   const int pages = (max_len + kKv8Page - 1) / kKv8Page;
-  unsigned ns = 1;
-  while (ns < 8 && units * ns < 2l * sms && (int)ns * kAttnWarps < pages) ns *= 2;
-  const unsigned u = (unsigned)units;
   const bool w = d.c.head_dim == 128;
   switch (dtype) {
-    case DT_F16: return w ? launch_attn_t<__half, 128>(d, u, ns, st) : launch_attn_t<__half, 64>(d, u, ns, st);
+    case DT_F16:
+      return w ? launch_attn_t<__half, 128>(d, units, pages, sms, st) : launch_attn_t<__half, 64>(d, units, pages, sms, st);
     case DT_BF16:
-      return w ? launch_attn_t<__nv_bfloat16, 128>(d, u, ns, st) : launch_attn_t<__nv_bfloat16, 64>(d, u, ns, st);
-    default: return w ? launch_attn_t<float, 128>(d, u, ns, st) : launch_attn_t<float, 64>(d, u, ns, st);
+      return w ? launch_attn_t<__nv_bfloat16, 128>(d, units, pages, sms, st)
+               : launch_attn_t<__nv_bfloat16, 64>(d, units, pages, sms, st);
+    default:
+      return w ? launch_attn_t<float, 128>(d, units, pages, sms, st) : launch_attn_t<float, 64>(d, units, pages, sms, st);
   }
 }
 

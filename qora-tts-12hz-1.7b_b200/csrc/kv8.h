@@ -1,6 +1,8 @@
 // kv8.h -- the 8-bit paged K/V cache: descriptors and launchers of its append
 // and attention kernels, and what the entry points on device pointers share.
 #pragma once
+#include <atomic>
+
 #include "../../include/qtts.h"
 #include "kernels.h"
 
@@ -25,6 +27,20 @@ class OnDeviceOf {
  private:
   int prev_ = -1;
 };
+
+// Runs `set` (function attributes, which belong to a device) the first time on
+// each device; `state` is one word a device, kept by the caller.
+constexpr int kMaxDevices = 64;
+template <typename F>
+cudaError_t once_per_device(std::atomic<int>* state, F set) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kMaxDevices && state[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  e = set();
+  if (e == cudaSuccess && dev < kMaxDevices) state[dev].store(1, std::memory_order_release);
+  return e;
+}
 
 struct Kv8AppendDesc {
   qtts_kv8_cache c;
