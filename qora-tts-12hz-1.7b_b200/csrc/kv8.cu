@@ -301,7 +301,6 @@ __device__ __forceinline__ uint32_t half2_of(uint32_t biased, uint32_t sel) {
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) { split_pair(a, b, hi, lo); }
 
 constexpr int kSlots = 8;
-constexpr int kAttnWarps = 4;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -320,7 +319,7 @@ __device__ __forceinline__ void cp_async_wait() {
 // chunks of a row change places so that the fragment reads below (8 lanes of
 // 16 bytes at a time: K two rows x four chunks, V four rows x two chunks) hit
 // every bank once.
-constexpr int kStages = 4;
+constexpr int kStages = 4, kStep = 2;
 template <int HD>
 struct Ring {
   static constexpr int kBlock = kKv8Page * HD;  // bytes of one K or V block
@@ -336,16 +335,16 @@ struct Ring {
   }
 };
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __grid_constant__ Kv8AttnDesc d) {
+template <typename T, int HD, int NW>
+__global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid_constant__ Kv8AttnDesc d) {
   constexpr int NT = HD / 8;   // dims a thread's V chunk holds, and n-tiles of the output
   constexpr int KJ = HD / 64;  // 64-dim halves of a row
   using R = Ring<HD>;
   extern __shared__ __align__(128) uint8_t ring[];
   float(*s_o)[kSlots][HD] = reinterpret_cast<float(*)[kSlots][HD]>(ring);  // after the pages: each warp's sums
   static_assert(R::kWarp >= kSlots * HD * 4, "the warps' sums lie over the ring");
-  __shared__ float s_scale[kAttnWarps][kStages][2];
-  __shared__ float s_m[kAttnWarps][kSlots], s_l[kAttnWarps][kSlots];
+  __shared__ float s_scale[NW][kStages][2];
+  __shared__ float s_m[NW][kSlots], s_l[NW][kSlots];
   __shared__ float s_po[kSlots][HD];
   __shared__ float s_pm[kSlots], s_pl[kSlots];
   pdl_launch_dependents();
@@ -393,29 +392,29 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __gr
     const int nslots = rows * nh;
     const bool on = g < nslots;
 
-    // this split's pages [pb, pe); the warp takes every kAttnWarps-th of them
+    // this split's pages [pb, pe); the warp takes every NW-th of them
     const int p0 = hi > 0 ? lo / kKv8Page : 0, p1 = (hi + kKv8Page - 1) / kKv8Page;
     const int share = (p1 - p0 + nsplit - 1) / nsplit;
     const int pb = p0 + split * share + warp, pe = min(p1, p0 + (split + 1) * share);
-    const int np = pb < pe ? (pe - pb + kAttnWarps - 1) / kAttnWarps : 0;
+    const int np = pb < pe ? (pe - pb + NW - 1) / NW : 0;
     const int* table = c.page_table + (size_t)seq * c.pages_per_seq;
     int entries = -1;        // lane i: the page of the 32 * k + i-th of them
     unsigned skip = 0;       // bit s: stage s holds no page
-    auto issue = [&](int i) {
+    auto issue_page = [&](int i) {
+      const int s = i % kStages;
+      skip |= 1u << s;
       if (i < np) {
         if ((i & 31) == 0) {
-          const int pg = pb + (i + lane) * kAttnWarps;
+          const int pg = pb + (i + lane) * NW;
           entries = pg < pe ? table[pg] : -1;
           if (pg < pe && (entries < 0 || entries >= c.n_pages)) {
             raise(d.flags, QTTS_KV8_BAD_PAGE);
             entries = -1;
           }
         }
-        const int page = __shfl_sync(kFull, entries, i & 31), s = i % kStages;
-        skip &= ~(1u << s);
-        if (page < 0) {
-          skip |= 1u << s;
-        } else {
+        const int page = __shfl_sync(kFull, entries, i & 31);
+        if (page >= 0) {
+          skip &= ~(1u << s);
           const int8_t* kb = block_codes(c, page, 0, kvh) + lane * 16;
           const int8_t* vb = block_codes(c, page, 1, kvh) + lane * 16;
           const uint32_t dst = ring_s + s * 2 * R::kBlock;
@@ -428,10 +427,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __gr
           if (lane < 2) cp_async4(scale_s + (s * 2 + lane) * 4, block_scale(c, page, lane, kvh));
         }
       }
+    };
+    auto issue = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) issue_page(i + k);
       cp_async_commit();  // one group a step, empty or not
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (int i = 0; i < kStages; i += kStep) issue(i);
 
     // this thread's slot: query fragments, scale, and the positions it sees
     uint32_t qa[KJ * 4][4];
@@ -474,51 +477,66 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __gr
       for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
     float m = -INFINITY, mo = -INFINITY, l = 0.0f;
 
-    for (int i = 0; i < np; ++i) {
-      cp_async_wait<kStages - 2>();
-      __syncwarp();  // every lane's copies of page i are there, and its reads of page i - 1 done
+    // kStep pages at a time: independent chains of products and one running
+    // maximum for all of them
+    for (int i = 0; i < np; i += kStep) {
+      cp_async_wait<kStages / kStep - 1>();
+      __syncwarp();  // every lane's copies of these pages are there
       const int st = i % kStages;
-      const bool skipped = (skip >> st) & 1;
-      issue(i + kStages - 1);
-      if (skipped) continue;
-      const uint8_t* kb = my_ring + st * 2 * R::kBlock;
-      const uint8_t* vb = kb + R::kBlock;
-      const float sk = s_scale[warp][st][0], sv = s_scale[warp][st][1];
-      const int at0 = (pb + i * kAttnWarps) * kKv8Page + 2 * t;
+      const uint8_t* base = my_ring + st * 2 * R::kBlock;
+      const int at0 = (pb + i * NW) * kKv8Page + 2 * t;
       // scores: positions 8n + 2t, + 1 of slot g in (acc[n][0] + 2^-11 acc[n][2], ...)
-      float acc[2][4] = {};
+      float acc[kStep][2][4] = {};
 #pragma unroll
       for (int j = 0; j < KJ; ++j) {
-        uint4 kw[2];
+        uint4 kw[kStep][2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) kw[n] = *reinterpret_cast<const uint4*>(kb + R::k_at(n * 8 + g, 16 * (t + 4 * j)));
+        for (int k = 0; k < kStep; ++k)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            kw[k][n] = *reinterpret_cast<const uint4*>(base + k * 2 * R::kBlock + R::k_at(n * 8 + g, 16 * (t + 4 * j)));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const uint32_t u = (e == 0 ? kw[n].x : e == 1 ? kw[n].y : e == 2 ? kw[n].z : kw[n].w) ^ 0x80808080u;
-            mma16816(acc[n], qa[j * 4 + e], half2_of(u, 0x4140), half2_of(u, 0x4342));
-          }
+          for (int k = 0; k < kStep; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint4& w = kw[k][n];
+              const uint32_t u = (e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w) ^ 0x80808080u;
+              mma16816(acc[k][n], qa[j * 4 + e], half2_of(u, 0x4140), half2_of(u, 0x4342));
+            }
       }
-      float s[2][2], pm = -INFINITY;
-      const float f = qscale * sk;
+      float s[kStep][2][2], pm[kStep], ev[kStep], fr[kStep];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int k = 0; k < kStep; ++k) {
+        const bool there = !((skip >> (st + k)) & 1);
+        const float f = qscale * s_scale[warp][st + k][0], sv = there ? s_scale[warp][st + k][1] : 0.0f;
+        pm[k] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int at = at0 + n * 8 + e;
-          s[n][e] = at >= see_lo && at < see_hi ? (acc[n][e] + acc[n][e + 2] * (1.0f / kSplitLoScale)) * f : -INFINITY;
-          pm = fmaxf(pm, s[n][e]);
-        }
-      pm = fmaxf(pm, __shfl_xor_sync(kFull, pm, 1));
-      pm = fmaxf(pm, __shfl_xor_sync(kFull, pm, 2));
-      // sv = fr * 2^ev; the output's running exponent follows score + ev, so
-      // that the weights times sv stay within f16 whatever the scales are
-      const int svb = __float_as_int(sv), svx = (svb >> 23) & 255;
-      const float ev = svx == 0 ? -126.0f : svx == 255 ? 0.0f : (float)(svx - 127);
-      const float fr = svx == 0 ? sv * 0x1p126f
-                                : svx == 255 ? sv : __int_as_float((svb & 0x807fffff) | 0x3f800000);
-      const float mn = fmaxf(m, pm), mon = fmaxf(mo, pm + ev);
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = at0 + k * NW * kKv8Page + n * 8 + e;
+            s[k][n][e] = there && at >= see_lo && at < see_hi
+                             ? (acc[k][n][e] + acc[k][n][e + 2] * (1.0f / kSplitLoScale)) * f : -INFINITY;
+            pm[k] = fmaxf(pm[k], s[k][n][e]);
+          }
+        // sv = fr * 2^ev; the output's running exponent follows score + ev, so
+        // that the weights times sv stay within f16 whatever the scales are
+        const int svb = __float_as_int(sv), svx = (svb >> 23) & 255;
+        ev[k] = svx == 0 ? -126.0f : svx == 255 ? 0.0f : (float)(svx - 127);
+        fr[k] = svx == 0 ? sv * 0x1p126f : svx == 255 ? sv : __int_as_float((svb & 0x807fffff) | 0x3f800000);
+      }
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) pm[k] = fmaxf(pm[k], __shfl_xor_sync(kFull, pm[k], 1));
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) pm[k] = fmaxf(pm[k], __shfl_xor_sync(kFull, pm[k], 2));
+      float mn = m, mon = mo;
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) {
+        mn = fmaxf(mn, pm[k]);
+        mon = fmaxf(mon, pm[k] + ev[k]);
+      }
       const float mz = mn == -INFINITY ? 0.0f : mn;
       l *= ex2(m - mz);
       const float beta = mo == mon ? 1.0f : ex2(mo - mon);
@@ -530,42 +548,48 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __gr
       }
       m = mn;
       mo = mon;
-      const float fac = mon == -INFINITY ? 0.0f : ex2(fminf(mz - mon + ev, 120.0f)) * fr;
-      uint32_t pa[4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float a = ex2(s[n][0] - mz), b = ex2(s[n][1] - mz);
-        l += a + b;
-        split_f16(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
-      }
-      uint32_t vw[4][NT / 4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, dims NT * g ...
+      for (int k = 0; k < kStep; ++k) {
+        const float fac = mon == -INFINITY ? 0.0f : ex2(fminf(mz - mon + ev[k], 120.0f)) * fr[k];
+        uint32_t pa[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint8_t* src = vb + R::v_at(2 * t + (e & 1) + (e >> 1) * 8, NT * g);
-        if (NT == 16) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src);
-          vw[e][0] = u.x;
-          vw[e][1] = u.y;
-          vw[e][NT / 4 - 2] = u.z;
-          vw[e][NT / 4 - 1] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(src);
-          vw[e][0] = u.x;
-          vw[e][1] = u.y;
+        for (int n = 0; n < 2; ++n) {
+          const float a = ex2(s[k][n][0] - mz), b = ex2(s[k][n][1] - mz);
+          l += a + b;
+          split_f16(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
+        }
+        const uint8_t* vb = base + k * 2 * R::kBlock + R::kBlock;
+        uint32_t vw[4][NT / 4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, dims NT * g ...
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint8_t* src = vb + R::v_at(2 * t + (e & 1) + (e >> 1) * 8, NT * g);
+          if (NT == 16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src);
+            vw[e][0] = u.x;
+            vw[e][1] = u.y;
+            vw[e][NT / 4 - 2] = u.z;
+            vw[e][NT / 4 - 1] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(src);
+            vw[e][0] = u.x;
+            vw[e][1] = u.y;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < NT / 4; ++q) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = vw[e][q] ^ 0x80808080u;
+          const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
+          const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
+          mma16816(o[q * 4 + 0], pa, half2_of(a01, 0x4140), half2_of(b01, 0x4140));
+          mma16816(o[q * 4 + 1], pa, half2_of(a01, 0x4342), half2_of(b01, 0x4342));
+          mma16816(o[q * 4 + 2], pa, half2_of(a23, 0x4140), half2_of(b23, 0x4140));
+          mma16816(o[q * 4 + 3], pa, half2_of(a23, 0x4342), half2_of(b23, 0x4342));
         }
       }
-#pragma unroll
-      for (int q = 0; q < NT / 4; ++q) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = vw[e][q] ^ 0x80808080u;
-        const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
-        const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
-        mma16816(o[q * 4 + 0], pa, half2_of(a01, 0x4140), half2_of(b01, 0x4140));
-        mma16816(o[q * 4 + 1], pa, half2_of(a01, 0x4342), half2_of(b01, 0x4342));
-        mma16816(o[q * 4 + 2], pa, half2_of(a23, 0x4140), half2_of(b23, 0x4140));
-        mma16816(o[q * 4 + 3], pa, half2_of(a23, 0x4342), half2_of(b23, 0x4342));
-      }
+      __syncwarp();  // every lane has read these pages
+      issue(i + kStages);
     }
     // join the warps, then the splits of the cluster, in their order
     l += __shfl_xor_sync(kFull, l, 1);
@@ -602,15 +626,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __gr
       if (e == 0 && d.lse)
         d.lse[orow * d.heads + head] = mx == -INFINITY ? -INFINITY : (mx + log2f(ll)) * 0.6931471805599453f;
     };
-    for (int i = tid; i < nslots * HD; i += kAttnWarps * 32) {
+    for (int i = tid; i < nslots * HD; i += NW * 32) {
       const int s = i / HD, e = i % HD;
       float mx = s_m[0][s];
 #pragma unroll
-      for (int w = 1; w < kAttnWarps; ++w) mx = fmaxf(mx, s_m[w][s]);
+      for (int w = 1; w < NW; ++w) mx = fmaxf(mx, s_m[w][s]);
       float sum = 0.0f, ll = 0.0f;
       if (mx > -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) {
+        for (int w = 0; w < NW; ++w) {
           const float k = ex2(s_m[w][s] - mx);
           sum += s_o[w][s][e] * k;
           ll += s_l[w][s] * k;
@@ -631,7 +655,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 3) kv8_attn_kernel(const __gr
       continue;
     }
     cluster.sync();
-    for (int i = tid + split * kAttnWarps * 32; i < nslots * HD; i += nsplit * kAttnWarps * 32) {
+    for (int i = tid + split * NW * 32; i < nslots * HD; i += nsplit * NW * 32) {
       const int s = i / HD, e = i % HD;
       float mx = -INFINITY, sum = 0.0f, ll = 0.0f;
       for (int r = 0; r < nsplit; ++r) {
@@ -657,21 +681,33 @@ cudaError_t launch_append_t(const Kv8AppendDesc& d, cudaStream_t st) {
                   LaunchOpts{true, 1}, d);
 }
 // Splits of a unit's pages: doubled while the CTAs do not fill the device
-// (three an SM) and every warp keeps two pages.  Clusters of 16 need an opt-in.
-template <typename T, int HD>
-cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, cudaStream_t st) {
-  constexpr int smem = kAttnWarps * Ring<HD>::kWarp;
+// (twelve warps an SM) and every warp keeps kStep pages.  Clusters of 16 need
+// an opt-in.
+template <typename T, int HD, int NW>
+cudaError_t launch_attn_w(const Kv8AttnDesc& d, long units, unsigned ns, cudaStream_t st) {
+  constexpr int smem = NW * Ring<HD>::kWarp;
   static std::atomic<int> ready[kMaxDevices];
   const cudaError_t set = once_per_device(ready, [] {
-    const cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e =
+        cudaFuncSetAttribute(kv8_attn_kernel<T, HD, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(kv8_attn_kernel<T, HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return cudaFuncSetAttribute(kv8_attn_kernel<T, HD, NW>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   });
   if (set != cudaSuccess) return set;
-  unsigned ns = 1;
-  while (ns < 16 && units * ns * 2 <= 3l * sms && pages >= (int)ns * 2 * kAttnWarps) ns *= 2;
-  return launch_k(kv8_attn_kernel<T, HD>, dim3((unsigned)units, ns), dim3(kAttnWarps * 32), smem, st,
-                  LaunchOpts{true, ns}, d);
+  return launch_k(kv8_attn_kernel<T, HD, NW>, dim3((unsigned)units, ns), dim3(NW * 32), smem, st, LaunchOpts{true, ns},
+                  d);
+}
+template <typename T, int HD>
+cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, cudaStream_t st) {
+  auto splits = [&](int warps) {
+    unsigned ns = 1;
+    while (ns < 16 && units * ns * 2 * warps <= 12l * sms && pages >= (int)ns * 2 * warps * kStep) ns *= 2;
+    return ns;
+  };
+  // few units over long caches: clusters of 16 CTAs of 4 warps leave two
+  // thirds of the SMs' warps unused, CTAs of 12 warps fill them
+  if (units * 16 * 4 < 6l * sms && pages >= 16 * 12) return launch_attn_w<T, HD, 12>(d, units, splits(12), st);
+  return launch_attn_w<T, HD, 4>(d, units, splits(4), st);
 }
 
 }  // namespace
