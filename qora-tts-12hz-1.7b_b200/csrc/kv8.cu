@@ -286,6 +286,32 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Integer sums start at the bits of 1.5 * 2^23, so that a sum of less than
+// 2^22 is read as a float by one subtraction.
+constexpr int kIntBias = 0x4B400000;
+constexpr float kFloatBias = 12582912.0f;
+// Four numbers of less than 2^22 as three signed bytes each (x = 65536 l0 +
+// 256 l1 + l2): the words of their l0, l1 and l2.
+__device__ __forceinline__ void limbs4(float4 v, float up, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
+  const float x[4] = {v.x, v.y, v.z, v.w};
+  w0 = w1 = w2 = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int y = __float2int_rn(x[i] * up);
+    w2 |= (uint32_t)(y & 255) << (8 * i);
+    y = (y - (int)(int8_t)(y & 255)) >> 8;
+    w1 |= (uint32_t)(y & 255) << (8 * i);
+    y = (y - (int)(int8_t)(y & 255)) >> 8;
+    w0 |= (uint32_t)(y & 255) << (8 * i);
+  }
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -436,13 +462,14 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
 #pragma unroll
     for (int i = 0; i < kStages; i += kStep) issue(i);
 
-    // this thread's slot: query fragments, scale, and the positions it sees
-    uint32_t qa[KJ * 4][4];
-    float qscale = 0.0f;
+    // this thread's slot: query limbs, scale, and the positions it sees
+    uint32_t q0[KJ * 4], q1[KJ * 4], q2[KJ * 4];
+    float qscale;
     int see_lo = 0, see_hi = 0;
     {
       float4 x[KJ][4];
       float big = 0.0f;
+      bool finite = true;
       const T* qp = static_cast<const T*>(d.q) + (size_t)(unit_row0 + slot_row) * d.ldq +
                     (size_t)(h0 + (on ? g % nh : 0)) * HD;
 #pragma unroll
@@ -450,21 +477,21 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[j][i] = on ? load4(qp + 16 * (t + 4 * j) + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-          big = fmaxf(big, fmaxf(fmaxf(fabsf(x[j][i].x), fabsf(x[j][i].y)), fmaxf(fabsf(x[j][i].z), fabsf(x[j][i].w))));
+          const float4 v = make_float4(fabsf(x[j][i].x), fabsf(x[j][i].y), fabsf(x[j][i].z), fabsf(x[j][i].w));
+          finite &= v.x <= FLT_MAX && v.y <= FLT_MAX && v.z <= FLT_MAX && v.w <= FLT_MAX;
+          big = fmaxf(big, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
         }
       big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
       big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
-      const int ef = (__float_as_int(big) >> 23) & 255;
-      const int ex = ef == 0 || ef == 255 ? 0 : ef - 127;
-      const float dn = ldexpf(1.0f, -ex);
-      qscale = ldexpf(d.scale * 1.4426950408889634f, ex);  // scores in units of log 2
+      finite = ((__ballot_sync(kFull, finite) >> (lane & 28)) & 15u) == 15u;
+      // big in [2^ex, 2^(ex+1)) becomes an integer in [2^21, 2^22)
+      const int ex = min(127, max(-100, ((__float_as_int(big) >> 23) & 255) - 127));
+      const float up = ldexpf(1.0f, 21 - ex);
+      qscale = finite ? ldexpf(d.scale * 1.4426950408889634f, ex - 21) : NAN;  // scores in units of log 2
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          split_f16(x[j][i].x * dn, x[j][i].y * dn, qa[j * 4 + i][0], qa[j * 4 + i][1]);
-          split_f16(x[j][i].z * dn, x[j][i].w * dn, qa[j * 4 + i][2], qa[j * 4 + i][3]);
-        }
+        for (int i = 0; i < 4; ++i) limbs4(x[j][i], up, q0[j * 4 + i], q1[j * 4 + i], q2[j * 4 + i]);
       if (on) {
         see_hi = slot_pos + 1;
         see_lo = d.window > 0 ? max(0, see_hi - d.window) : 0;
@@ -485,27 +512,26 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       const int st = i % kStages;
       const uint8_t* base = my_ring + st * 2 * R::kBlock;
       const int at0 = (pb + i * NW) * kKv8Page + 2 * t;
-      // scores: positions 8n + 2t, + 1 of slot g in (acc[n][0] + 2^-11 acc[n][2], ...)
-      float acc[kStep][2][4] = {};
+      // scores of positions 8n + 2t, + 1 of slot g: l0, l1 in hi, l2 in lo
+      int hi_[kStep][2][4], lo_[kStep][2][4];
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        uint4 kw[kStep][2];
+      for (int k = 0; k < kStep; ++k)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) hi_[k][n][e] = lo_[k][n][e] = kIntBias;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
 #pragma unroll
         for (int k = 0; k < kStep; ++k)
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-            kw[k][n] = *reinterpret_cast<const uint4*>(base + k * 2 * R::kBlock + R::k_at(n * 8 + g, 16 * (t + 4 * j)));
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int k = 0; k < kStep; ++k)
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint4& w = kw[k][n];
-              const uint32_t u = (e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w) ^ 0x80808080u;
-              mma16816(acc[k][n], qa[j * 4 + e], half2_of(u, 0x4140), half2_of(u, 0x4342));
-            }
-      }
+          for (int n = 0; n < 2; ++n) {
+            const uint4 w = *reinterpret_cast<const uint4*>(base + k * 2 * R::kBlock + R::k_at(n * 8 + g, 16 * (t + 4 * j)));
+            imma16832(hi_[k][n], q0[j * 4], q1[j * 4], q0[j * 4 + 1], q1[j * 4 + 1], w.x, w.y);
+            imma16832(lo_[k][n], q2[j * 4], 0, q2[j * 4 + 1], 0, w.x, w.y);
+            imma16832(hi_[k][n], q0[j * 4 + 2], q1[j * 4 + 2], q0[j * 4 + 3], q1[j * 4 + 3], w.z, w.w);
+            imma16832(lo_[k][n], q2[j * 4 + 2], 0, q2[j * 4 + 3], 0, w.z, w.w);
+          }
       float s[kStep][2][2], pm[kStep], ev[kStep], fr[kStep];
 #pragma unroll
       for (int k = 0; k < kStep; ++k) {
@@ -518,7 +544,10 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
           for (int e = 0; e < 2; ++e) {
             const int at = at0 + k * NW * kKv8Page + n * 8 + e;
             s[k][n][e] = there && at >= see_lo && at < see_hi
-                             ? (acc[k][n][e] + acc[k][n][e + 2] * (1.0f / kSplitLoScale)) * f : -INFINITY;
+                             ? f * fmaf(__int_as_float(hi_[k][n][e]) - kFloatBias, 65536.0f,
+                                        fmaf(__int_as_float(hi_[k][n][e + 2]) - kFloatBias, 256.0f,
+                                             __int_as_float(lo_[k][n][e]) - kFloatBias))
+                             : -INFINITY;
             pm[k] = fmaxf(pm[k], s[k][n][e]);
           }
         // sv = fr * 2^ev; the output's running exponent follows score + ev, so
