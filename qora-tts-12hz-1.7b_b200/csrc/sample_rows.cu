@@ -51,57 +51,68 @@ struct SampleRowsDesc {
   float* logprob = nullptr;
 };
 
-// Order keys: larger for a larger logit, equal for the two zeros, 0 for what is
-// never drawn (NaN, -inf).  A 16-bit logit has a 16-bit key.
+// Order keys: larger for a larger logit, equal for the two zeros, at most kNone
+// for what is never drawn (NaN, -inf).  A 16-bit logit has a 16-bit key.
 template <typename T>
 struct Key {  // f16, bf16
   using Stored = uint16_t;
-  static __device__ __forceinline__ float f32(uint32_t bits) {
-    const uint16_t b = (uint16_t)bits;
-    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(b));
-    else return __uint_as_float((uint32_t)b << 16);
-  }
-  static __device__ __forceinline__ uint32_t of(uint32_t bits) {
-    constexpr uint32_t inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    const uint32_t mag = bits & 0x7fffu;
-    const uint32_t k = bits & 0x8000u ? 0x8000u - mag : 0x8000u + mag;
-    return mag > inf || bits == (0x8000u | inf) ? 0u : k;
-  }
+  static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  static constexpr uint32_t kNone = 0x8000u - kInf;
   static __device__ __forceinline__ float value(uint32_t k) {
-    return f32(k >= 0x8000u ? k - 0x8000u : 0x8000u | (0x8000u - k));
+    const uint32_t bits = k >= 0x8000u ? k - 0x8000u : 0x8000u | (0x8000u - k);
+    if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((uint16_t)bits));
+    else return __uint_as_float(bits << 16);
+  }
+  // two logits' keys: 0x8000 + magnitude, or 0x8000 - magnitude
+  static __device__ __forceinline__ uint32_t of2(uint32_t w, uint32_t& most) {
+    const uint32_t sign = (w >> 15) & 0x00010001u;
+    uint32_t k = (w ^ (sign * 0x7fffu) ^ 0x80008000u) + sign;
+    if (__vmaxu2(k, 0x80008000u + kInf * 0x00010001u) != 0x80008000u + kInf * 0x00010001u) {  // a NaN
+      if ((k & 0xffffu) > 0x8000u + kInf) k &= 0xffff0000u;
+      if ((k >> 16) > 0x8000u + kInf) k &= 0xffffu;
+    }
+    most = __vmaxu2(most, k);
+    return k;
+  }
+  static __device__ __forceinline__ uint32_t of(uint32_t bits, uint32_t& most) {
+    return of2(bits, most) & 0xffffu;  // (the upper half, +0, is no largest key: see larger())
   }
 };
 template <>
 struct Key<float> {
   using Stored = uint32_t;
-  static __device__ __forceinline__ uint32_t of(uint32_t bits) {
-    const float l = __uint_as_float(bits);
-    return l > -INFINITY ? f32_order_key(l) : 0u;
-  }
+  static constexpr uint32_t kNone = 0u;
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+  }
+  static __device__ __forceinline__ uint32_t of(uint32_t bits, uint32_t& most) {
+    const float l = __uint_as_float(bits);
+    const uint32_t k = l > -INFINITY ? f32_order_key(l) : 0u;
+    most = max(most, k);
+    return k;
   }
 };
 __device__ __forceinline__ u64 place_of(uint32_t key, int index) { return ((u64)key << 32) | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t key_in(u64 place) { return (uint32_t)(place >> 32); }
 
 struct Weigh {
-  float top;  // the largest logit
+  float top;        // the largest logit
   float inv_tf;
-  double inv_t;
+  double inv_t, top_d;
+  bool infinite;    // top is: the infinite logits share, whatever the temperature
   const double* exp2_32;  // 2^(i / 32)
   __device__ __forceinline__ double z(float l) const {
-    const double x = ((double)l - (double)top) * inv_t;
-    return l == top ? 0.0 : x <= 0.0 ? x : -INFINITY;  // an infinite top over an infinite temperature is no number
+    if (infinite) return l == top ? 0.0 : -INFINITY;
+    return ((double)l - top_d) * inv_t;
   }
-  // false: the weight is surely 0 (z < -34 whatever the f32 roundings)
-  __device__ __forceinline__ bool counts(float l) const { return !((top - l) * inv_tf > 34.0f); }
-  // exp(z) 2^45 to the nearest integer: z = n ln2/32 + r, exp(r) by its series
-  // to r^5 (|r| < 0.011: 2e-15), 2^(n/32) by table and exponent.  Below -33
-  // (a weight of less than 1/8 of 2^-45) it is 0.
+  // false: the weight is 0 (z < -33.9 whatever the f32 roundings)
+  __device__ __forceinline__ bool counts(float l) const {
+    return infinite ? l == top : !((top - l) * inv_tf > 34.0f);
+  }
+  // exp(z) 2^45 to the nearest integer, for z of -35 to 0: z = n ln2/32 + r,
+  // exp(r) by its series to r^5 (|r| < 0.011: 2e-15), 2^(n/32) by table and
+  // exponent
   __device__ __forceinline__ u64 of_z(double x) const {
-    const bool some = x > -33.0;
-    x = some ? x : -33.0;
     const double shift = 0x1.8p52;
     const double nd = __fma_rn(x, 46.166241308446828, shift);  // 32 / ln 2
     const int n = __double2loint(nd);
@@ -114,9 +125,9 @@ struct Weigh {
     const double t = exp2_32[n & 31];
     const double s = __hiloint2double(__double2hiint(t) + (((n >> 5) + kFix) << 20), __double2loint(t));
     const double w = __fma_rn(s, p, 0x1p52);  // the sum's mantissa is the integer
-    return some ? (u64)(__double_as_longlong(w) - __double_as_longlong(0x1p52)) : 0;
+    return (u64)(__double_as_longlong(w) - __double_as_longlong(0x1p52));
   }
-  __device__ __forceinline__ u64 operator()(float l) const { return of_z(z(l)); }
+  __device__ __forceinline__ u64 operator()(float l) const { return counts(l) ? of_z(z(l)) : 0; }
 };
 
 // Histogram bins: counts, and weights as three words of 15 bits, whose sums of
@@ -133,8 +144,9 @@ struct Bins {
   __device__ __forceinline__ u64 weight(int b) const { return (u64)w[0][b] + ((u64)w[1][b] << 15) + ((u64)w[2][b] << 30); }
 };
 
-constexpr int kFew = 32;  // tokens that one warp puts in order
-struct Shared {
+constexpr int kFew = 32;      // tokens that a search leaves to one warp
+constexpr int kSmall = 64;    // tokens whose filters and draw one warp does alone
+struct alignas(16) Shared {
   Bins bins;
   union {
     u64 list[kList];
@@ -146,11 +158,13 @@ struct Shared {
   u64 weight[kList];  // of the list; before it is made, this CTA's part of the list
   u64 few[kFew], few_weight[kFew];
   double exp2_32[32];
-  u64 scan[33];
-  u64 word[4];            // what this CTA tells the cluster
+  u64 scan[32];
+  unsigned scan32[32];
+  u64 word[2];            // what this CTA tells the cluster
+  unsigned key_word[2];
   unsigned part[32];      // tokens in this CTA's part of the list, by warp
   unsigned offset[8 * 32];
-  u64 found_before;
+  u64 found_before, found_at;
   unsigned found_bin, found_n, n;
 };
 
@@ -170,9 +184,9 @@ struct Block {
     __syncthreads();
     if (lane == 0) sh.scan[warp] = v;
     __syncthreads();
-    v = sh.scan[0];
+    v = sh.scan[lane & (kWarps - 1)];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) v = op(v, sh.scan[w]);
+    for (int o = kWarps / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(kFull, v, o));
     return v;
   }
   __device__ __forceinline__ u64 sum(u64 v) {
@@ -183,6 +197,20 @@ struct Block {
   }
   __device__ __forceinline__ u64 least(u64 v) {
     return reduce(v, [](u64 a, u64 b) { return a < b ? a : b; });
+  }
+  __device__ __forceinline__ unsigned sum32(unsigned v) {
+    v = __reduce_add_sync(kFull, v);
+    __syncthreads();
+    if (lane == 0) sh.scan32[warp] = v;
+    __syncthreads();
+    return __reduce_add_sync(kFull, lane < kWarps ? sh.scan32[lane] : 0u);
+  }
+  __device__ __forceinline__ unsigned most32(unsigned v) {
+    v = __reduce_max_sync(kFull, v);
+    __syncthreads();
+    if (lane == 0) sh.scan32[warp] = v;
+    __syncthreads();
+    return __reduce_max_sync(kFull, lane < kWarps ? sh.scan32[lane] : 0u);
   }
   // exclusive prefix over the threads, and the total
   __device__ __forceinline__ u64 prefix(u64 v, u64* total) {
@@ -195,15 +223,15 @@ struct Block {
     __syncthreads();
     if (lane == 31) sh.scan[warp] = x;
     __syncthreads();
-    u64 before = 0, all = 0;
+    u64 s = lane < kWarps ? sh.scan[lane] : 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const u64 s = sh.scan[w];
-      if (w < warp) before += s;
-      all += s;
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const u64 y = __shfl_up_sync(kFull, s, o);
+      if (lane >= o) s += y;
     }
-    *total = all;
-    return before + x - v;
+    *total = __shfl_sync(kFull, s, kWarps - 1);
+    const u64 before = __shfl_sync(kFull, s, max(0, warp - 1));
+    return (warp ? before : 0) + x - v;
   }
   __device__ __forceinline__ void clear(Mode mode) {
     for (int i = tid; i < kBins; i += TH) {
@@ -242,18 +270,20 @@ struct Block {
     __syncthreads();
     return target;
   }
-  // The entry of the list (all in [lo, hi], or 0: not taking part), from the
-  // largest down, at which the running count or weight reaches `target` (at
-  // least 1).  Histograms narrow the range until a warp can order what is left.
-  __device__ u64 select(Mode mode, int n, u64 lo, u64 hi, u64 target) {
+  // The entry of the list (0: not taking part), from the largest down, at which
+  // the running count or weight reaches `target` (at least 1).  The first
+  // histogram goes by first_bin(place), the next ones by the places of the bin
+  // that holds the target, until one warp can order what is left.
+  template <typename FirstBin>
+  __device__ u64 select(Mode mode, int n, u64 target, FirstBin first_bin) {
+    u64 lo = 1, hi = ~0ull;
+    int s = -1, bin = 0;
     for (;;) {
-      const u64 span = hi - lo;
-      const int s = span < kBins ? 0 : 64 - __clzll(span) - 10;
       clear(mode);
       for (int i = tid; i < n; i += TH) {
         const u64 c = sh.list[i];
-        if (c < lo || c > hi || c == 0) continue;
-        const int b = (int)((hi - c) >> s);
+        if (c < lo || c > hi) continue;
+        const int b = s < 0 ? first_bin(c) : (int)((hi - c) >> s);
         atomicAdd(&sh.bins.count[b], 1u);
         if (mode == WEIGHT) sh.bins.add(b, sh.weight[i]);
       }
@@ -262,29 +292,45 @@ struct Block {
                     [&](int b) { return mode == COUNT ? (u64)sh.bins.count[b] : sh.bins.weight(b); },
                     [&](int b) { return sh.bins.count[b]; });
       target -= sh.found_before;
-      hi -= (u64)sh.found_bin << s;
-      const u64 width = (1ull << s) - 1;
-      if (hi - lo > width) lo = hi - width;
-      if (sh.found_n > kFew) continue;
+      bin = sh.found_bin;
+      if (s >= 0) {
+        hi -= (u64)bin << s;
+        const u64 width = (1ull << s) - 1;
+        if (hi - lo > width) lo = hi - width;
+      }
+      auto inside = [&](u64 c) { return c >= lo && c <= hi && (s >= 0 || first_bin(c) == bin); };
+      if (sh.found_n <= kFew) {
+        for (int i = tid; i < n; i += TH) {
+          const u64 c = sh.list[i];
+          if (inside(c)) {
+            const unsigned at = atomicAdd(&sh.n, 1u);
+            sh.few[at] = c;
+            sh.few_weight[at] = mode == COUNT ? 1 : sh.weight[i];
+          }
+        }
+        __syncthreads();
+        if (warp == 0) {  // the weight at or above each lane's entry
+          const int m = sh.n;
+          const u64 c = lane < m ? sh.few[lane] : 0, w = lane < m ? sh.few_weight[lane] : 0;
+          u64 incl = 0;
+          for (int i = 0; i < m; ++i) incl += sh.few[i] >= c ? sh.few_weight[i] : 0;
+          if (lane < m && incl >= target && incl - w < target) sh.found_at = c;
+        }
+        __syncthreads();
+        return sh.found_at;
+      }
+      u64 a = ~0ull, z = 0;
       for (int i = tid; i < n; i += TH) {
         const u64 c = sh.list[i];
-        if (c >= lo && c <= hi && c) {
-          const unsigned at = atomicAdd(&sh.n, 1u);
-          sh.few[at] = c;
-          sh.few_weight[at] = mode == COUNT ? 1 : sh.weight[i];
+        if (inside(c)) {
+          a = c < a ? c : a;
+          z = c > z ? c : z;
         }
       }
-      __syncthreads();
-      // every warp for itself: the weight at or above this lane's entry
-      const bool have = lane < (int)sh.n;
-      const u64 c = have ? sh.few[lane] : 0, w = have ? sh.few_weight[lane] : 0;
-      u64 incl = 0;
-      for (int i = 0; i < (int)sh.n; ++i) {
-        const u64 ci = sh.few[i], wi = sh.few_weight[i];
-        if (ci >= c) incl += wi;
-      }
-      const bool at = have && incl >= target && incl - w < target;
-      return __shfl_sync(kFull, c, __ffs(__ballot_sync(kFull, at)) - 1);
+      lo = least(a);
+      hi = most(z);
+      const u64 span = hi - lo;
+      s = span < kBins ? 0 : 64 - __clzll(span) - 10;
     }
   }
 };
@@ -306,6 +352,7 @@ struct Filters {
   bool use_p;
   double zmin;
   float u;
+  float bins_per_unit;
 };
 
 __device__ __forceinline__ void answer(const SampleRowsDesc& d, int row, int token, int kept, double logw, u64 total) {
@@ -314,15 +361,90 @@ __device__ __forceinline__ void answer(const SampleRowsDesc& d, int row, int tok
   if (d.logprob) d.logprob[row] = token < 0 ? -INFINITY : (float)(logw - log((double)total * (1.0 / (1ull << kFix))));
 }
 
-// All filters and the draw on a list that holds every token they can keep, in
-// the order of the indices; its places lie in [lo, hi], or are 0.
+// The bin of a key in the histogram over (top - l) / T, 32 bins a unit.
+template <typename T>
+struct FirstBin {
+  float top, per_unit;
+  __device__ __forceinline__ int key(uint32_t k) const {
+    const float l = Key<T>::value(k), x = (top - l) * per_unit;
+    return l == top ? 0 : x < (float)(kBins - 1) ? (int)x : kBins - 1;
+  }
+  __device__ __forceinline__ int operator()(u64 place) const { return key(key_in(place)); }
+};
+
+// All filters and the draw on a list of at most kSmall tokens that holds every
+// one they can keep, in the order of the indices: one warp, each lane's two
+// tokens against all of them.
+template <typename T>
+__device__ void draw_small(Shared& sh, const SampleRowsDesc& d, const Weigh& weigh, const Filters& f, int row, int n) {
+  const int lane = threadIdx.x & 31;
+  u64 c[2], w[2], sum = 0;
+  double z[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = lane * 2 + j;
+    c[j] = i < n ? sh.list[i] : 0;
+    const float l = Key<T>::value(key_in(c[j]));
+    z[j] = weigh.z(l);
+    w[j] = c[j] && weigh.counts(l) ? weigh.of_z(z[j]) : 0;
+    if (i < kSmall) sh.weight[i] = w[j];
+  }
+  __syncwarp();
+  u64 above[2] = {0, 0};
+  int rank[2] = {0, 0};
+  for (int i = 0; i < n; ++i) {
+    const u64 ci = sh.list[i], wi = sh.weight[i];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool before = ci > c[j];
+      rank[j] += before && ci;
+      above[j] += before ? wi : 0;
+    }
+  }
+  bool keep[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    keep[j] = c[j] != 0 && (f.k == 0 || rank[j] < f.k);
+    sum += keep[j] ? w[j] : 0;
+  }
+  if (f.use_p) {  // a token whose weight before it reaches the target is not kept
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    const u64 target = nucleus(f.p, sum);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) keep[j] = keep[j] && above[j] < target;
+  }
+  u64 own = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    keep[j] = keep[j] && z[j] >= f.zmin;
+    if (!keep[j]) w[j] = 0;
+    own += w[j];
+  }
+  const unsigned cnt = __reduce_add_sync(kFull, (unsigned)keep[0] + (unsigned)keep[1]);
+  u64 incl = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(kFull, incl, o);
+    if (lane >= o) incl += y;
+  }
+  const u64 total = __shfl_sync(kFull, incl, 31), goal = goal_of(f.u, total);
+  u64 run = incl - own;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (run <= goal && goal < run + w[j]) answer(d, row, (int)~(uint32_t)c[j], (int)cnt, z[j], total);
+    run += w[j];
+  }
+}
+
+// The same on a longer list.
 template <typename T, int TH>
-__device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Weigh& weigh, const Filters& f, int row,
-                               int n, u64 lo, u64 hi) {
+__device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Weigh& weigh, const Filters& f, int row, int n) {
   constexpr int N = kList / TH;  // entries of a thread: they stay in registers, next to each other in the list
   Shared& sh = bk.sh;
+  const FirstBin<T> first_bin{weigh.top, f.bins_per_unit};
   u64 last = 1;
-  if (f.k > 0 && f.k < n) last = bk.select(COUNT, n, lo, hi, f.k);
+  if (f.k > 0 && f.k < n) last = bk.select(COUNT, n, f.k, first_bin);
   const int each = (n + TH - 1) / TH, i0 = min(n, (int)threadIdx.x * each), i1 = min(n, i0 + each);
   u64 c[N], w[N], total = 0;
   double z[N];
@@ -330,12 +452,10 @@ __device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Wei
   for (int j = 0; j < N; ++j) {
     c[j] = i0 + j < i1 ? sh.list[i0 + j] : 0;
     if (c[j] < last) c[j] = 0;
-    z[j] = c[j] ? weigh.z(Key<T>::value(key_in(c[j]))) : -INFINITY;
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
+    const float l = Key<T>::value(key_in(c[j]));
+    z[j] = weigh.z(l);
     w[j] = 0;
-    if (j < each) w[j] = weigh.of_z(z[j]);
+    if (c[j] && weigh.counts(l)) w[j] = weigh.of_z(z[j]);
     total += w[j];
   }
   if (f.use_p) {
@@ -346,26 +466,25 @@ __device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Wei
         sh.list[i0 + j] = c[j];
         sh.weight[i0 + j] = w[j];
       }
-    last = bk.select(WEIGHT, n, lo, hi, nucleus(f.p, total));
+    last = bk.select(WEIGHT, n, nucleus(f.p, total), first_bin);
   }
   u64 own = 0;
   unsigned cnt = 0;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const bool keep = c[j] >= last && c[j] && z[j] >= f.zmin;
+    const bool keep = c[j] >= last && z[j] >= f.zmin;
     if (!keep) w[j] = 0;
     cnt += keep;
     own += w[j];
   }
   u64 sum;
   u64 run = bk.prefix(own, &sum);
-  cnt = (unsigned)bk.sum(cnt);
+  cnt = bk.sum32(cnt);
   const u64 goal = goal_of(f.u, sum);
   if (run <= goal && goal < run + own) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (run <= goal && goal < run + w[j])
-        answer(d, row, (int)~(uint32_t)c[j], (int)cnt, z[j], sum);
+      if (run <= goal && goal < run + w[j]) answer(d, row, (int)~(uint32_t)c[j], (int)cnt, z[j], sum);
       run += w[j];
     }
   }
@@ -397,46 +516,44 @@ template <typename T, int TH>
 struct Slice {
   const typename Key<T>::Stored* keys;
   int n, base;  // base: the first one's index
-  // f(i, key, place) of every column, kUnroll at a time
+  // f(key, place) of every column that can be drawn
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
 #pragma unroll 4
     for (int i = threadIdx.x; i < n; i += TH) {
       const uint32_t k = keys[i];
-      f(i, k, place_of(k, base + i));
+      if (k > Key<T>::kNone) f(k, place_of(k, base + i));
     }
   }
-  // f(i, key, weight) of columns [first, last) step `step` whose place is at
+  // f(i, key, z, weight) of columns [first, last) step `step` whose place is at
   // least `floor`: four independent chains of f64 arithmetic
   template <typename F>
   __device__ __forceinline__ void weighed(int first, int last, int step, u64 floor, const Weigh& weigh, F f) const {
+    const uint32_t floor_key = key_in(floor);
     for (int i0 = first; i0 < last; i0 += 4 * step) {
       uint32_t k[4];
       float l[4];
-      bool on[4], any = false;
+      bool on[4], heavy[4], any = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = i0 + j * step;
         k[j] = i < last ? keys[i] : 0u;
-        on[j] = k[j] != 0 && place_of(k[j], base + i) >= floor;
-        l[j] = Key<T>::value(on[j] ? k[j] : 1u);
-        any |= on[j] && weigh.counts(l[j]);
+        on[j] = k[j] > floor_key || (k[j] == floor_key && i < last && place_of(k[j], base + i) >= floor);
+        l[j] = Key<T>::value(k[j]);
+        heavy[j] = on[j] && weigh.counts(l[j]);
+        any |= heavy[j];
       }
-      if (any) {
-        u64 w[4];
-        double z[4];
+      u64 w[4] = {0, 0, 0, 0};
+      double z[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] = weigh.z(l[j]);
+      for (int j = 0; j < 4; ++j) z[j] = weigh.z(l[j]);
+      if (any) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = weigh.of_z(z[j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (on[j]) f(i0 + j * step, k[j], z[j], w[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (on[j]) f(i0 + j * step, k[j], weigh.z(l[j]), 0ull);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (on[j]) f(i0 + j * step, k[j], z[j], heavy[j] ? w[j] : 0ull);
     }
   }
 };
@@ -445,24 +562,20 @@ struct Slice {
 // of the tokens at or above `lo` reaches target(total).
 template <typename T, int TH, typename Target>
 __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<T, TH>& sl, Mode mode, Target target_of,
-                              u64 lo, u64 hi, const Weigh& weigh, float bins_per_unit) {
+                              u64 lo, const Weigh& weigh, float bins_per_unit) {
   Shared& sh = bk.sh;
   const int tid = threadIdx.x;
   const unsigned ranks = cl.num_blocks(), rank = cl.block_rank();
-  // level 0: bins of (top - l) / T; then, where a bin holds more than a list,
-  // bins of the places [lo, hi]
-  auto first_bin = [&](uint32_t k) {
-    const float l = Key<T>::value(k), x = (weigh.top - l) * bins_per_unit;
-    return l == weigh.top ? 0 : x < (float)(kBins - 1) ? (int)x : kBins - 1;
-  };
+  const FirstBin<T> first_bin{weigh.top, bins_per_unit};
+  u64 hi = ~0ull;
   int s = -1;
   u64 target = 0;
   for (;;) {
     bk.clear(mode);
-    auto bin_of = [&](uint32_t k, u64 c) { return s < 0 ? first_bin(k) : (int)((hi - c) >> s); };
+    auto bin_of = [&](uint32_t k, u64 c) { return s < 0 ? first_bin.key(k) : (int)((hi - c) >> s); };
     if (mode == COUNT) {
-      sl.each([&](int, uint32_t k, u64 c) {
-        if (k != 0 && c >= lo && c <= hi) atomicAdd(&sh.bins.count[bin_of(k, c)], 1u);
+      sl.each([&](uint32_t k, u64 c) {
+        if (c >= lo && c <= hi) atomicAdd(&sh.bins.count[bin_of(k, c)], 1u);
       });
     } else {
       sl.weighed(tid, sl.n, TH, lo, weigh, [&](int i, uint32_t k, double, u64 w) {
@@ -490,23 +603,23 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
     target = bk.find([&](u64 total) { return s < 0 ? target_of(total) : target; },
                      [&](int b) { return cl.map_shared_rank(sh.merged.weight, b / share)[b]; },
                      [&](int b) { return cl.map_shared_rank(sh.merged.count, b / share)[b]; });
-    const int bin0 = sh.found_bin;
+    const int bin = sh.found_bin;
     const unsigned count = sh.found_n;
     target -= sh.found_before;
     if (s >= 0) {
-      hi -= (u64)bin0 << s;
+      hi -= (u64)bin << s;
       const u64 width = (1ull << s) - 1;
       if (hi - lo > width) lo = hi - width;
     }
-    auto inside = [&](uint32_t k, u64 c) { return k != 0 && c >= lo && c <= hi && (s >= 0 || first_bin(k) == bin0); };
+    auto inside = [&](uint32_t k, u64 c) { return c >= lo && c <= hi && (s >= 0 || first_bin.key(k) == bin); };
     if (count <= kList) {
       // every CTA gathers the bin's tokens from all, each from its own part
-      u64 a = ~0ull, z = 0;
-      sl.each([&](int, uint32_t k, u64 c) {
+      sl.each([&](uint32_t k, u64 c) {
         if (inside(k, c)) sh.weight[atomicAdd(&sh.n, 1u)] = c;  // (the weights are filled in below)
       });
       cl.sync();
       unsigned at = 0;
+      u64 a = ~0ull, z = 0;
       for (unsigned r = 0; r < ranks; ++r) {
         const unsigned m = *cl.map_shared_rank(&sh.n, r);
         const u64* from = cl.map_shared_rank(sh.weight, r);
@@ -523,11 +636,14 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
       cl.sync();
       if (mode == WEIGHT)
         for (unsigned i = tid; i < at; i += TH) sh.weight[i] = weigh(Key<T>::value(key_in(sh.list[i])));
-      return bk.select(mode, (int)at, a, z, target);
+      // the bin's places spread evenly over the first histogram
+      const u64 span = z - a;
+      const int shift = span < kBins ? 0 : 64 - __clzll(span) - 10;
+      return bk.select(mode, (int)at, target, [&](u64 c) { return (int)((z - c) >> shift); });
     }
     // the range of the bin's places
     u64 a = ~0ull, z = 0;
-    sl.each([&](int, uint32_t k, u64 c) {
+    sl.each([&](uint32_t k, u64 c) {
       if (inside(k, c)) {
         a = c < a ? c : a;
         z = c > z ? c : z;
@@ -553,53 +669,74 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
   }
 }
 
-// Reads columns [0, n) at src; put(i, key) for each.  16 bytes a load where the
-// row starts on that boundary.
-template <typename T, int TH, typename Put>
-__device__ __forceinline__ void read_columns(const T* src, int n, Put put) {
+// Reads columns [0, n) at src into keys and returns the largest key: 16 bytes a
+// load and a store where the row starts on that boundary (keys always do).
+template <typename T, int TH>
+__device__ __forceinline__ uint32_t read_columns(const T* src, int n, typename Key<T>::Stored* keys) {
+  using K = Key<T>;
   constexpr int E = 16 / sizeof(T);
+  uint32_t most = 0;
   int done = 0;
   if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
     const uint4* v = reinterpret_cast<const uint4*>(src);
     const int nv = n / E;
 #pragma unroll 4
     for (int i = threadIdx.x; i < nv; i += TH) {
-      const uint4 u = __ldcs(v + i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (E == 4) {
-          put(i * E + j, Key<T>::of(w[j]));
-        } else {
-          put(i * E + 2 * j, Key<T>::of(w[j] & 0xffffu));
-          put(i * E + 2 * j + 1, Key<T>::of(w[j] >> 16));
-        }
-      }
+      uint4 u = __ldcs(v + i);
+      if constexpr (E == 4) u = make_uint4(K::of(u.x, most), K::of(u.y, most), K::of(u.z, most), K::of(u.w, most));
+      else u = make_uint4(K::of2(u.x, most), K::of2(u.y, most), K::of2(u.z, most), K::of2(u.w, most));
+      reinterpret_cast<uint4*>(keys)[i] = u;
     }
     done = nv * E;
   }
+  if constexpr (E == 8) most = max(most & 0xffffu, most >> 16);
 #pragma unroll 8
   for (int i = done + threadIdx.x; i < n; i += TH) {
-    if constexpr (E == 4) put(i, Key<T>::of(reinterpret_cast<const uint32_t*>(src)[i]));
-    else put(i, Key<T>::of(reinterpret_cast<const uint16_t*>(src)[i]));
+    uint32_t one = 0, k;
+    if constexpr (E == 4) k = K::of(reinterpret_cast<const uint32_t*>(src)[i], one);
+    else k = K::of(reinterpret_cast<const uint16_t*>(src)[i], one);
+    keys[i] = (typename K::Stored)k;
+    most = max(most, k);
   }
+  return most;
+}
+
+// One warp: a bound that `each` of the m keys reach, and hardly more (the low
+// bits of a 32-bit key are left at 0); 1 above kNone if there are fewer.
+template <typename T>
+__device__ __forceinline__ uint32_t bound_of(const unsigned* k, int m, int each) {
+  constexpr int kTopBit = sizeof(T) == 4 ? 31 : 15, kLowBit = sizeof(T) == 4 ? 10 : 0;
+  const int lane = threadIdx.x & 31;
+  uint32_t v[16], bound = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = j * 32 + lane < m ? k[j * 32 + lane] : 0u;
+#pragma unroll 1
+  for (int b = kTopBit; b >= kLowBit; --b) {
+    const uint32_t t = bound | (1u << b);
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) c += v[j] >= t;
+    if (__reduce_add_sync(kFull, c) >= (unsigned)each) bound = t;
+  }
+  return max(bound, Key<T>::kNone + 1);
 }
 
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid_constant__ SampleRowsDesc d) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
+  static_assert(sizeof(Shared) % 16 == 0, "the keys start on 16 bytes");
+  static_assert(TH <= 512, "bound_of takes 16 keys a lane");
   auto* keys = reinterpret_cast<typename Key<T>::Stored*>(smem + sizeof(Shared));
   if (threadIdx.x < 32) sh.exp2_32[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
   pdl_launch_dependents();
   pdl_wait();
   cg::cluster_group cl = cg::this_cluster();
-  constexpr int kWarps = TH / 32;
+  constexpr int kWarps = TH / 32, kPart = kList / kWarps;  // tokens of a warp's part of the list
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x;
   const unsigned rank = cl.block_rank(), ranks = cl.num_blocks();
   const int base = (int)rank * d.per, n = max(0, min(d.per, d.V - base));
   const T* src = static_cast<const T*>(d.logits) + (size_t)row * d.ld + base;
-  const bool short_row = d.V <= kList;  // the row is the list
   Block<TH> bk(sh);
   Filters f;
   const float temp = d.temperature ? d.temperature[row] : 1.0f;
@@ -609,108 +746,155 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   f.u = d.u[row];
   f.use_p = f.p < 1.0f;
   if (f.k < 0 || f.k >= d.V) f.k = 0;
+  f.bins_per_unit = 32.0f / temp;
+  const bool greedy = !(temp > 0.0f);
+  // small top-k: the list is what lies above a bound
+  const bool bounded = !greedy && f.k > 0 && f.k <= kList / 2 && f.k * 4 <= (int)ranks * TH;
+  const int each = bounded ? (f.k + ranks - 1) / ranks : 0;
 
-  // ---- the row, and the first token of the order ---------------------------------
-  uint32_t my_key = 0;
-  int my_at = 0;
-  read_columns<T, TH>(src, n, [&](int i, uint32_t k) {
-    if (short_row) sh.list[i] = k ? place_of(k, i) : 0ull;
-    else keys[i] = (typename Key<T>::Stored)k;
-    if (k > my_key || (k == my_key && i < my_at)) {
-      my_key = k;
-      my_at = i;
+  // ---- the row, its largest key and the bound ----------------------------------------
+  const uint32_t my_key = read_columns<T, TH>(src, n, keys);
+  unsigned* maxima = reinterpret_cast<unsigned*>(sh.weight);
+  maxima[tid] = my_key;
+  uint32_t top = bk.most32(my_key), bound = 0;
+  if (bounded && warp == 0) bound = bound_of<T>(maxima, TH, each);
+  if (ranks > 1) {
+    if (tid == 0) {
+      sh.key_word[0] = top;
+      sh.key_word[1] = bound;
     }
-  });
-  u64 best = bk.most(my_key ? place_of(my_key, base + my_at) : 0ull);
-  if (!short_row) {
-    if (tid == 0) sh.word[2] = best;
     cl.sync();
+    bound = ~0u;
     for (unsigned r = 0; r < ranks; ++r) {
-      const u64 x = cl.map_shared_rank(sh.word, r)[2];
-      best = best > x ? best : x;
+      const unsigned* w = cl.map_shared_rank(sh.key_word, r);
+      top = max(top, w[0]);
+      bound = min(bound, w[1]);
     }
+  } else {
+    if (tid == 0) sh.key_word[1] = bound;
+    __syncthreads();
+    bound = sh.key_word[1];
   }
-  if (best == 0 || !(temp > 0.0f)) {
-    if (rank == 0 && tid == 0) answer(d, row, best == 0 ? -1 : (int)~(uint32_t)best, best != 0, 0.0, 1ull << kFix);
-    if (!short_row) cl.sync();  // no CTA leaves while its word is read
+  if (top <= Key<T>::kNone || greedy) {
+    // the first column with the largest key
+    unsigned at = 0xffffffffu;
+    if (top > Key<T>::kNone)
+      for (int i = tid; i < n; i += TH)
+        if (keys[i] == top) at = min(at, (unsigned)(base + i));
+    at = ~bk.most32(~at);
+    if (ranks > 1) {
+      if (tid == 0) sh.word[0] = at;
+      cl.sync();
+      for (unsigned r = 0; r < ranks; ++r) at = min(at, (unsigned)cl.map_shared_rank(sh.word, r)[0]);
+      cl.sync();  // no CTA leaves while its word is read
+    }
+    if (rank == 0 && tid == 0) answer(d, row, (int)at, at != 0xffffffffu, 0.0, 1ull << kFix);
     return;
   }
   Weigh weigh;
-  weigh.top = Key<T>::value(key_in(best));
+  weigh.top = Key<T>::value(top);
   weigh.inv_tf = 1.0f / temp;
   weigh.inv_t = 1.0 / (double)temp;
+  weigh.top_d = weigh.top;
+  weigh.infinite = isinf(weigh.top);
   weigh.exp2_32 = sh.exp2_32;
   f.zmin = mp > 0.0f ? log((double)fminf(mp, 1.0f)) : -INFINITY;
-  const u64 lowest = 1ull << 32;  // the least place that can be drawn
-  if (short_row) {
-    draw_from_list<T>(bk, d, weigh, f, row, n, lowest, best);
-    return;
-  }
-  const Slice<T, TH> sl{keys, n, base};
-  const int seg = (d.per + kWarps - 1) / kWarps, s0 = min(n, warp * seg), s1 = min(n, s0 + seg);  // a warp's columns
+  const int seg = ((d.per + kWarps - 1) / kWarps + 7) / 8 * 8;  // a warp's columns
+  const int s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
 
-  // ---- small top-k: the list of what lies above a bound ---------------------------
-  if (f.k > 0 && f.k <= kList / 2 && f.k * 4 <= (int)ranks * TH) {
-    constexpr int kPart = kList / kWarps;  // tokens of a warp's part
-    sh.list[tid] = my_key ? place_of(my_key, tid) : 0ull;
-    __syncthreads();
-    const int each = (f.k + ranks - 1) / ranks;
-    uint32_t bound = 1;
-    if (bk.sum(my_key != 0) >= (u64)each) bound = key_in(bk.select(COUNT, TH, lowest, ~0ull, each));
-    if (tid == 0) sh.word[0] = bound;
-    cl.sync();
-    for (unsigned r = 0; r < ranks; ++r) bound = min(bound, (uint32_t)cl.map_shared_rank(sh.word, r)[0]);
+  // ---- a list: what lies above the bound, or a short row ---------------------------
+  if (bounded) {
     unsigned mine = 0;
-    for (int i0 = s0; i0 < s1; i0 += 128) {  // in the order of the columns
-      uint32_t k[4];
+    for (int i0 = s0; i0 < s1; i0 += 256) {  // eight columns a lane, in their order
+      const int i = i0 + lane * 8;
+      unsigned hits = 0;
+      uint32_t k[8];
+      if (i < s1) {
+        if constexpr (sizeof(T) == 2) {
+          const uint4 u = *reinterpret_cast<const uint4*>(keys + i);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * 32 + lane;
-        k[j] = i < s1 ? keys[i] : 0u;
-      }
+          for (int j = 0; j < 4; ++j) {
+            k[2 * j] = w[j] & 0xffffu;
+            k[2 * j + 1] = w[j] >> 16;
+          }
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(keys + i), v = *reinterpret_cast<const uint4*>(keys + i + 4);
+          k[0] = u.x, k[1] = u.y, k[2] = u.z, k[3] = u.w, k[4] = v.x, k[5] = v.y, k[6] = v.z, k[7] = v.w;
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned hits = __ballot_sync(kFull, k[j] >= bound);
-        const unsigned at = mine + __popc(hits & ((1u << lane) - 1));
-        if (k[j] >= bound && at < kPart) sh.weight[warp * kPart + at] = place_of(k[j], base + i0 + j * 32 + lane);
-        mine += __popc(hits);
+        for (int j = 0; j < 8; ++j) hits |= (i + j < s1 && k[j] >= bound) ? 1u << j : 0u;
       }
+      if (!__any_sync(kFull, hits)) continue;
+      unsigned at = __popc(hits);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(kFull, at, o);
+        if (lane >= o) at += y;
+      }
+      const unsigned all = __shfl_sync(kFull, at, 31);
+      at += mine - __popc(hits);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((hits >> j) & 1) {
+          if (at < kPart) sh.weight[warp * kPart + at] = place_of(k[j], base + i + j);
+          ++at;
+        }
+      mine += all;
     }
     if (lane == 0) sh.part[warp] = mine;
-    cl.sync();
+    if (ranks > 1) cl.sync();
+    else __syncthreads();
     const int parts = (int)ranks * kWarps;  // at most 8 * 16
-    const unsigned m = tid < parts ? cl.map_shared_rank(sh.part, tid / kWarps)[tid % kWarps] : 0u;
+    unsigned m = 0;
+    if (tid < parts) m = ranks > 1 ? cl.map_shared_rank(sh.part, tid / kWarps)[tid % kWarps] : sh.part[tid];
     u64 total;
     const u64 at = bk.prefix(m, &total);
-    const bool fits = total <= kList && __syncthreads_and(m <= (unsigned)kPart);
+    const bool fits = __syncthreads_and(total <= kList && m <= (unsigned)kPart);
     if (fits) {
       if (rank == 0) {
         if (tid < parts) sh.offset[tid] = ((unsigned)at << 12) | m;
         __syncthreads();
         for (int p = warp; p < parts; p += kWarps) {
           const unsigned o = sh.offset[p] >> 12, c = sh.offset[p] & 4095u;
-          const u64* from = cl.map_shared_rank(sh.weight, p / kWarps) + (p % kWarps) * kPart;
+          const u64* from = (ranks > 1 ? cl.map_shared_rank(sh.weight, p / kWarps) : sh.weight) + (p % kWarps) * kPart;
           for (unsigned i = lane; i < c; i += 32) sh.list[o + i] = from[i];
         }
       }
-      cl.sync();
-      if (rank == 0) draw_from_list<T>(bk, d, weigh, f, row, (int)total, place_of(bound, 0x7fffffff), best);
+      if (ranks > 1) cl.sync();
+      else __syncthreads();
+      if (rank != 0) return;
+      if (total <= kSmall) {
+        if (warp == 0) draw_small<T>(sh, d, weigh, f, row, (int)total);
+      } else {
+        draw_from_list<T>(bk, d, weigh, f, row, (int)total);
+      }
       return;
     }
-    cl.sync();
+    if (ranks > 1) cl.sync();
+  }
+  if (d.V <= kList) {
+    for (int i = tid; i < n; i += TH) {
+      const uint32_t k = keys[i];
+      sh.list[i] = k > Key<T>::kNone ? place_of(k, i) : 0ull;
+    }
+    __syncthreads();
+    draw_from_list<T>(bk, d, weigh, f, row, n);
+    return;
   }
 
   // ---- otherwise: the last kept place by histograms over the cluster ----------------
-  const float bins_per_unit = 32.0f / temp;
-  u64 last = lowest;
+  const Slice<T, TH> sl{keys, n, base};
+  u64 last = (u64)(Key<T>::kNone + 1) << 32;
   if (f.k > 0)
-    last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, best, weigh, bins_per_unit);
+    last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, weigh, f.bins_per_unit);
   if (f.use_p)
-    last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, best, weigh,
-                          bins_per_unit);
+    last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, weigh,
+                          f.bins_per_unit);
 
   // ---- the draw: a warp's columns, then the threads of the CTA over that warp's ----
-  u64 sum = 0, cnt = 0;
+  u64 sum = 0;
+  unsigned cnt = 0;
   sl.weighed(s0 + lane, s1, 32, last, weigh, [&](int, uint32_t, double z, u64 w) {
     const bool keep = z >= f.zmin;
     sum += keep ? w : 0;
@@ -718,8 +902,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   });
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-  cnt = bk.sum(cnt);
-  __syncthreads();
+  cnt = bk.sum32(cnt);
   if (lane == 0) sh.scan[warp] = sum;
   __syncthreads();
   u64 mine = 0;
@@ -730,8 +913,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   if (goal < run || goal >= run + mine) return;  // another CTA's
   int w = 0;
   while (goal >= run + sh.scan[w]) run += sh.scan[w++];
-  const int t0 = min(n, w * seg), t1 = min(n, t0 + seg), each = (t1 - t0 + TH - 1) / TH;
-  const int a0 = min(t1, t0 + tid * each), a1 = min(t1, a0 + each);
+  const int t0 = min(n, w * seg), t1 = min(n, t0 + seg), more = (t1 - t0 + TH - 1) / TH;
+  const int a0 = min(t1, t0 + tid * more), a1 = min(t1, a0 + more);
   u64 own = 0, all;
   sl.weighed(a0, a1, 1, last, weigh, [&](int, uint32_t, double z, u64 w) { own += z >= f.zmin ? w : 0; });
   u64 at = run + bk.prefix(own, &all);
@@ -746,7 +929,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
 template <typename T, int TH>
 cudaError_t launch_t(const SampleRowsDesc& d, int n_rows, int ranks, cudaStream_t st) {
   constexpr size_t key = sizeof(typename Key<T>::Stored);
-  const size_t smem = sizeof(Shared) + (d.V <= kList ? 0 : (size_t)d.per * key);
+  const size_t smem = sizeof(Shared) + (size_t)d.per * key;
   static std::atomic<int> ready[kMaxDevices];
   const cudaError_t e = once_per_device(ready, [] {
     return cudaFuncSetAttribute(sample_rows_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize,

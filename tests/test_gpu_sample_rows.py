@@ -54,7 +54,7 @@ def check(qtts, x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, dtype="f32
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("V", [1, 2, 31, 32, 33, 100, 1000, 2048, 5000, 40000])
+@pytest.mark.parametrize("V", [1, 2, 31, 32, 33, 100, 1000, 2048, 2049, 4000, 5000, 40000])
 def test_filters(qtts, V, dtype):
     rng = np.random.default_rng(V)
     n = 24
