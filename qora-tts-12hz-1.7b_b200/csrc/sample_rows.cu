@@ -7,9 +7,8 @@
 // w = exp((l - largest) / T) are integers of 2^-45 (f64 arithmetic), whose
 // sums do not depend on their order.
 //
-// A row of at most kList logits is a list in one CTA's shared memory.  A longer
-// row lies in the shared memory of a cluster of CTAs, its logits read from HBM
-// once, and is cut down to a list:
+// A row is cut down to a list of at most kList tokens in one CTA's shared memory:
+//   a short row is one;
 //   small top-k: the least of the CTAs' own (k / CTAs)-th largest thread
 //     maxima has k logits above it and few more; those are the list;
 //   otherwise a histogram over (largest - l) / T of counts (top-k) or weights
@@ -17,7 +16,8 @@
 //     tokens are the list.
 // In a list the token at which the running count or weight reaches a target is
 // found by histograms over the range that still holds it, until one warp can
-// put the rest in order.
+// put the rest in order.  A long row is shared by a cluster of CTAs, which read
+// it from HBM once and from the L2 cache in the passes after the first.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -55,7 +55,6 @@ struct SampleRowsDesc {
 // for what is never drawn (NaN, -inf).  A 16-bit logit has a 16-bit key.
 template <typename T>
 struct Key {  // f16, bf16
-  using Stored = uint16_t;
   static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   static constexpr uint32_t kNone = 0x8000u - kInf;
   static __device__ __forceinline__ float value(uint32_t k) {
@@ -63,8 +62,14 @@ struct Key {  // f16, bf16
     if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((uint16_t)bits));
     else return __uint_as_float(bits << 16);
   }
+  static __device__ __forceinline__ uint32_t near(float l) {  // the key of the nearest T
+    uint32_t bits, unused = 0;
+    if constexpr (std::is_same<T, __half>::value) bits = __half_as_ushort(__float2half_rn(l));
+    else bits = __bfloat16_as_ushort(__float2bfloat16_rn(l));
+    return of_word(bits, unused) & 0xffffu;
+  }
   // two logits' keys: 0x8000 + magnitude, or 0x8000 - magnitude
-  static __device__ __forceinline__ uint32_t of2(uint32_t w, uint32_t& most) {
+  static __device__ __forceinline__ uint32_t of_word(uint32_t w, uint32_t& most) {
     const uint32_t sign = (w >> 15) & 0x00010001u;
     uint32_t k = (w ^ (sign * 0x7fffu) ^ 0x80008000u) + sign;
     if (__vmaxu2(k, 0x80008000u + kInf * 0x00010001u) != 0x80008000u + kInf * 0x00010001u) {  // a NaN
@@ -74,18 +79,18 @@ struct Key {  // f16, bf16
     most = __vmaxu2(most, k);
     return k;
   }
-  static __device__ __forceinline__ uint32_t of(uint32_t bits, uint32_t& most) {
-    return of2(bits, most) & 0xffffu;  // (the upper half, +0, is no largest key: see larger())
-  }
 };
 template <>
 struct Key<float> {
-  using Stored = uint32_t;
   static constexpr uint32_t kNone = 0u;
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
   }
-  static __device__ __forceinline__ uint32_t of(uint32_t bits, uint32_t& most) {
+  static __device__ __forceinline__ uint32_t near(float l) {
+    uint32_t unused = 0;
+    return of_word(__float_as_uint(l), unused);
+  }
+  static __device__ __forceinline__ uint32_t of_word(uint32_t bits, uint32_t& most) {
     const float l = __uint_as_float(bits);
     const uint32_t k = l > -INFINITY ? f32_order_key(l) : 0u;
     most = max(most, k);
@@ -96,23 +101,26 @@ __device__ __forceinline__ u64 place_of(uint32_t key, int index) { return ((u64)
 __device__ __forceinline__ uint32_t key_in(u64 place) { return (uint32_t)(place >> 32); }
 
 struct Weigh {
-  float top;        // the largest logit
-  float inv_tf;
-  double inv_t, top_d;
-  bool infinite;    // top is: the infinite logits share, whatever the temperature
+  float top;              // the largest logit
+  float light;            // about top - 36 T: what lies below weighs nothing
+  double top_d, inv_t;
+  bool infinite;          // top is: the infinite logits share, whatever the temperature
   const double* exp2_32;  // 2^(i / 32)
+  __device__ __forceinline__ Weigh(float t, float temp, const double* table) : top(t), exp2_32(table) {
+    light = top - 36.0f * temp;
+    top_d = top;
+    inv_t = 1.0 / (double)temp;
+    infinite = isinf(top);
+  }
   __device__ __forceinline__ double z(float l) const {
     if (infinite) return l == top ? 0.0 : -INFINITY;
     return ((double)l - top_d) * inv_t;
   }
-  // false: the weight is 0 (z < -33.9 whatever the f32 roundings)
-  __device__ __forceinline__ bool counts(float l) const {
-    return infinite ? l == top : !((top - l) * inv_tf > 34.0f);
-  }
-  // exp(z) 2^45 to the nearest integer, for z of -35 to 0: z = n ln2/32 + r,
-  // exp(r) by its series to r^5 (|r| < 0.011: 2e-15), 2^(n/32) by table and
-  // exponent
-  __device__ __forceinline__ u64 of_z(double x) const {
+  // exp(z) 2^45 to the nearest integer, for a finite top and z of -500 to 0:
+  // z = n ln2/32 + r, exp(r) by its series to r^5 (|r| < 0.011: 2e-15),
+  // 2^(n/32) by table and exponent
+  __device__ __forceinline__ u64 finite(float l) const {
+    const double x = ((double)l - top_d) * inv_t;
     const double shift = 0x1.8p52;
     const double nd = __fma_rn(x, 46.166241308446828, shift);  // 32 / ln 2
     const int n = __double2loint(nd);
@@ -127,7 +135,10 @@ struct Weigh {
     const double w = __fma_rn(s, p, 0x1p52);  // the sum's mantissa is the integer
     return (u64)(__double_as_longlong(w) - __double_as_longlong(0x1p52));
   }
-  __device__ __forceinline__ u64 operator()(float l) const { return counts(l) ? of_z(z(l)) : 0; }
+  __device__ __forceinline__ u64 operator()(float l) const {
+    if (infinite) return l == top ? 1ull << kFix : 0;
+    return z(l) > -36.0 ? finite(l) : 0;
+  }
 };
 
 // Histogram bins: counts, and weights as three words of 15 bits, whose sums of
@@ -163,7 +174,7 @@ struct alignas(16) Shared {
   u64 word[2];            // what this CTA tells the cluster
   unsigned key_word[2];
   unsigned part[32];      // tokens in this CTA's part of the list, by warp
-  unsigned offset[8 * 32];
+  unsigned offset[16 * 16];
   u64 found_before, found_at;
   unsigned found_bin, found_n, n;
 };
@@ -350,7 +361,7 @@ struct Filters {
   int k;  // 0: off
   float p;
   bool use_p;
-  double zmin;
+  u64 min_place;  // min-p: the least place that it keeps
   float u;
   float bins_per_unit;
 };
@@ -386,7 +397,7 @@ __device__ void draw_small(Shared& sh, const SampleRowsDesc& d, const Weigh& wei
     c[j] = i < n ? sh.list[i] : 0;
     const float l = Key<T>::value(key_in(c[j]));
     z[j] = weigh.z(l);
-    w[j] = c[j] && weigh.counts(l) ? weigh.of_z(z[j]) : 0;
+    w[j] = c[j] ? weigh(l) : 0;
     if (i < kSmall) sh.weight[i] = w[j];
   }
   __syncwarp();
@@ -417,7 +428,7 @@ __device__ void draw_small(Shared& sh, const SampleRowsDesc& d, const Weigh& wei
   u64 own = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    keep[j] = keep[j] && z[j] >= f.zmin;
+    keep[j] = keep[j] && c[j] >= f.min_place;
     if (!keep[j]) w[j] = 0;
     own += w[j];
   }
@@ -455,7 +466,7 @@ __device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Wei
     const float l = Key<T>::value(key_in(c[j]));
     z[j] = weigh.z(l);
     w[j] = 0;
-    if (c[j] && weigh.counts(l)) w[j] = weigh.of_z(z[j]);
+    if (c[j]) w[j] = weigh(l);
     total += w[j];
   }
   if (f.use_p) {
@@ -468,11 +479,12 @@ __device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Wei
       }
     last = bk.select(WEIGHT, n, nucleus(f.p, total), first_bin);
   }
+  last = last > f.min_place ? last : f.min_place;
   u64 own = 0;
   unsigned cnt = 0;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const bool keep = c[j] >= last && z[j] >= f.zmin;
+    const bool keep = c[j] >= last;
     if (!keep) w[j] = 0;
     cnt += keep;
     own += w[j];
@@ -511,49 +523,117 @@ __device__ __forceinline__ void cluster_sum(cg::cluster_group& cl, Shared& sh, u
   cl.sync();
 }
 
-// One CTA's columns [0, n) of the row, the keys in shared memory.
+// One CTA's columns [0, n) of the row, as vectors of E columns: 16 bytes a load
+// where the row starts on that boundary.  A short row's keys are kept.
 template <typename T, int TH>
 struct Slice {
-  const typename Key<T>::Stored* keys;
-  int n, base;  // base: the first one's index
+  using K = Key<T>;
+  static constexpr int E = 16 / sizeof(T);
+  const T* src;
+  int n, nv, base;  // columns, vectors, the first column's index
+  bool aligned;
+  uint4* kept;      // shared memory, or null
+
+  __device__ __forceinline__ uint4 raw(int v) const {
+    if (aligned && (v + 1) * E <= n) return reinterpret_cast<const uint4*>(src)[v];
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (E == 4) {
+        w[j] = v * E + j < n ? reinterpret_cast<const uint32_t*>(src)[v * E + j] : 0xff800000u;
+      } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+        const uint32_t none = 0x8000u | K::kInf;  // -inf behind the last column
+        const int i = v * E + 2 * j;
+        w[j] = (i < n ? h[i] : none) | ((i + 1 < n ? h[i + 1] : none) << 16);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ uint4 to_keys(uint4 u, uint32_t (&most)[4]) const {
+    return make_uint4(K::of_word(u.x, most[0]), K::of_word(u.y, most[1]), K::of_word(u.z, most[2]),
+                      K::of_word(u.w, most[3]));
+  }
+  // the first pass: the thread's largest key in each place of a vector
+  // (E == 8: two in a word)
+  __device__ __forceinline__ void largest(uint32_t (&most)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most[j] = 0;
+    for (int v0 = threadIdx.x; v0 < nv; v0 += 4 * TH) {
+      uint4 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v0 + j * TH < nv) u[j] = raw(v0 + j * TH);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v0 + j * TH < nv) {
+          u[j] = to_keys(u[j], most);
+          if (kept) kept[v0 + j * TH] = u[j];
+        }
+    }
+  }
+  // later passes: the keys of a vector (none where v is no vector)
+  __device__ __forceinline__ void keys(int v, bool is, uint32_t (&k)[E]) const {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    uint32_t most[4] = {0, 0, 0, 0};
+    if (is) u = kept ? kept[v] : to_keys(raw(v), most);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (E == 4) {
+        k[j] = w[j];
+      } else {
+        k[2 * j] = w[j] & 0xffffu;
+        k[2 * j + 1] = w[j] >> 16;
+      }
+    }
+  }
   // f(key, place) of every column that can be drawn
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += TH) {
-      const uint32_t k = keys[i];
-      if (k > Key<T>::kNone) f(k, place_of(k, base + i));
+#pragma unroll 2
+    for (int v = threadIdx.x; v < nv; v += TH) {
+      uint32_t k[E];
+      keys(v, true, k);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (k[j] > K::kNone) f(k[j], place_of(k[j], base + v * E + j));
     }
   }
-  // f(i, key, z, weight) of columns [first, last) step `step` whose place is at
-  // least `floor`: four independent chains of f64 arithmetic
+  // f(i, key, weight) of the columns of vectors [first, last) step `step` whose
+  // place is at least `floor`: four independent chains of f64 arithmetic
   template <typename F>
   __device__ __forceinline__ void weighed(int first, int last, int step, u64 floor, const Weigh& weigh, F f) const {
     const uint32_t floor_key = key_in(floor);
-    for (int i0 = first; i0 < last; i0 += 4 * step) {
-      uint32_t k[4];
-      float l[4];
-      bool on[4], heavy[4], any = false;
+    // Keys below that of `light` have z < -35; keys from it on z > -73, as a T
+    // so near to the largest that 36 T is less than half a step gives its key.
+    const uint32_t heavy = K::near(weigh.light);
+#pragma unroll 1
+    for (int v = first; v < last; v += step) {
+      uint32_t kk[E];
+      keys(v, true, kk);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * step;
-        k[j] = i < last ? keys[i] : 0u;
-        on[j] = k[j] > floor_key || (k[j] == floor_key && i < last && place_of(k[j], base + i) >= floor);
-        l[j] = Key<T>::value(k[j]);
-        heavy[j] = on[j] && weigh.counts(l[j]);
-        any |= heavy[j];
+      for (int h = 0; h < E; h += 4) {
+        const uint32_t* k = kk + h;
+        const int i0 = v * E + h;
+        u64 w[4] = {0, 0, 0, 0};
+        if (weigh.infinite) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = weigh(K::value(k[j]));
+        } else if (max(max(k[0], k[1]), max(k[2], k[3])) >= heavy) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = weigh.finite(K::value(k[j]));
+            if (k[j] < heavy) w[j] = 0;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bool on = k[j] >= floor_key;
+          if (k[j] == floor_key) on = place_of(k[j], base + i0 + j) >= floor;
+          if (on) f(i0 + j, k[j], w[j]);
+        }
       }
-      u64 w[4] = {0, 0, 0, 0};
-      double z[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) z[j] = weigh.z(l[j]);
-      if (any) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = weigh.of_z(z[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (on[j]) f(i0 + j * step, k[j], z[j], heavy[j] ? w[j] : 0ull);
     }
   }
 };
@@ -578,7 +658,7 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
         if (c >= lo && c <= hi) atomicAdd(&sh.bins.count[bin_of(k, c)], 1u);
       });
     } else {
-      sl.weighed(tid, sl.n, TH, lo, weigh, [&](int i, uint32_t k, double, u64 w) {
+      sl.weighed(tid, sl.nv, TH, lo, weigh, [&](int i, uint32_t k, u64 w) {
         const u64 c = place_of(k, sl.base + i);
         if (c > hi) return;
         const int b = bin_of(k, c);
@@ -669,65 +749,41 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
   }
 }
 
-// Reads columns [0, n) at src into keys and returns the largest key: 16 bytes a
-// load and a store where the row starts on that boundary (keys always do).
-template <typename T, int TH>
-__device__ __forceinline__ uint32_t read_columns(const T* src, int n, typename Key<T>::Stored* keys) {
-  using K = Key<T>;
-  constexpr int E = 16 / sizeof(T);
-  uint32_t most = 0;
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-    const uint4* v = reinterpret_cast<const uint4*>(src);
-    const int nv = n / E;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += TH) {
-      uint4 u = __ldcs(v + i);
-      if constexpr (E == 4) u = make_uint4(K::of(u.x, most), K::of(u.y, most), K::of(u.z, most), K::of(u.w, most));
-      else u = make_uint4(K::of2(u.x, most), K::of2(u.y, most), K::of2(u.z, most), K::of2(u.w, most));
-      reinterpret_cast<uint4*>(keys)[i] = u;
-    }
-    done = nv * E;
-  }
-  if constexpr (E == 8) most = max(most & 0xffffu, most >> 16);
-#pragma unroll 8
-  for (int i = done + threadIdx.x; i < n; i += TH) {
-    uint32_t one = 0, k;
-    if constexpr (E == 4) k = K::of(reinterpret_cast<const uint32_t*>(src)[i], one);
-    else k = K::of(reinterpret_cast<const uint16_t*>(src)[i], one);
-    keys[i] = (typename K::Stored)k;
-    most = max(most, k);
-  }
-  return most;
-}
-
-// One warp: a bound that `each` of the m keys reach, and hardly more (the low
-// bits of a 32-bit key are left at 0); 1 above kNone if there are fewer.
-template <typename T>
-__device__ __forceinline__ uint32_t bound_of(const unsigned* k, int m, int each) {
+// One warp: a bound that `each` of its keys v (N a lane) reach, and hardly more
+// (the low bits of a 32-bit key are left at 0); 1 above kNone if there are fewer.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&v)[N], int each) {
   constexpr int kTopBit = sizeof(T) == 4 ? 31 : 15, kLowBit = sizeof(T) == 4 ? 10 : 0;
-  const int lane = threadIdx.x & 31;
-  uint32_t v[16], bound = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = j * 32 + lane < m ? k[j * 32 + lane] : 0u;
+  uint32_t bound = 0;
 #pragma unroll 1
   for (int b = kTopBit; b >= kLowBit; --b) {
     const uint32_t t = bound | (1u << b);
     unsigned c = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) c += v[j] >= t;
+    for (int j = 0; j < N; ++j) c += v[j] >= t;
     if (__reduce_add_sync(kFull, c) >= (unsigned)each) bound = t;
   }
   return max(bound, Key<T>::kNone + 1);
+}
+
+// The least key that min-p keeps: the lowest with z >= log(min_p).
+template <typename T>
+__device__ __forceinline__ uint32_t min_p_key(float min_p, uint32_t top, float temp, const Weigh& weigh) {
+  const double zmin = log((double)fminf(min_p, 1.0f));
+  // the value in f64, one or two keys around its nearest T
+  uint32_t k = Key<T>::near((float)(weigh.top_d + zmin * (double)temp));
+  if (weigh.infinite) return top;
+  k = min(max(k, Key<T>::kNone + 1), top);
+  while (k > Key<T>::kNone + 1 && weigh.z(Key<T>::value(k - 1)) >= zmin) --k;
+  while (k < top && !(weigh.z(Key<T>::value(k)) >= zmin)) ++k;
+  return k;
 }
 
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid_constant__ SampleRowsDesc d) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
-  static_assert(sizeof(Shared) % 16 == 0, "the keys start on 16 bytes");
-  static_assert(TH <= 512, "bound_of takes 16 keys a lane");
-  auto* keys = reinterpret_cast<typename Key<T>::Stored*>(smem + sizeof(Shared));
+  static_assert(TH <= 512, "the bound takes 16 maxima a lane");
   if (threadIdx.x < 32) sh.exp2_32[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
   pdl_launch_dependents();
   pdl_wait();
@@ -736,7 +792,14 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x;
   const unsigned rank = cl.block_rank(), ranks = cl.num_blocks();
   const int base = (int)rank * d.per, n = max(0, min(d.per, d.V - base));
-  const T* src = static_cast<const T*>(d.logits) + (size_t)row * d.ld + base;
+  constexpr int E = Slice<T, TH>::E;
+  Slice<T, TH> sl;
+  sl.src = static_cast<const T*>(d.logits) + (size_t)row * d.ld + base;
+  sl.n = n;
+  sl.nv = (n + E - 1) / E;
+  sl.base = base;
+  sl.aligned = (reinterpret_cast<uintptr_t>(sl.src) & 15) == 0;
+  sl.kept = d.V <= kList ? reinterpret_cast<uint4*>(smem + sizeof(Shared)) : nullptr;
   Block<TH> bk(sh);
   Filters f;
   const float temp = d.temperature ? d.temperature[row] : 1.0f;
@@ -749,15 +812,43 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   f.bins_per_unit = 32.0f / temp;
   const bool greedy = !(temp > 0.0f);
   // small top-k: the list is what lies above a bound
-  const bool bounded = !greedy && f.k > 0 && f.k <= kList / 2 && f.k * 4 <= (int)ranks * TH;
-  const int each = bounded ? (f.k + ranks - 1) / ranks : 0;
+  // (of the threads' maxima if they are four times as many, else of each warp's
+  // maxima in every place of the vectors, which needs fewer hits a warp)
+  const bool bounded = !greedy && f.k > 0 && f.k <= kList / 2;
+  const bool by_threads = f.k * 4 <= (int)ranks * TH;
+  const int sharers = by_threads ? ranks : ranks * kWarps, each = bounded ? (f.k + sharers - 1) / sharers : 0;
 
   // ---- the row, its largest key and the bound ----------------------------------------
-  const uint32_t my_key = read_columns<T, TH>(src, n, keys);
+  uint32_t most[4];
+  sl.largest(most);
+  uint32_t bound = 0;
+  uint32_t my_key = max(max(most[0], most[1]), max(most[2], most[3]));
+  if constexpr (E == 8) {
+    my_key = 0;
+    uint32_t half[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      half[2 * j] = most[j] & 0xffffu;
+      half[2 * j + 1] = most[j] >> 16;
+      my_key = max(my_key, max(half[2 * j], half[2 * j + 1]));
+    }
+    if (bounded && !by_threads) bound = bound_of<T>(half, each);
+  } else {
+    if (bounded && !by_threads) bound = bound_of<T>(most, each);
+  }
   unsigned* maxima = reinterpret_cast<unsigned*>(sh.weight);
   maxima[tid] = my_key;
-  uint32_t top = bk.most32(my_key), bound = 0;
-  if (bounded && warp == 0) bound = bound_of<T>(maxima, TH, each);
+  uint32_t top = bk.most32(my_key);
+  if (bounded && by_threads) {
+    if (warp == 0) {
+      uint32_t v[TH / 32];
+#pragma unroll
+      for (int j = 0; j < TH / 32; ++j) v[j] = maxima[j * 32 + lane];
+      bound = bound_of<T>(v, each);
+    }
+  } else if (bounded) {
+    bound = ~bk.most32(~bound);  // the least of the warps'
+  }
   if (ranks > 1) {
     if (tid == 0) {
       sh.key_word[0] = top;
@@ -779,8 +870,9 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     // the first column with the largest key
     unsigned at = 0xffffffffu;
     if (top > Key<T>::kNone)
-      for (int i = tid; i < n; i += TH)
-        if (keys[i] == top) at = min(at, (unsigned)(base + i));
+      sl.each([&](uint32_t k, u64 c) {
+        if (k == top) at = min(at, ~(uint32_t)c);
+      });
     at = ~bk.most32(~at);
     if (ranks > 1) {
       if (tid == 0) sh.word[0] = at;
@@ -791,40 +883,21 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     if (rank == 0 && tid == 0) answer(d, row, (int)at, at != 0xffffffffu, 0.0, 1ull << kFix);
     return;
   }
-  Weigh weigh;
-  weigh.top = Key<T>::value(top);
-  weigh.inv_tf = 1.0f / temp;
-  weigh.inv_t = 1.0 / (double)temp;
-  weigh.top_d = weigh.top;
-  weigh.infinite = isinf(weigh.top);
-  weigh.exp2_32 = sh.exp2_32;
-  f.zmin = mp > 0.0f ? log((double)fminf(mp, 1.0f)) : -INFINITY;
-  const int seg = ((d.per + kWarps - 1) / kWarps + 7) / 8 * 8;  // a warp's columns
-  const int s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
+  const Weigh weigh(Key<T>::value(top), temp, sh.exp2_32);
+  f.min_place = (u64)(mp > 0.0f ? min_p_key<T>(mp, top, temp, weigh) : Key<T>::kNone + 1) << 32;
+  const int seg = (sl.nv + kWarps - 1) / kWarps, v0 = min(sl.nv, warp * seg), v1 = min(sl.nv, v0 + seg);  // a warp's vectors
 
   // ---- a list: what lies above the bound, or a short row ---------------------------
   if (bounded) {
     unsigned mine = 0;
-    for (int i0 = s0; i0 < s1; i0 += 256) {  // eight columns a lane, in their order
-      const int i = i0 + lane * 8;
+#pragma unroll 2
+    for (int w0 = v0; w0 < v1; w0 += 32) {  // in the order of the columns
+      const int v = w0 + lane;
       unsigned hits = 0;
-      uint32_t k[8];
-      if (i < s1) {
-        if constexpr (sizeof(T) == 2) {
-          const uint4 u = *reinterpret_cast<const uint4*>(keys + i);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      uint32_t k[E];
+      sl.keys(v, v < v1, k);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            k[2 * j] = w[j] & 0xffffu;
-            k[2 * j + 1] = w[j] >> 16;
-          }
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(keys + i), v = *reinterpret_cast<const uint4*>(keys + i + 4);
-          k[0] = u.x, k[1] = u.y, k[2] = u.z, k[3] = u.w, k[4] = v.x, k[5] = v.y, k[6] = v.z, k[7] = v.w;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) hits |= (i + j < s1 && k[j] >= bound) ? 1u << j : 0u;
-      }
+      for (int j = 0; j < E; ++j) hits |= k[j] >= bound ? 1u << j : 0u;
       if (!__any_sync(kFull, hits)) continue;
       unsigned at = __popc(hits);
 #pragma unroll
@@ -835,9 +908,9 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
       const unsigned all = __shfl_sync(kFull, at, 31);
       at += mine - __popc(hits);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < E; ++j)
         if ((hits >> j) & 1) {
-          if (at < kPart) sh.weight[warp * kPart + at] = place_of(k[j], base + i + j);
+          if (at < kPart) sh.weight[warp * kPart + at] = place_of(k[j], base + v * E + j);
           ++at;
         }
       mine += all;
@@ -845,7 +918,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     if (lane == 0) sh.part[warp] = mine;
     if (ranks > 1) cl.sync();
     else __syncthreads();
-    const int parts = (int)ranks * kWarps;  // at most 8 * 16
+    const int parts = (int)ranks * kWarps;  // at most 16 * 16
     unsigned m = 0;
     if (tid < parts) m = ranks > 1 ? cl.map_shared_rank(sh.part, tid / kWarps)[tid % kWarps] : sh.part[tid];
     u64 total;
@@ -874,9 +947,12 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     if (ranks > 1) cl.sync();
   }
   if (d.V <= kList) {
-    for (int i = tid; i < n; i += TH) {
-      const uint32_t k = keys[i];
-      sh.list[i] = k > Key<T>::kNone ? place_of(k, i) : 0ull;
+    for (int v = tid; v < sl.nv; v += TH) {
+      uint32_t k[E];
+      sl.keys(v, true, k);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (v * E + j < n) sh.list[v * E + j] = k[j] > Key<T>::kNone ? place_of(k[j], v * E + j) : 0ull;
     }
     __syncthreads();
     draw_from_list<T>(bk, d, weigh, f, row, n);
@@ -884,7 +960,6 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   }
 
   // ---- otherwise: the last kept place by histograms over the cluster ----------------
-  const Slice<T, TH> sl{keys, n, base};
   u64 last = (u64)(Key<T>::kNone + 1) << 32;
   if (f.k > 0)
     last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, weigh, f.bins_per_unit);
@@ -892,13 +967,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, weigh,
                           f.bins_per_unit);
 
-  // ---- the draw: a warp's columns, then the threads of the CTA over that warp's ----
+  // ---- the draw: a warp's vectors, then the threads of the CTA over that warp's ----
+  last = last > f.min_place ? last : f.min_place;
   u64 sum = 0;
   unsigned cnt = 0;
-  sl.weighed(s0 + lane, s1, 32, last, weigh, [&](int, uint32_t, double z, u64 w) {
-    const bool keep = z >= f.zmin;
-    sum += keep ? w : 0;
-    cnt += keep;
+  sl.weighed(v0 + lane, v1, 32, last, weigh, [&](int, uint32_t, u64 w) {
+    sum += w;
+    ++cnt;
   });
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
@@ -913,38 +988,40 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   if (goal < run || goal >= run + mine) return;  // another CTA's
   int w = 0;
   while (goal >= run + sh.scan[w]) run += sh.scan[w++];
-  const int t0 = min(n, w * seg), t1 = min(n, t0 + seg), more = (t1 - t0 + TH - 1) / TH;
+  const int t0 = min(sl.nv, w * seg), t1 = min(sl.nv, t0 + seg), more = (t1 - t0 + TH - 1) / TH;
   const int a0 = min(t1, t0 + tid * more), a1 = min(t1, a0 + more);
   u64 own = 0, all;
-  sl.weighed(a0, a1, 1, last, weigh, [&](int, uint32_t, double z, u64 w) { own += z >= f.zmin ? w : 0; });
+  sl.weighed(a0, a1, 1, last, weigh, [&](int, uint32_t, u64 w) { own += w; });
   u64 at = run + bk.prefix(own, &all);
   if (goal < at || goal >= at + own) return;
-  sl.weighed(a0, a1, 1, last, weigh, [&](int i, uint32_t, double z, u64 w) {
-    if (!(z >= f.zmin)) return;
-    if (at <= goal && goal < at + w) answer(d, row, base + i, (int)count, z, total);
+  sl.weighed(a0, a1, 1, last, weigh, [&](int i, uint32_t k, u64 w) {
+    if (at <= goal && goal < at + w) answer(d, row, base + i, (int)count, weigh.z(Key<T>::value(k)), total);
     at += w;
   });
 }
 
 template <typename T, int TH>
 cudaError_t launch_t(const SampleRowsDesc& d, int n_rows, int ranks, cudaStream_t st) {
-  constexpr size_t key = sizeof(typename Key<T>::Stored);
-  const size_t smem = sizeof(Shared) + (size_t)d.per * key;
+  const size_t smem = sizeof(Shared) + (d.V <= kList ? kList * sizeof(T) : 0);
   static std::atomic<int> ready[kMaxDevices];
-  const cudaError_t e = once_per_device(ready, [] {
-    return cudaFuncSetAttribute(sample_rows_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(sizeof(Shared) + QTTS_SAMPLE_ROWS_MAX_V / 8 * key));
+  const cudaError_t set = once_per_device(ready, [] {
+    const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)(sizeof(Shared) + kList * sizeof(T)));
+    if (e != cudaSuccess) return e;
+    return cudaFuncSetAttribute(sample_rows_kernel<T, TH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   });
-  if (e != cudaSuccess) return e;
+  if (set != cudaSuccess) return set;
   return launch_k(sample_rows_kernel<T, TH>, dim3(n_rows, ranks), dim3(TH), smem, st,
                   LaunchOpts{true, (unsigned)ranks}, d);
 }
 template <typename T>
 cudaError_t launch(SampleRowsDesc d, int n_rows, int sms, cudaStream_t st) {
-  // A cluster's CTAs hold at most 32768 logits each; rows that do not fill the
-  // device are spread over more, down to 4096 logits a CTA.
+  // Rows that do not fill the device (two CTAs an SM) are spread over more
+  // CTAs, down to 4096 logits each; kMaxSlice keeps the histograms' words in
+  // 32 bits.
+  constexpr int kMaxSlice = 98304;
   int ranks = 1;
-  while (ranks < 8 && (d.V > ranks * 32768 || (d.V > ranks * 4096 && (long)n_rows * ranks < 2l * sms))) ranks *= 2;
+  while (ranks < 16 && (d.V > ranks * kMaxSlice || (d.V > ranks * 4096 && (long)n_rows * ranks <= sms))) ranks *= 2;
   d.per = ((d.V + ranks - 1) / ranks + 31) / 32 * 32;
   return d.V <= kList ? launch_t<T, 256>(d, n_rows, 1, st) : launch_t<T, 512>(d, n_rows, ranks, st);
 }
