@@ -51,51 +51,56 @@ struct SampleRowsDesc {
   float* logprob = nullptr;
 };
 
-// Order keys: larger for a larger logit, equal for the two zeros, at most kNone
-// for what is never drawn (NaN, -inf).  A 16-bit logit has a 16-bit key.
+// Order keys: larger for a larger logit, equal for the two zeros.  Those of NaN
+// lie above kInf or (sign bit set) below kNone, that of -inf is kNone: a row
+// with a key above kInf is read again with such keys set to 0, and what is at
+// most kNone is never drawn.  A 16-bit logit has a 16-bit key.
 template <typename T>
 struct Key {  // f16, bf16
-  static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  static constexpr uint32_t kNone = 0x8000u - kInf;
+  static constexpr uint32_t kInfBits = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  static constexpr uint32_t kInf = 0x8000u + kInfBits, kNone = 0x8000u - kInfBits;
   static __device__ __forceinline__ float value(uint32_t k) {
     const uint32_t bits = k >= 0x8000u ? k - 0x8000u : 0x8000u | (0x8000u - k);
     if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((uint16_t)bits));
     else return __uint_as_float(bits << 16);
   }
   static __device__ __forceinline__ uint32_t near(float l) {  // the key of the nearest T
-    uint32_t bits, unused = 0;
+    uint32_t bits;
     if constexpr (std::is_same<T, __half>::value) bits = __half_as_ushort(__float2half_rn(l));
     else bits = __bfloat16_as_ushort(__float2bfloat16_rn(l));
-    return of_word(bits, unused) & 0xffffu;
+    return of_word(bits) & 0xffffu;
   }
   // two logits' keys: 0x8000 + magnitude, or 0x8000 - magnitude
-  static __device__ __forceinline__ uint32_t of_word(uint32_t w, uint32_t& most) {
+  static __device__ __forceinline__ uint32_t of_word(uint32_t w) {
     const uint32_t sign = (w >> 15) & 0x00010001u;
-    uint32_t k = (w ^ (sign * 0x7fffu) ^ 0x80008000u) + sign;
-    if (__vmaxu2(k, 0x80008000u + kInf * 0x00010001u) != 0x80008000u + kInf * 0x00010001u) {  // a NaN
-      if ((k & 0xffffu) > 0x8000u + kInf) k &= 0xffff0000u;
-      if ((k >> 16) > 0x8000u + kInf) k &= 0xffffu;
-    }
-    most = __vmaxu2(most, k);
+    return (w ^ (sign * 0x7fffu) ^ 0x80008000u) + sign;
+  }
+  static __device__ __forceinline__ uint32_t without_nan(uint32_t k) {
+    if ((k & 0xffffu) > kInf) k &= 0xffff0000u;
+    if ((k >> 16) > kInf) k &= 0xffffu;
     return k;
   }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t largest(uint32_t w) { return max(w & 0xffffu, w >> 16); }
 };
 template <>
 struct Key<float> {
-  static constexpr uint32_t kNone = 0u;
+  static constexpr uint32_t kInf = 0xff800000u, kNone = 0x00800000u;
   static __device__ __forceinline__ float value(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+    return __uint_as_float(k >= 0x80000000u ? k - 0x80000000u : 0x80000000u | (0x80000000u - k));
   }
-  static __device__ __forceinline__ uint32_t near(float l) {
-    uint32_t unused = 0;
-    return of_word(__float_as_uint(l), unused);
+  static __device__ __forceinline__ uint32_t near(float l) { return of_word(__float_as_uint(l)); }
+  static __device__ __forceinline__ uint32_t of_word(uint32_t w) {  // 2^31 + magnitude, or 2^31 - magnitude
+    const int sign = (int)w >> 31;
+    return (uint32_t)(((int)(w & 0x7fffffffu) ^ sign) - sign) + 0x80000000u;
   }
-  static __device__ __forceinline__ uint32_t of_word(uint32_t bits, uint32_t& most) {
-    const float l = __uint_as_float(bits);
-    const uint32_t k = l > -INFINITY ? f32_order_key(l) : 0u;
-    most = max(most, k);
-    return k;
-  }
+  static __device__ __forceinline__ uint32_t without_nan(uint32_t k) { return k > kInf ? 0u : k; }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ uint32_t largest(uint32_t w) { return w; }
 };
 __device__ __forceinline__ u64 place_of(uint32_t key, int index) { return ((u64)key << 32) | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t key_in(u64 place) { return (uint32_t)(place >> 32); }
@@ -171,6 +176,7 @@ struct alignas(16) Shared {
   double exp2_32[32];
   u64 scan[32];
   unsigned scan32[32];
+  unsigned tally[2][2][32];
   u64 word[2];            // what this CTA tells the cluster
   unsigned key_word[2];
   unsigned part[32];      // tokens in this CTA's part of the list, by warp
@@ -531,7 +537,7 @@ struct Slice {
   static constexpr int E = 16 / sizeof(T);
   const T* src;
   int n, nv, base;  // columns, vectors, the first column's index
-  bool aligned;
+  bool aligned, nan;
   uint4* kept;      // shared memory, or null
 
   __device__ __forceinline__ uint4 raw(int v) const {
@@ -543,19 +549,20 @@ struct Slice {
         w[j] = v * E + j < n ? reinterpret_cast<const uint32_t*>(src)[v * E + j] : 0xff800000u;
       } else {
         const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-        const uint32_t none = 0x8000u | K::kInf;  // -inf behind the last column
+        const uint32_t none = 0x8000u | K::kInfBits;  // -inf behind the last column
         const int i = v * E + 2 * j;
         w[j] = (i < n ? h[i] : none) | ((i + 1 < n ? h[i + 1] : none) << 16);
       }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ uint4 to_keys(uint4 u, uint32_t (&most)[4]) const {
-    return make_uint4(K::of_word(u.x, most[0]), K::of_word(u.y, most[1]), K::of_word(u.z, most[2]),
-                      K::of_word(u.w, most[3]));
+  __device__ __forceinline__ uint4 to_keys(uint4 u) const {
+    u = make_uint4(K::of_word(u.x), K::of_word(u.y), K::of_word(u.z), K::of_word(u.w));
+    if (nan) u = make_uint4(K::without_nan(u.x), K::without_nan(u.y), K::without_nan(u.z), K::without_nan(u.w));
+    return u;
   }
-  // the first pass: the thread's largest key in each place of a vector
-  // (E == 8: two in a word)
+  // the first pass: the thread's largest key in each place of a vector (E == 8:
+  // two in a word)
   __device__ __forceinline__ void largest(uint32_t (&most)[4]) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) most[j] = 0;
@@ -567,16 +574,21 @@ struct Slice {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (v0 + j * TH < nv) {
-          u[j] = to_keys(u[j], most);
+          u[j] = to_keys(u[j]);
           if (kept) kept[v0 + j * TH] = u[j];
+          most[0] = K::larger(most[0], u[j].x);
+          most[1] = K::larger(most[1], u[j].y);
+          most[2] = K::larger(most[2], u[j].z);
+          most[3] = K::larger(most[3], u[j].w);
         }
     }
   }
-  // later passes: the keys of a vector (none where v is no vector)
-  __device__ __forceinline__ void keys(int v, bool is, uint32_t (&k)[E]) const {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    uint32_t most[4] = {0, 0, 0, 0};
-    if (is) u = kept ? kept[v] : to_keys(raw(v), most);
+  // later passes: the keys of a vector, in words
+  __device__ __forceinline__ uint4 words(int v) const { return kept ? kept[v] : to_keys(raw(v)); }
+  static __device__ __forceinline__ uint32_t largest_of(uint4 u) {
+    return K::largest(K::larger(K::larger(u.x, u.y), K::larger(u.z, u.w)));
+  }
+  static __device__ __forceinline__ void apart(uint4 u, uint32_t (&k)[E]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -594,7 +606,7 @@ struct Slice {
 #pragma unroll 2
     for (int v = threadIdx.x; v < nv; v += TH) {
       uint32_t k[E];
-      keys(v, true, k);
+      apart(words(v), k);
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (k[j] > K::kNone) f(k[j], place_of(k[j], base + v * E + j));
@@ -611,7 +623,7 @@ struct Slice {
 #pragma unroll 1
     for (int v = first; v < last; v += step) {
       uint32_t kk[E];
-      keys(v, true, kk);
+      apart(words(v), kk);
 #pragma unroll
       for (int h = 0; h < E; h += 4) {
         const uint32_t* k = kk + h;
@@ -749,19 +761,48 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
   }
 }
 
-// One warp: a bound that `each` of its keys v (N a lane) reach, and hardly more
-// (the low bits of a 32-bit key are left at 0); 1 above kNone if there are fewer.
+// The largest key, but for low bits of a 32-bit one left at 0, that at least
+// `each` of the CTA's keys v (N a thread) reach; 1 above kNone if there are
+// fewer.  Two bits a step, one barrier each.
+template <typename T, int TH, int N>
+__device__ __forceinline__ uint32_t bound_of(Block<TH>& bk, const uint32_t (&v)[N], unsigned each) {
+  constexpr int kTop = sizeof(T) == 4 ? 30 : 14, kLow = sizeof(T) == 4 ? 10 : 0;
+  uint32_t bound = 0;
+  int turn = 0;
+#pragma unroll 1
+  for (int b = kTop; b >= kLow; b -= 2, turn ^= 1) {
+    unsigned c[3] = {0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) c[q] += v[j] >= (bound | ((uint32_t)(q + 1) << b));
+    const unsigned ab = __reduce_add_sync(kFull, c[0] | c[1] << 16), cc = __reduce_add_sync(kFull, c[2]);
+    if (bk.lane == 0) {
+      bk.sh.tally[turn][0][bk.warp] = ab;
+      bk.sh.tally[turn][1][bk.warp] = cc;
+    }
+    __syncthreads();
+    const bool in = bk.lane < Block<TH>::kWarps;
+    const unsigned all = __reduce_add_sync(kFull, in ? bk.sh.tally[turn][0][bk.lane] : 0u);
+    const unsigned third = __reduce_add_sync(kFull, in ? bk.sh.tally[turn][1][bk.lane] : 0u);
+    const uint32_t q = third >= each ? 3 : (all >> 16) >= each ? 2 : (all & 0xffffu) >= each ? 1 : 0;
+    bound |= q << b;
+  }
+  return max(bound, Key<T>::kNone + 1);
+}
+
+// The same by one warp, without barriers, for its keys alone.
 template <typename T, int N>
-__device__ __forceinline__ uint32_t bound_of(const uint32_t (&v)[N], int each) {
-  constexpr int kTopBit = sizeof(T) == 4 ? 31 : 15, kLowBit = sizeof(T) == 4 ? 10 : 0;
+__device__ __forceinline__ uint32_t warp_bound_of(const uint32_t (&v)[N], unsigned each) {
+  constexpr int kTop = sizeof(T) == 4 ? 31 : 15, kLow = sizeof(T) == 4 ? 10 : 0;
   uint32_t bound = 0;
 #pragma unroll 1
-  for (int b = kTopBit; b >= kLowBit; --b) {
+  for (int b = kTop; b >= kLow; --b) {
     const uint32_t t = bound | (1u << b);
     unsigned c = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) c += v[j] >= t;
-    if (__reduce_add_sync(kFull, c) >= (unsigned)each) bound = t;
+    if (__reduce_add_sync(kFull, c) >= each) bound = t;
   }
   return max(bound, Key<T>::kNone + 1);
 }
@@ -783,7 +824,6 @@ template <typename T, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid_constant__ SampleRowsDesc d) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
-  static_assert(TH <= 512, "the bound takes 16 maxima a lane");
   if (threadIdx.x < 32) sh.exp2_32[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
   pdl_launch_dependents();
   pdl_wait();
@@ -812,59 +852,54 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   f.bins_per_unit = 32.0f / temp;
   const bool greedy = !(temp > 0.0f);
   // small top-k: the list is what lies above a bound
-  // (of the threads' maxima if they are four times as many, else of each warp's
-  // maxima in every place of the vectors, which needs fewer hits a warp)
-  const bool bounded = !greedy && f.k > 0 && f.k <= kList / 2;
-  const bool by_threads = f.k * 4 <= (int)ranks * TH;
-  const int sharers = by_threads ? ranks : ranks * kWarps, each = bounded ? (f.k + sharers - 1) / sharers : 0;
+  const bool bounded = !greedy && f.k > 0 && f.k <= kList / 2 && f.k * 4 <= (int)ranks * TH * E;
+  const unsigned each = bounded ? (f.k + ranks - 1) / ranks : 0;
+  // 256 rows of 2048, k = 50: 8.0 us with one warp and a maximum a thread, 10.5
+  // us with the whole CTA and all maxima, which a larger k needs
+  const bool by_warp = f.k * 4 <= (int)ranks * TH;
 
   // ---- the row, its largest key and the bound ----------------------------------------
-  uint32_t most[4];
-  sl.largest(most);
-  uint32_t bound = 0;
-  uint32_t my_key = max(max(most[0], most[1]), max(most[2], most[3]));
-  if constexpr (E == 8) {
-    my_key = 0;
-    uint32_t half[8];
+  uint32_t top = 0, bound = 0;
+  sl.nan = false;
+  for (;;) {
+    uint32_t most[4], maxima[E];
+    sl.largest(most);
+    sl.apart(make_uint4(most[0], most[1], most[2], most[3]), maxima);
+    top = bk.most32(sl.largest_of(make_uint4(most[0], most[1], most[2], most[3])));
+    if (bounded && by_warp) {
+      unsigned* own = reinterpret_cast<unsigned*>(sh.weight);
+      own[tid] = sl.largest_of(make_uint4(most[0], most[1], most[2], most[3]));
+      __syncthreads();
+      if (warp == 0) {
+        uint32_t v[kWarps];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      half[2 * j] = most[j] & 0xffffu;
-      half[2 * j + 1] = most[j] >> 16;
-      my_key = max(my_key, max(half[2 * j], half[2 * j + 1]));
+        for (int j = 0; j < kWarps; ++j) v[j] = own[j * 32 + lane];
+        bound = warp_bound_of<T>(v, each);
+      }
+      if (ranks == 1) {
+        if (tid == 0) sh.key_word[1] = bound;
+        __syncthreads();
+        bound = sh.key_word[1];
+      }
+    } else if (bounded) {
+      bound = bound_of<T, TH>(bk, maxima, each);
     }
-    if (bounded && !by_threads) bound = bound_of<T>(half, each);
-  } else {
-    if (bounded && !by_threads) bound = bound_of<T>(most, each);
-  }
-  unsigned* maxima = reinterpret_cast<unsigned*>(sh.weight);
-  maxima[tid] = my_key;
-  uint32_t top = bk.most32(my_key);
-  if (bounded && by_threads) {
-    if (warp == 0) {
-      uint32_t v[TH / 32];
-#pragma unroll
-      for (int j = 0; j < TH / 32; ++j) v[j] = maxima[j * 32 + lane];
-      bound = bound_of<T>(v, each);
+    if (ranks > 1) {
+      if (tid == 0) {
+        sh.key_word[0] = top;
+        sh.key_word[1] = bound;
+      }
+      cl.sync();
+      bound = ~0u;
+      for (unsigned r = 0; r < ranks; ++r) {
+        const unsigned* w = cl.map_shared_rank(sh.key_word, r);
+        top = max(top, w[0]);
+        bound = min(bound, w[1]);
+      }
     }
-  } else if (bounded) {
-    bound = ~bk.most32(~bound);  // the least of the warps'
-  }
-  if (ranks > 1) {
-    if (tid == 0) {
-      sh.key_word[0] = top;
-      sh.key_word[1] = bound;
-    }
-    cl.sync();
-    bound = ~0u;
-    for (unsigned r = 0; r < ranks; ++r) {
-      const unsigned* w = cl.map_shared_rank(sh.key_word, r);
-      top = max(top, w[0]);
-      bound = min(bound, w[1]);
-    }
-  } else {
-    if (tid == 0) sh.key_word[1] = bound;
-    __syncthreads();
-    bound = sh.key_word[1];
+    if (top <= Key<T>::kInf || sl.nan) break;
+    sl.nan = true;  // the same again without them
+    if (ranks > 1) cl.sync();
   }
   if (top <= Key<T>::kNone || greedy) {
     // the first column with the largest key
@@ -893,12 +928,14 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
 #pragma unroll 2
     for (int w0 = v0; w0 < v1; w0 += 32) {  // in the order of the columns
       const int v = w0 + lane;
-      unsigned hits = 0;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (v < v1) u = sl.words(v);
+      if (!__any_sync(kFull, sl.largest_of(u) >= bound)) continue;
       uint32_t k[E];
-      sl.keys(v, v < v1, k);
+      sl.apart(u, k);
+      unsigned hits = 0;
 #pragma unroll
       for (int j = 0; j < E; ++j) hits |= k[j] >= bound ? 1u << j : 0u;
-      if (!__any_sync(kFull, hits)) continue;
       unsigned at = __popc(hits);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -949,7 +986,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   if (d.V <= kList) {
     for (int v = tid; v < sl.nv; v += TH) {
       uint32_t k[E];
-      sl.keys(v, true, k);
+      sl.apart(sl.words(v), k);
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (v * E + j < n) sh.list[v * E + j] = k[j] > Key<T>::kNone ? place_of(k[j], v * E + j) : 0ull;
