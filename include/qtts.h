@@ -289,6 +289,7 @@ QTTS_API int qtts_q4_quantize(const float* data, int k, int n, uint8_t* packed, 
 #define QTTS_KV8_BAD_ROW 1    /* seq past n_seqs, or a position outside the sequence's pages */
 #define QTTS_KV8_BAD_PAGE 2   /* a page table entry outside [0, n_pages) */
 #define QTTS_KV8_ROPE_RANGE 4 /* a position outside the rotation tables (left unrotated) */
+#define QTTS_KV8_TIMEOUT 8    /* a bounded device wait (1 s) ran out: outputs undefined */
 typedef struct {
   int8_t* codes;
   float* scales;

@@ -5,58 +5,19 @@
 // [page][K|V][kv_head][16][head_dim], one f32 scale per [page][K|V][kv_head];
 // an element's value is code * scale.
 #include <cooperative_groups.h>
-#include <cuda_bf16.h>
 #include <float.h>
 
 #include <algorithm>
 
 #include "common.cuh"
 #include "engine.h"
-#include "kv8.h"
+#include "kv8.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace qtts {
 
 namespace {
-
-constexpr unsigned kFull = 0xffffffffu;
-
-// ---- four consecutive elements of a row --------------------------------------
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                     __uint_as_float(u.y & 0xffff0000u));
-}
-__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
-__device__ __forceinline__ void store4(__half* p, float4 v) {
-  *reinterpret_cast<uint2*>(p) =
-      make_uint2(half2_bits(__floats2half2_rn(v.x, v.y)), half2_bits(__floats2half2_rn(v.z, v.w)));
-}
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-  *reinterpret_cast<uint2*>(p) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
-
-__device__ __forceinline__ void raise(int* flags, int bit) {
-  if (flags) atomicOr(flags, bit);
-}
-
-// codes and scale of (page, K = 0 / V = 1, kv head)
-__device__ __forceinline__ int8_t* block_codes(const qtts_kv8_cache& c, int page, int which, int h) {
-  return c.codes + (size_t)page * c.page_stride + (size_t)(which * c.kv_heads + h) * kKv8Page * c.head_dim;
-}
-__device__ __forceinline__ float* block_scale(const qtts_kv8_cache& c, int page, int which, int h) {
-  return c.scales + (size_t)page * c.scale_stride + which * c.kv_heads + h;
-}
 
 // ---- append --------------------------------------------------------------------
 // A head's row of HD values lies on HD / 4 lanes, four consecutive values each,
@@ -312,21 +273,8 @@ __device__ __forceinline__ void limbs4(float4 v, float up, uint32_t& w0, uint32_
     w0 |= (uint32_t)(y & 255) << (8 * i);
   }
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// Two bytes of w ^ 0x80808080 (a code + 128) become the f16 pair 1024 + (code +
-// 128) by a byte permute onto 0x64; subtracting 1152 is exact.
-__device__ __forceinline__ uint32_t half2_of(uint32_t biased, uint32_t sel) {
-  uint32_t r = __byte_perm(biased, 0x64646464u, sel);
-  const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
-  return half2_bits(h);
-}
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) { split_pair(a, b, hi, lo); }
-
 constexpr int kSlots = 8;
+constexpr int kTileSlots = 32;  // query heads of a sequence's rows from which the tile kernel takes over
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -552,9 +500,7 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
           }
         // sv = fr * 2^ev; the output's running exponent follows score + ev, so
         // that the weights times sv stay within f16 whatever the scales are
-        const int svb = __float_as_int(sv), svx = (svb >> 23) & 255;
-        ev[k] = svx == 0 ? -126.0f : svx == 255 ? 0.0f : (float)(svx - 127);
-        fr[k] = svx == 0 ? sv * 0x1p126f : svx == 255 ? sv : __int_as_float((svb & 0x807fffff) | 0x3f800000);
+        split_scale(sv, ev[k], fr[k]);
       }
 #pragma unroll
       for (int k = 0; k < kStep; ++k) pm[k] = fmaxf(pm[k], __shfl_xor_sync(kFull, pm[k], 1));
@@ -585,7 +531,7 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
         for (int n = 0; n < 2; ++n) {
           const float a = ex2(s[k][n][0] - mz), b = ex2(s[k][n][1] - mz);
           l += a + b;
-          split_f16(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
+          split_pair(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
         }
         const uint8_t* vb = base + k * 2 * R::kBlock + R::kBlock;
         uint32_t vw[4][NT / 4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9, dims NT * g ...
@@ -760,6 +706,7 @@ cudaError_t launch_kv8_append(Kv8AppendDesc d, int dtype, int sms, cudaStream_t 
 
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st) {
   const int group = d.heads / d.c.kv_heads;
+  if ((long)max_rows * group >= kTileSlots) return launch_kv8_tile(d, dtype, max_rows, max_len, sms, st);
   d.unit_heads = std::min(group, kSlots);
   d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
   d.group_rows = std::max(1, std::min(max_rows, kSlots / d.unit_heads));

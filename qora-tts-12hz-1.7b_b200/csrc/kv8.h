@@ -77,5 +77,7 @@ struct Kv8AttnDesc {
   int unit_heads = 1;   // query heads of a unit
 };
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st);
+// The same for many rows: tiles of 128 slots on the tensor cores (kv8_tile.cu).
+cudaError_t launch_kv8_tile(Kv8AttnDesc d, int dtype, int max_rows, int len, int sms, cudaStream_t st);
 
 }  // namespace qtts

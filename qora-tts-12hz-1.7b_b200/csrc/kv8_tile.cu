@@ -1,0 +1,745 @@
+// kv8_tile.cu -- attention of many rows over the 8-bit paged cache (sm_100a):
+// chunks of a prompt, or every frame of an utterance.
+//
+// A CTA takes 128 slots (query heads of consecutive rows that share a K/V head)
+// and walks over the cache in tiles of 128 positions:
+//   S = Q K^T     tcgen05.mma, Q and K in shared memory, S (f32) in TMEM
+//   P = softmax   a thread per slot reads its row of S, keeps the running
+//                 maximum and sum, and writes P as f16 over S
+//   O += P V      tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
+// Four warps do the softmax, four turn the codes of the next tile into f16
+// operands (exact: a code has 8 bits), one issues the products.  Two CTAs an SM
+// fill each other's waits.
+//
+// Queries are scaled by a power of two to at most 2, which f16 holds exactly
+// for 16-bit types; f32 queries are split into f16 hi + lo, and so is P then
+// (rounding to 2^-25 of the largest), two products each and one CTA an SM.
+// The V scales are folded into P, relative to a running exponent of their own,
+// so that P stays within f16 whatever the scales are; O is rescaled only when
+// that exponent has grown by 6 (P then reaches 2^7).
+//
+// A tile of rows may span sequences: its segments (runs of rows of one
+// sequence) are taken one after the other, with the other slots masked.
+#include <cooperative_groups.h>
+#include <float.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "engine.h"
+#include "kv8.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace qtts {
+
+namespace {
+
+constexpr int kTileM = 128, kTileN = 128, kTilePages = kTileN / kKv8Page;
+constexpr int kSoft = 128, kConvert = 128;  // threads of the softmax and of the conversion
+constexpr int kTileThreads = kSoft + kConvert + 32;
+constexpr uint32_t kTmemCols = 256;  // S and P: 0..127, O: 128..
+constexpr unsigned long long kWaitNs = 1000000000ull;
+
+struct TileSegment {
+  int row0, rows, seq, lo, hi;  // rows of the tile, and the positions [lo, hi) that any of them sees
+};
+struct TileShared {
+  uint64_t k_full, v_full, s_full, p_full, o_full, fin;
+  uint32_t tmem;
+  int abort;
+  int n_segments;
+  int seq[kTileM], pos[kTileM];
+  TileSegment segment[kTileM];
+  float scale[2][kTilePages][4];  // K scale, exponent and fraction of the V scale, 1 if the page is there
+  float m[kTileM], l[kTileM];
+};
+
+template <typename T, int HD>
+struct TileCfg {
+  static constexpr bool kSplit = sizeof(T) == 4;
+  static constexpr int kHalf = kTileM * HD * 2;  // bytes of a 128-row f16 operand
+  static constexpr int kQ = 0, kK = kHalf * (kSplit ? 2 : 1), kV = kK + kHalf;
+  static constexpr int kOps = kV + kHalf;
+  static constexpr int kUsed = kOps + (int)sizeof(TileShared);
+  // per SM: two, and by shared memory never more, as TMEM holds two (a third
+  // would wait for it, and its cluster for the third)
+  static constexpr int kCtas = kSplit && HD == 128 ? 1 : 2;
+  static constexpr int kSmem = kUsed > 80 * 1024 ? kUsed : 80 * 1024;
+};
+
+// Operands have no swizzle, 16-byte core-matrix rows.  Q and K (K-major): row r,
+// 8-dim chunk c at (r/8) * 16 HD + c * 128 + (r%8) * 16.  V (MN-major): position
+// p, 8-dim group g at g * 2048 + (p/8) * 128 + (p%8) * 16.  In both the leading
+// offset is 128 bytes and a 16-deep step advances the start by 256.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t stride) {
+  return ((addr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) | (1ull << 46);
+}
+// kind::f16, D f32, A and B f16, A K-major
+__host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void commit_to(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_of(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bar_init(uint64_t* bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_of(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(bar)) : "memory");
+}
+// Waits for the phase, at most kWaitNs or until another thread has given up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity, int* abort) {
+  const uint32_t a = smem_of(bar);
+  unsigned long long t0 = 0;
+  for (unsigned it = 0;; ++it) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((it & 255u) == 255u) {
+      if (*reinterpret_cast<volatile int*>(abort)) return false;
+      unsigned long long t;
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > kWaitNs) {
+        *reinterpret_cast<volatile int*>(abort) = 1;
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void smem_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void store16(uint8_t* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(a, b, c, d);
+}
+// plain f16 hi + lo (lo unscaled: the values are at most 128)
+__device__ __forceinline__ uint32_t pack_half(float a, float b) { return half2_bits(__floats2half2_rn(a, b)); }
+__device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return pack_half(a - h.x, b - h.y);
+}
+
+// What the parts of a CTA share: its place in the work and its operands.
+template <typename T, int HD>
+struct TileJob {
+  using C = TileCfg<T, HD>;
+  const Kv8AttnDesc& d;
+  TileShared& sh;
+  uint8_t* ops;
+  int row0, rows, kvh, h0, nh, nsplit, split;
+  uint32_t tmem;
+
+  __device__ __forceinline__ void tiles(const TileSegment& g, int& p0, int& p1, int& t0, int& t1) const {
+    p0 = g.lo / kKv8Page;
+    p1 = (g.hi + kKv8Page - 1) / kKv8Page;
+    const int nt = g.hi > 0 && g.seq >= 0 ? (p1 - p0 + kTilePages - 1) / kTilePages : 0;
+    const int share = (nt + nsplit - 1) / nsplit;
+    t0 = min(nt, split * share);
+    t1 = min(nt, t0 + share);
+  }
+};
+
+// ---- codes to operands -----------------------------------------------------------
+template <typename T, int HD>
+struct Converter {
+  using J = TileJob<T, HD>;
+  static constexpr int N = HD / 16;  // 16-byte pieces of a thread, per operand
+  const J& job;
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  uint4 k[N], v[N];
+  int ids = -1;       // lanes 0..7: the tile's pages
+  float sk = 0.0f, sv = 0.0f;
+
+  __device__ explicit Converter(const J& j) : job(j) {}
+  // piece i: positions 8 at a time, dims 16 at a time
+  __device__ __forceinline__ int block_of(int i) const { return HD == 128 ? warp + 4 * (i >> 1) : warp + 4 * i; }
+  __device__ __forceinline__ int chunk_of(int i) const { return HD == 128 ? (lane >> 3) + 4 * (i & 1) : lane >> 3; }
+
+  __device__ __forceinline__ int pages(const int* table, int p0, int p1, int tile) {
+    const qtts_kv8_cache& c = job.d.c;
+    const int pg = p0 + tile * kTilePages + lane;
+    int id = -1;
+    if (lane < kTilePages && pg < p1) {
+      id = table[pg];
+      if (id < 0 || id >= c.n_pages) {
+        raise(job.d.flags, QTTS_KV8_BAD_PAGE);
+        id = -1;
+      }
+    }
+    return id;
+  }
+  __device__ __forceinline__ void fetch(int which, uint4 (&r)[N]) const {
+    const qtts_kv8_cache& c = job.d.c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int b = block_of(i), page = __shfl_sync(kFull, ids, b >> 1);
+      r[i] = make_uint4(0, 0, 0, 0);
+      if (page >= 0)
+        r[i] = *reinterpret_cast<const uint4*>(block_codes(c, page, which, job.kvh) + ((b & 1) * 8 + (lane & 7)) * HD +
+                                               chunk_of(i) * 16);
+    }
+  }
+  __device__ __forceinline__ void fetch_scales() {
+    sk = sv = 0.0f;
+    if (ids >= 0) {
+      sk = *block_scale(job.d.c, ids, 0, job.kvh);
+      sv = *block_scale(job.d.c, ids, 1, job.kvh);
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* p, int next, uint4 u) const {  // 16 dims: two core-matrix rows
+    const uint2 a = halves_of(u.x), b = halves_of(u.y), c = halves_of(u.z), d = halves_of(u.w);
+    store16(p, a.x, a.y, b.x, b.y);
+    store16(p + next, c.x, c.y, d.x, d.y);
+  }
+  __device__ __forceinline__ void put_k() const {
+    uint8_t* base = job.ops + J::C::kK;
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(base + block_of(i) * (16 * HD) + chunk_of(i) * 256 + (lane & 7) * 16, 128, k[i]);
+  }
+  __device__ __forceinline__ void put_v() const {
+    uint8_t* base = job.ops + J::C::kV;
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, v[i]);
+  }
+  // One segment; `it` counts the CTA's tiles.
+  __device__ bool run(const TileSegment& g, int& it) {
+    TileShared& sh = job.sh;
+    int p0, p1, t0, t1;
+    job.tiles(g, p0, p1, t0, t1);
+    if (t0 == t1) return true;
+    const int* table = job.d.c.page_table + (size_t)g.seq * job.d.c.pages_per_seq;
+    ids = pages(table, p0, p1, t0);
+    fetch(0, k);
+    fetch(1, v);
+    fetch_scales();
+    for (int t = t0; t < t1; ++t, ++it) {
+      const int next = t + 1 < t1 ? pages(table, p0, p1, t + 1) : -1;
+      if (it > 0 && !bar_wait(&sh.s_full, (it - 1) & 1, &sh.abort)) return false;
+      if (warp == 0 && lane < kTilePages) {
+        float ev, fr;
+        split_scale(sv, ev, fr);
+        float* s = sh.scale[it & 1][lane];
+        s[0] = sk;
+        s[1] = ev;
+        s[2] = fr;
+        s[3] = ids >= 0 ? 1.0f : 0.0f;
+      }
+      put_k();
+      smem_to_async();
+      bar_arrive(&sh.k_full);
+      ids = next;
+      if (t + 1 < t1) {
+        fetch(0, k);
+        fetch_scales();
+      }
+      if (it > 0 && !bar_wait(&sh.o_full, (it - 1) & 1, &sh.abort)) return false;
+      put_v();
+      smem_to_async();
+      bar_arrive(&sh.v_full);
+      if (t + 1 < t1) fetch(1, v);
+    }
+    return true;
+  }
+};
+
+// ---- the products ------------------------------------------------------------------
+template <typename T, int HD>
+__device__ bool issue_products(const TileJob<T, HD>& job, const TileSegment& g, int& it) {
+  using C = TileCfg<T, HD>;
+  TileShared& sh = job.sh;
+  constexpr uint32_t score = instruction(kTileN, false), value = instruction(HD, true);
+  const uint32_t q = smem_of(job.ops + C::kQ), k = smem_of(job.ops + C::kK), v = smem_of(job.ops + C::kV);
+  const uint32_t s = job.tmem, o = job.tmem + kTileN;
+  const bool one = (threadIdx.x & 31) == 0;
+  int p0, p1, t0, t1;
+  job.tiles(g, p0, p1, t0, t1);
+  for (int t = t0; t < t1; ++t, ++it) {
+    // P of the tile before lies where S goes
+    bool ok = it == 0 || bar_wait(&sh.o_full, (it - 1) & 1, &sh.abort);
+    ok = ok && bar_wait(&sh.k_full, it & 1, &sh.abort);
+    if (!__all_sync(kFull, ok)) return false;
+    if (one) {
+      tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e)
+        mma_ss(s, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), score, e > 0);
+      if (C::kSplit) {
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e)
+          mma_ss(s, operand(q + C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), score, true);
+      }
+      commit_to(&sh.s_full);
+      // a plain arrival besides the products' own: it passes on what the
+      // converters wrote (the scales) to who waits for S
+      bar_arrive(&sh.s_full);
+    }
+    __syncwarp();
+    ok = bar_wait(&sh.p_full, it & 1, &sh.abort);
+    ok = ok && bar_wait(&sh.v_full, it & 1, &sh.abort);
+    if (!__all_sync(kFull, ok)) return false;
+    if (one) {
+      tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < kTileN / 16; ++e) {
+        const uint32_t p = s + 32 * (e >> 1) + 8 * (e & 1);
+        mma_ts(o, p, operand(v + e * 256, 2048), value, t > t0 || e > 0);
+        if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), value, true);
+      }
+      commit_to(&sh.o_full);
+    }
+    __syncwarp();
+  }
+  return true;
+}
+
+// ---- softmax -----------------------------------------------------------------------
+template <typename T, int HD>
+struct Softmax {
+  using J = TileJob<T, HD>;
+  using C = TileCfg<T, HD>;
+  const J& job;
+  const int slot = threadIdx.x, row, head;
+  const uint32_t lanes = (uint32_t)(threadIdx.x & ~31) << 16;  // this warp's TMEM lanes
+  float qs = 0.0f;
+  float m, mo, l;
+  int see_lo, see_hi;
+
+  __device__ explicit Softmax(const J& j) : job(j), row((int)threadIdx.x / j.nh), head((int)threadIdx.x % j.nh) {}
+
+  // The slot's query as the operand's row, scaled by a power of two.
+  __device__ void put_query() {
+    const bool on = row < job.rows && job.sh.seq[row] >= 0;
+    const T* src = static_cast<const T*>(job.d.q) + (size_t)(job.row0 + (on ? row : 0)) * job.d.ldq +
+                   (size_t)(job.h0 + head) * HD;
+    float big = 0.0f;
+    bool finite = true;
+    if (on) {
+#pragma unroll 8
+      for (int c = 0; c < HD / 4; ++c) {
+        const float4 x = load4(src + 4 * c);
+        const float a = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        finite &= fabsf(x.x) <= FLT_MAX && fabsf(x.y) <= FLT_MAX && fabsf(x.z) <= FLT_MAX && fabsf(x.w) <= FLT_MAX;
+        big = fmaxf(big, a);
+      }
+    }
+    const bool use = on && finite;
+    const int ex = min(126, max(-120, ((__float_as_int(big) >> 23) & 255) - 127));
+    const float dn = ldexpf(1.0f, -ex);
+    qs = finite ? ldexpf(job.d.scale * 1.4426950408889634f, ex) : NAN;  // scores in units of log 2
+    uint8_t* dst = job.ops + C::kQ + (slot >> 3) * (16 * HD) + (slot & 7) * 16;
+#pragma unroll 4
+    for (int c = 0; c < HD / 8; ++c) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+      if (use) {
+        a = load4(src + 8 * c);
+        b = load4(src + 8 * c + 4);
+      }
+      a = make_float4(a.x * dn, a.y * dn, a.z * dn, a.w * dn);
+      b = make_float4(b.x * dn, b.y * dn, b.z * dn, b.w * dn);
+      const uint32_t h0 = pack_half(a.x, a.y), h1 = pack_half(a.z, a.w), h2 = pack_half(b.x, b.y), h3 = pack_half(b.z, b.w);
+      store16(dst + c * 128, h0, h1, h2, h3);
+      if (C::kSplit)
+        store16(dst + C::kHalf + c * 128, pack_rest(a.x, a.y, h0), pack_rest(a.z, a.w, h1), pack_rest(b.x, b.y, h2),
+                pack_rest(b.z, b.w, h3));
+    }
+  }
+
+  // One tile whose first position is `at`; MASK: some slot of the warp does not
+  // see all of it.
+  template <bool MASK>
+  __device__ __forceinline__ void tile(int at, const float (*sc)[4]) {
+    const uint32_t s = job.tmem + lanes, o = s + kTileN;
+    const unsigned width = (unsigned)(see_hi - see_lo), from = (unsigned)(at - see_lo);
+    float pm[kTilePages], f[kTilePages];
+#pragma unroll
+    for (int k = 0; k < kTilePages; ++k) {
+      f[k] = qs * sc[k][0];
+      pm[k] = -INFINITY;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float x[32];
+      tmem_load(s + 32 * c, x);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int k = 2 * c + (e >> 4);
+        float y = x[e] * f[k];
+        if (MASK && !(from + 32 * c + e < width && sc[k][3] != 0.0f)) y = -INFINITY;
+        pm[k] = fmaxf(pm[k], y);
+      }
+    }
+    float mn = m, mon = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kTilePages; ++k) {
+      mn = fmaxf(mn, pm[k]);
+      mon = fmaxf(mon, pm[k] + sc[k][1]);
+    }
+    // (mo of -inf: nothing is in O yet)
+    const bool grow = mon > mo + 6.0f, rescale = grow && mo > -INFINITY;
+    if (__any_sync(kFull, rescale)) {
+      const float beta = rescale ? ex2(mo - mon) : 1.0f;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        float x[32];
+        tmem_load(o + 32 * c, x);
+        uint32_t r[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(x[16 * h + e] * beta);
+          tmem_store16(o + 32 * c + 16 * h, r);
+        }
+      }
+    }
+    if (grow || mo == -INFINITY) mo = mon;
+    const float mz = mn == -INFINITY ? 0.0f : mn;
+    l *= ex2(m - mz);
+    m = mn;
+    float fac[kTilePages], part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kTilePages; ++k)
+      fac[k] = mo == -INFINITY ? 0.0f : ex2(fminf(mz - mo + sc[k][1], 120.0f)) * sc[k][2];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float x[32];
+      tmem_load(s + 32 * c, x);
+      uint32_t hi[16], lo[16];
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const int k = 2 * c + (e >> 4);
+        float p[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          p[j] = ex2(fmaf(x[e + j], f[k], -mz));
+          if (MASK && !(from + 32 * c + e + j < width && sc[k][3] != 0.0f)) p[j] = 0.0f;
+          part[(e + j) & 3] += p[j];
+          p[j] *= fac[k];
+        }
+        hi[e / 2] = pack_half(p[0], p[1]);
+        if (C::kSplit) lo[e / 2] = pack_rest(p[0], p[1], hi[e / 2]);
+      }
+      tmem_store16(s + 32 * c, hi);
+      if (C::kSplit) tmem_store16(s + 32 * c + 16, lo);
+    }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+
+  __device__ bool run(const TileSegment& g, int& it) {
+    TileShared& sh = job.sh;
+    int p0, p1, t0, t1;
+    job.tiles(g, p0, p1, t0, t1);
+    const bool mine = row >= g.row0 && row < g.row0 + g.rows;
+    see_hi = mine ? max(0, sh.pos[row] + 1) : 0;
+    see_lo = mine && job.d.window > 0 ? max(0, see_hi - job.d.window) : 0;
+    m = mo = -INFINITY;
+    l = 0.0f;
+    for (int t = t0; t < t1; ++t, ++it) {
+      const int at = (p0 + t * kTilePages) * kKv8Page;
+      if (!__all_sync(kFull, bar_wait(&sh.s_full, it & 1, &sh.abort))) return false;
+      tc_fence_after();
+      const float(*sc)[4] = sh.scale[it & 1];
+      bool pages = true;
+#pragma unroll
+      for (int k = 0; k < kTilePages; ++k) pages &= sc[k][3] != 0.0f;
+      // a slot of another segment has no say: its row is never read
+      const bool all = !mine || (see_lo <= at && see_hi >= at + kTileN);
+      if (pages && __all_sync(kFull, all)) tile<false>(at, sc);
+      else tile<true>(at, sc);
+      tmem_store_wait();
+      tc_fence_before();
+      bar_arrive(&sh.p_full);
+    }
+    if (t1 > t0) {
+      if (!__all_sync(kFull, bar_wait(&sh.o_full, (it - 1) & 1, &sh.abort))) return false;
+      tc_fence_after();
+    }
+    return true;
+  }
+
+  // O of the finished segment, relative to the maximum m: f(first dim, 32 values)
+  template <typename F>
+  __device__ __forceinline__ void output(bool any, F f) const {
+    const float back = m == -INFINITY || mo == -INFINITY ? 0.0f : ex2(mo - m);
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      float x[32];
+      if (any) {
+        tmem_load(job.tmem + lanes + kTileN + 32 * c, x);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] *= back;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+      }
+      f(32 * c, x);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_row(T* p, const float (&x)[32], float mul) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 4)
+    store4(p + e, make_float4(x[e] * mul, x[e + 1] * mul, x[e + 2] * mul, x[e + 3] * mul));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
+    kv8_tile_kernel(const __grid_constant__ Kv8AttnDesc d) {
+  using C = TileCfg<T, HD>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  TileShared& sh = *reinterpret_cast<TileShared*>(smem + C::kOps);
+  pdl_wait();
+  const qtts_kv8_cache& c = d.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int per = c.kv_heads * d.head_chunks, units = gridDim.x / per;
+  const int unit = units - 1 - (int)blockIdx.x / per, rest = blockIdx.x % per;  // the last rows see most: first
+  const int group = d.heads / c.kv_heads, hc = rest % d.head_chunks;
+  TileJob<T, HD> job{d, sh, smem};
+  job.kvh = rest / d.head_chunks;
+  job.h0 = job.kvh * group + hc * d.unit_heads;
+  job.nh = min(d.unit_heads, group - hc * d.unit_heads);
+  job.row0 = unit * d.group_rows;
+  job.rows = min(d.group_rows, d.n_rows - job.row0);
+  job.nsplit = gridDim.y;
+  job.split = blockIdx.y;
+  const int cap = c.pages_per_seq * kKv8Page;
+
+  // ---- rows, segments, barriers, TMEM, queries ------------------------------------
+  for (int i = tid; i < kTileM; i += kTileThreads) {
+    int seq = -1, pos = -1;
+    if (i < job.rows) {
+      seq = d.seq[job.row0 + i];
+      pos = d.pos[job.row0 + i];
+      if (seq >= 0 && (seq >= c.n_seqs || pos >= cap)) {
+        raise(d.flags, QTTS_KV8_BAD_ROW);
+        if (seq >= c.n_seqs) seq = -1;
+        pos = min(pos, cap - 1);
+      }
+    }
+    sh.seq[i] = seq;
+    sh.pos[i] = pos;
+    sh.segment[i] = TileSegment{0, 0, -1, 0x7fffffff, 0};
+  }
+  if (tid == 0) {
+    bar_init(&sh.k_full, kConvert);
+    bar_init(&sh.v_full, kConvert);
+    bar_init(&sh.s_full, 2);
+    bar_init(&sh.p_full, kSoft);
+    bar_init(&sh.o_full, 1);
+    bar_init(&sh.fin, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    sh.abort = 0;
+  }
+  if (warp == kTileThreads / 32 - 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&sh.tmem)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  __syncthreads();
+  if (warp == kTileThreads / 32 - 1) {  // runs of rows of one sequence
+    int n = 0;
+    for (int r0 = 0; r0 < job.rows; r0 += 32) {
+      const int r = r0 + lane;
+      const bool in = r < job.rows;
+      const bool start = in && (r == 0 || sh.seq[r] != sh.seq[r - 1]);
+      const unsigned starts = __ballot_sync(kFull, start);
+      const int g = n + __popc(starts & (kFull >> (31 - lane))) - 1;
+      if (start) {
+        sh.segment[g].row0 = r;
+        sh.segment[g].seq = sh.seq[r];
+      }
+      __syncwarp();
+      if (in) {
+        atomicAdd(&sh.segment[g].rows, 1);
+        const int p = sh.pos[r];
+        if (p >= 0) {
+          atomicMax(&sh.segment[g].hi, p + 1);
+          atomicMin(&sh.segment[g].lo, d.window > 0 ? max(0, p + 1 - d.window) : 0);
+        }
+      }
+      n += __popc(starts);
+      __syncwarp();
+    }
+    if (lane == 0) sh.n_segments = n;
+  }
+  Softmax<T, HD> soft(job);
+  if (tid < kSoft) {
+    soft.put_query();
+    smem_to_async();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  job.tmem = sh.tmem;
+
+  Converter<T, HD> conv(job);
+  bool ok = true;
+  int it = 0;
+  for (int g = 0; g < sh.n_segments; ++g) {
+    const TileSegment seg = sh.segment[g];
+    if (seg.seq < 0) continue;  // padding
+    if (ok) {
+      if (tid < kSoft) ok = soft.run(seg, it);
+      else if (tid < kSoft + kConvert) ok = conv.run(seg, it);
+      else ok = issue_products<T, HD>(job, seg, it);
+    }
+    const bool mine = tid < kSoft && soft.row >= seg.row0 && soft.row < seg.row0 + seg.rows;
+    int p0, p1, t0, t1;
+    job.tiles(seg, p0, p1, t0, t1);
+    if (job.nsplit == 1) {
+      if (tid < kSoft && ok) {
+        const size_t row = job.row0 + soft.row;
+        const int head = job.h0 + soft.head;
+        const bool none = soft.m == -INFINITY && soft.l == soft.l;
+        const float inv = none ? 0.0f : __fdiv_rn(1.0f, soft.l);
+        T* out = static_cast<T*>(d.out) + row * d.ldo + (size_t)head * HD;
+        soft.output(t1 > t0, [&](int e, const float(&x)[32]) {
+          if (mine) store_row(out + e, x, inv);
+        });
+        if (mine && d.lse)
+          d.lse[row * d.heads + head] = none ? -INFINITY : (soft.m + log2f(soft.l)) * 0.6931471805599453f;
+        tc_fence_before();
+      }
+      continue;
+    }
+    // join the splits of the cluster, in their order: O over the K and V operands
+    float* sums = reinterpret_cast<float*>(smem + C::kK);
+    __syncthreads();
+    if (tid < kSoft) {
+      soft.output(t1 > t0 && ok, [&](int e, const float(&x)[32]) { store_row(sums + soft.slot * HD + e, x, 1.0f); });
+      sh.m[tid] = soft.l == soft.l ? soft.m : INFINITY;  // a NaN sum makes the join NaN
+      sh.l[tid] = soft.l;
+      tc_fence_before();
+    }
+    cluster.sync();
+    const int first = seg.row0 * job.nh, n = seg.rows * job.nh * HD;
+    for (int i = tid + job.split * kTileThreads; i < n; i += job.nsplit * kTileThreads) {
+      const int s = first + i / HD, e = i % HD;
+      float mx = -INFINITY, sum = 0.0f, ll = 0.0f;
+      for (int r = 0; r < job.nsplit; ++r) {
+        const float rm = *cluster.map_shared_rank(&sh.m[s], r), rl = *cluster.map_shared_rank(&sh.l[s], r),
+                    ro = *cluster.map_shared_rank(&sums[s * HD + e], r);
+        const float mn = fmaxf(mx, rm);
+        if (mn == -INFINITY) continue;
+        const float a = ex2(mx - mn), b = ex2(rm - mn);
+        sum = sum * a + ro * b;
+        ll = ll * a + rl * b;
+        mx = mn;
+      }
+      const size_t row = job.row0 + s / job.nh;
+      const int head = job.h0 + s % job.nh;
+      const float v = mx == -INFINITY ? 0.0f : __fdiv_rn(sum, ll);
+      T* op = static_cast<T*>(d.out) + row * d.ldo + (size_t)head * HD + e;
+      if constexpr (sizeof(T) == 4) *op = v;
+      else *op = T(v);
+      if (e == 0 && d.lse)
+        d.lse[row * d.heads + head] = mx == -INFINITY ? -INFINITY : (mx + log2f(ll)) * 0.6931471805599453f;
+    }
+    cluster.sync();  // no CTA goes on while its sums are read
+  }
+  // A dependent kernel may start now: it could take TMEM that a CTA of this one
+  // still had to get, had it started before the allocation.
+  pdl_launch_dependents();
+  // every product is done (a wait that ran out leaves some in flight) before TMEM goes
+  __syncthreads();
+  if (tid == kTileThreads - 32) commit_to(&sh.fin);
+  if (warp == kTileThreads / 32 - 1) {
+    int plain = 0;
+    bar_wait(&sh.fin, 0, &plain);
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(job.tmem), "r"(kTmemCols));
+  }
+  if (tid == 0 && sh.abort) raise(d.flags, QTTS_KV8_TIMEOUT);
+}
+
+template <typename T, int HD>
+cudaError_t launch_tile_t(const Kv8AttnDesc& d, long units, int len, int sms, cudaStream_t st) {
+  using C = TileCfg<T, HD>;
+  static std::atomic<int> ready[kMaxDevices];
+  const cudaError_t set = once_per_device(ready, [] {
+    return cudaFuncSetAttribute(kv8_tile_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  if (set != cudaSuccess) return set;
+  // the cache is split while the CTAs do not fill the device and keep two tiles
+  unsigned ns = 1;
+  const int tiles = (len + kTileN - 1) / kTileN;
+  while (ns < 8 && units * ns * 2 <= (long)C::kCtas * sms && tiles >= (int)ns * 4) ns *= 2;
+  return launch_k(kv8_tile_kernel<T, HD>, dim3((unsigned)units, ns), dim3(kTileThreads), (size_t)C::kSmem, st,
+                  LaunchOpts{true, ns}, d);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_tile(Kv8AttnDesc d, int dtype, int max_rows, int len, int sms, cudaStream_t st) {
+  const int group = d.heads / d.c.kv_heads;
+  d.unit_heads = std::min(group, kTileM);
+  d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
+  // rows of a tile: what 128 slots hold, or a sequence's rows in equal shares
+  const int most = kTileM / d.unit_heads, parts = (max_rows + most - 1) / most;
+  d.group_rows = std::min(most, (max_rows + parts - 1) / parts);
+  const long units = ((long)d.n_rows + d.group_rows - 1) / d.group_rows * d.c.kv_heads * d.head_chunks;
+  const bool w = d.c.head_dim == 128;
+  switch (dtype) {
+    case DT_F16:
+      return w ? launch_tile_t<__half, 128>(d, units, len, sms, st) : launch_tile_t<__half, 64>(d, units, len, sms, st);
+    case DT_BF16:
+      return w ? launch_tile_t<__nv_bfloat16, 128>(d, units, len, sms, st)
+               : launch_tile_t<__nv_bfloat16, 64>(d, units, len, sms, st);
+    default:
+      return w ? launch_tile_t<float, 128>(d, units, len, sms, st) : launch_tile_t<float, 64>(d, units, len, sms, st);
+  }
+}
+
+}  // namespace qtts

@@ -500,7 +500,7 @@ def expf_dev(x_ptr, y_ptr, n, stream=0):
 
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2}  # qtts.h QTTS_F32 / QTTS_F16 / QTTS_BF16
 KV8_PAGE = 16  # positions per page
-KV8_BAD_ROW, KV8_BAD_PAGE, KV8_ROPE_RANGE = 1, 2, 4  # bits of the flags word
+KV8_BAD_ROW, KV8_BAD_PAGE, KV8_ROPE_RANGE, KV8_TIMEOUT = 1, 2, 4, 8  # bits of the flags word
 SAMPLE_ROWS_MAX_V = 262144
 
 
