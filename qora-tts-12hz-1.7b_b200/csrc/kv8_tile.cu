@@ -8,8 +8,8 @@
 //                 maximum and sum, and writes P as f16 over S
 //   O += P V      tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
 // Four warps do the softmax, four turn the codes of the next tile into f16
-// operands (exact: a code has 8 bits), one issues the products.  Two CTAs an SM
-// fill each other's waits.
+// operands (exact: a code has 8 bits), and the first of these issues the
+// products.  Two CTAs an SM fill each other's waits.
 //
 // Queries are scaled by a power of two to at most 2, which f16 holds exactly
 // for 16-bit types; f32 queries are split into f16 hi + lo, and so is P then
@@ -37,7 +37,7 @@ namespace {
 
 constexpr int kTileM = 128, kTileN = 128, kTilePages = kTileN / kKv8Page;
 constexpr int kSoft = 128, kConvert = 128;  // threads of the softmax and of the conversion
-constexpr int kTileThreads = kSoft + kConvert + 32;
+constexpr int kTileThreads = kSoft + kConvert;
 constexpr uint32_t kTmemCols = 256;  // S and P: 0..127, O: 128..
 constexpr unsigned long long kWaitNs = 1000000000ull;
 
@@ -52,6 +52,7 @@ struct TileShared {
   int seq[kTileM], pos[kTileM];
   TileSegment segment[kTileM];
   float scale[2][kTilePages][4];  // K scale, exponent and fraction of the V scale, 1 if the page is there
+  float log_v[2][kTilePages];     // log2 of the V scale; NaN keeps a page from the short way (Softmax::tile)
   float m[kTileM], l[kTileM];
 };
 
@@ -132,6 +133,10 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity, int* ab
     }
   }
 }
+// The same for a warp as one, so that it stays together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, int* abort) {
+  return __all_sync(kFull, bar_wait(bar, parity, abort));
+}
 __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
   uint32_t r[32];
   asm volatile(
@@ -146,6 +151,44 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
       : "memory");
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+// 64 columns: two loads, one wait
+__device__ __forceinline__ void tmem_load64(uint32_t addr, float (&v)[64]) {
+  uint32_t r[64];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t* q = r + 32 * h;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]),
+          "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]), "=r"(q[16]),
+          "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]), "=r"(q[24]),
+          "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+        : "r"(addr + 32 * h)
+        : "memory");
+  }
+  // the wait takes the registers through it, so that no use moves above it
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t* q = r + 32 * h;
+    if (h == 0)
+      asm volatile("tcgen05.wait::ld.sync.aligned;"
+                   : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
+                     "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]),
+                     "+r"(q[16]), "+r"(q[17]), "+r"(q[18]), "+r"(q[19]), "+r"(q[20]), "+r"(q[21]), "+r"(q[22]),
+                     "+r"(q[23]), "+r"(q[24]), "+r"(q[25]), "+r"(q[26]), "+r"(q[27]), "+r"(q[28]), "+r"(q[29]),
+                     "+r"(q[30]), "+r"(q[31])::"memory");
+    else
+      asm volatile(""
+                   : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
+                     "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]),
+                     "+r"(q[16]), "+r"(q[17]), "+r"(q[18]), "+r"(q[19]), "+r"(q[20]), "+r"(q[21]), "+r"(q[22]),
+                     "+r"(q[23]), "+r"(q[24]), "+r"(q[25]), "+r"(q[26]), "+r"(q[27]), "+r"(q[28]), "+r"(q[29]),
+                     "+r"(q[30]), "+r"(q[31])::"memory");
+  }
+#pragma unroll
+  for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j]);
 }
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -251,6 +294,49 @@ struct Converter {
 #pragma unroll
     for (int i = 0; i < N; ++i) put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, v[i]);
   }
+  // Issues S = Q K^T of tile `it`, once its K is there.
+  __device__ __forceinline__ bool score(int it) const {
+    TileShared& sh = job.sh;
+    constexpr uint32_t idesc = instruction(kTileN, false);
+    if (!warp_wait(&sh.k_full, it & 1, &sh.abort)) return false;
+    if (lane == 0) {
+      const uint32_t q = smem_of(job.ops + J::C::kQ), k = smem_of(job.ops + J::C::kK);
+      tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e)
+        mma_ss(job.tmem, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, e > 0);
+      if (J::C::kSplit) {
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e)
+          mma_ss(job.tmem, operand(q + J::C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, true);
+      }
+      commit_to(&sh.s_full);
+      // a plain arrival besides the products' own: it passes on what the
+      // converters wrote (the scales) to who waits for S
+      bar_arrive(&sh.s_full);
+    }
+    __syncwarp();
+    return true;
+  }
+  // Issues O += P V of tile `it`, once its P and V are there.
+  __device__ __forceinline__ bool weigh(int it, bool first) const {
+    TileShared& sh = job.sh;
+    constexpr uint32_t idesc = instruction(HD, true);
+    if (!warp_wait(&sh.v_full, it & 1, &sh.abort) || !warp_wait(&sh.p_full, it & 1, &sh.abort)) return false;
+    if (lane == 0) {
+      const uint32_t v = smem_of(job.ops + J::C::kV), o = job.tmem + kTileN;
+      tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < kTileN / 16; ++e) {
+        const uint32_t p = job.tmem + 32 * (e >> 1) + 8 * (e & 1);
+        mma_ts(o, p, operand(v + e * 256, 2048), idesc, !first || e > 0);
+        if (J::C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
+      }
+      commit_to(&sh.o_full);
+    }
+    __syncwarp();
+    return true;
+  }
   // One segment; `it` counts the CTA's tiles.
   __device__ bool run(const TileSegment& g, int& it) {
     TileShared& sh = job.sh;
@@ -264,8 +350,8 @@ struct Converter {
     fetch_scales();
     for (int t = t0; t < t1; ++t, ++it) {
       const int next = t + 1 < t1 ? pages(table, p0, p1, t + 1) : -1;
-      if (it > 0 && !bar_wait(&sh.s_full, (it - 1) & 1, &sh.abort)) return false;
-      if (warp == 0 && lane < kTilePages) {
+      if (it > 0 && !warp_wait(&sh.s_full, (it - 1) & 1, &sh.abort)) return false;  // K is free
+      if (warp == 1 && lane < kTilePages) {
         float ev, fr;
         split_scale(sv, ev, fr);
         float* s = sh.scale[it & 1][lane];
@@ -273,6 +359,7 @@ struct Converter {
         s[1] = ev;
         s[2] = fr;
         s[3] = ids >= 0 ? 1.0f : 0.0f;
+        sh.log_v[it & 1][lane] = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX ? log2f(sv) : NAN;
       }
       put_k();
       smem_to_async();
@@ -282,67 +369,106 @@ struct Converter {
         fetch(0, k);
         fetch_scales();
       }
-      if (it > 0 && !bar_wait(&sh.o_full, (it - 1) & 1, &sh.abort)) return false;
+      // the products of the tile before, then this one's scores: P of the tile
+      // before lies where S goes
+      if (warp == 0 && t > t0 && !weigh(it - 1, t - 1 == t0)) return false;
+      if (it > 0 && !warp_wait(&sh.o_full, (it - 1) & 1, &sh.abort)) return false;  // V (and S) is free
+      if (warp == 0 && !score(it)) return false;
       put_v();
       smem_to_async();
       bar_arrive(&sh.v_full);
       if (t + 1 < t1) fetch(1, v);
     }
-    return true;
+    return warp != 0 || weigh(it - 1, t1 - 1 == t0);
   }
 };
 
-// ---- the products ------------------------------------------------------------------
-template <typename T, int HD>
-__device__ bool issue_products(const TileJob<T, HD>& job, const TileSegment& g, int& it) {
-  using C = TileCfg<T, HD>;
-  TileShared& sh = job.sh;
-  constexpr uint32_t score = instruction(kTileN, false), value = instruction(HD, true);
-  const uint32_t q = smem_of(job.ops + C::kQ), k = smem_of(job.ops + C::kK), v = smem_of(job.ops + C::kV);
-  const uint32_t s = job.tmem, o = job.tmem + kTileN;
-  const bool one = (threadIdx.x & 31) == 0;
-  int p0, p1, t0, t1;
-  job.tiles(g, p0, p1, t0, t1);
-  for (int t = t0; t < t1; ++t, ++it) {
-    // P of the tile before lies where S goes
-    bool ok = it == 0 || bar_wait(&sh.o_full, (it - 1) & 1, &sh.abort);
-    ok = ok && bar_wait(&sh.k_full, it & 1, &sh.abort);
-    if (!__all_sync(kFull, ok)) return false;
-    if (one) {
-      tc_fence_after();
+// ---- softmax -----------------------------------------------------------------------
+struct Running {
+  float m, mo, l;  // largest score, exponent of O, sum of exp2(score - m)
+};
+
+// The running exponent of O follows max(score + exponent of the V scale); O is
+// rescaled when it has grown by 6.  (mo of -inf: nothing is in O yet.)
+template <int HD>
+__device__ __forceinline__ void grow_to(float mon, float& mo, uint32_t o) {
+  const bool grow = mon > mo + 6.0f, rescale = grow && mo > -INFINITY;
+  if (__any_sync(kFull, rescale)) {
+    const float beta = rescale ? ex2(mo - mon) : 1.0f;
+#pragma unroll 1
+    for (int c = 0; c < HD / 32; ++c) {
+      float x[32];
+      tmem_load(o + 32 * c, x);
+      uint32_t r[16];
 #pragma unroll
-      for (int e = 0; e < HD / 16; ++e)
-        mma_ss(s, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), score, e > 0);
-      if (C::kSplit) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int e = 0; e < HD / 16; ++e)
-          mma_ss(s, operand(q + C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), score, true);
+        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(x[16 * h + e] * beta);
+        tmem_store16(o + 32 * c + 16 * h, r);
       }
-      commit_to(&sh.s_full);
-      // a plain arrival besides the products' own: it passes on what the
-      // converters wrote (the scales) to who waits for S
-      bar_arrive(&sh.s_full);
     }
-    __syncwarp();
-    ok = bar_wait(&sh.p_full, it & 1, &sh.abort);
-    ok = ok && bar_wait(&sh.v_full, it & 1, &sh.abort);
-    if (!__all_sync(kFull, ok)) return false;
-    if (one) {
-      tc_fence_after();
-#pragma unroll
-      for (int e = 0; e < kTileN / 16; ++e) {
-        const uint32_t p = s + 32 * (e >> 1) + 8 * (e & 1);
-        mma_ts(o, p, operand(v + e * 256, 2048), value, t > t0 || e > 0);
-        if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), value, true);
-      }
-      commit_to(&sh.o_full);
-    }
-    __syncwarp();
   }
-  return true;
+  if (grow || mo == -INFINITY) mo = mon;
 }
 
-// ---- softmax -----------------------------------------------------------------------
+// Any tile: S at columns s (this warp's lanes), of which this slot sees positions
+// from .. from + width relative to its first.
+template <int HD, bool SPLIT>
+__device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, unsigned width, float qs,
+                                          const float (*sc)[4]) {
+  float mn = r.m, mon = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float x[32];
+    tmem_load(s + 32 * c, x);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float* k = sc[2 * c + q];
+      const float f = qs * k[0];
+      float pm = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (from + 32 * c + 16 * q + e < width) pm = fmaxf(pm, x[16 * q + e] * f);
+      if (k[3] != 0.0f) {
+        mn = fmaxf(mn, pm);
+        mon = fmaxf(mon, pm + k[1]);
+      }
+    }
+  }
+  grow_to<HD>(mon, r.mo, s + kTileN);
+  const float mz = mn == -INFINITY ? 0.0f : mn;
+  r.l *= ex2(r.m - mz);
+  r.m = mn;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float x[32];
+    tmem_load(s + 32 * c, x);
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float* k = sc[2 * c + q];
+      const float f = qs * k[0];
+      const float fac = r.mo == -INFINITY ? 0.0f : ex2(fminf(mz - r.mo + k[1], 120.0f)) * k[2];
+      const unsigned at = k[3] != 0.0f ? from + 32 * c + 16 * q : 0x80000000u;  // (no width reaches it)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float p[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          p[j] = at + e + j < width ? ex2(fmaf(x[16 * q + e + j], f, -mz)) : 0.0f;
+          r.l += p[j];
+          p[j] *= fac;
+        }
+        hi[8 * q + e / 2] = pack_half(p[0], p[1]);
+        if (SPLIT) lo[8 * q + e / 2] = pack_rest(p[0], p[1], hi[8 * q + e / 2]);
+      }
+    }
+    tmem_store16(s + 32 * c, hi);
+    if (SPLIT) tmem_store16(s + 32 * c + 16, lo);
+  }
+  return r;
+}
+
 template <typename T, int HD>
 struct Softmax {
   using J = TileJob<T, HD>;
@@ -394,84 +520,71 @@ struct Softmax {
     }
   }
 
-  // One tile whose first position is `at`; MASK: some slot of the warp does not
-  // see all of it.
-  template <bool MASK>
-  __device__ __forceinline__ void tile(int at, const float (*sc)[4]) {
-    const uint32_t s = job.tmem + lanes, o = s + kTileN;
-    const unsigned width = (unsigned)(see_hi - see_lo), from = (unsigned)(at - see_lo);
-    float pm[kTilePages], f[kTilePages];
+  // One tile that every slot of the warp sees in whole, of pages with ordinary
+  // scales: the weights times the V scale come straight from the exponential,
+  // exp2(score + log2 sv - mo), and the sum l from their sum per page.  False if
+  // the exponents are too far apart for that (nothing is done then).
+  __device__ __forceinline__ bool tile_short(const float (*sc)[4], const float* log_v) {
+    const uint32_t s = job.tmem + lanes;
+    float pm[kTilePages];
 #pragma unroll
-    for (int k = 0; k < kTilePages; ++k) {
-      f[k] = qs * sc[k][0];
-      pm[k] = -INFINITY;
-    }
+    for (int c = 0; c < 2; ++c) {
+      float x[64];
+      tmem_load64(s + 64 * c, x);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float x[32];
-      tmem_load(s + 32 * c, x);
+      for (int k = 0; k < 4; ++k) {
+        float a = fmaxf(x[16 * k], x[16 * k + 1]), b = fmaxf(x[16 * k + 2], x[16 * k + 3]);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int k = 2 * c + (e >> 4);
-        float y = x[e] * f[k];
-        if (MASK && !(from + 32 * c + e < width && sc[k][3] != 0.0f)) y = -INFINITY;
-        pm[k] = fmaxf(pm[k], y);
+        for (int e = 4; e < 16; e += 4) {
+          a = fmaxf(fmaxf(a, x[16 * k + e]), x[16 * k + e + 1]);
+          b = fmaxf(fmaxf(b, x[16 * k + e + 2]), x[16 * k + e + 3]);
+        }
+        pm[4 * c + k] = fmaxf(a, b);
       }
     }
     float mn = m, mon = -INFINITY;
+    bool near = qs >= 0.0f;  // (a negative or NaN scale goes the long way)
 #pragma unroll
     for (int k = 0; k < kTilePages; ++k) {
-      mn = fmaxf(mn, pm[k]);
-      mon = fmaxf(mon, pm[k] + sc[k][1]);
+      const float y = pm[k] * (qs * sc[k][0]);
+      mn = fmaxf(mn, y);
+      mon = fmaxf(mon, y + sc[k][1]);
+      near &= y - mn > -1000.0f;
     }
-    // (mo of -inf: nothing is in O yet)
-    const bool grow = mon > mo + 6.0f, rescale = grow && mo > -INFINITY;
-    if (__any_sync(kFull, rescale)) {
-      const float beta = rescale ? ex2(mo - mon) : 1.0f;
-#pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        float x[32];
-        tmem_load(o + 32 * c, x);
-        uint32_t r[16];
+    const float mo_new = mon > mo + 6.0f || mo == -INFINITY ? mon : mo;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(x[16 * h + e] * beta);
-          tmem_store16(o + 32 * c + 16 * h, r);
-        }
-      }
-    }
-    if (grow || mo == -INFINITY) mo = mon;
-    const float mz = mn == -INFINITY ? 0.0f : mn;
-    l *= ex2(m - mz);
+    for (int k = 0; k < kTilePages; ++k) near &= fabsf(mn + log_v[k] - mo_new) < 40.0f;
+    if (!__all_sync(kFull, near)) return false;
+    grow_to<HD>(mon, mo, s + kTileN);
+    l *= ex2(m - mn);
     m = mn;
-    float fac[kTilePages], part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kTilePages; ++k)
-      fac[k] = mo == -INFINITY ? 0.0f : ex2(fminf(mz - mo + sc[k][1], 120.0f)) * sc[k][2];
+    for (int c = 0; c < 2; ++c) {
+      float x[64];
+      tmem_load64(s + 64 * c, x);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float x[32];
-      tmem_load(s + 32 * c, x);
-      uint32_t hi[16], lo[16];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hi[16], lo[16];
 #pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        const int k = 2 * c + (e >> 4);
-        float p[2];
+        for (int q = 0; q < 2; ++q) {
+          const int k = 4 * c + 2 * h + q;
+          const float f = qs * sc[k][0], off = log_v[k] - mo;
+          float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          p[j] = ex2(fmaf(x[e + j], f[k], -mz));
-          if (MASK && !(from + 32 * c + e + j < width && sc[k][3] != 0.0f)) p[j] = 0.0f;
-          part[(e + j) & 3] += p[j];
-          p[j] *= fac[k];
+          for (int e = 0; e < 16; e += 2) {
+            const float p0 = ex2(fmaf(x[32 * h + 16 * q + e], f, off)), p1 = ex2(fmaf(x[32 * h + 16 * q + e + 1], f, off));
+            sum0 += p0;
+            sum1 += p1;
+            hi[8 * q + e / 2] = pack_half(p0, p1);
+            if (C::kSplit) lo[8 * q + e / 2] = pack_rest(p0, p1, hi[8 * q + e / 2]);
+          }
+          l = fmaf(sum0 + sum1, ex2(-off - m), l);
         }
-        hi[e / 2] = pack_half(p[0], p[1]);
-        if (C::kSplit) lo[e / 2] = pack_rest(p[0], p[1], hi[e / 2]);
+        tmem_store16(s + 64 * c + 32 * h, hi);
+        if (C::kSplit) tmem_store16(s + 64 * c + 32 * h + 16, lo);
       }
-      tmem_store16(s + 32 * c, hi);
-      if (C::kSplit) tmem_store16(s + 32 * c + 16, lo);
     }
-    l += (part[0] + part[1]) + (part[2] + part[3]);
+    return true;
   }
 
   __device__ bool run(const TileSegment& g, int& it) {
@@ -485,22 +598,28 @@ struct Softmax {
     l = 0.0f;
     for (int t = t0; t < t1; ++t, ++it) {
       const int at = (p0 + t * kTilePages) * kKv8Page;
-      if (!__all_sync(kFull, bar_wait(&sh.s_full, it & 1, &sh.abort))) return false;
+      if (!warp_wait(&sh.s_full, it & 1, &sh.abort)) return false;
       tc_fence_after();
       const float(*sc)[4] = sh.scale[it & 1];
-      bool pages = true;
+      const float* log_v = sh.log_v[it & 1];
+      bool plain = true;
 #pragma unroll
-      for (int k = 0; k < kTilePages; ++k) pages &= sc[k][3] != 0.0f;
+      for (int k = 0; k < kTilePages; ++k) plain &= log_v[k] == log_v[k];
       // a slot of another segment has no say: its row is never read
       const bool all = !mine || (see_lo <= at && see_hi >= at + kTileN);
-      if (pages && __all_sync(kFull, all)) tile<false>(at, sc);
-      else tile<true>(at, sc);
+      if (!(plain && __all_sync(kFull, all)) || !tile_short(sc, log_v)) {
+        const Running r = tile_long<HD, C::kSplit>(Running{m, mo, l}, job.tmem + lanes, (unsigned)(at - see_lo),
+                                                   (unsigned)(see_hi - see_lo), qs, sc);
+        m = r.m;
+        mo = r.mo;
+        l = r.l;
+      }
       tmem_store_wait();
       tc_fence_before();
       bar_arrive(&sh.p_full);
     }
     if (t1 > t0) {
-      if (!__all_sync(kFull, bar_wait(&sh.o_full, (it - 1) & 1, &sh.abort))) return false;
+      if (!warp_wait(&sh.o_full, (it - 1) & 1, &sh.abort)) return false;
       tc_fence_after();
     }
     return true;
@@ -582,13 +701,13 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.abort = 0;
   }
-  if (warp == kTileThreads / 32 - 1) {
+  if (warp == kSoft / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&sh.tmem)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   __syncthreads();
-  if (warp == kTileThreads / 32 - 1) {  // runs of rows of one sequence
+  if (warp == kSoft / 32) {  // runs of rows of one sequence
     int n = 0;
     for (int r0 = 0; r0 < job.rows; r0 += 32) {
       const int r = r0 + lane;
@@ -632,8 +751,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
     if (seg.seq < 0) continue;  // padding
     if (ok) {
       if (tid < kSoft) ok = soft.run(seg, it);
-      else if (tid < kSoft + kConvert) ok = conv.run(seg, it);
-      else ok = issue_products<T, HD>(job, seg, it);
+      else ok = conv.run(seg, it);
     }
     const bool mine = tid < kSoft && soft.row >= seg.row0 && soft.row < seg.row0 + seg.rows;
     int p0, p1, t0, t1;
@@ -694,8 +812,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
   pdl_launch_dependents();
   // every product is done (a wait that ran out leaves some in flight) before TMEM goes
   __syncthreads();
-  if (tid == kTileThreads - 32) commit_to(&sh.fin);
-  if (warp == kTileThreads / 32 - 1) {
+  if (tid == kSoft) commit_to(&sh.fin);
+  if (warp == kSoft / 32) {
     int plain = 0;
     bar_wait(&sh.fin, 0, &plain);
     tc_fence_after();
