@@ -75,6 +75,7 @@ struct Kv8AttnDesc {
   int group_rows = 1;   // rows of one unit
   int head_chunks = 1;  // units along the query heads of one K/V head
   int unit_heads = 1;   // query heads of a unit
+  int halves = 1;       // tile kernel: halves of 128 slots of a unit
 };
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st);
 // The same for many rows: tiles of 128 slots on the tensor cores (kv8_tile.cu).

@@ -1,19 +1,20 @@
 // kv8_tile.cu -- attention of many rows over the 8-bit paged cache (sm_100a):
 // chunks of a prompt, or every frame of an utterance.
 //
-// A CTA takes 128 slots (query heads of consecutive rows that share a K/V head)
-// and walks over the cache in tiles of 128 positions:
+// A CTA takes one or two halves of 128 slots (query heads of consecutive rows
+// that share a K/V head) and walks over the cache in tiles of 128 positions:
 //   S = Q K^T     tcgen05.mma, Q and K in shared memory, S (f32) in TMEM
 //   P = softmax   a thread per slot reads its row of S, keeps the running
 //                 maximum and sum, and writes P as f16 over S
 //   O += P V      tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
-// Four warps do the softmax, four turn the codes of the next tile into f16
-// operands (exact: a code has 8 bits), and the first of these issues the
-// products.  Two CTAs an SM fill each other's waits.
+// Four warps a half do the softmax, four turn codes into f16 operands (exact: a
+// code has 8 bits), up to two tiles ahead, and one issues the products: those of
+// one half run while the other half is in its softmax.
 //
 // Queries are scaled by a power of two to at most 2, which f16 holds exactly
 // for 16-bit types; f32 queries are split into f16 hi + lo, and so is P then
-// (rounding to 2^-25 of the largest), two products each and one CTA an SM.
+// (rounding to 2^-25 of the largest), two products each; the two operands of a
+// split query take the room of two halves, so that f32 has one half.
 // The V scales are folded into P, relative to a running exponent of their own,
 // so that P stays within f16 whatever the scales are; O is rescaled only when
 // that exponent has grown by 6 (P then reaches 2^7).
@@ -36,37 +37,39 @@ namespace qtts {
 namespace {
 
 constexpr int kTileM = 128, kTileN = 128, kTilePages = kTileN / kKv8Page;
-constexpr int kSoft = 128, kConvert = 128;  // threads of the softmax and of the conversion
-constexpr int kTileThreads = kSoft + kConvert;
-constexpr uint32_t kTmemCols = 256;  // S and P: 0..127, O: 128..
+constexpr int kSoft = 256, kConvert = 128;  // threads of the softmax (two halves) and of the conversion
+constexpr int kTileThreads = kSoft + kConvert + 32;
+constexpr uint32_t kTmemCols = 512;  // half h: S and P at 256 h, O at 256 h + 128
 constexpr unsigned long long kWaitNs = 1000000000ull;
+constexpr int kScales = 4;  // tiles of scales kept: a half may be two tiles behind the conversion
 
 struct TileSegment {
-  int row0, rows, seq, lo, hi;  // rows of the tile, and the positions [lo, hi) that any of them sees
+  int row0, rows, seq, lo, hi;  // rows of the unit, and the positions [lo, hi) that any of them sees
 };
 struct TileShared {
-  uint64_t k_full, v_full, s_full, p_full, o_full, fin;
+  uint64_t k_full[2], k_free[2], v_full[2], v_free[2];  // by buffer
+  uint64_t s_full[2], p_full[2], o_full[2];             // by half
+  uint64_t fin;
   uint32_t tmem;
   int abort;
   int n_segments;
-  int seq[kTileM], pos[kTileM];
-  TileSegment segment[kTileM];
-  float scale[2][kTilePages][4];  // K scale, exponent and fraction of the V scale, 1 if the page is there
-  float log_v[2][kTilePages];     // log2 of the V scale; NaN keeps a page from the short way (Softmax::tile)
-  float m[kTileM], l[kTileM];
+  int seq[2 * kTileM], pos[2 * kTileM];
+  TileSegment segment[2 * kTileM];
+  // K scale, exponent and fraction of the V scale (-1: no page), and log2 of the
+  // V scale; NaN keeps a page from the short way (Softmax::tile_short)
+  float4 scale[kScales][kTilePages];
+  float m[2 * kTileM], l[2 * kTileM];
 };
 
 template <typename T, int HD>
 struct TileCfg {
   static constexpr bool kSplit = sizeof(T) == 4;
   static constexpr int kHalf = kTileM * HD * 2;  // bytes of a 128-row f16 operand
-  static constexpr int kQ = 0, kK = kHalf * (kSplit ? 2 : 1), kV = kK + kHalf;
-  static constexpr int kOps = kV + kHalf;
+  static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + 2 * kHalf, kOps = kV + 2 * kHalf;
   static constexpr int kUsed = kOps + (int)sizeof(TileShared);
-  // per SM: two, and by shared memory never more, as TMEM holds two (a third
-  // would wait for it, and its cluster for the third)
-  static constexpr int kCtas = kSplit && HD == 128 ? 1 : 2;
-  static constexpr int kSmem = kUsed > 80 * 1024 ? kUsed : 80 * 1024;
+  // One CTA an SM, as it takes all of TMEM (a second would wait for it, and its
+  // cluster for the second).
+  static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
 };
 
 // Operands have no swizzle, 16-byte core-matrix rows.  Q and K (K-major): row r,
@@ -152,44 +155,6 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
 }
-// 64 columns: two loads, one wait
-__device__ __forceinline__ void tmem_load64(uint32_t addr, float (&v)[64]) {
-  uint32_t r[64];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t* q = r + 32 * h;
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]),
-          "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]), "=r"(q[16]),
-          "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]), "=r"(q[24]),
-          "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
-        : "r"(addr + 32 * h)
-        : "memory");
-  }
-  // the wait takes the registers through it, so that no use moves above it
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t* q = r + 32 * h;
-    if (h == 0)
-      asm volatile("tcgen05.wait::ld.sync.aligned;"
-                   : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
-                     "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]),
-                     "+r"(q[16]), "+r"(q[17]), "+r"(q[18]), "+r"(q[19]), "+r"(q[20]), "+r"(q[21]), "+r"(q[22]),
-                     "+r"(q[23]), "+r"(q[24]), "+r"(q[25]), "+r"(q[26]), "+r"(q[27]), "+r"(q[28]), "+r"(q[29]),
-                     "+r"(q[30]), "+r"(q[31])::"memory");
-    else
-      asm volatile(""
-                   : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
-                     "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]),
-                     "+r"(q[16]), "+r"(q[17]), "+r"(q[18]), "+r"(q[19]), "+r"(q[20]), "+r"(q[21]), "+r"(q[22]),
-                     "+r"(q[23]), "+r"(q[24]), "+r"(q[25]), "+r"(q[26]), "+r"(q[27]), "+r"(q[28]), "+r"(q[29]),
-                     "+r"(q[30]), "+r"(q[31])::"memory");
-  }
-#pragma unroll
-  for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j]);
-}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -219,7 +184,7 @@ struct TileJob {
   const Kv8AttnDesc& d;
   TileShared& sh;
   uint8_t* ops;
-  int row0, rows, kvh, h0, nh, nsplit, split;
+  int row0, rows, kvh, h0, nh, nsplit, split, halves;
   uint32_t tmem;
 
   __device__ __forceinline__ void tiles(const TileSegment& g, int& p0, int& p1, int& t0, int& t1) const {
@@ -229,6 +194,10 @@ struct TileJob {
     const int share = (nt + nsplit - 1) / nsplit;
     t0 = min(nt, split * share);
     t1 = min(nt, t0 + share);
+  }
+  // whether half h holds rows of the segment
+  __device__ __forceinline__ bool takes(const TileSegment& g, int h) const {
+    return h < halves && g.row0 * nh < (h + 1) * kTileM && (g.row0 + g.rows) * nh > h * kTileM;
   }
 };
 
@@ -284,58 +253,15 @@ struct Converter {
     store16(p, a.x, a.y, b.x, b.y);
     store16(p + next, c.x, c.y, d.x, d.y);
   }
-  __device__ __forceinline__ void put_k() const {
-    uint8_t* base = job.ops + J::C::kK;
+  __device__ __forceinline__ void put_k(int b) const {
+    uint8_t* base = job.ops + J::C::kK + b * J::C::kHalf;
 #pragma unroll
     for (int i = 0; i < N; ++i) put(base + block_of(i) * (16 * HD) + chunk_of(i) * 256 + (lane & 7) * 16, 128, k[i]);
   }
-  __device__ __forceinline__ void put_v() const {
-    uint8_t* base = job.ops + J::C::kV;
+  __device__ __forceinline__ void put_v(int b) const {
+    uint8_t* base = job.ops + J::C::kV + b * J::C::kHalf;
 #pragma unroll
     for (int i = 0; i < N; ++i) put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, v[i]);
-  }
-  // Issues S = Q K^T of tile `it`, once its K is there.
-  __device__ __forceinline__ bool score(int it) const {
-    TileShared& sh = job.sh;
-    constexpr uint32_t idesc = instruction(kTileN, false);
-    if (!warp_wait(&sh.k_full, it & 1, &sh.abort)) return false;
-    if (lane == 0) {
-      const uint32_t q = smem_of(job.ops + J::C::kQ), k = smem_of(job.ops + J::C::kK);
-      tc_fence_after();
-#pragma unroll
-      for (int e = 0; e < HD / 16; ++e)
-        mma_ss(job.tmem, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, e > 0);
-      if (J::C::kSplit) {
-#pragma unroll
-        for (int e = 0; e < HD / 16; ++e)
-          mma_ss(job.tmem, operand(q + J::C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, true);
-      }
-      commit_to(&sh.s_full);
-      // a plain arrival besides the products' own: it passes on what the
-      // converters wrote (the scales) to who waits for S
-      bar_arrive(&sh.s_full);
-    }
-    __syncwarp();
-    return true;
-  }
-  // Issues O += P V of tile `it`, once its P and V are there.
-  __device__ __forceinline__ bool weigh(int it, bool first) const {
-    TileShared& sh = job.sh;
-    constexpr uint32_t idesc = instruction(HD, true);
-    if (!warp_wait(&sh.v_full, it & 1, &sh.abort) || !warp_wait(&sh.p_full, it & 1, &sh.abort)) return false;
-    if (lane == 0) {
-      const uint32_t v = smem_of(job.ops + J::C::kV), o = job.tmem + kTileN;
-      tc_fence_after();
-#pragma unroll
-      for (int e = 0; e < kTileN / 16; ++e) {
-        const uint32_t p = job.tmem + 32 * (e >> 1) + 8 * (e & 1);
-        mma_ts(o, p, operand(v + e * 256, 2048), idesc, !first || e > 0);
-        if (J::C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
-      }
-      commit_to(&sh.o_full);
-    }
-    __syncwarp();
-    return true;
   }
   // One segment; `it` counts the CTA's tiles.
   __device__ bool run(const TileSegment& g, int& it) {
@@ -348,38 +274,112 @@ struct Converter {
     fetch(0, k);
     fetch(1, v);
     fetch_scales();
+    int next = t0 + 1 < t1 ? pages(table, p0, p1, t0 + 1) : -1;
     for (int t = t0; t < t1; ++t, ++it) {
-      const int next = t + 1 < t1 ? pages(table, p0, p1, t + 1) : -1;
-      if (it > 0 && !warp_wait(&sh.s_full, (it - 1) & 1, &sh.abort)) return false;  // K is free
-      if (warp == 1 && lane < kTilePages) {
+      const int b = it & 1;
+      const unsigned before = (unsigned)((it >> 1) - 1) & 1u;  // the buffer's last use
+      if (it > 1 && !warp_wait(&sh.k_free[b], before, &sh.abort)) return false;
+      if (warp == 0 && lane < kTilePages) {
         float ev, fr;
         split_scale(sv, ev, fr);
-        float* s = sh.scale[it & 1][lane];
-        s[0] = sk;
-        s[1] = ev;
-        s[2] = fr;
-        s[3] = ids >= 0 ? 1.0f : 0.0f;
-        sh.log_v[it & 1][lane] = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX ? log2f(sv) : NAN;
+        const bool plain = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX;
+        sh.scale[it % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : -1.0f, plain ? log2f(sv) : NAN);
       }
-      put_k();
+      put_k(b);
       smem_to_async();
-      bar_arrive(&sh.k_full);
+      bar_arrive(&sh.k_full[b]);
       ids = next;
       if (t + 1 < t1) {
         fetch(0, k);
         fetch_scales();
       }
-      // the products of the tile before, then this one's scores: P of the tile
-      // before lies where S goes
-      if (warp == 0 && t > t0 && !weigh(it - 1, t - 1 == t0)) return false;
-      if (it > 0 && !warp_wait(&sh.o_full, (it - 1) & 1, &sh.abort)) return false;  // V (and S) is free
-      if (warp == 0 && !score(it)) return false;
-      put_v();
+      next = t + 2 < t1 ? pages(table, p0, p1, t + 2) : -1;
+      if (it > 1 && !warp_wait(&sh.v_free[b], before, &sh.abort)) return false;
+      put_v(b);
       smem_to_async();
-      bar_arrive(&sh.v_full);
+      bar_arrive(&sh.v_full[b]);
       if (t + 1 < t1) fetch(1, v);
     }
-    return warp != 0 || weigh(it - 1, t1 - 1 == t0);
+    return true;
+  }
+};
+
+// ---- the products ------------------------------------------------------------------
+template <typename T, int HD>
+struct Products {
+  using J = TileJob<T, HD>;
+  using C = TileCfg<T, HD>;
+  const J& job;
+  const int lane = threadIdx.x & 31;
+  int done[2] = {0, 0};  // tiles of each half
+
+  __device__ explicit Products(const J& j) : job(j) {}
+  // S = Q K^T of half h with K of buffer b; last: no other half reads K after it
+  __device__ __forceinline__ bool score(int h, int b, bool last) {
+    TileShared& sh = job.sh;
+    constexpr uint32_t idesc = instruction(kTileN, false);
+    // P of the half's tile before lies where S goes
+    if (done[h] > 0 && !warp_wait(&sh.o_full[h], (done[h] - 1) & 1, &sh.abort)) return false;
+    if (lane == 0) {
+      const uint32_t q = smem_of(job.ops + C::kQ) + h * C::kHalf, k = smem_of(job.ops + C::kK) + b * C::kHalf;
+      const uint32_t s = job.tmem + 256 * h;
+      tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e)
+        mma_ss(s, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, e > 0);
+      if (C::kSplit) {
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e)
+          mma_ss(s, operand(q + C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, true);
+      }
+      commit_to(&sh.s_full[h]);
+      if (last) commit_to(&sh.k_free[b]);
+      // a plain arrival besides the products' own: it passes on what the
+      // converters wrote (the scales) to who waits for S
+      bar_arrive(&sh.s_full[h]);
+    }
+    __syncwarp();
+    return true;
+  }
+  // O += P V of half h with V of buffer b
+  __device__ __forceinline__ bool weigh(int h, int b, bool first, bool last) {
+    TileShared& sh = job.sh;
+    constexpr uint32_t idesc = instruction(HD, true);
+    if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
+    if (lane == 0) {
+      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h, o = s + kTileN;
+      tc_fence_after();
+#pragma unroll
+      for (int e = 0; e < kTileN / 16; ++e) {
+        const uint32_t p = s + 32 * (e >> 1) + 8 * (e & 1);
+        mma_ts(o, p, operand(v + e * 256, 2048), idesc, !first || e > 0);
+        if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
+      }
+      commit_to(&sh.o_full[h]);
+      if (last) commit_to(&sh.v_free[b]);
+    }
+    __syncwarp();
+    ++done[h];
+    return true;
+  }
+  __device__ bool run(const TileSegment& g, int& it) {
+    TileShared& sh = job.sh;
+    int p0, p1, t0, t1;
+    job.tiles(g, p0, p1, t0, t1);
+    const bool one = job.takes(g, 0), two = job.takes(g, 1);
+    // half 1 is half a tile behind half 0: while one is in its softmax the
+    // other's products run
+    for (int t = t0; t < t1; ++t, ++it) {
+      const int b = it & 1, before = (it - 1) & 1;
+      const unsigned use = (unsigned)(it >> 1) & 1u;
+      if (!warp_wait(&sh.k_full[b], use, &sh.abort)) return false;
+      if (one && !score(0, b, !two)) return false;
+      if (two && t > t0 && !weigh(1, before, t - 1 == t0, true)) return false;
+      if (two && !score(1, b, true)) return false;
+      if (!warp_wait(&sh.v_full[b], use, &sh.abort)) return false;
+      if (one && !weigh(0, b, t == t0, !two)) return false;
+    }
+    return !two || t0 == t1 || weigh(1, (it - 1) & 1, t1 - 1 == t0, true);
   }
 };
 
@@ -415,7 +415,7 @@ __device__ __forceinline__ void grow_to(float mon, float& mo, uint32_t o) {
 // from .. from + width relative to its first.
 template <int HD, bool SPLIT>
 __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, unsigned width, float qs,
-                                          const float (*sc)[4]) {
+                                          const float4* sc) {
   float mn = r.m, mon = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
@@ -423,15 +423,15 @@ __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, 
     tmem_load(s + 32 * c, x);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const float* k = sc[2 * c + q];
-      const float f = qs * k[0];
+      const float4 k = sc[2 * c + q];
+      const float f = qs * k.x;
       float pm = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (from + 32 * c + 16 * q + e < width) pm = fmaxf(pm, x[16 * q + e] * f);
-      if (k[3] != 0.0f) {
+      if (k.z != -1.0f) {
         mn = fmaxf(mn, pm);
-        mon = fmaxf(mon, pm + k[1]);
+        mon = fmaxf(mon, pm + k.y);
       }
     }
   }
@@ -446,10 +446,10 @@ __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, 
     uint32_t hi[16], lo[16];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const float* k = sc[2 * c + q];
-      const float f = qs * k[0];
-      const float fac = r.mo == -INFINITY ? 0.0f : ex2(fminf(mz - r.mo + k[1], 120.0f)) * k[2];
-      const unsigned at = k[3] != 0.0f ? from + 32 * c + 16 * q : 0x80000000u;  // (no width reaches it)
+      const float4 k = sc[2 * c + q];
+      const float f = qs * k.x;
+      const float fac = r.mo == -INFINITY ? 0.0f : ex2(fminf(mz - r.mo + k.y, 120.0f)) * k.z;
+      const unsigned at = k.z != -1.0f ? from + 32 * c + 16 * q : 0x80000000u;  // (no width reaches it)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         float p[2];
@@ -474,13 +474,16 @@ struct Softmax {
   using J = TileJob<T, HD>;
   using C = TileCfg<T, HD>;
   const J& job;
-  const int slot = threadIdx.x, row, head;
-  const uint32_t lanes = (uint32_t)(threadIdx.x & ~31) << 16;  // this warp's TMEM lanes
+  const int half = threadIdx.x >> 7, slot = threadIdx.x, row, head;
   float qs = 0.0f;
   float m, mo, l;
   int see_lo, see_hi;
+  int done = 0;  // tiles of this half
 
   __device__ explicit Softmax(const J& j) : job(j), row((int)threadIdx.x / j.nh), head((int)threadIdx.x % j.nh) {}
+  __device__ __forceinline__ uint32_t columns() const {
+    return job.tmem + 256 * half + ((threadIdx.x & 96u) << 16);
+  }
 
   // The slot's query as the operand's row, scaled by a power of two.
   __device__ void put_query() {
@@ -502,7 +505,7 @@ struct Softmax {
     const int ex = min(126, max(-120, ((__float_as_int(big) >> 23) & 255) - 127));
     const float dn = ldexpf(1.0f, -ex);
     qs = finite ? ldexpf(job.d.scale * 1.4426950408889634f, ex) : NAN;  // scores in units of log 2
-    uint8_t* dst = job.ops + C::kQ + (slot >> 3) * (16 * HD) + (slot & 7) * 16;
+    uint8_t* dst = job.ops + C::kQ + half * C::kHalf + ((slot & 127) >> 3) * (16 * HD) + (slot & 7) * 16;
 #pragma unroll 4
     for (int c = 0; c < HD / 8; ++c) {
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
@@ -524,65 +527,64 @@ struct Softmax {
   // scales: the weights times the V scale come straight from the exponential,
   // exp2(score + log2 sv - mo), and the sum l from their sum per page.  False if
   // the exponents are too far apart for that (nothing is done then).
-  __device__ __forceinline__ bool tile_short(const float (*sc)[4], const float* log_v) {
-    const uint32_t s = job.tmem + lanes;
-    float pm[kTilePages];
+  __device__ __forceinline__ bool tile_short(const float4* sc) {
+    const uint32_t s = columns();
+    float pm[kTilePages], f[kTilePages], log_v[kTilePages];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float x[64];
-      tmem_load64(s + 64 * c, x);
+    for (int c = 0; c < 4; ++c) {
+      float x[32];
+      tmem_load(s + 32 * c, x);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         float a = fmaxf(x[16 * k], x[16 * k + 1]), b = fmaxf(x[16 * k + 2], x[16 * k + 3]);
 #pragma unroll
         for (int e = 4; e < 16; e += 4) {
           a = fmaxf(fmaxf(a, x[16 * k + e]), x[16 * k + e + 1]);
           b = fmaxf(fmaxf(b, x[16 * k + e + 2]), x[16 * k + e + 3]);
         }
-        pm[4 * c + k] = fmaxf(a, b);
+        pm[2 * c + k] = fmaxf(a, b);
       }
     }
     float mn = m, mon = -INFINITY;
     bool near = qs >= 0.0f;  // (a negative or NaN scale goes the long way)
 #pragma unroll
     for (int k = 0; k < kTilePages; ++k) {
-      const float y = pm[k] * (qs * sc[k][0]);
+      const float4 z = sc[k];
+      f[k] = qs * z.x;
+      log_v[k] = z.w;
+      const float y = pm[k] * f[k];
       mn = fmaxf(mn, y);
-      mon = fmaxf(mon, y + sc[k][1]);
-      near &= y - mn > -1000.0f;
+      mon = fmaxf(mon, y + z.y);
     }
     const float mo_new = mon > mo + 6.0f || mo == -INFINITY ? mon : mo;
 #pragma unroll
-    for (int k = 0; k < kTilePages; ++k) near &= fabsf(mn + log_v[k] - mo_new) < 40.0f;
+    for (int k = 0; k < kTilePages; ++k) near &= fabsf(mn + log_v[k] - mo_new) < 40.0f;  // (false for NaN)
     if (!__all_sync(kFull, near)) return false;
     grow_to<HD>(mon, mo, s + kTileN);
     l *= ex2(m - mn);
     m = mn;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float x[64];
-      tmem_load64(s + 64 * c, x);
+    for (int c = 0; c < 4; ++c) {
+      float x[32];
+      tmem_load(s + 32 * c, x);
+      uint32_t hi[16], lo[16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t hi[16], lo[16];
+      for (int q = 0; q < 2; ++q) {
+        const int k = 2 * c + q;
+        const float off = log_v[k] - mo;
+        float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int k = 4 * c + 2 * h + q;
-          const float f = qs * sc[k][0], off = log_v[k] - mo;
-          float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float p0 = ex2(fmaf(x[32 * h + 16 * q + e], f, off)), p1 = ex2(fmaf(x[32 * h + 16 * q + e + 1], f, off));
-            sum0 += p0;
-            sum1 += p1;
-            hi[8 * q + e / 2] = pack_half(p0, p1);
-            if (C::kSplit) lo[8 * q + e / 2] = pack_rest(p0, p1, hi[8 * q + e / 2]);
-          }
-          l = fmaf(sum0 + sum1, ex2(-off - m), l);
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = ex2(fmaf(x[16 * q + e], f[k], off)), p1 = ex2(fmaf(x[16 * q + e + 1], f[k], off));
+          sum0 += p0;
+          sum1 += p1;
+          hi[8 * q + e / 2] = pack_half(p0, p1);
+          if (C::kSplit) lo[8 * q + e / 2] = pack_rest(p0, p1, hi[8 * q + e / 2]);
         }
-        tmem_store16(s + 64 * c + 32 * h, hi);
-        if (C::kSplit) tmem_store16(s + 64 * c + 32 * h + 16, lo);
+        l = fmaf(sum0 + sum1, ex2(-off - m), l);
       }
+      tmem_store16(s + 32 * c, hi);
+      if (C::kSplit) tmem_store16(s + 32 * c + 16, lo);
     }
     return true;
   }
@@ -596,19 +598,19 @@ struct Softmax {
     see_lo = mine && job.d.window > 0 ? max(0, see_hi - job.d.window) : 0;
     m = mo = -INFINITY;
     l = 0.0f;
-    for (int t = t0; t < t1; ++t, ++it) {
+    if (!job.takes(g, half)) {
+      it += t1 - t0;
+      return true;
+    }
+    for (int t = t0; t < t1; ++t, ++it, ++done) {
       const int at = (p0 + t * kTilePages) * kKv8Page;
-      if (!warp_wait(&sh.s_full, it & 1, &sh.abort)) return false;
+      if (!warp_wait(&sh.s_full[half], done & 1, &sh.abort)) return false;
       tc_fence_after();
-      const float(*sc)[4] = sh.scale[it & 1];
-      const float* log_v = sh.log_v[it & 1];
-      bool plain = true;
-#pragma unroll
-      for (int k = 0; k < kTilePages; ++k) plain &= log_v[k] == log_v[k];
+      const float4* sc = sh.scale[it % kScales];
       // a slot of another segment has no say: its row is never read
       const bool all = !mine || (see_lo <= at && see_hi >= at + kTileN);
-      if (!(plain && __all_sync(kFull, all)) || !tile_short(sc, log_v)) {
-        const Running r = tile_long<HD, C::kSplit>(Running{m, mo, l}, job.tmem + lanes, (unsigned)(at - see_lo),
+      if (!__all_sync(kFull, all) || !tile_short(sc)) {
+        const Running r = tile_long<HD, C::kSplit>(Running{m, mo, l}, columns(), (unsigned)(at - see_lo),
                                                    (unsigned)(see_hi - see_lo), qs, sc);
         m = r.m;
         mo = r.mo;
@@ -616,10 +618,10 @@ struct Softmax {
       }
       tmem_store_wait();
       tc_fence_before();
-      bar_arrive(&sh.p_full);
+      bar_arrive(&sh.p_full[half]);
     }
     if (t1 > t0) {
-      if (!warp_wait(&sh.o_full, (it - 1) & 1, &sh.abort)) return false;
+      if (!warp_wait(&sh.o_full[half], (done - 1) & 1, &sh.abort)) return false;
       tc_fence_after();
     }
     return true;
@@ -633,7 +635,7 @@ struct Softmax {
     for (int c = 0; c < HD / 32; ++c) {
       float x[32];
       if (any) {
-        tmem_load(job.tmem + lanes + kTileN + 32 * c, x);
+        tmem_load(columns() + kTileN + 32 * c, x);
 #pragma unroll
         for (int e = 0; e < 32; ++e) x[e] *= back;
       } else {
@@ -653,7 +655,7 @@ __device__ __forceinline__ void store_row(T* p, const float (&x)[32], float mul)
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
+__global__ void __launch_bounds__(kTileThreads, 1)
     kv8_tile_kernel(const __grid_constant__ Kv8AttnDesc d) {
   using C = TileCfg<T, HD>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -673,10 +675,11 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
   job.rows = min(d.group_rows, d.n_rows - job.row0);
   job.nsplit = gridDim.y;
   job.split = blockIdx.y;
+  job.halves = d.halves;
   const int cap = c.pages_per_seq * kKv8Page;
 
   // ---- rows, segments, barriers, TMEM, queries ------------------------------------
-  for (int i = tid; i < kTileM; i += kTileThreads) {
+  for (int i = tid; i < 2 * kTileM; i += kTileThreads) {
     int seq = -1, pos = -1;
     if (i < job.rows) {
       seq = d.seq[job.row0 + i];
@@ -692,22 +695,27 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
     sh.segment[i] = TileSegment{0, 0, -1, 0x7fffffff, 0};
   }
   if (tid == 0) {
-    bar_init(&sh.k_full, kConvert);
-    bar_init(&sh.v_full, kConvert);
-    bar_init(&sh.s_full, 2);
-    bar_init(&sh.p_full, kSoft);
-    bar_init(&sh.o_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sh.k_full[i], kConvert);
+      bar_init(&sh.v_full[i], kConvert);
+      bar_init(&sh.k_free[i], 1);
+      bar_init(&sh.v_free[i], 1);
+      bar_init(&sh.s_full[i], 2);
+      bar_init(&sh.p_full[i], kTileM);
+      bar_init(&sh.o_full[i], 1);
+    }
     bar_init(&sh.fin, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.abort = 0;
   }
-  if (warp == kSoft / 32) {
+  constexpr int kLast = kTileThreads / 32 - 1;  // the warp of the products
+  if (warp == kLast) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&sh.tmem)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   __syncthreads();
-  if (warp == kSoft / 32) {  // runs of rows of one sequence
+  if (warp == kLast) {  // runs of rows of one sequence
     int n = 0;
     for (int r0 = 0; r0 < job.rows; r0 += 32) {
       const int r = r0 + lane;
@@ -734,7 +742,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
     if (lane == 0) sh.n_segments = n;
   }
   Softmax<T, HD> soft(job);
-  if (tid < kSoft) {
+  const bool softmax = tid < kTileM * d.halves;  // (the second half's warps have nothing to do with one half)
+  if (softmax) {
     soft.put_query();
     smem_to_async();
   }
@@ -744,20 +753,22 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
   job.tmem = sh.tmem;
 
   Converter<T, HD> conv(job);
+  Products<T, HD> products(job);
   bool ok = true;
   int it = 0;
   for (int g = 0; g < sh.n_segments; ++g) {
     const TileSegment seg = sh.segment[g];
     if (seg.seq < 0) continue;  // padding
     if (ok) {
-      if (tid < kSoft) ok = soft.run(seg, it);
-      else ok = conv.run(seg, it);
+      if (softmax) ok = soft.run(seg, it);
+      else if (warp == kLast) ok = products.run(seg, it);
+      else if (tid >= kSoft) ok = conv.run(seg, it);
     }
-    const bool mine = tid < kSoft && soft.row >= seg.row0 && soft.row < seg.row0 + seg.rows;
+    const bool mine = softmax && soft.row >= seg.row0 && soft.row < seg.row0 + seg.rows;
     int p0, p1, t0, t1;
     job.tiles(seg, p0, p1, t0, t1);
     if (job.nsplit == 1) {
-      if (tid < kSoft && ok) {
+      if (softmax && ok && job.takes(seg, soft.half)) {
         const size_t row = job.row0 + soft.row;
         const int head = job.h0 + soft.head;
         const bool none = soft.m == -INFINITY && soft.l == soft.l;
@@ -775,7 +786,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
     // join the splits of the cluster, in their order: O over the K and V operands
     float* sums = reinterpret_cast<float*>(smem + C::kK);
     __syncthreads();
-    if (tid < kSoft) {
+    if (softmax && job.takes(seg, soft.half)) {
       soft.output(t1 > t0 && ok, [&](int e, const float(&x)[32]) { store_row(sums + soft.slot * HD + e, x, 1.0f); });
       sh.m[tid] = soft.l == soft.l ? soft.m : INFINITY;  // a NaN sum makes the join NaN
       sh.l[tid] = soft.l;
@@ -812,8 +823,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<T, HD>::kCtas)
   pdl_launch_dependents();
   // every product is done (a wait that ran out leaves some in flight) before TMEM goes
   __syncthreads();
-  if (tid == kSoft) commit_to(&sh.fin);
-  if (warp == kSoft / 32) {
+  if (tid == kLast * 32) commit_to(&sh.fin);
+  if (warp == kLast) {
     int plain = 0;
     bar_wait(&sh.fin, 0, &plain);
     tc_fence_after();
@@ -833,7 +844,7 @@ cudaError_t launch_tile_t(const Kv8AttnDesc& d, long units, int len, int sms, cu
   // the cache is split while the CTAs do not fill the device and keep two tiles
   unsigned ns = 1;
   const int tiles = (len + kTileN - 1) / kTileN;
-  while (ns < 8 && units * ns * 2 <= (long)C::kCtas * sms && tiles >= (int)ns * 4) ns *= 2;
+  while (ns < 8 && units * ns * 2 <= sms && tiles >= (int)ns * 4) ns *= 2;
   return launch_k(kv8_tile_kernel<T, HD>, dim3((unsigned)units, ns), dim3(kTileThreads), (size_t)C::kSmem, st,
                   LaunchOpts{true, ns}, d);
 }
@@ -844,10 +855,15 @@ cudaError_t launch_kv8_tile(Kv8AttnDesc d, int dtype, int max_rows, int len, int
   const int group = d.heads / d.c.kv_heads;
   d.unit_heads = std::min(group, kTileM);
   d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
-  // rows of a tile: what 128 slots hold, or a sequence's rows in equal shares
-  const int most = kTileM / d.unit_heads, parts = (max_rows + most - 1) / most;
-  d.group_rows = std::min(most, (max_rows + parts - 1) / parts);
-  const long units = ((long)d.n_rows + d.group_rows - 1) / d.group_rows * d.c.kv_heads * d.head_chunks;
+  // Rows of a unit: what its slots hold, or a sequence's rows in equal shares.
+  // Two halves (16-bit rows) where the units still fill the device.
+  long units = 0;
+  for (d.halves = dtype == DT_F32 ? 1 : 2;; d.halves = 1) {
+    const int most = d.halves * kTileM / d.unit_heads, parts = (max_rows + most - 1) / most;
+    d.group_rows = std::min(most, (max_rows + parts - 1) / parts);
+    units = ((long)d.n_rows + d.group_rows - 1) / d.group_rows * d.c.kv_heads * d.head_chunks;
+    if (d.halves == 1 || (units >= sms && d.group_rows * d.unit_heads > kTileM)) break;
+  }
   const bool w = d.c.head_dim == 128;
   switch (dtype) {
     case DT_F16:
