@@ -8,8 +8,11 @@
 //                 maximum and sum, and writes P as f16 over S
 //   O += P V      tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
 // Four warps a half do the softmax, four turn codes into f16 operands (exact: a
-// code has 8 bits), up to two tiles ahead, and one issues the products: those of
-// one half run while the other half is in its softmax.
+// code has 8 bits), up to two tiles ahead for K, and one issues the products:
+// those of one half run while the other half is in its softmax.  The codes of
+// the next tile are on their way to shared memory meanwhile (asynchronous
+// copies; held in registers instead, they were spilled, and a tile took 8000
+// cycles, of which the conversion waited 4500 for them).
 //
 // Queries are scaled by a power of two to at most 2, which f16 holds exactly
 // for 16-bit types; f32 queries are split into f16 hi + lo, and so is P then
@@ -47,7 +50,8 @@ struct TileSegment {
   int row0, rows, seq, lo, hi;  // rows of the unit, and the positions [lo, hi) that any of them sees
 };
 struct TileShared {
-  uint64_t k_full[2], k_free[2], v_full[2], v_free[2];  // by buffer
+  uint64_t k_full[2], k_free[2];                        // by buffer
+  uint64_t v_full, v_free;
   uint64_t s_full[2], p_full[2], o_full[2];             // by half
   uint64_t fin;
   uint32_t tmem;
@@ -65,7 +69,9 @@ template <typename T, int HD>
 struct TileCfg {
   static constexpr bool kSplit = sizeof(T) == 4;
   static constexpr int kHalf = kTileM * HD * 2;  // bytes of a 128-row f16 operand
-  static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + 2 * kHalf, kOps = kV + 2 * kHalf;
+  // Q (two halves, or hi and lo), two of K, one of V, and the raw codes of a tile
+  static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + 2 * kHalf, kRaw = kV + kHalf, kOps = kRaw + kHalf;
+  static_assert(kTileM * HD * 4 * (kSplit ? 1 : 2) <= 4 * kHalf, "the halves' sums lie over K, V and the codes");
   static constexpr int kUsed = kOps + (int)sizeof(TileShared);
   // One CTA an SM, as it takes all of TMEM (a second would wait for it, and its
   // cluster for the second).
@@ -208,11 +214,11 @@ struct Converter {
   static constexpr int N = HD / 16;  // 16-byte pieces of a thread, per operand
   const J& job;
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  uint4 k[N], v[N];
-  int ids = -1;       // lanes 0..7: the tile's pages
+  uint4* raw;    // this thread's pieces: K at raw[i * kConvert], V N of them on
   float sk = 0.0f, sv = 0.0f;
 
-  __device__ explicit Converter(const J& j) : job(j) {}
+  __device__ explicit Converter(const J& j)
+      : job(j), raw(reinterpret_cast<uint4*>(j.ops + J::C::kRaw) + (threadIdx.x & (kConvert - 1))) {}
   // piece i: positions 8 at a time, dims 16 at a time
   __device__ __forceinline__ int block_of(int i) const { return HD == 128 ? warp + 4 * (i >> 1) : warp + 4 * i; }
   __device__ __forceinline__ int chunk_of(int i) const { return HD == 128 ? (lane >> 3) + 4 * (i & 1) : lane >> 3; }
@@ -230,18 +236,21 @@ struct Converter {
     }
     return id;
   }
-  __device__ __forceinline__ void fetch(int which, uint4 (&r)[N]) const {
+  // starts the copies of K or V of the tile whose pages lanes 0..7 hold in `ids`
+  // (zeros for a missing one); the pieces there have been read
+  __device__ __forceinline__ void fetch(int which, int ids) const {
     const qtts_kv8_cache& c = job.d.c;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int b = block_of(i), page = __shfl_sync(kFull, ids, b >> 1);
-      r[i] = make_uint4(0, 0, 0, 0);
-      if (page >= 0)
-        r[i] = *reinterpret_cast<const uint4*>(block_codes(c, page, which, job.kvh) + ((b & 1) * 8 + (lane & 7)) * HD +
-                                               chunk_of(i) * 16);
+      const int8_t* src = block_codes(c, max(page, 0), which, job.kvh) + ((b & 1) * 8 + (lane & 7)) * HD + chunk_of(i) * 16;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(raw + (which * N + i) * kConvert)),
+                   "l"(src), "r"(page >= 0 ? 16 : 0)
+                   : "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  __device__ __forceinline__ void fetch_scales() {
+  __device__ __forceinline__ void fetch_scales(int ids) {
     sk = sv = 0.0f;
     if (ids >= 0) {
       sk = *block_scale(job.d.c, ids, 0, job.kvh);
@@ -256,12 +265,14 @@ struct Converter {
   __device__ __forceinline__ void put_k(int b) const {
     uint8_t* base = job.ops + J::C::kK + b * J::C::kHalf;
 #pragma unroll
-    for (int i = 0; i < N; ++i) put(base + block_of(i) * (16 * HD) + chunk_of(i) * 256 + (lane & 7) * 16, 128, k[i]);
+    for (int i = 0; i < N; ++i)
+      put(base + block_of(i) * (16 * HD) + chunk_of(i) * 256 + (lane & 7) * 16, 128, raw[i * kConvert]);
   }
-  __device__ __forceinline__ void put_v(int b) const {
-    uint8_t* base = job.ops + J::C::kV + b * J::C::kHalf;
+  __device__ __forceinline__ void put_v() const {
+    uint8_t* base = job.ops + J::C::kV;
 #pragma unroll
-    for (int i = 0; i < N; ++i) put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, v[i]);
+    for (int i = 0; i < N; ++i)
+      put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, raw[(N + i) * kConvert]);
   }
   // One segment; `it` counts the CTA's tiles.
   __device__ bool run(const TileSegment& g, int& it) {
@@ -270,36 +281,50 @@ struct Converter {
     job.tiles(g, p0, p1, t0, t1);
     if (t0 == t1) return true;
     const int* table = job.d.c.page_table + (size_t)g.seq * job.d.c.pages_per_seq;
-    ids = pages(table, p0, p1, t0);
-    fetch(0, k);
-    fetch(1, v);
-    fetch_scales();
-    int next = t0 + 1 < t1 ? pages(table, p0, p1, t0 + 1) : -1;
-    for (int t = t0; t < t1; ++t, ++it) {
-      const int b = it & 1;
-      const unsigned before = (unsigned)((it >> 1) - 1) & 1u;  // the buffer's last use
-      if (it > 1 && !warp_wait(&sh.k_free[b], before, &sh.abort)) return false;
-      if (warp == 0 && lane < kTilePages) {
-        float ev, fr;
-        split_scale(sv, ev, fr);
-        const bool plain = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX;
-        sh.scale[it % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : -1.0f, plain ? log2f(sv) : NAN);
+    // K of a tile is put before V of the one before it: V waits for the products
+    // of the tile before that
+    int ids = pages(table, p0, p1, t0), next = pages(table, p0, p1, t0 + 1);
+    fetch(0, ids);
+    fetch_scales(ids);
+    asm volatile("cp.async.commit_group;" ::: "memory");  // (so that K is the older of two groups from the start)
+    const int it0 = it;
+    for (int t = t0; t <= t1; ++t) {
+      const int i = it0 + t - t0;
+      if (t < t1) {
+        const int b = i & 1;
+        const int after = pages(table, p0, p1, t + 2);
+        if (i > 1 && !warp_wait(&sh.k_free[b], (unsigned)((i >> 1) - 1) & 1u, &sh.abort)) return false;
+        if (warp == 0 && lane < kTilePages) {
+          float ev, fr;
+          split_scale(sv, ev, fr);
+          const bool plain = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX;
+          sh.scale[i % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : -1.0f, plain ? log2f(sv) : NAN);
+        }
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // this thread's K
+        put_k(b);
+        smem_to_async();
+        bar_arrive(&sh.k_full[b]);
+        fetch(0, next);
+        fetch_scales(next);
+        if (t > t0) {
+          if (i > 1 && !warp_wait(&sh.v_free, (unsigned)(i - 2) & 1u, &sh.abort)) return false;
+          asm volatile("cp.async.wait_group 1;" ::: "memory");  // this thread's V
+          put_v();
+          smem_to_async();
+          bar_arrive(&sh.v_full);
+        }
+        fetch(1, ids);
+        ids = next;
+        next = after;
+      } else {
+        if (i > 1 && !warp_wait(&sh.v_free, (unsigned)(i - 2) & 1u, &sh.abort)) return false;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        put_v();
+        smem_to_async();
+        bar_arrive(&sh.v_full);
       }
-      put_k(b);
-      smem_to_async();
-      bar_arrive(&sh.k_full[b]);
-      ids = next;
-      if (t + 1 < t1) {
-        fetch(0, k);
-        fetch_scales();
-      }
-      next = t + 2 < t1 ? pages(table, p0, p1, t + 2) : -1;
-      if (it > 1 && !warp_wait(&sh.v_free[b], before, &sh.abort)) return false;
-      put_v(b);
-      smem_to_async();
-      bar_arrive(&sh.v_full[b]);
-      if (t + 1 < t1) fetch(1, v);
     }
+    it = it0 + t1 - t0;
     return true;
   }
 };
@@ -341,13 +366,13 @@ struct Products {
     __syncwarp();
     return true;
   }
-  // O += P V of half h with V of buffer b
-  __device__ __forceinline__ bool weigh(int h, int b, bool first, bool last) {
+  // O += P V of half h; last: no other half reads V after it
+  __device__ __forceinline__ bool weigh(int h, bool first, bool last) {
     TileShared& sh = job.sh;
     constexpr uint32_t idesc = instruction(HD, true);
     if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
     if (lane == 0) {
-      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h, o = s + kTileN;
+      const uint32_t v = smem_of(job.ops + C::kV), s = job.tmem + 256 * h, o = s + kTileN;
       tc_fence_after();
 #pragma unroll
       for (int e = 0; e < kTileN / 16; ++e) {
@@ -356,7 +381,7 @@ struct Products {
         if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
       }
       commit_to(&sh.o_full[h]);
-      if (last) commit_to(&sh.v_free[b]);
+      if (last) commit_to(&sh.v_free);
     }
     __syncwarp();
     ++done[h];
@@ -370,16 +395,16 @@ struct Products {
     // half 1 is half a tile behind half 0: while one is in its softmax the
     // other's products run
     for (int t = t0; t < t1; ++t, ++it) {
-      const int b = it & 1, before = (it - 1) & 1;
+      const int b = it & 1;
       const unsigned use = (unsigned)(it >> 1) & 1u;
       if (!warp_wait(&sh.k_full[b], use, &sh.abort)) return false;
       if (one && !score(0, b, !two)) return false;
-      if (two && t > t0 && !weigh(1, before, t - 1 == t0, true)) return false;
+      if (two && t > t0 && !weigh(1, t - 1 == t0, true)) return false;
       if (two && !score(1, b, true)) return false;
-      if (!warp_wait(&sh.v_full[b], use, &sh.abort)) return false;
-      if (one && !weigh(0, b, t == t0, !two)) return false;
+      if (!warp_wait(&sh.v_full, it & 1, &sh.abort)) return false;
+      if (one && !weigh(0, t == t0, !two)) return false;
     }
-    return !two || t0 == t1 || weigh(1, (it - 1) & 1, t1 - 1 == t0, true);
+    return !two || t0 == t1 || weigh(1, t1 - 1 == t0, true);
   }
 };
 
@@ -697,13 +722,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.k_full[i], kConvert);
-      bar_init(&sh.v_full[i], kConvert);
       bar_init(&sh.k_free[i], 1);
-      bar_init(&sh.v_free[i], 1);
       bar_init(&sh.s_full[i], 2);
       bar_init(&sh.p_full[i], kTileM);
       bar_init(&sh.o_full[i], 1);
     }
+    bar_init(&sh.v_full, kConvert);
+    bar_init(&sh.v_free, 1);
     bar_init(&sh.fin, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.abort = 0;
