@@ -8,11 +8,12 @@
 //                 maximum and sum, and writes P as f16 over S
 //   O += P V      tcgen05.mma, P from TMEM, V in shared memory, O in TMEM
 // Four warps a half do the softmax, four turn codes into f16 operands (exact: a
-// code has 8 bits), up to two tiles ahead for K, and one issues the products:
-// those of one half run while the other half is in its softmax.  The codes of
-// the next tile are on their way to shared memory meanwhile (asynchronous
-// copies; held in registers instead, they were spilled, and a tile took 8000
-// cycles, of which the conversion waited 4500 for them).
+// code has 8 bits), two tiles ahead at most, and one issues the products in an
+// order that keeps the halves half a tile apart: those of one run while the
+// other is in its softmax.  (A warp a half let them fall into step: 183 instead
+// of 165 us for four chunks of 1000 rows.)  The next codes to convert are on their way to shared memory
+// meanwhile (asynchronous copies; held in registers instead, they were spilled,
+// and a tile took 8000 cycles, of which the conversion waited 4500 for them).
 //
 // Queries are scaled by a power of two to at most 2, which f16 holds exactly
 // for 16-bit types; f32 queries are split into f16 hi + lo, and so is P then
@@ -41,7 +42,7 @@ namespace {
 
 constexpr int kTileM = 128, kTileN = 128, kTilePages = kTileN / kKv8Page;
 constexpr int kSoft = 256, kConvert = 128;  // threads of the softmax (two halves) and of the conversion
-constexpr int kTileThreads = kSoft + kConvert + 32;
+constexpr int kTileThreads = kSoft + kConvert + 32;  // and a warp that issues the products
 constexpr uint32_t kTmemCols = 512;  // half h: S and P at 256 h, O at 256 h + 128
 constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr int kScales = 4;  // tiles of scales kept: a half may be two tiles behind the conversion
@@ -50,8 +51,7 @@ struct TileSegment {
   int row0, rows, seq, lo, hi;  // rows of the unit, and the positions [lo, hi) that any of them sees
 };
 struct TileShared {
-  uint64_t k_full[2], k_free[2];                        // by buffer
-  uint64_t v_full, v_free;
+  uint64_t k_full[2], k_free[2], v_full[2], v_free[2];  // by buffer
   uint64_t s_full[2], p_full[2], o_full[2];             // by half
   uint64_t fin;
   uint32_t tmem;
@@ -69,9 +69,9 @@ template <typename T, int HD>
 struct TileCfg {
   static constexpr bool kSplit = sizeof(T) == 4;
   static constexpr int kHalf = kTileM * HD * 2;  // bytes of a 128-row f16 operand
-  // Q (two halves, or hi and lo), two of K, one of V, and the raw codes of a tile
-  static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + 2 * kHalf, kRaw = kV + kHalf, kOps = kRaw + kHalf;
-  static_assert(kTileM * HD * 4 * (kSplit ? 1 : 2) <= 4 * kHalf, "the halves' sums lie over K, V and the codes");
+  // Q (two halves, or hi and lo), two of K and V, and the raw codes of one
+  static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + 2 * kHalf, kRaw = kV + 2 * kHalf, kOps = kRaw + kHalf / 2;
+  static_assert(kTileM * HD * 4 * (kSplit ? 1 : 2) <= 4 * kHalf, "the halves' sums lie over K and V");
   static constexpr int kUsed = kOps + (int)sizeof(TileShared);
   // One CTA an SM, as it takes all of TMEM (a second would wait for it, and its
   // cluster for the second).
@@ -146,20 +146,33 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity, int* ab
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, int* abort) {
   return __all_sync(kFull, bar_wait(bar, parity, abort));
 }
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns on their way into r, which may be read after tmem_wait(r).
+__device__ __forceinline__ void tmem_start(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&q)[32], float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
+                 "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]),
+                 "+r"(q[16]), "+r"(q[17]), "+r"(q[18]), "+r"(q[19]), "+r"(q[20]), "+r"(q[21]), "+r"(q[22]), "+r"(q[23]),
+                 "+r"(q[24]), "+r"(q[25]), "+r"(q[26]), "+r"(q[27]), "+r"(q[28]), "+r"(q[29]), "+r"(q[30]), "+r"(q[31])
+               :
+               : "memory");
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(q[j]);
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_start(addr, r);
+  tmem_wait(r, v);
 }
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -214,7 +227,7 @@ struct Converter {
   static constexpr int N = HD / 16;  // 16-byte pieces of a thread, per operand
   const J& job;
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  uint4* raw;    // this thread's pieces: K at raw[i * kConvert], V N of them on
+  uint4* raw;  // this thread's pieces at raw[i * kConvert]
   float sk = 0.0f, sv = 0.0f;
 
   __device__ explicit Converter(const J& j)
@@ -244,7 +257,7 @@ struct Converter {
     for (int i = 0; i < N; ++i) {
       const int b = block_of(i), page = __shfl_sync(kFull, ids, b >> 1);
       const int8_t* src = block_codes(c, max(page, 0), which, job.kvh) + ((b & 1) * 8 + (lane & 7)) * HD + chunk_of(i) * 16;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(raw + (which * N + i) * kConvert)),
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(raw + i * kConvert)),
                    "l"(src), "r"(page >= 0 ? 16 : 0)
                    : "memory");
     }
@@ -268,11 +281,11 @@ struct Converter {
     for (int i = 0; i < N; ++i)
       put(base + block_of(i) * (16 * HD) + chunk_of(i) * 256 + (lane & 7) * 16, 128, raw[i * kConvert]);
   }
-  __device__ __forceinline__ void put_v() const {
-    uint8_t* base = job.ops + J::C::kV;
+  __device__ __forceinline__ void put_v(int b) const {
+    uint8_t* base = job.ops + J::C::kV + b * J::C::kHalf;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, raw[(N + i) * kConvert]);
+      put(base + chunk_of(i) * 4096 + block_of(i) * 128 + (lane & 7) * 16, 2048, raw[i * kConvert]);
   }
   // One segment; `it` counts the CTA's tiles.
   __device__ bool run(const TileSegment& g, int& it) {
@@ -281,50 +294,35 @@ struct Converter {
     job.tiles(g, p0, p1, t0, t1);
     if (t0 == t1) return true;
     const int* table = job.d.c.page_table + (size_t)g.seq * job.d.c.pages_per_seq;
-    // K of a tile is put before V of the one before it: V waits for the products
-    // of the tile before that
     int ids = pages(table, p0, p1, t0), next = pages(table, p0, p1, t0 + 1);
     fetch(0, ids);
     fetch_scales(ids);
-    asm volatile("cp.async.commit_group;" ::: "memory");  // (so that K is the older of two groups from the start)
-    const int it0 = it;
-    for (int t = t0; t <= t1; ++t) {
-      const int i = it0 + t - t0;
-      if (t < t1) {
-        const int b = i & 1;
-        const int after = pages(table, p0, p1, t + 2);
-        if (i > 1 && !warp_wait(&sh.k_free[b], (unsigned)((i >> 1) - 1) & 1u, &sh.abort)) return false;
-        if (warp == 0 && lane < kTilePages) {
-          float ev, fr;
-          split_scale(sv, ev, fr);
-          const bool plain = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX;
-          sh.scale[i % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : -1.0f, plain ? log2f(sv) : NAN);
-        }
-        asm volatile("cp.async.wait_group 1;" ::: "memory");  // this thread's K
-        put_k(b);
-        smem_to_async();
-        bar_arrive(&sh.k_full[b]);
-        fetch(0, next);
-        fetch_scales(next);
-        if (t > t0) {
-          if (i > 1 && !warp_wait(&sh.v_free, (unsigned)(i - 2) & 1u, &sh.abort)) return false;
-          asm volatile("cp.async.wait_group 1;" ::: "memory");  // this thread's V
-          put_v();
-          smem_to_async();
-          bar_arrive(&sh.v_full);
-        }
-        fetch(1, ids);
-        ids = next;
-        next = after;
-      } else {
-        if (i > 1 && !warp_wait(&sh.v_free, (unsigned)(i - 2) & 1u, &sh.abort)) return false;
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        put_v();
-        smem_to_async();
-        bar_arrive(&sh.v_full);
+    for (int t = t0; t < t1; ++t, ++it) {
+      const int b = it & 1;
+      const unsigned before = (unsigned)((it >> 1) - 1) & 1u;  // the buffers' last use
+      const int after = pages(table, p0, p1, t + 2);
+      if (it > 1 && !warp_wait(&sh.k_free[b], before, &sh.abort)) return false;
+      if (warp == 0 && lane < kTilePages) {
+        float ev, fr;
+        split_scale(sv, ev, fr);
+        const bool plain = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX;
+        sh.scale[it % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : -1.0f, plain ? log2f(sv) : NAN);
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");  // this thread's own copies
+      put_k(b);
+      smem_to_async();
+      bar_arrive(&sh.k_full[b]);
+      fetch(1, ids);
+      fetch_scales(next);
+      if (it > 1 && !warp_wait(&sh.v_free[b], before, &sh.abort)) return false;
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      put_v(b);
+      smem_to_async();
+      bar_arrive(&sh.v_full[b]);
+      if (t + 1 < t1) fetch(0, next);
+      ids = next;
+      next = after;
     }
-    it = it0 + t1 - t0;
     return true;
   }
 };
@@ -339,8 +337,8 @@ struct Products {
   int done[2] = {0, 0};  // tiles of each half
 
   __device__ explicit Products(const J& j) : job(j) {}
-  // S = Q K^T of half h with K of buffer b; last: no other half reads K after it
-  __device__ __forceinline__ bool score(int h, int b, bool last) {
+  // S = Q K^T of half h with K of buffer b; last: no other half reads this K
+  __device__ __forceinline__ bool score(int h, int b, bool last) const {
     TileShared& sh = job.sh;
     constexpr uint32_t idesc = instruction(kTileN, false);
     // P of the half's tile before lies where S goes
@@ -366,13 +364,14 @@ struct Products {
     __syncwarp();
     return true;
   }
-  // O += P V of half h; last: no other half reads V after it
-  __device__ __forceinline__ bool weigh(int h, bool first, bool last) {
+  // O += P V of half h with V of buffer b; last: no other half reads this V
+  __device__ __forceinline__ bool weigh(int h, int b, bool first, bool last) {
     TileShared& sh = job.sh;
     constexpr uint32_t idesc = instruction(HD, true);
     if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
+    ++done[h];
     if (lane == 0) {
-      const uint32_t v = smem_of(job.ops + C::kV), s = job.tmem + 256 * h, o = s + kTileN;
+      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h, o = s + kTileN;
       tc_fence_after();
 #pragma unroll
       for (int e = 0; e < kTileN / 16; ++e) {
@@ -381,10 +380,9 @@ struct Products {
         if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
       }
       commit_to(&sh.o_full[h]);
-      if (last) commit_to(&sh.v_free);
+      if (last) commit_to(&sh.v_free[b]);
     }
     __syncwarp();
-    ++done[h];
     return true;
   }
   __device__ bool run(const TileSegment& g, int& it) {
@@ -392,19 +390,17 @@ struct Products {
     int p0, p1, t0, t1;
     job.tiles(g, p0, p1, t0, t1);
     const bool one = job.takes(g, 0), two = job.takes(g, 1);
-    // half 1 is half a tile behind half 0: while one is in its softmax the
-    // other's products run
     for (int t = t0; t < t1; ++t, ++it) {
       const int b = it & 1;
       const unsigned use = (unsigned)(it >> 1) & 1u;
       if (!warp_wait(&sh.k_full[b], use, &sh.abort)) return false;
       if (one && !score(0, b, !two)) return false;
-      if (two && t > t0 && !weigh(1, t - 1 == t0, true)) return false;
+      if (two && t > t0 && !weigh(1, b ^ 1, t - 1 == t0, true)) return false;
       if (two && !score(1, b, true)) return false;
-      if (!warp_wait(&sh.v_full, it & 1, &sh.abort)) return false;
-      if (one && !weigh(0, t == t0, !two)) return false;
+      if (!warp_wait(&sh.v_full[b], use, &sh.abort)) return false;
+      if (one && !weigh(0, b, t == t0, !two)) return false;
     }
-    return !two || t0 == t1 || weigh(1, t1 - 1 == t0, true);
+    return !two || t0 == t1 || weigh(1, (it - 1) & 1, t1 - 1 == t0, true);
   }
 };
 
@@ -553,12 +549,22 @@ struct Softmax {
   // exp2(score + log2 sv - mo), and the sum l from their sum per page.  False if
   // the exponents are too far apart for that (nothing is done then).
   __device__ __forceinline__ bool tile_short(const float4* sc) {
+    // (each load of 32 columns is on its way while the one before is worked on)
     const uint32_t s = columns();
+    uint32_t r[2][32];
     float pm[kTilePages], f[kTilePages], log_v[kTilePages];
+    tmem_start(s, r[0]);
+#pragma unroll
+    for (int k = 0; k < kTilePages; ++k) {
+      const float4 z = sc[k];
+      f[k] = qs * z.x;
+      log_v[k] = z.w;
+    }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       float x[32];
-      tmem_load(s + 32 * c, x);
+      tmem_wait(r[c & 1], x);
+      tmem_start(s + 32 * ((c + 1) & 3), r[(c + 1) & 1]);  // (after the last, the first again)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         float a = fmaxf(x[16 * k], x[16 * k + 1]), b = fmaxf(x[16 * k + 2], x[16 * k + 3]);
@@ -567,31 +573,32 @@ struct Softmax {
           a = fmaxf(fmaxf(a, x[16 * k + e]), x[16 * k + e + 1]);
           b = fmaxf(fmaxf(b, x[16 * k + e + 2]), x[16 * k + e + 3]);
         }
-        pm[2 * c + k] = fmaxf(a, b);
+        pm[2 * c + k] = fmaxf(a, b) * f[2 * c + k];
       }
     }
     float mn = m, mon = -INFINITY;
     bool near = qs >= 0.0f;  // (a negative or NaN scale goes the long way)
 #pragma unroll
     for (int k = 0; k < kTilePages; ++k) {
-      const float4 z = sc[k];
-      f[k] = qs * z.x;
-      log_v[k] = z.w;
-      const float y = pm[k] * f[k];
-      mn = fmaxf(mn, y);
-      mon = fmaxf(mon, y + z.y);
+      mn = fmaxf(mn, pm[k]);
+      mon = fmaxf(mon, pm[k] + log_v[k]);
     }
     const float mo_new = mon > mo + 6.0f || mo == -INFINITY ? mon : mo;
 #pragma unroll
     for (int k = 0; k < kTilePages; ++k) near &= fabsf(mn + log_v[k] - mo_new) < 40.0f;  // (false for NaN)
-    if (!__all_sync(kFull, near)) return false;
+    if (!__all_sync(kFull, near)) {
+      float x[32];
+      tmem_wait(r[0], x);  // the load on its way
+      return false;
+    }
     grow_to<HD>(mon, mo, s + kTileN);
     l *= ex2(m - mn);
     m = mn;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       float x[32];
-      tmem_load(s + 32 * c, x);
+      tmem_wait(r[c & 1], x);
+      if (c < 3) tmem_start(s + 32 * (c + 1), r[(c + 1) & 1]);
       uint32_t hi[16], lo[16];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -722,13 +729,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       bar_init(&sh.k_full[i], kConvert);
+      bar_init(&sh.v_full[i], kConvert);
       bar_init(&sh.k_free[i], 1);
+      bar_init(&sh.v_free[i], 1);
       bar_init(&sh.s_full[i], 2);
       bar_init(&sh.p_full[i], kTileM);
       bar_init(&sh.o_full[i], 1);
     }
-    bar_init(&sh.v_full, kConvert);
-    bar_init(&sh.v_free, 1);
     bar_init(&sh.fin, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.abort = 0;
