@@ -881,8 +881,9 @@ int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t l
   d.flags = flags;
   const int cap = cache->pages_per_seq * kKv8Page;
   int len = max_len == 0 ? cap : std::min(max_len, cap);
-  if (window > 0) len = std::min(len, window + std::max(1, max_rows) - 1);
-  return launched(launch_kv8_attention(d, dtype, max_rows == 0 ? 1 : max_rows, len, on.sm_count, (cudaStream_t)stream));
+  max_rows = std::max(1, std::min(max_rows, n_rows));
+  if (window > 0) len = (int)std::min<int64_t>(len, (int64_t)window + max_rows - 1);
+  return launched(launch_kv8_attention(d, dtype, max_rows, len, on.sm_count, (cudaStream_t)stream));
 } catch (...) {
   return QTTS_ERR_OOM;
 }

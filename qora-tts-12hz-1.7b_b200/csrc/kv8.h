@@ -76,6 +76,7 @@ struct Kv8AttnDesc {
   int head_chunks = 1;  // units along the query heads of one K/V head
   int unit_heads = 1;   // query heads of a unit
   int halves = 1;       // tile kernel: halves of 128 slots of a unit
+  int seq_units = 1;    // tile kernel: units of a sequence of max_rows rows
 };
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st);
 // The same for many rows: tiles of 128 slots on the tensor cores (kv8_tile.cu).
