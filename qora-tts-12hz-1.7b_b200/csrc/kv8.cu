@@ -27,14 +27,38 @@ namespace {
 // RMS norm over the head (the formula of the q/k/v epilogue): the mean of
 // squares is summed in f64 (order-free to f32, so that a code does not depend
 // on the reduction tree), everything after it is one f32 rounding per step.
-template <int HD>
-__device__ __forceinline__ float4 head_norm(float4 x, float4 g) {
-  double ss = (double)x.x * x.x + (double)x.y * x.y + (double)x.z * x.z + (double)x.w * x.w;
+//
+// N heads (or tokens) at a time: their sums of squares are reduced together (at
+// each step half of the lanes keep one half of the values), after which lane j
+// of a head's lanes holds the sum of value j % N; the square root and the
+// division, a few dozen instructions, are done once for all of them.
+template <int HD, int N>
+__device__ __forceinline__ void head_norm(float4 (&x)[N], float4 g) {
+  constexpr int L = HD / 4;  // lanes of a head
+  static_assert((N & (N - 1)) == 0 && N <= L, "values are halved between lanes");
+  const int lane = threadIdx.x & 31;
+  double ss[N];
 #pragma unroll
-  for (int o = HD / 8; o; o >>= 1) ss += __shfl_xor_sync(kFull, ss, o);
-  const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn((float)(ss / HD), 1e-6f)));
-  return make_float4(__fmul_rn(__fmul_rn(x.x, inv), g.x), __fmul_rn(__fmul_rn(x.y, inv), g.y),
-                     __fmul_rn(__fmul_rn(x.z, inv), g.z), __fmul_rn(__fmul_rn(x.w, inv), g.w));
+  for (int i = 0; i < N; ++i)
+    ss[i] = (double)x[i].x * x[i].x + (double)x[i].y * x[i].y + (double)x[i].z * x[i].z + (double)x[i].w * x[i].w;
+#pragma unroll
+  for (int n = N / 2; n; n >>= 1) {  // lane bit n: which half of the values this lane keeps
+    const bool up = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const double give = up ? ss[i] : ss[i + n], keep = up ? ss[i + n] : ss[i];
+      ss[i] = keep + __shfl_xor_sync(kFull, give, n);
+    }
+  }
+#pragma unroll
+  for (int o = N; o < L; o <<= 1) ss[0] += __shfl_xor_sync(kFull, ss[0], o);
+  const float own = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn((float)(ss[0] / HD), 1e-6f)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float inv = __shfl_sync(kFull, own, (lane & ~(N - 1)) | i);
+    x[i] = make_float4(__fmul_rn(__fmul_rn(x[i].x, inv), g.x), __fmul_rn(__fmul_rn(x[i].y, inv), g.y),
+                       __fmul_rn(__fmul_rn(x[i].z, inv), g.z), __fmul_rn(__fmul_rn(x[i].w, inv), g.w));
+  }
 }
 // (a, b) -> (a cos - b sin, b cos + a sin) of the two halves, products and sum
 // rounded one by one (no contraction)
@@ -73,21 +97,29 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
   return codes4(v, ratio);
 }
 
+// Tokens of a block that registers hold in a chunk of a prompt.  16 chunks of
+// 611 rows: 66 us with 4; 122, 78 and 73 us with 16, 8 and 2 (fewer need more
+// passes, more leave fewer warps an SM to hide the loads).
+constexpr int kAppendKeep = 4;
 // Rows [chunk * d.chunk, + d.chunk): every block (run of rows of one sequence,
 // consecutive positions, one page) that starts there, for one K or V head.
-template <typename T, int HD>
+// Registers hold KEEP tokens of a block; a longer one is read and worked out
+// once for its maximum and once more for its codes.
+template <typename T, int HD, int KEEP>
 __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int h) {
-  constexpr int LPT = HD / 4, TPW = 32 / LPT, STEPS = kKv8Page / TPW;  // lanes per token, tokens per step
+  constexpr int LPT = HD / 4, TPW = 32 / LPT, STEPS = KEEP / TPW;  // lanes per token, tokens per step
   const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
   const bool upper = (lane % LPT) >= LPT / 2;
   const qtts_kv8_cache& c = d.c;
   // lane i holds row first + i; a block that starts in the chunk ends before lane 32
   const int first = chunk * d.chunk - 1, row = first + lane;
-  int seq = -1, pos = -1;
+  int seq = -1, pos = -1, rope = -1;
   if (row >= 0 && row < d.n_rows) {
     seq = d.seq[row];
     pos = d.pos[row];
+    rope = d.rope_pos ? d.rope_pos[row] : pos;
   }
+  const bool turn = which == 0 && d.rope_cos != nullptr;
   const bool ok = seq >= 0 && seq < c.n_seqs && pos >= 0 && pos < c.pages_per_seq * kKv8Page;
   if (seq >= 0 && !ok && lane >= 1 && lane <= d.chunk) raise(d.flags, QTTS_KV8_BAD_ROW);
   const int pseq = __shfl_up_sync(kFull, seq, 1), ppos = __shfl_up_sync(kFull, pos, 1);
@@ -113,37 +145,53 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
     const float had = slot0 ? *sp : 0.0f;
     float4 x[STEPS];
     float big = 0.0f;
+    // the angles of a step's token (none: 1 and 0)
+    auto angles = [&](int t, float4& cs, float4& sn) {
+      const int rp = __shfl_sync(kFull, rope, min(31, i + t));
+      cs = make_float4(1.f, 1.f, 1.f, 1.f);
+      sn = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (t >= n) return;
+      if (rp >= 0 && rp < d.rope_rows) {
+        cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+        sn = load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+      } else {
+        raise(d.flags, QTTS_KV8_ROPE_RANGE);
+      }
+    };
+    // x = tokens t0 .. t0 + KEEP of the block, normed and rotated; their largest
+    auto tokens = [&](int t0) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (s * TPW >= n) break;
-      const int t = s * TPW + sub;
-      if (t < n) x[s] = load4(src + (size_t)(first + i + t) * ld + (size_t)h * HD + d0);
-    }
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      if (s * TPW >= n) break;
-      const int t = s * TPW + sub;
-      if (which == 0) {
-        if (d.k_norm) x[s] = head_norm<HD>(x[s], g);
-        if (d.rope_cos) {
-          float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (t < n) {
-            const int rp = d.rope_pos ? d.rope_pos[first + i + t] : bpos + t;
-            if (rp >= 0 && rp < d.rope_rows) {
-              cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
-              sn = load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2));
-            } else {
-              raise(d.flags, QTTS_KV8_ROPE_RANGE);
-            }
-          }
-          x[s] = rotate<HD>(x[s], cs, sn, upper);
+      for (int s = 0; s < STEPS; ++s) {
+        const int t = t0 + s * TPW + sub;
+        x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (t < n) x[s] = load4(src + (size_t)(first + i + t) * ld + (size_t)h * HD + d0);
+      }
+      float4 cs, sn;
+      if (turn) angles(t0 + sub, cs, sn);  // (of each step while the one before is worked on)
+      if (which == 0 && d.k_norm) {
+        if (STEPS > 1 && n - t0 <= TPW) {  // one step
+          float4 one[1] = {x[0]};
+          head_norm<HD, 1>(one, g);
+          x[0] = one[0];
+        } else {
+          head_norm<HD, STEPS>(x, g);
         }
       }
-      if (t < n)
-        big = fmaxf(big, fmaxf(fmaxf(finite_abs(x[s].x), finite_abs(x[s].y)),
-                               fmaxf(finite_abs(x[s].z), finite_abs(x[s].w))));
-    }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        if (t0 + s * TPW >= n) break;
+        if (turn) {
+          const float4 c0 = cs, s0 = sn;
+          if (s + 1 < STEPS && t0 + (s + 1) * TPW < n) angles(t0 + (s + 1) * TPW + sub, cs, sn);
+          x[s] = rotate<HD>(x[s], c0, s0, upper);
+        }
+        if (t0 + s * TPW + sub < n)
+          big = fmaxf(big, fmaxf(fmaxf(finite_abs(x[s].x), finite_abs(x[s].y)),
+                                 fmaxf(finite_abs(x[s].z), finite_abs(x[s].w))));
+      }
+    };
+#pragma unroll 1
+    for (int t0 = 0; t0 < n; t0 += KEEP) tokens(t0);
 #pragma unroll
     for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, o));
     // 127 steps to the largest value; the floor keeps 1 / scale finite
@@ -163,30 +211,38 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
       }
     }
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+#pragma unroll 1
+    for (int t0 = 0; t0 < n; t0 += KEEP) {
+      if (n > KEEP) tokens(t0);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      if (s * TPW >= n) break;
-      const int t = s * TPW + sub;
-      if (t < n) *reinterpret_cast<uint32_t*>(codes + (slot0 + t) * HD + d0) = codes4(x[s], inv);
+      for (int s = 0; s < STEPS; ++s) {
+        const int t = t0 + s * TPW + sub;
+        if (t < n) *reinterpret_cast<uint32_t*>(codes + (slot0 + t) * HD + d0) = codes4(x[s], inv);
+      }
     }
     if (lane == 0) *sp = scale;
   }
 }
 
-constexpr int kQHeads = 4;  // query heads of one warp
-
-template <typename T, int HD>
+// NH query heads of one row, from h0 on.
+template <typename T, int HD, int NH>
 __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
-  constexpr int LPT = HD / 4, TPW = 32 / LPT;
+  constexpr int LPT = HD / 4, TPW = 32 / LPT, N = NH / TPW;
   const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
   const bool upper = (lane % LPT) >= LPT / 2;
-  const int seq = d.seq[row], pos = d.pos[row];
+  const int seq = d.seq[row], pos = d.pos[row], rp = d.rope_pos ? d.rope_pos[row] : pos;
+  const T* src = static_cast<const T*>(d.q) + (size_t)row * d.ldq;
+  T* dst = static_cast<T*>(d.q_out) + (size_t)row * d.ldqo;
+  float4 x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int h = h0 + i * TPW + sub;
+    x[i] = h < d.heads ? load4(src + (size_t)h * HD + d0) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   if (seq < 0 || seq >= d.c.n_seqs || pos < 0 || pos >= d.c.pages_per_seq * kKv8Page) return;  // flagged with K and V
-  const float4 g = norm_weight(d.q_norm, d0);
   float4 cs, sn;
   bool turn = d.rope_cos != nullptr;
   if (turn) {
-    const int rp = d.rope_pos ? d.rope_pos[row] : pos;
     turn = rp >= 0 && rp < d.rope_rows;
     if (turn) {
       cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
@@ -195,41 +251,32 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
       raise(d.flags, QTTS_KV8_ROPE_RANGE);
     }
   }
-  const T* src = static_cast<const T*>(d.q) + (size_t)row * d.ldq;
-  T* dst = static_cast<T*>(d.q_out) + (size_t)row * d.ldqo;
-  constexpr int N = kQHeads / TPW;
-  float4 x[N];
+  if (d.q_norm) head_norm<HD, N>(x, norm_weight(d.q_norm, d0));
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int h = h0 + i * TPW + sub;
-    x[i] = h < d.heads ? load4(src + (size_t)h * HD + d0) : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int h = h0 + i * TPW + sub;
-    if (d.q_norm) x[i] = head_norm<HD>(x[i], g);
     if (turn) x[i] = rotate<HD>(x[i], cs, sn, upper);
     if (h < d.heads) store4(dst + (size_t)h * HD + d0, x[i]);
   }
 }
 
 // A warp takes the blocks that start in a chunk of rows, for one K or V head
-// (they are its alone: the block's scale needs all of its new tokens, which
-// stay in registers between the maximum and the codes), or kQHeads query heads
-// of one row.  HBM-bound: every input is read once, every output written once,
-// and a block that grows has its earlier codes read and written again.
-template <typename T, int HD>
+// (they are its alone: the block's scale needs all of its new tokens), or NH
+// query heads of one row.  HBM-bound: every input is read from HBM once, every
+// output written once, and a block that grows has its earlier codes read and
+// written again.
+template <typename T, int HD, int KEEP, int NH>
 __global__ void __launch_bounds__(128) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
   pdl_launch_dependents();
   pdl_wait();
   const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (w < d.kv_warps) {
     const int per = 2 * d.c.kv_heads, j = (int)(w % per);
-    append_blocks<T, HD>(d, (int)(w / per), j & 1, j >> 1);
-  } else if (w < d.n_warps) {
-    const int per = (d.heads + kQHeads - 1) / kQHeads;
+    append_blocks<T, HD, KEEP>(d, (int)(w / per), j & 1, j >> 1);
+  } else {
+    const int per = (d.heads + NH - 1) / NH;
     const long i = w - d.kv_warps;
-    rotate_queries<T, HD>(d, (int)(i / per), (int)(i % per) * kQHeads);
+    if (per > 0 && i < (long)d.n_rows * per) rotate_queries<T, HD, NH>(d, (int)(i / per), (int)(i % per) * NH);
   }
 }
 
@@ -651,9 +698,12 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
 }
 
 template <typename T, int HD>
-cudaError_t launch_append_t(const Kv8AppendDesc& d, cudaStream_t st) {
-  return launch_k(kv8_append_kernel<T, HD>, dim3((unsigned)((d.n_warps + 3) / 4)), dim3(128), 0, st,
-                  LaunchOpts{true, 1}, d);
+cudaError_t launch_append_t(const Kv8AppendDesc& d, bool single, cudaStream_t st) {
+  auto run = [&](auto kernel, int nh) {
+    const long warps = d.kv_warps + (d.q ? (long)d.n_rows * ((d.heads + nh - 1) / nh) : 0);
+    return launch_k(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, st, LaunchOpts{true, 1}, d);
+  };
+  return single ? run(kv8_append_kernel<T, HD, 128 / HD, 4>, 4) : run(kv8_append_kernel<T, HD, kAppendKeep, 8>, 8);
 }
 // Splits of a unit's pages: doubled while the CTAs do not fill the device
 // (twelve warps an SM) and every warp keeps kStep pages.  Clusters of 16 need
@@ -695,12 +745,14 @@ cudaError_t launch_kv8_append(Kv8AppendDesc d, int dtype, int sms, cudaStream_t 
   auto kv_warps = [&] { return ((long)d.n_rows + d.chunk - 1) / d.chunk * 2 * d.c.kv_heads; };
   while (d.chunk < kKv8Page && kv_warps() > (long)sms * 64) d.chunk *= 2;
   d.kv_warps = kv_warps();
-  d.n_warps = d.kv_warps + (d.q ? (long)d.n_rows * ((d.heads + kQHeads - 1) / kQHeads) : 0);
+  // fewer rows than twice the sequences: mostly single tokens
+  const bool single = d.n_rows < 2l * d.c.n_seqs;
   const bool w = d.c.head_dim == 128;
   switch (dtype) {
-    case DT_F16: return w ? launch_append_t<__half, 128>(d, st) : launch_append_t<__half, 64>(d, st);
-    case DT_BF16: return w ? launch_append_t<__nv_bfloat16, 128>(d, st) : launch_append_t<__nv_bfloat16, 64>(d, st);
-    default: return w ? launch_append_t<float, 128>(d, st) : launch_append_t<float, 64>(d, st);
+    case DT_F16: return w ? launch_append_t<__half, 128>(d, single, st) : launch_append_t<__half, 64>(d, single, st);
+    case DT_BF16:
+      return w ? launch_append_t<__nv_bfloat16, 128>(d, single, st) : launch_append_t<__nv_bfloat16, 64>(d, single, st);
+    default: return w ? launch_append_t<float, 128>(d, single, st) : launch_append_t<float, 64>(d, single, st);
   }
 }
 

@@ -55,8 +55,7 @@ struct Kv8AppendDesc {
   int n_rows = 0;
   int* flags = nullptr;
   int chunk = 1;       // rows whose blocks one warp looks for (1, 2, 4, 8 or 16)
-  long kv_warps = 0;   // warps of K / V blocks; the q warps follow them
-  long n_warps = 0;
+  long kv_warps = 0;   // warps of K / V blocks
 };
 cudaError_t launch_kv8_append(Kv8AppendDesc d, int dtype, int sms, cudaStream_t st);
 
