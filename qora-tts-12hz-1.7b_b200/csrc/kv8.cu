@@ -61,19 +61,19 @@ __device__ __forceinline__ void head_norm(float4 (&x)[N], float4 g) {
   }
 }
 // (a, b) -> (a cos - b sin, b cos + a sin) of the two halves, products and sum
-// rounded one by one (no contraction)
+// rounded one by one (no contraction); s is -sin on the lanes of the first half
+// (a product's sign change is exact).
 template <int HD>
-__device__ __forceinline__ float4 rotate(float4 x, float4 c, float4 s, bool upper) {
-  float4 y;
-  y.x = __shfl_xor_sync(kFull, x.x, HD / 8);
-  y.y = __shfl_xor_sync(kFull, x.y, HD / 8);
-  y.z = __shfl_xor_sync(kFull, x.z, HD / 8);
-  y.w = __shfl_xor_sync(kFull, x.w, HD / 8);
-  const float sg = upper ? 1.0f : -1.0f;  // a product's sign change is exact
-  return make_float4(__fadd_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x) * sg),
-                     __fadd_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y) * sg),
-                     __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z) * sg),
-                     __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w) * sg));
+__device__ __forceinline__ float4 rotate(float4 x, float4 c, float4 s) {
+  const float4 y = make_float4(__shfl_xor_sync(kFull, x.x, HD / 8), __shfl_xor_sync(kFull, x.y, HD / 8),
+                               __shfl_xor_sync(kFull, x.z, HD / 8), __shfl_xor_sync(kFull, x.w, HD / 8));
+  return make_float4(__fadd_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)),
+                     __fadd_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
+                     __fadd_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)),
+                     __fadd_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
+}
+__device__ __forceinline__ float4 signed_sin(float4 s, bool upper) {
+  return upper ? s : make_float4(-s.x, -s.y, -s.z, -s.w);
 }
 __device__ __forceinline__ float4 norm_weight(const __half* w, int d0) {
   return w ? load4(w + d0) : make_float4(1.f, 1.f, 1.f, 1.f);
@@ -91,6 +91,18 @@ __device__ __forceinline__ uint32_t code_of(float v, float inv) {
 __device__ __forceinline__ uint32_t codes4(float4 v, float inv) {
   return code_of(v.x, inv) | (code_of(v.y, inv) << 8) | (code_of(v.z, inv) << 16) | (code_of(v.w, inv) << 24);
 }
+// The same for finite values of at most 127 steps: the sum with 1.5 * 2^23
+// rounds to the nearest, ties to even, and its low byte is the code.
+__device__ __forceinline__ uint32_t small_codes4(float4 v, float inv) {
+  const float b = 12582912.0f;
+  const uint32_t x = __float_as_uint(__fadd_rn(__fmul_rn(v.x, inv), b)), y = __float_as_uint(__fadd_rn(__fmul_rn(v.y, inv), b)),
+                 z = __float_as_uint(__fadd_rn(__fmul_rn(v.z, inv), b)), w = __float_as_uint(__fadd_rn(__fmul_rn(v.w, inv), b));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t abs_bits4(float4 v) {
+  return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+}
 __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
   const float4 v = make_float4((float)(int8_t)(w & 0xff), (float)(int8_t)((w >> 8) & 0xff),
                                (float)(int8_t)((w >> 16) & 0xff), (float)(int8_t)(w >> 24));
@@ -103,10 +115,10 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
 constexpr int kAppendKeep = 4;
 // Rows [chunk * d.chunk, + d.chunk): every block (run of rows of one sequence,
 // consecutive positions, one page) that starts there, for one K or V head.
-// Registers hold KEEP tokens of a block; a longer one is read and worked out
-// once for its maximum and once more for its codes.
+// KEEP tokens are worked out at a time; between the maximum and the codes those
+// of a longer block lie in `kept`, this lane's part of shared memory.
 template <typename T, int HD, int KEEP>
-__device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int h) {
+__device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int h, float4* kept) {
   constexpr int LPT = HD / 4, TPW = 32 / LPT, STEPS = KEEP / TPW;  // lanes per token, tokens per step
   const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
   const bool upper = (lane % LPT) >= LPT / 2;
@@ -144,7 +156,7 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
     int8_t* codes = block_codes(c, page, which, h);
     const float had = slot0 ? *sp : 0.0f;
     float4 x[STEPS];
-    float big = 0.0f;
+    uint32_t most = 0;  // the largest |value|'s bits, above those of FLT_MAX if one is not finite
     // the angles of a step's token (none: 1 and 0)
     auto angles = [&](int t, float4& cs, float4& sn) {
       const int rp = __shfl_sync(kFull, rope, min(31, i + t));
@@ -153,7 +165,7 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
       if (t >= n) return;
       if (rp >= 0 && rp < d.rope_rows) {
         cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
-        sn = load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+        sn = signed_sin(load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2)), upper);
       } else {
         raise(d.flags, QTTS_KV8_ROPE_RANGE);
       }
@@ -183,17 +195,34 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
         if (turn) {
           const float4 c0 = cs, s0 = sn;
           if (s + 1 < STEPS && t0 + (s + 1) * TPW < n) angles(t0 + (s + 1) * TPW + sub, cs, sn);
-          x[s] = rotate<HD>(x[s], c0, s0, upper);
+          x[s] = rotate<HD>(x[s], c0, s0);
         }
-        if (t0 + s * TPW + sub < n)
-          big = fmaxf(big, fmaxf(fmaxf(finite_abs(x[s].x), finite_abs(x[s].y)),
-                                 fmaxf(finite_abs(x[s].z), finite_abs(x[s].w))));
+        if (t0 + s * TPW + sub < n) most = max(most, abs_bits4(x[s]));
+        if (n > KEEP) kept[(t0 / TPW + s) * 32] = x[s];
       }
+    };
+    auto each = [&](auto f) {  // f(x, token) for what this lane holds
+#pragma unroll 1
+      for (int t0 = 0; t0 < n; t0 += KEEP)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          const int t = t0 + s * TPW + sub;
+          if (t < n) f(n > KEEP ? kept[(t0 / TPW + s) * 32] : x[s], t);
+        }
     };
 #pragma unroll 1
     for (int t0 = 0; t0 < n; t0 += KEEP) tokens(t0);
+    most = __reduce_max_sync(kFull, most);
+    float big = __uint_as_float(most);
+    const bool finite = most <= 0x7f7fffffu;
+    if (!finite) {
+      big = 0.0f;
+      each([&](float4 v, int) {
+        big = fmaxf(big, fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
+      });
 #pragma unroll
-    for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, o));
+      for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, o));
+    }
     // 127 steps to the largest value; the floor keeps 1 / scale finite
     const float need = big > 0.0f ? fmaxf(__fmul_rn(big, (float)(1.0 / 127.0)), FLT_MIN) : 0.0f;
     float scale = need;
@@ -211,15 +240,9 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
       }
     }
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-#pragma unroll 1
-    for (int t0 = 0; t0 < n; t0 += KEEP) {
-      if (n > KEEP) tokens(t0);
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int t = t0 + s * TPW + sub;
-        if (t < n) *reinterpret_cast<uint32_t*>(codes + (slot0 + t) * HD + d0) = codes4(x[s], inv);
-      }
-    }
+    auto put = [&](int t, uint32_t w) { *reinterpret_cast<uint32_t*>(codes + (slot0 + t) * HD + d0) = w; };
+    if (finite) each([&](float4 v, int t) { put(t, small_codes4(v, inv)); });
+    else each([&](float4 v, int t) { put(t, codes4(v, inv)); });
     if (lane == 0) *sp = scale;
   }
 }
@@ -246,7 +269,7 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
     turn = rp >= 0 && rp < d.rope_rows;
     if (turn) {
       cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
-      sn = load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+      sn = signed_sin(load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2)), upper);
     } else {
       raise(d.flags, QTTS_KV8_ROPE_RANGE);
     }
@@ -255,7 +278,7 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int h = h0 + i * TPW + sub;
-    if (turn) x[i] = rotate<HD>(x[i], cs, sn, upper);
+    if (turn) x[i] = rotate<HD>(x[i], cs, sn);
     if (h < d.heads) store4(dst + (size_t)h * HD + d0, x[i]);
   }
 }
@@ -269,10 +292,12 @@ template <typename T, int HD, int KEEP, int NH>
 __global__ void __launch_bounds__(128) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int kSteps = kKv8Page * HD / 128;  // float4 of a lane for a block's tokens
+  __shared__ float4 s_kept[4][kSteps][32];
   const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (w < d.kv_warps) {
     const int per = 2 * d.c.kv_heads, j = (int)(w % per);
-    append_blocks<T, HD, KEEP>(d, (int)(w / per), j & 1, j >> 1);
+    append_blocks<T, HD, KEEP>(d, (int)(w / per), j & 1, j >> 1, &s_kept[threadIdx.x >> 5][0][threadIdx.x & 31]);
   } else {
     const int per = (d.heads + NH - 1) / NH;
     const long i = w - d.kv_warps;
