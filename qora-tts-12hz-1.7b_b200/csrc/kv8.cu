@@ -109,6 +109,12 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
   return codes4(v, ratio);
 }
 
+// four elements as they lie in memory
+template <typename T>
+struct alignas(4 * sizeof(T)) Raw4 {
+  uint32_t w[sizeof(T)];
+};
+
 // Tokens of a block that registers hold in a chunk of a prompt.  16 chunks of
 // 611 rows: 66 us with 4; 122, 78 and 73 us with 16, 8 and 2 (fewer need more
 // passes, more leave fewer warps an SM to hide the loads).
@@ -170,14 +176,20 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
         raise(d.flags, QTTS_KV8_ROPE_RANGE);
       }
     };
+    Raw4<T> raw[STEPS];  // the next tokens, on their way while the ones before are worked on
+    const T* from = src + (size_t)(first + i + sub) * ld + (size_t)h * HD + d0;
+    auto read = [&](int t0) {
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        raw[s] = Raw4<T>{};
+        if (t0 + s * TPW + sub < n) raw[s] = *reinterpret_cast<const Raw4<T>*>(from + (size_t)(t0 + s * TPW) * ld);
+      }
+    };
     // x = tokens t0 .. t0 + KEEP of the block, normed and rotated; their largest
     auto tokens = [&](int t0) {
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int t = t0 + s * TPW + sub;
-        x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (t < n) x[s] = load4(src + (size_t)(first + i + t) * ld + (size_t)h * HD + d0);
-      }
+      for (int s = 0; s < STEPS; ++s) x[s] = load4(reinterpret_cast<const T*>(&raw[s]));
+      if (t0 + KEEP < n) read(t0 + KEEP);
       float4 cs, sn;
       if (turn) angles(t0 + sub, cs, sn);  // (of each step while the one before is worked on)
       if (which == 0 && d.k_norm) {
@@ -210,6 +222,7 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
           if (t < n) f(n > KEEP ? kept[(t0 / TPW + s) * 32] : x[s], t);
         }
     };
+    read(0);
 #pragma unroll 1
     for (int t0 = 0; t0 < n; t0 += KEEP) tokens(t0);
     most = __reduce_max_sync(kFull, most);
