@@ -260,10 +260,12 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
   }
 }
 
-// NH query heads of one row, from h0 on.
-template <typename T, int HD, int NH>
+constexpr int kQHeads = 4;  // query heads of a warp
+
+// kQHeads query heads of one row, from h0 on.
+template <typename T, int HD>
 __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
-  constexpr int LPT = HD / 4, TPW = 32 / LPT, N = NH / TPW;
+  constexpr int LPT = HD / 4, TPW = 32 / LPT, N = kQHeads / TPW;
   const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
   const bool upper = (lane % LPT) >= LPT / 2;
   const int seq = d.seq[row], pos = d.pos[row], rp = d.rope_pos ? d.rope_pos[row] : pos;
@@ -297,12 +299,12 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
 }
 
 // A warp takes the blocks that start in a chunk of rows, for one K or V head
-// (they are its alone: the block's scale needs all of its new tokens), or NH
-// query heads of one row.  HBM-bound: every input is read from HBM once, every
+// (they are its alone: the block's scale needs all of its new tokens), or
+// kQHeads query heads of one row.  HBM-bound: every input is read from HBM once, every
 // output written once, and a block that grows has its earlier codes read and
 // written again.
-template <typename T, int HD, int KEEP, int NH>
-__global__ void __launch_bounds__(128) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
+template <typename T, int HD, int KEEP>
+__global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kSteps = kKv8Page * HD / 128;  // float4 of a lane for a block's tokens
@@ -312,9 +314,9 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const __grid_constant__
     const int per = 2 * d.c.kv_heads, j = (int)(w % per);
     append_blocks<T, HD, KEEP>(d, (int)(w / per), j & 1, j >> 1, &s_kept[threadIdx.x >> 5][0][threadIdx.x & 31]);
   } else {
-    const int per = (d.heads + NH - 1) / NH;
+    const int per = (d.heads + kQHeads - 1) / kQHeads;
     const long i = w - d.kv_warps;
-    if (per > 0 && i < (long)d.n_rows * per) rotate_queries<T, HD, NH>(d, (int)(i / per), (int)(i % per) * NH);
+    if (per > 0 && i < (long)d.n_rows * per) rotate_queries<T, HD>(d, (int)(i / per), (int)(i % per) * kQHeads);
   }
 }
 
@@ -737,11 +739,9 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
 
 template <typename T, int HD>
 cudaError_t launch_append_t(const Kv8AppendDesc& d, bool single, cudaStream_t st) {
-  auto run = [&](auto kernel, int nh) {
-    const long warps = d.kv_warps + (d.q ? (long)d.n_rows * ((d.heads + nh - 1) / nh) : 0);
-    return launch_k(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, st, LaunchOpts{true, 1}, d);
-  };
-  return single ? run(kv8_append_kernel<T, HD, 128 / HD, 4>, 4) : run(kv8_append_kernel<T, HD, kAppendKeep, 8>, 8);
+  const long warps = d.kv_warps + (d.q ? (long)d.n_rows * ((d.heads + kQHeads - 1) / kQHeads) : 0);
+  const auto kernel = single ? kv8_append_kernel<T, HD, 128 / HD> : kv8_append_kernel<T, HD, kAppendKeep>;
+  return launch_k(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, st, LaunchOpts{true, 1}, d);
 }
 // Splits of a unit's pages: doubled while the CTAs do not fill the device
 // (twelve warps an SM) and every warp keeps kStep pages.  Clusters of 16 need
@@ -767,9 +767,23 @@ cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, 
     while (ns < 16 && units * ns * 2 * warps <= 12l * sms && pages >= (int)ns * 2 * warps * kStep) ns *= 2;
     return ns;
   };
-  // few units over long caches: clusters of 16 CTAs of 4 warps leave two
-  // thirds of the SMs' warps unused, CTAs of 12 warps fill them
-  if (units * 16 * 4 < 6l * sms && pages >= 16 * 12) return launch_attn_w<T, HD, 12>(d, units, splits(12), st);
+  // Few units over long caches: clusters of 16 CTAs of 4 warps leave two thirds
+  // of the SMs' warps unused, CTAs of 12 warps, one an SM, fill them.  Clusters
+  // of up to 16, as many as there are units, have to fit the GPU's processing
+  // clusters at once: 8 units over 32003 positions take 42 us with 16 CTAs each
+  // (two waves) and 29 with the 10 that fit.
+  if (units * 16 * 4 < 6l * sms && pages >= 16 * 12) {
+    unsigned ns = 16;
+    for (; ns > 8; --ns) {
+      g_occ_query = true;
+      g_occ_clusters = 0;
+      const cudaError_t e = launch_attn_w<T, HD, 12>(d, units, ns, st);
+      g_occ_query = false;
+      if (e != cudaSuccess) return e;
+      if (g_occ_clusters >= units) break;
+    }
+    return launch_attn_w<T, HD, 12>(d, units, ns, st);
+  }
   return launch_attn_w<T, HD, 4>(d, units, splits(4), st);
 }
 
