@@ -361,7 +361,6 @@ __device__ __forceinline__ void limbs4(float4 v, float up, uint32_t& w0, uint32_
   }
 }
 constexpr int kSlots = 8;
-constexpr int kTileSlots = 32;  // query heads of a sequence's rows from which the tile kernel takes over
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -743,9 +742,8 @@ cudaError_t launch_append_t(const Kv8AppendDesc& d, bool single, cudaStream_t st
   const auto kernel = single ? kv8_append_kernel<T, HD, 128 / HD> : kv8_append_kernel<T, HD, kAppendKeep>;
   return launch_k(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, st, LaunchOpts{true, 1}, d);
 }
-// Splits of a unit's pages: doubled while the CTAs do not fill the device
-// (twelve warps an SM) and every warp keeps kStep pages.  Clusters of 16 need
-// an opt-in.
+// NW warps a CTA, a unit's pages split over clusters of ns CTAs (more than 8
+// need an opt-in).
 template <typename T, int HD, int NW>
 cudaError_t launch_attn_w(const Kv8AttnDesc& d, long units, unsigned ns, cudaStream_t st) {
   constexpr int smem = NW * Ring<HD>::kWarp;
@@ -761,30 +759,47 @@ cudaError_t launch_attn_w(const Kv8AttnDesc& d, long units, unsigned ns, cudaStr
                   d);
 }
 template <typename T, int HD>
-cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, cudaStream_t st) {
-  auto splits = [&](int warps) {
-    unsigned ns = 1;
-    while (ns < 16 && units * ns * 2 * warps <= 12l * sms && pages >= (int)ns * 2 * warps * kStep) ns *= 2;
-    return ns;
-  };
-  // Few units over long caches: clusters of 16 CTAs of 4 warps leave two thirds
-  // of the SMs' warps unused, CTAs of 12 warps, one an SM, fill them.  Clusters
-  // of up to 16, as many as there are units, have to fit the GPU's processing
-  // clusters at once: 8 units over 32003 positions take 42 us with 16 CTAs each
-  // (two waves) and 29 with the 10 that fit.
-  if (units * 16 * 4 < 6l * sms && pages >= 16 * 12) {
-    unsigned ns = 16;
-    for (; ns > 8; --ns) {
-      g_occ_query = true;
-      g_occ_clusters = 0;
-      const cudaError_t e = launch_attn_w<T, HD, 12>(d, units, ns, st);
-      g_occ_query = false;
-      if (e != cudaSuccess) return e;
-      if (g_occ_clusters >= units) break;
-    }
-    return launch_attn_w<T, HD, 12>(d, units, ns, st);
+cudaError_t launch_attn_by(const Kv8AttnDesc& d, long units, int warps, unsigned ns, cudaStream_t st) {
+  switch (warps) {
+    case 12: return launch_attn_w<T, HD, 12>(d, units, ns, st);
+    case 4: return launch_attn_w<T, HD, 4>(d, units, ns, st);
+    case 3: return launch_attn_w<T, HD, 3>(d, units, ns, st);
+    default: return launch_attn_w<T, HD, 2>(d, units, ns, st);
   }
-  return launch_attn_w<T, HD, 4>(d, units, splits(4), st);
+}
+// clusters of such a launch that fit the device at once
+template <typename T, int HD>
+long attn_clusters(const Kv8AttnDesc& d, long units, int warps, unsigned ns, cudaStream_t st) {
+  g_occ_query = true;
+  g_occ_clusters = 0;
+  const cudaError_t e = launch_attn_by<T, HD>(d, units, warps, ns, st);
+  g_occ_query = false;
+  return e == cudaSuccess ? g_occ_clusters : 0;
+}
+template <typename T, int HD>
+cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, cudaStream_t st) {
+  // CTAs that fit the device at once (12 warps an SM), of the fewest steps a
+  // warp, a cluster counting like 0.4 of a step and a warp more like 0.07: 8
+  // units of 17 pages take 7.0 us as 4 x 4 warps, 7.6 as 12; 512 units of 19
+  // pages 15.0 us with 3 warps, 17.4 with 2, 20.1 with 4 (two waves); 8 units of
+  // 2001 pages 29 us as 10 x 12 warps.  Clusters of more than 8 have to fit the
+  // GPU's processing clusters (16 x 12 warps: two waves, 42 us).
+  int best_w = 0;
+  unsigned best_n = 1;
+  double best = 1e30;
+  for (const int w : {12, 4, 3, 2})
+    for (unsigned n = 1; n <= 16 && units * n <= (long)(12 / w) * sms && (n == 1 || (int)n * w <= pages); ++n) {
+      const int each = (pages + (int)n * w - 1) / ((int)n * w);
+      const double t = (each + kStep - 1) / kStep + (n > 1 ? 0.4 : 0.0) + 0.07 * w;
+      if (t >= best || (n > 8 && attn_clusters<T, HD>(d, units, w, n, st) < units)) continue;
+      best = t;
+      best_w = w;
+      best_n = n;
+    }
+  // More units than that: small CTAs where a unit is short (2048 units of 19
+  // pages: 48 us with 2 warps, 58 with 4; of 192 pages: 326 and 296).
+  if (best_w == 0) best_w = pages <= 32 ? 2 : 4;
+  return launch_attn_by<T, HD>(d, units, best_w, best_n, st);
 }
 
 }  // namespace
@@ -810,11 +825,29 @@ cudaError_t launch_kv8_append(Kv8AppendDesc d, int dtype, int sms, cudaStream_t 
 
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st) {
   const int group = d.heads / d.c.kv_heads;
-  if ((long)max_rows * group >= kTileSlots) return launch_kv8_tile(d, dtype, max_rows, max_len, sms, st);
   d.unit_heads = std::min(group, kSlots);
   d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
   d.group_rows = std::max(1, std::min(max_rows, kSlots / d.unit_heads));
   const long units = ((long)d.n_rows + d.group_rows - 1) / d.group_rows * d.c.kv_heads * d.head_chunks;
+  // what a unit of `rows` rows sees: the mean of a causal chunk, or its window
+  auto seen = [&](int rows) {
+    const long mean = std::max(1l, (long)max_len - max_rows / 2);
+    return d.window > 0 ? std::min(mean, (long)d.window + rows - 1) : mean;
+  };
+  // Units of 8 slots here, or tiles of 128 (kv8_tile.cu)?  Both as measured, in
+  // us: a unit costs 0.0085 and 0.0009 a page (of 128 dims) over 7; a CTA of
+  // tiles 10 and 2.2 a tile over 4, one an SM at a time.  One sequence's 100
+  // rows over 100 positions (16 heads, 8 K/V heads of 128): 10.3 here and 16 in
+  // tiles; 8 such sequences: 27 and 16; 4 of 64 rows over 4000: 102 and 45; 16
+  // rows over 1000: 12 and 20; 500 rows of 16 heads of 64, window 72: 13.5 and 20.
+  if (max_rows > 1) {
+    const double here = 7.0 + units * (0.0085 + 0.0009 * d.c.head_dim / 128 * ((seen(d.group_rows) + kKv8Page - 1) / kKv8Page));
+    Kv8AttnDesc t = d;
+    const TilePlan plan = plan_kv8_tile(t, dtype, max_rows, max_len, sms);
+    const long tiles = (seen(t.group_rows) + 127) / 128, waves = (plan.units * plan.splits + sms - 1) / sms;
+    if (4.0 + waves * (10.0 + 2.2 * t.halves * ((tiles + plan.splits - 1) / plan.splits)) < here)
+      return launch_kv8_tile(t, plan, dtype, st);
+  }
   const int pages = (max_len + kKv8Page - 1) / kKv8Page;
   const bool w = d.c.head_dim == 128;
   switch (dtype) {

@@ -79,6 +79,12 @@ struct Kv8AttnDesc {
 };
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st);
 // The same for many rows: tiles of 128 slots on the tensor cores (kv8_tile.cu).
-cudaError_t launch_kv8_tile(Kv8AttnDesc d, int dtype, int max_rows, int len, int sms, cudaStream_t st);
+// The plan fills the descriptor's shape of a unit.
+struct TilePlan {
+  long units;
+  unsigned splits;  // CTAs of a cluster that share a unit's positions
+};
+TilePlan plan_kv8_tile(Kv8AttnDesc& d, int dtype, int max_rows, int max_len, int sms);
+cudaError_t launch_kv8_tile(const Kv8AttnDesc& d, const TilePlan& plan, int dtype, cudaStream_t st);
 
 }  // namespace qtts

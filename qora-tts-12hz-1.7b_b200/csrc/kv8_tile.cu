@@ -40,7 +40,7 @@ namespace qtts {
 
 namespace {
 
-constexpr int kTileM = 128, kTileN = 128, kTilePages = kTileN / kKv8Page;
+constexpr int kTileM = 128, kTilePos = 128, kTilePages = kTilePos / kKv8Page;
 constexpr int kSoft = 256, kConvert = 128;  // threads of the softmax (two halves) and of the conversion
 constexpr int kTileThreads = kSoft + kConvert + 32;  // and a warp that issues the products
 constexpr uint32_t kTmemCols = 512;  // half h: S and P at 256 h, O at 256 h + 128
@@ -53,7 +53,7 @@ struct TileSegment {
 struct TileShared {
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2];  // by buffer
   uint64_t s_full[2], p_full[2], o_full[2];             // by half
-  uint64_t fin;
+  uint64_t q_full, fin;
   uint32_t tmem;
   int abort;
   int n_segments;
@@ -340,7 +340,7 @@ struct Products {
   // S = Q K^T of half h with K of buffer b; last: no other half reads this K
   __device__ __forceinline__ bool score(int h, int b, bool last) const {
     TileShared& sh = job.sh;
-    constexpr uint32_t idesc = instruction(kTileN, false);
+    constexpr uint32_t idesc = instruction(kTilePos, false);
     // P of the half's tile before lies where S goes
     if (done[h] > 0 && !warp_wait(&sh.o_full[h], (done[h] - 1) & 1, &sh.abort)) return false;
     if (lane == 0) {
@@ -371,10 +371,10 @@ struct Products {
     if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
     ++done[h];
     if (lane == 0) {
-      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h, o = s + kTileN;
+      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h, o = s + kTilePos;
       tc_fence_after();
 #pragma unroll
-      for (int e = 0; e < kTileN / 16; ++e) {
+      for (int e = 0; e < kTilePos / 16; ++e) {
         const uint32_t p = s + 32 * (e >> 1) + 8 * (e & 1);
         mma_ts(o, p, operand(v + e * 256, 2048), idesc, !first || e > 0);
         if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
@@ -456,7 +456,7 @@ __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, 
       }
     }
   }
-  grow_to<HD>(mon, r.mo, s + kTileN);
+  grow_to<HD>(mon, r.mo, s + kTilePos);
   const float mz = mn == -INFINITY ? 0.0f : mn;
   r.l *= ex2(r.m - mz);
   r.m = mn;
@@ -514,7 +514,7 @@ struct Softmax {
     float big = 0.0f;
     bool finite = true;
     if (on) {
-#pragma unroll 8
+#pragma unroll 16
       for (int c = 0; c < HD / 4; ++c) {
         const float4 x = load4(src + 4 * c);
         const float a = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
@@ -591,7 +591,7 @@ struct Softmax {
       tmem_wait(r[0], x);  // the load on its way
       return false;
     }
-    grow_to<HD>(mon, mo, s + kTileN);
+    grow_to<HD>(mon, mo, s + kTilePos);
     l *= ex2(m - mn);
     m = mn;
 #pragma unroll
@@ -640,7 +640,7 @@ struct Softmax {
       tc_fence_after();
       const float4* sc = sh.scale[it % kScales];
       // a slot of another segment has no say: its row is never read
-      const bool all = !mine || (see_lo <= at && see_hi >= at + kTileN);
+      const bool all = !mine || (see_lo <= at && see_hi >= at + kTilePos);
       if (!__all_sync(kFull, all) || !tile_short(sc)) {
         const Running r = tile_long<HD, C::kSplit>(Running{m, mo, l}, columns(), (unsigned)(at - see_lo),
                                                    (unsigned)(see_hi - see_lo), qs, sc);
@@ -667,7 +667,7 @@ struct Softmax {
     for (int c = 0; c < HD / 32; ++c) {
       float x[32];
       if (any) {
-        tmem_load(columns() + kTileN + 32 * c, x);
+        tmem_load(columns() + kTilePos + 32 * c, x);
 #pragma unroll
         for (int e = 0; e < 32; ++e) x[e] *= back;
       } else {
@@ -741,6 +741,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bar_init(&sh.p_full[i], kTileM);
       bar_init(&sh.o_full[i], 1);
     }
+    bar_init(&sh.q_full, kTileM * d.halves);
     bar_init(&sh.fin, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.abort = 0;
@@ -780,10 +781,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   Softmax<T, HD> soft(job);
   const bool softmax = tid < kTileM * d.halves;  // (the second half's warps have nothing to do with one half)
-  if (softmax) {
-    soft.put_query();
-    smem_to_async();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -793,6 +790,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   Products<T, HD> products(job);
   bool ok = true;
   int it = 0;
+  if (softmax) {  // (while the first codes are on their way)
+    soft.put_query();
+    smem_to_async();
+    bar_arrive(&sh.q_full);
+  }
+  if (warp == kLast) ok = warp_wait(&sh.q_full, 0, &sh.abort);
   for (int g = 0; g < sh.n_segments; ++g) {
     const TileSegment seg = sh.segment[g];
     if (seg.seq < 0) continue;  // padding
@@ -871,47 +874,48 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 }
 
 template <typename T, int HD>
-cudaError_t launch_tile_t(const Kv8AttnDesc& d, long units, int len, int sms, cudaStream_t st) {
+cudaError_t launch_tile_t(const Kv8AttnDesc& d, const TilePlan& plan, cudaStream_t st) {
   using C = TileCfg<T, HD>;
   static std::atomic<int> ready[kMaxDevices];
   const cudaError_t set = once_per_device(ready, [] {
     return cudaFuncSetAttribute(kv8_tile_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   if (set != cudaSuccess) return set;
-  // the cache is split while the CTAs do not fill the device and keep two tiles
-  unsigned ns = 1;
-  const int tiles = (len + kTileN - 1) / kTileN;
-  while (ns < 8 && units * ns * 2 <= sms && tiles >= (int)ns * 4) ns *= 2;
-  return launch_k(kv8_tile_kernel<T, HD>, dim3((unsigned)units, ns), dim3(kTileThreads), (size_t)C::kSmem, st,
-                  LaunchOpts{true, ns}, d);
+  return launch_k(kv8_tile_kernel<T, HD>, dim3((unsigned)plan.units, plan.splits), dim3(kTileThreads), (size_t)C::kSmem,
+                  st, LaunchOpts{true, plan.splits}, d);
 }
 
 }  // namespace
 
-cudaError_t launch_kv8_tile(Kv8AttnDesc d, int dtype, int max_rows, int len, int sms, cudaStream_t st) {
+TilePlan plan_kv8_tile(Kv8AttnDesc& d, int dtype, int max_rows, int max_len, int sms) {
   const int group = d.heads / d.c.kv_heads;
   d.unit_heads = std::min(group, kTileM);
   d.head_chunks = (group + d.unit_heads - 1) / d.unit_heads;
   // Rows of a unit: what its slots hold, or a sequence's rows in equal shares.
   // Two halves (16-bit rows) where the units still fill the device.
-  long units = 0;
+  TilePlan plan{0, 1};
   for (d.halves = dtype == DT_F32 ? 1 : 2;; d.halves = 1) {
     const int most = d.halves * kTileM / d.unit_heads, parts = (max_rows + most - 1) / most;
     d.group_rows = std::min(most, (max_rows + parts - 1) / parts);
     d.seq_units = (max_rows + d.group_rows - 1) / d.group_rows;
     const long all = ((long)d.n_rows + d.group_rows - 1) / d.group_rows;
-    units = (all + d.seq_units - 1) / d.seq_units * d.seq_units * d.c.kv_heads * d.head_chunks;
-    if (d.halves == 1 || (units >= sms && d.group_rows * d.unit_heads > kTileM)) break;
+    plan.units = (all + d.seq_units - 1) / d.seq_units * d.seq_units * d.c.kv_heads * d.head_chunks;
+    if (d.halves == 1 || (plan.units >= sms && d.group_rows * d.unit_heads > kTileM)) break;
   }
+  // the positions are split while the CTAs do not fill the device and keep two tiles
+  const int seen = d.window > 0 ? (int)std::min<long>(max_len, (long)d.window + d.group_rows - 1) : max_len;
+  const int tiles = (seen + kTilePos - 1) / kTilePos;
+  while (plan.splits < 8 && plan.units * plan.splits * 2 <= sms && tiles >= (int)plan.splits * 4) plan.splits *= 2;
+  return plan;
+}
+
+cudaError_t launch_kv8_tile(const Kv8AttnDesc& d, const TilePlan& plan, int dtype, cudaStream_t st) {
   const bool w = d.c.head_dim == 128;
   switch (dtype) {
-    case DT_F16:
-      return w ? launch_tile_t<__half, 128>(d, units, len, sms, st) : launch_tile_t<__half, 64>(d, units, len, sms, st);
+    case DT_F16: return w ? launch_tile_t<__half, 128>(d, plan, st) : launch_tile_t<__half, 64>(d, plan, st);
     case DT_BF16:
-      return w ? launch_tile_t<__nv_bfloat16, 128>(d, units, len, sms, st)
-               : launch_tile_t<__nv_bfloat16, 64>(d, units, len, sms, st);
-    default:
-      return w ? launch_tile_t<float, 128>(d, units, len, sms, st) : launch_tile_t<float, 64>(d, units, len, sms, st);
+      return w ? launch_tile_t<__nv_bfloat16, 128>(d, plan, st) : launch_tile_t<__nv_bfloat16, 64>(d, plan, st);
+    default: return w ? launch_tile_t<float, 128>(d, plan, st) : launch_tile_t<float, 64>(d, plan, st);
   }
 }
 

@@ -350,6 +350,112 @@ def test_long_caches(qtts, length, rows):
     check_attention(qtts, p, rng, seq, pos, 2, "f32", max_rows=rows)
 
 
+# Enough rows that tiles of 128 slots take over (the choice weighs the units of
+# eight slots against them), with everything that can go wrong in a tile.
+MANY = [(0, 57, 100), (-1, 3, 4), (1, 0, 130), (2, 300, 99), (3, -5, 60), (3, 55, 40), (-1, 0, 33), (4, 399, 1), (5, 128, 128),
+        (6, 1, 97), (0, 0, 64), (7, 250, 150)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,heads,kvh", [(128, 16, 8), (64, 16, 16), (128, 16, 1), (64, 12, 4)])
+@pytest.mark.parametrize("window", [0, 20, 200])
+def test_tiles(qtts, hd, heads, kvh, dtype, window):
+    rng = np.random.default_rng(hd + heads + window)
+    p = Pool(qtts, rng, 8, 25, kvh, hd, layers=2)
+    seq, pos = rows_of(MANY)
+    check_attention(qtts, p, rng, seq, pos, heads, dtype, window=window, max_rows=100, max_len=400, ldx=8)
+
+
+@pytest.mark.parametrize("dtype,halves", [("f32", 1), ("bf16", 1), ("bf16", 2)])
+def test_tiles_split_and_whole(qtts, dtype, halves):
+    # few units over long caches, whose positions a cluster shares; and so many
+    # that a CTA takes two halves
+    rng = np.random.default_rng(halves)
+    if halves == 1:
+        p = Pool(qtts, rng, 2, 190, 2, 128)
+        seq, pos = rows_of([(1, 2600, 400), (0, 500, 11)])
+        check_attention(qtts, p, rng, seq, pos, 4, dtype, max_rows=400)
+    else:
+        p = Pool(qtts, rng, 12, 40, 8, 64)
+        seq, pos = rows_of([(s, 200 + 7 * s, 256) for s in range(12)])
+        check_attention(qtts, p, rng, seq, pos, 16, dtype, max_rows=256)
+
+
+def test_tiles_of_scales_far_apart(qtts):
+    rng = np.random.default_rng(21)
+    p = Pool(qtts, rng, 8, 20, 8, 64)
+    p.scales[:, 1] *= (10.0 ** rng.integers(-9, 10, p.scales[:, 1].shape)).astype(np.float32)
+    p.scales[p.table[0, 2], 1] = 0.0
+    p.scales[p.table[0, 3], 0] = 0.0
+    p.scales[p.table[1, :12], 1] = 0.0
+    p.scales[p.table[2, 5], 0] *= -1.0  # no append makes a negative scale, but its value is defined
+    p.scales[p.table[:, 19]] = np.nan
+    p.d_scales[:, 0] = dev(p.scales)
+    seq, pos = rows_of([(s, 203, 100) for s in range(8)])
+    for dtype in ("f32", "bf16"):
+        check_attention(qtts, p, rng, seq, pos, 16, dtype, max_rows=100)
+    check_attention(qtts, p, rng, seq, pos, 16, "f32", max_rows=100, scale=-0.05)
+
+
+def test_tiles_keep_not_a_number_and_bad_pages_apart(qtts):
+    rng = np.random.default_rng(22)
+    p = Pool(qtts, rng, 8, 14, 8, 64)
+    seq, pos = rows_of([(s, 100, 100) for s in range(8)])
+    p.table[3, 4] = -1
+    p.table[5, 12] = 1 << 30
+    p.d_table.copy_(dev(p.table))
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check_attention(qtts, p, rng, seq, pos, 16, "f32", max_rows=100, flags=flags)
+    assert flags.item() == qtts.KV8_BAD_PAGE
+    seq = seq.copy()
+    pos = pos.copy()
+    seq[200:210], pos[777] = 8, 14 * 16
+    flags.zero_()
+    q = rng.standard_normal((800, 16 * 64)).astype(np.float32)
+    big = dev(q)
+    big[100, 5] = float("nan")
+    big[333, 64 * 7] = float("-inf")
+    out = torch.full_like(big, 5.0)
+    t = dev(seq.astype(np.int32)), dev(pos.astype(np.int32))
+    qtts.kv8_attention_dev(p.cache, big.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), 800, 16,
+                           max_rows=100, flags_ptr=flags.data_ptr())
+    torch.cuda.synchronize()
+    assert flags.item() == qtts.KV8_BAD_PAGE | qtts.KV8_BAD_ROW
+    nan = torch.isnan(out.view(800, 16, 64)).all(-1)
+    assert bool(nan[100, 0]) and bool(nan[333, 7]) and int(torch.isnan(out).sum()) == 128
+    assert bool((out[200:210] == 5.0).all())
+
+
+def test_tiles_in_a_graph_and_on_two_streams_at_once(qtts):
+    rng = np.random.default_rng(23)
+    p = Pool(qtts, rng, 8, 14, 8, 64)
+    seq, pos = rows_of([(s, 100, 100) for s in range(8)])
+    t = dev(seq), dev(pos)
+    q = [torch.randn(800, 1024, device="cuda") for _ in range(2)]
+    want = [torch.zeros_like(x) for x in q]
+    got = [torch.zeros_like(x) for x in q]
+
+    def call(i, out, stream):
+        qtts.kv8_attention_dev(p.cache, q[i].data_ptr(), out[i].data_ptr(), t[0].data_ptr(), t[1].data_ptr(), 800, 16,
+                               max_rows=100, stream=stream)
+
+    for i in range(2):
+        call(i, want, 0)
+    torch.cuda.synchronize()
+    st = [torch.cuda.Stream() for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], stream=st[i]):
+            for _ in range(3):
+                call(i, got, st[i].cuda_stream)
+    for _ in range(3):
+        for i in range(2):
+            with torch.cuda.stream(st[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_offsets_past_32_bits(qtts):
     # pages 400 MB apart: the last one lies past 4 GB of codes
     rng = np.random.default_rng(16)
