@@ -779,10 +779,10 @@ long attn_clusters(const Kv8AttnDesc& d, long units, int warps, unsigned ns, cud
 template <typename T, int HD>
 cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, cudaStream_t st) {
   // CTAs that fit the device at once (12 warps an SM), of the fewest steps a
-  // warp, a cluster counting like 0.4 of a step and a warp more like 0.07: 8
-  // units of 17 pages take 7.0 us as 4 x 4 warps, 7.6 as 12; 512 units of 19
-  // pages 15.0 us with 3 warps, 17.4 with 2, 20.1 with 4 (two waves); 8 units of
-  // 2001 pages 29 us as 10 x 12 warps.  Clusters of more than 8 have to fit the
+  // warp, a cluster of n counting like 0.4 + 0.1 n steps and a warp like 0.05:
+  // 512 units of 19 pages take 15.0 us with 3 warps, 17.4 with 2, 20.1 with 4
+  // (two waves); 128 units of 63 pages 16.5 us with 12 warps, 21.2 as 6 x 2; 256
+  // of 63 pages 21.6 us as 2 x 3, 23.6 with 4; 8 of 2001 pages 29 us as 10 x 12.  Clusters of more than 8 have to fit the
   // GPU's processing clusters (16 x 12 warps: two waves, 42 us).
   int best_w = 0;
   unsigned best_n = 1;
@@ -790,7 +790,7 @@ cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, 
   for (const int w : {12, 4, 3, 2})
     for (unsigned n = 1; n <= 16 && units * n <= (long)(12 / w) * sms && (n == 1 || (int)n * w <= pages); ++n) {
       const int each = (pages + (int)n * w - 1) / ((int)n * w);
-      const double t = (each + kStep - 1) / kStep + (n > 1 ? 0.4 : 0.0) + 0.07 * w;
+      const double t = (each + kStep - 1) / kStep + (n > 1 ? 0.4 + 0.1 * n : 0.0) + 0.05 * w;
       if (t >= best || (n > 8 && attn_clusters<T, HD>(d, units, w, n, st) < units)) continue;
       best = t;
       best_w = w;
@@ -836,7 +836,7 @@ cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max
   };
   // Units of 8 slots here, or tiles of 128 (kv8_tile.cu)?  Both as measured, in
   // us: a unit costs 0.0085 and 0.0009 a page (of 128 dims) over 7; a CTA of
-  // tiles 10 and 2.2 a tile over 4, one an SM at a time.  One sequence's 100
+  // tiles 10 and 2.2 a tile over 4 (10 with splits), one an SM at a time.  One sequence's 100
   // rows over 100 positions (16 heads, 8 K/V heads of 128): 10.3 here and 16 in
   // tiles; 8 such sequences: 27 and 16; 4 of 64 rows over 4000: 102 and 45; 16
   // rows over 1000: 12 and 20; 500 rows of 16 heads of 64, window 72: 13.5 and 20.
@@ -845,7 +845,7 @@ cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max
     Kv8AttnDesc t = d;
     const TilePlan plan = plan_kv8_tile(t, dtype, max_rows, max_len, sms);
     const long tiles = (seen(t.group_rows) + 127) / 128, waves = (plan.units * plan.splits + sms - 1) / sms;
-    if (4.0 + waves * (10.0 + 2.2 * t.halves * ((tiles + plan.splits - 1) / plan.splits)) < here)
+    if ((plan.splits > 1 ? 10.0 : 4.0) + waves * (10.0 + 2.2 * t.halves * ((tiles + plan.splits - 1) / plan.splits)) < here)
       return launch_kv8_tile(t, plan, dtype, st);
   }
   const int pages = (max_len + kKv8Page - 1) / kKv8Page;

@@ -685,6 +685,12 @@ __device__ __forceinline__ void store_row(T* p, const float (&x)[32], float mul)
   for (int e = 0; e < 32; e += 4)
     store4(p + e, make_float4(x[e] * mul, x[e + 1] * mul, x[e + 2] * mul, x[e + 3] * mul));
 }
+// A split's sums: dim e of slot s, groups of four dims changing places by the
+// slot, so that the slots of a warp write to eight places at once, not to one.
+template <int HD>
+__device__ __forceinline__ int sum_at(int s, int e) {
+  return s * HD + (e ^ ((s & 7) << 2));
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -827,7 +833,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     float* sums = reinterpret_cast<float*>(smem + C::kK);
     __syncthreads();
     if (softmax && job.takes(seg, soft.half)) {
-      soft.output(t1 > t0 && ok, [&](int e, const float(&x)[32]) { store_row(sums + soft.slot * HD + e, x, 1.0f); });
+      soft.output(t1 > t0 && ok, [&](int e0, const float(&x)[32]) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          store4(sums + sum_at<HD>(soft.slot, e0 + e), make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+      });
       sh.m[tid] = soft.l == soft.l ? soft.m : INFINITY;  // a NaN sum makes the join NaN
       sh.l[tid] = soft.l;
       tc_fence_before();
@@ -839,7 +849,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float mx = -INFINITY, sum = 0.0f, ll = 0.0f;
       for (int r = 0; r < job.nsplit; ++r) {
         const float rm = *cluster.map_shared_rank(&sh.m[s], r), rl = *cluster.map_shared_rank(&sh.l[s], r),
-                    ro = *cluster.map_shared_rank(&sums[s * HD + e], r);
+                    ro = *cluster.map_shared_rank(&sums[sum_at<HD>(s, e)], r);
         const float mn = fmaxf(mx, rm);
         if (mn == -INFINITY) continue;
         const float a = ex2(mx - mn), b = ex2(rm - mn);
