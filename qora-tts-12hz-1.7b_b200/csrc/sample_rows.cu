@@ -811,13 +811,20 @@ __device__ __forceinline__ uint32_t warp_bound_of(const uint32_t (&v)[N], unsign
 template <typename T>
 __device__ __forceinline__ uint32_t min_p_key(float min_p, uint32_t top, float temp, const Weigh& weigh) {
   const double zmin = log((double)fminf(min_p, 1.0f));
-  // the value in f64, one or two keys around its nearest T
-  uint32_t k = Key<T>::near((float)(weigh.top_d + zmin * (double)temp));
   if (weigh.infinite) return top;
-  k = min(max(k, Key<T>::kNone + 1), top);
-  while (k > Key<T>::kNone + 1 && weigh.z(Key<T>::value(k - 1)) >= zmin) --k;
-  while (k < top && !(weigh.z(Key<T>::value(k)) >= zmin)) ++k;
-  return k;
+  auto keeps = [&](uint32_t k) { return weigh.z(Key<T>::value(k)) >= zmin; };
+  // between a key that is not kept and one that is: mostly two keys around the
+  // nearest T of the value in f64
+  uint32_t lo = Key<T>::kNone, hi = top;
+  const uint32_t k = min(max(Key<T>::near((float)(weigh.top_d + zmin * (double)temp)), lo), hi);
+  if (k > lo + 2 && !keeps(k - 2)) lo = k - 2;
+  if (k + 2 < hi && keeps(k + 2)) hi = k + 2;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (keeps(mid)) hi = mid;
+    else lo = mid;
+  }
+  return hi;
 }
 
 template <typename T, int TH>

@@ -110,6 +110,23 @@ def test_special_logits(qtts):
         check(qtts, x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [300, 40000])
+def test_min_p_where_many_keys_weigh_the_same(qtts, V, dtype):
+    # an infinite temperature makes every finite logit the heaviest; a largest
+    # logit of -log(min_p) T puts the border next to zero, where logits are dense
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((10, V)).astype(np.float32)
+    x[:, ::7] = -np.inf
+    x[5:] = np.minimum(x[5:], 0.5) * np.float32(1e-7)
+    x[5:, 3] = np.float32(np.log(2.0))
+    u = rng.random(10).astype(np.float32)
+    T = np.array([np.inf] * 5 + [1.0] * 5, np.float32)
+    for m in (0.5, 1.0, 1e-6):
+        check(qtts, x, u, temperature=T, min_p=m, dtype=dtype)
+        check(qtts, x, u, temperature=T, min_p=m, top_k=20, dtype=dtype)
+
+
 def test_uniform_numbers_at_the_ends(qtts):
     rng = np.random.default_rng(6)
     u = np.array([0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, np.nan, 0.5, 1e-30], np.float32)
