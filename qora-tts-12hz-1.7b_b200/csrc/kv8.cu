@@ -611,7 +611,8 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       mo = mon;
 #pragma unroll
       for (int k = 0; k < kStep; ++k) {
-        const float fac = mon == -INFINITY ? 0.0f : ex2(fminf(mz - mon + ev[k], 120.0f)) * fr[k];
+        // (a page that the slot does not see has no say, even with an infinite or NaN scale)
+        const float fac = pm[k] == -INFINITY ? 0.0f : ex2(fminf(mz - mon + ev[k], 120.0f)) * fr[k];
         uint32_t pa[4];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -885,11 +886,11 @@ OnDeviceOf::OnDeviceOf(const void* p) {
     return;
   }
   if (cur != a.device) prev_ = cur;
-  static int sms[64] = {0};
-  int n = a.device >= 0 && a.device < 64 ? sms[a.device] : 0;
+  static std::atomic<int> sms[kMaxDevices];
+  int n = a.device >= 0 && a.device < kMaxDevices ? sms[a.device].load(std::memory_order_relaxed) : 0;
   if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, a.device) != cudaSuccess || n <= 0) n = 148;
-    if (a.device >= 0 && a.device < 64) sms[a.device] = n;
+    if (a.device >= 0 && a.device < kMaxDevices) sms[a.device].store(n, std::memory_order_relaxed);
   }
   sm_count = n;
 }

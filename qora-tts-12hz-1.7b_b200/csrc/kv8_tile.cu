@@ -45,6 +45,7 @@ constexpr int kSoft = 256, kConvert = 128;  // threads of the softmax (two halve
 constexpr int kTileThreads = kSoft + kConvert + 32;  // and a warp that issues the products
 constexpr uint32_t kTmemCols = 512;  // half h: S and P at 256 h, O at 256 h + 128
 constexpr unsigned long long kWaitNs = 1000000000ull;
+constexpr float kNoPage = 4.0f;  // no fraction of a scale (split_scale)
 constexpr int kScales = 4;  // tiles of scales kept: a half may be two tiles behind the conversion
 
 struct TileSegment {
@@ -59,7 +60,7 @@ struct TileShared {
   int n_segments;
   int seq[2 * kTileM], pos[2 * kTileM];
   TileSegment segment[2 * kTileM];
-  // K scale, exponent and fraction of the V scale (-1: no page), and log2 of the
+  // K scale, exponent and fraction of the V scale (kNoPage: none), and log2 of the
   // V scale; NaN keeps a page from the short way (Softmax::tile_short)
   float4 scale[kScales][kTilePages];
   float m[2 * kTileM], l[2 * kTileM];
@@ -306,7 +307,7 @@ struct Converter {
         float ev, fr;
         split_scale(sv, ev, fr);
         const bool plain = ids >= 0 && sk >= 0.0f && sv >= FLT_MIN && sv <= FLT_MAX;
-        sh.scale[it % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : -1.0f, plain ? log2f(sv) : NAN);
+        sh.scale[it % kScales][lane] = make_float4(sk, ev, ids >= 0 ? fr : kNoPage, plain ? log2f(sv) : NAN);
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");  // this thread's own copies
       put_k(b);
@@ -450,7 +451,7 @@ __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, 
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (from + 32 * c + 16 * q + e < width) pm = fmaxf(pm, x[16 * q + e] * f);
-      if (k.z != -1.0f) {
+      if (k.z != kNoPage) {
         mn = fmaxf(mn, pm);
         mon = fmaxf(mon, pm + k.y);
       }
@@ -470,15 +471,16 @@ __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, 
       const float4 k = sc[2 * c + q];
       const float f = qs * k.x;
       const float fac = r.mo == -INFINITY ? 0.0f : ex2(fminf(mz - r.mo + k.y, 120.0f)) * k.z;
-      const unsigned at = k.z != -1.0f ? from + 32 * c + 16 * q : 0x80000000u;  // (no width reaches it)
+      const unsigned at = k.z != kNoPage ? from + 32 * c + 16 * q : 0x80000000u;  // (no width reaches it)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         float p[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          p[j] = at + e + j < width ? ex2(fmaf(x[16 * q + e + j], f, -mz)) : 0.0f;
-          r.l += p[j];
-          p[j] *= fac;
+          const bool seen = at + e + j < width;
+          const float w = seen ? ex2(fmaf(x[16 * q + e + j], f, -mz)) : 0.0f;
+          r.l += w;
+          p[j] = seen ? w * fac : 0.0f;  // (fac may be infinite or NaN)
         }
         hi[8 * q + e / 2] = pack_half(p[0], p[1]);
         if (SPLIT) lo[8 * q + e / 2] = pack_rest(p[0], p[1], hi[8 * q + e / 2]);

@@ -350,6 +350,53 @@ def test_long_caches(qtts, length, rows):
     check_attention(qtts, p, rng, seq, pos, 2, "f32", max_rows=rows)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 100])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_page_out_of_sight_may_have_any_scale(qtts, rows, window):
+    # pages that some rows of a unit see and others do not, ahead of them or
+    # behind their window, with scales of NaN and infinity
+    rng = np.random.default_rng(16)
+    heads, hd, n_seqs = 16, 64, 8
+    p = Pool(qtts, rng, n_seqs, 20, 8, hd)
+    seq, pos = rows_of([(s, 156, rows) for s in range(n_seqs)])
+    q = rng.standard_normal((len(seq), heads * hd)).astype(np.float32)
+    good, _ = check_attention(qtts, p, rng, seq, pos, heads, "f32", window=window, max_rows=rows, q=q)
+    bad = np.zeros(20, bool)
+    bad[[2, 11]] = True
+    if not window:
+        bad[2] = False
+    p.d_scales[dev(p.table[::2, bad].astype(np.int64)).reshape(-1), 0, 1] = float("inf")
+    p.d_scales[dev(p.table[1::2, bad].astype(np.int64)).reshape(-1), 0] = float("nan")
+    out = torch.full_like(good, 5.0)
+    t = dev(q), dev(seq), dev(pos)
+    qtts.kv8_attention_dev(p.cache, t[0].data_ptr(), out.data_ptr(), t[1].data_ptr(), t[2].data_ptr(), len(seq), heads,
+                           window=window, scale=hd ** -0.5, max_rows=rows)
+    torch.cuda.synchronize()
+    lo = np.maximum(0, pos + 1 - window) if window else 0 * pos
+    clean = dev(~((bad[None] & (np.arange(20)[None] * 16 <= pos[:, None]) & (np.arange(20)[None] * 16 + 15 >= lo[:, None])).any(1)))
+    assert 0 < int(clean.sum()) and (rows < 100 or int(clean.sum()) < len(seq))
+    # either result is off by at most this (check_attention's bound, by the largest |q|_1 |k|)
+    vals = np.abs(p.codes.astype(np.float64)).max((3, 4)) * np.abs(p.scales)
+    most = hd ** -0.5 * np.abs(q).reshape(len(seq), heads, hd).sum(-1).max() * vals[:, 0].max()
+    tol = vals[:, 1].max() * (2 * most * (hd / 16 + 8) * 2.0 ** -23 + 2.0 ** -20 + (300 / 16 + 32) * 2.0 ** -23)
+    tol += HALF_STEP["f32"] * vals[:, 1].max()
+    assert bool(((out - good).abs()[clean] <= 2 * tol).all())
+    assert not bool(torch.isfinite(out[~clean]).all(-1).any())
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_negative_scales(qtts, rows):
+    # no append makes one, but its value is defined
+    rng = np.random.default_rng(17)
+    p = Pool(qtts, rng, 8, 20, 8, 64)
+    p.scales[::3, 1] = -1.0
+    p.scales[1::3, 1] = -0.03
+    p.scales[::5, 0] *= -1.0
+    p.d_scales[:, 0] = dev(p.scales)
+    seq, pos = rows_of([(s, 320 - rows - s, rows) for s in range(8)])
+    check_attention(qtts, p, rng, seq, pos, 16, "f32", max_rows=rows)
+
+
 # Enough rows that tiles of 128 slots take over (the choice weighs the units of
 # eight slots against them), with everything that can go wrong in a tile.
 MANY = [(0, 57, 100), (-1, 3, 4), (1, 0, 130), (2, 300, 99), (3, -5, 60), (3, 55, 40), (-1, 0, 33), (4, 399, 1), (5, 128, 128),
