@@ -106,6 +106,7 @@ __device__ __forceinline__ u64 place_of(uint32_t key, int index) { return ((u64)
 __device__ __forceinline__ uint32_t key_in(u64 place) { return (uint32_t)(place >> 32); }
 
 struct Weigh {
+  static constexpr double kStepsPerUnit = 46.166241308446828;  // 32 / ln 2
   float top;              // the largest logit
   float light;            // about top - 36 T: what lies below weighs nothing
   double top_d, inv_t;
@@ -125,10 +126,18 @@ struct Weigh {
   // z = n ln2/32 + r, exp(r) by its series to r^5 (|r| < 0.011: 2e-15),
   // 2^(n/32) by table and exponent
   __device__ __forceinline__ u64 finite(float l) const {
+    int n;
+    return finite(l, n);
+  }
+  // n of such a z: it never falls as l grows
+  __device__ __forceinline__ int steps(float l) const {
+    return __double2loint(__fma_rn(((double)l - top_d) * inv_t, kStepsPerUnit, 0x1.8p52));
+  }
+  __device__ __forceinline__ u64 finite(float l, int& n) const {
     const double x = ((double)l - top_d) * inv_t;
     const double shift = 0x1.8p52;
-    const double nd = __fma_rn(x, 46.166241308446828, shift);  // 32 / ln 2
-    const int n = __double2loint(nd);
+    const double nd = __fma_rn(x, kStepsPerUnit, shift);
+    n = __double2loint(nd);
     const double r = __fma_rn(nd - shift, -0.021660849392498290, x);  // ln 2 / 32
     double p = __fma_rn(r, 1.0 / 120.0, 1.0 / 24.0);
     p = __fma_rn(p, r, 1.0 / 6.0);
@@ -166,10 +175,7 @@ struct alignas(16) Shared {
   Bins bins;
   union {
     u64 list[kList];
-    struct {  // cluster: this CTA's share of the merged bins, read before any list is made
-      u64 weight[kBins];
-      unsigned count[kBins];
-    } merged;
+    u64 merged[kBins];  // cluster: this CTA's share of the bins, read before any list is made
   };
   u64 weight[kList];  // of the list; before it is made, this CTA's part of the list
   u64 few[kFew], few_weight[kFew];
@@ -508,24 +514,35 @@ __device__ void draw_from_list(Block<TH>& bk, const SampleRowsDesc& d, const Wei
   }
 }
 
-// Words that each CTA of a cluster tells the others: sums, and the sum of lower ranks.
+// Over the lanes of a warp; every lane gets the result.
+template <typename Op>
+__device__ __forceinline__ u64 over_lanes(u64 v, Op op) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+__device__ __forceinline__ u64 lanes_sum(u64 v) {
+  return over_lanes(v, [](u64 a, u64 b) { return a + b; });
+}
+// What the CTAs of a cluster (at most 16) tell each other is read by a lane a
+// CTA, as one read of another SM's shared memory takes hundreds of cycles.  (A
+// row of 151936 logits over 16 CTAs with top-p: CTA after CTA 37 us.)
+template <typename V>
+__device__ __forceinline__ V of_lane_rank(cg::cluster_group& cl, V* word, V none) {
+  const unsigned r = threadIdx.x & 31;
+  return r < cl.num_blocks() ? *cl.map_shared_rank(word, r) : none;
+}
+// Sums of all CTAs, and of the CTAs of lower ranks.
 __device__ __forceinline__ void cluster_sum(cg::cluster_group& cl, Shared& sh, u64 a, u64 b, u64* ta, u64* tb, u64* before_a) {
   if (threadIdx.x == 0) {
     sh.word[0] = a;
     sh.word[1] = b;
   }
   cl.sync();
-  u64 sa = 0, sb = 0, before = 0;
-  for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-    const u64* w = cl.map_shared_rank(sh.word, r);
-    const u64 x = w[0];
-    if (r < cl.block_rank()) before += x;
-    sa += x;
-    sb += w[1];
-  }
-  *ta = sa;
-  *tb = sb;
-  *before_a = before;
+  const u64 x = of_lane_rank<u64>(cl, &sh.word[0], 0), y = of_lane_rank<u64>(cl, &sh.word[1], 0);
+  *ta = lanes_sum(x);
+  *tb = lanes_sum(y);
+  *before_a = lanes_sum((threadIdx.x & 31) < cl.block_rank() ? x : 0);
   cl.sync();
 }
 
@@ -600,146 +617,270 @@ struct Slice {
       }
     }
   }
-  // f(key, place) of every column that can be drawn
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-#pragma unroll 2
-    for (int v = threadIdx.x; v < nv; v += TH) {
-      uint32_t k[E];
-      apart(words(v), k);
+  // f(key, place) of the columns whose places lie in [lo, hi] (lo above kNone), as
+  // long as go(); the loads of four vectors are on their way at once
+  template <typename F, typename Go>
+  __device__ __forceinline__ void between(u64 lo, u64 hi, F f, Go go) const {
+    const uint32_t k0 = key_in(lo), span = key_in(hi) - k0;
+#pragma unroll 1
+    for (int v0 = threadIdx.x; v0 < nv && go(); v0 += 4 * TH) {
+      uint4 u[4];
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (k[j] > K::kNone) f(k[j], place_of(k[j], base + v * E + j));
+      for (int j = 0; j < 4; ++j)
+        if (v0 + j * TH < nv) u[j] = kept ? kept[v0 + j * TH] : raw(v0 + j * TH);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (v0 + j * TH >= nv) break;
+        uint32_t k[E];
+        apart(kept ? u[j] : to_keys(u[j]), k);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (k[e] - k0 <= span) {
+            const u64 c = place_of(k[e], base + (v0 + j * TH) * E + e);
+            if (c >= lo && c <= hi) f(k[e], c);
+          }
+      }
     }
   }
-  // f(i, key, weight) of the columns of vectors [first, last) step `step` whose
-  // place is at least `floor`: four independent chains of f64 arithmetic
   template <typename F>
-  __device__ __forceinline__ void weighed(int first, int last, int step, u64 floor, const Weigh& weigh, F f) const {
-    const uint32_t floor_key = key_in(floor);
+  __device__ __forceinline__ void between(u64 lo, u64 hi, F f) const {
+    between(lo, hi, f, [] { return true; });
+  }
+  // The logits of a vector of a long row, as they are: NaN compares like what
+  // is never drawn.
+  __device__ __forceinline__ void logits(int v, float (&l)[E]) const {
+    const uint4 u = raw(v);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (E == 4) {
+        l[j] = __uint_as_float(w[j]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        l[2 * j] = __half2float(__ushort_as_half((uint16_t)(w[j] & 0xffffu)));
+        l[2 * j + 1] = __half2float(__ushort_as_half((uint16_t)(w[j] >> 16)));
+      } else {
+        l[2 * j] = __uint_as_float(w[j] << 16);
+        l[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  }
+  // A floor (a place) in terms of logits and columns of this slice
+  struct Floor {
+    float l, heavy;  // what lies below heavy weighs nothing
+    int last;        // the last column that reaches the floor with a logit of l
+    __device__ __forceinline__ bool operator()(float x, int i) const { return x > l || (x == l && i <= last); }
+  };
+  __device__ __forceinline__ Floor floor_of(u64 floor, const Weigh& weigh) const {
+    const long last = (long)(uint32_t)~(uint32_t)floor - base;
     // Keys below that of `light` have z < -35; keys from it on z > -73, as a T
     // so near to the largest that 36 T is less than half a step gives its key.
-    const uint32_t heavy = K::near(weigh.light);
+    return Floor{K::value(key_in(floor)), K::value(max(K::near(weigh.light), K::kNone + 1)),
+                 (int)max(-1l, min(last, (long)n))};
+  }
+  // f(i, logit, weight, steps) of the columns of vectors [first, last) step
+  // `step` that reach the floor: four independent chains of f64 arithmetic
+  template <typename F>
+  __device__ __forceinline__ void weighed(int first, int last, int step, const Floor& floor, const Weigh& weigh, F f) const {
 #pragma unroll 1
     for (int v = first; v < last; v += step) {
-      uint32_t kk[E];
-      apart(words(v), kk);
+      float l[E];
+      logits(v, l);
 #pragma unroll
       for (int h = 0; h < E; h += 4) {
-        const uint32_t* k = kk + h;
-        const int i0 = v * E + h;
+        const float* x = l + h;
         u64 w[4] = {0, 0, 0, 0};
+        int steps[4] = {0, 0, 0, 0};
         if (weigh.infinite) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = weigh(K::value(k[j]));
-        } else if (max(max(k[0], k[1]), max(k[2], k[3])) >= heavy) {
+          for (int j = 0; j < 4; ++j) w[j] = x[j] == weigh.top ? 1ull << kFix : 0;
+        } else if (fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= floor.heavy) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            w[j] = weigh.finite(K::value(k[j]));
-            if (k[j] < heavy) w[j] = 0;
+            const bool on = x[j] >= floor.heavy;  // (not NaN, not far below the range of `finite`)
+            const u64 y = weigh.finite(on ? x[j] : weigh.top, steps[j]);
+            w[j] = on ? y : 0;
           }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          bool on = k[j] >= floor_key;
-          if (k[j] == floor_key) on = place_of(k[j], base + i0 + j) >= floor;
-          if (on) f(i0 + j, k[j], w[j]);
+          const int i = v * E + h + j;
+          if (floor(x[j], i)) f(i, x[j], w[j], steps[j]);
         }
       }
     }
   }
+  // Weight and number of the columns of a warp's vectors [first, last) that
+  // reach a floor that few do: each lane puts theirs in a column of shared
+  // memory (TH x 16 floats), and the weights are worked out a row at a time.
+  __device__ __forceinline__ void gathered(int first, int last, const Floor& floor, const Weigh& weigh, float* column,
+                                           u64& sum, unsigned& count) const {
+    constexpr int kDeep = 16;
+    const int lane = threadIdx.x & 31;
+    float* own = column + threadIdx.x;
+    int have = 0;
+    auto work_out = [&] {
+      const int rows = __reduce_max_sync(kFull, have);
+#pragma unroll 1
+      for (int r = 0; r < rows; r += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float l = r + j < have ? own[(r + j) * TH] : weigh.top;
+          const bool on = r + j < have && (weigh.infinite ? l == weigh.top : l >= floor.heavy);
+          const u64 y = weigh.infinite ? 1ull << kFix : weigh.finite(on ? l : weigh.top);
+          sum += on ? y : 0;
+        }
+      }
+      have = 0;
+    };
+#pragma unroll 2
+    for (int v0 = first; v0 < last; v0 += 32) {
+      if (__any_sync(kFull, have > kDeep - E)) work_out();
+      const int v = v0 + lane;
+      if (v < last) {
+        float l[E];
+        logits(v, l);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (floor(l[j], v * E + j)) {
+            own[have * TH] = l[j];
+            ++have;
+            ++count;
+          }
+      }
+    }
+    work_out();
+  }
 };
+
+// The lowest of the keys (kNone, top] for which keeps() holds, which it does for
+// `top` and for every key above one; mostly within two keys of `guess`.
+template <typename T, typename Keeps>
+__device__ __forceinline__ uint32_t lowest_key(uint32_t top, float guess, Keeps keeps) {
+  uint32_t lo = Key<T>::kNone, hi = top;
+  const uint32_t k = min(max(Key<T>::near(guess), lo), hi);
+  if (k > lo + 2 && !keeps(k - 2)) lo = k - 2;
+  if (k + 2 < hi && keeps(k + 2)) hi = k + 2;
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (keeps(mid)) hi = mid;
+    else lo = mid;
+  }
+  return hi;
+}
 
 // The whole cluster's search for the place at which the running count or weight
 // of the tokens at or above `lo` reaches target(total).
 template <typename T, int TH, typename Target>
 __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<T, TH>& sl, Mode mode, Target target_of,
-                              u64 lo, const Weigh& weigh, float bins_per_unit) {
+                              u64 lo, uint32_t top, const Weigh& weigh, float bins_per_unit) {
+  using K = Key<T>;
   Shared& sh = bk.sh;
   const int tid = threadIdx.x;
   const unsigned ranks = cl.num_blocks(), rank = cl.block_rank();
   const FirstBin<T> first_bin{weigh.top, bins_per_unit};
-  u64 hi = ~0ull;
+  const auto floor = sl.floor_of(lo, weigh);
+  // the first histogram's bin of a key: over (top - l) / T for counts; for
+  // weights the steps of ln2 / 32 that their arithmetic has at hand
+  auto bin_of_steps = [&](int steps) { return min(-steps, kBins - 1); };
+  auto bin_of_key = [&](uint32_t k) {
+    if (mode == COUNT) return first_bin.key(k);
+    const float l = K::value(k);
+    if (weigh.infinite) return l == weigh.top ? 0 : kBins - 1;
+    return l >= floor.heavy ? bin_of_steps(weigh.steps(l)) : kBins - 1;
+  };
+  u64 hi = ((u64)top << 32) | 0xffffffffu;
   int s = -1;
   u64 target = 0;
   for (;;) {
     bk.clear(mode);
-    auto bin_of = [&](uint32_t k, u64 c) { return s < 0 ? first_bin.key(k) : (int)((hi - c) >> s); };
     if (mode == COUNT) {
-      sl.each([&](uint32_t k, u64 c) {
-        if (c >= lo && c <= hi) atomicAdd(&sh.bins.count[bin_of(k, c)], 1u);
-      });
+      sl.between(lo, hi, [&](uint32_t k, u64 c) { atomicAdd(&sh.bins.count[s < 0 ? first_bin.key(k) : (int)((hi - c) >> s)], 1u); });
     } else {
-      sl.weighed(tid, sl.nv, TH, lo, weigh, [&](int i, uint32_t k, u64 w) {
-        const u64 c = place_of(k, sl.base + i);
-        if (c > hi) return;
-        const int b = bin_of(k, c);
-        atomicAdd(&sh.bins.count[b], 1u);
+      sl.weighed(tid, sl.nv, TH, floor, weigh, [&](int i, float l, u64 w, int steps) {
+        int b = bin_of_steps(steps);
+        if (s >= 0) {
+          const u64 c = place_of(K::near(l), sl.base + i);
+          if (c < lo || c > hi) return;
+          b = (int)((hi - c) >> s);
+        }
         sh.bins.add(b, w);
       });
     }
     cl.sync();
+    // each CTA adds up its share of the bins, a thread a CTA's bin
     const int share = kBins / ranks, b0 = rank * share;  // ranks: a power of two
-    for (int b = b0 + tid; b < b0 + share; b += TH) {
-      unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < kBins / TH; ++j) {
+      const int i = tid + j * TH, b = b0 + i % share;
+      const Bins* o = cl.map_shared_rank(&sh.bins, i / share);
+      sh.weight[i] = mode == COUNT ? o->count[b] : o->weight(b);
+    }
+    __syncthreads();
+    for (int i = tid; i < share; i += TH) {
       u64 w = 0;
-      for (unsigned r = 0; r < ranks; ++r) {
-        const Bins* o = cl.map_shared_rank(&sh.bins, r);
-        c += o->count[b];
-        if (mode == WEIGHT) w += o->weight(b);
-      }
-      sh.merged.count[b] = c;
-      sh.merged.weight[b] = mode == COUNT ? c : w;
+#pragma unroll 4
+      for (unsigned r = 0; r < ranks; ++r) w += sh.weight[r * share + i];
+      sh.merged[b0 + i] = w;
     }
     cl.sync();
     target = bk.find([&](u64 total) { return s < 0 ? target_of(total) : target; },
-                     [&](int b) { return cl.map_shared_rank(sh.merged.weight, b / share)[b]; },
-                     [&](int b) { return cl.map_shared_rank(sh.merged.count, b / share)[b]; });
+                     [&](int b) { return cl.map_shared_rank(sh.merged, b / share)[b]; }, [](int) { return 0u; });
     const int bin = sh.found_bin;
-    const unsigned count = sh.found_n;
     target -= sh.found_before;
     if (s >= 0) {
       hi -= (u64)bin << s;
       const u64 width = (1ull << s) - 1;
       if (hi - lo > width) lo = hi - width;
+    } else {
+      // the bin's keys: two warps look for its ends
+      if (tid < 64) {
+        const int most = tid < 32 ? bin : bin - 1;
+        const float unit = mode == COUNT ? (bin + (tid < 32)) / bins_per_unit
+                                         : (float)((bin + (tid < 32 ? 0.5 : -0.5)) / (Weigh::kStepsPerUnit * weigh.inv_t));
+        const uint32_t k = most < 0 ? top + 1 : lowest_key<T>(top, weigh.top - unit, [&](uint32_t x) { return bin_of_key(x) <= most; });
+        if ((tid & 31) == 0) sh.key_word[tid >> 5] = k;
+      }
+      __syncthreads();
+      const u64 k0 = (u64)sh.key_word[0] << 32, k1 = ((u64)sh.key_word[1] << 32) - 1;
+      lo = k0 > lo ? k0 : lo;
+      hi = k1 < hi ? k1 : hi;
     }
-    auto inside = [&](uint32_t k, u64 c) { return c >= lo && c <= hi && (s >= 0 || first_bin.key(k) == bin); };
-    if (count <= kList) {
-      // every CTA gathers the bin's tokens from all, each from its own part
-      sl.each([&](uint32_t k, u64 c) {
-        if (inside(k, c)) sh.weight[atomicAdd(&sh.n, 1u)] = c;  // (the weights are filled in below)
-      });
-      cl.sync();
-      unsigned at = 0;
+    // every CTA gathers the bin's tokens from all, each from its own part
+    volatile unsigned* count = &sh.n;
+    sl.between(lo, hi, [&](uint32_t, u64 c) {
+      const unsigned at = atomicAdd(&sh.n, 1u);
+      if (at < kList) sh.weight[at] = c;  // (the weights are filled in below)
+    }, [&] { return *count <= kList; });
+    cl.sync();
+    const unsigned m = of_lane_rank<unsigned>(cl, &sh.n, 0u), all = __reduce_add_sync(kFull, m);
+    if (all <= kList) {
+      // warp w takes part w / ranks of the tokens of CTA w % ranks
+      const unsigned r = bk.warp % ranks, mine = __shfl_sync(kFull, m, r);
+      const unsigned before = __reduce_add_sync(kFull, bk.lane < (int)r ? m : 0u);
+      const u64* from = cl.map_shared_rank(sh.weight, r);
       u64 a = ~0ull, z = 0;
-      for (unsigned r = 0; r < ranks; ++r) {
-        const unsigned m = *cl.map_shared_rank(&sh.n, r);
-        const u64* from = cl.map_shared_rank(sh.weight, r);
-        for (unsigned i = tid; i < m; i += TH) {
-          const u64 c = from[i];
-          sh.list[at + i] = c;
-          a = c < a ? c : a;
-          z = c > z ? c : z;
-        }
-        at += m;
+#pragma unroll 4
+      for (unsigned i = bk.warp / ranks * 32 + bk.lane; i < mine; i += TH / ranks) {
+        const u64 c = from[i];
+        sh.list[before + i] = c;
+        a = c < a ? c : a;
+        z = c > z ? c : z;
       }
       a = bk.least(a);
       z = bk.most(z);
       cl.sync();
       if (mode == WEIGHT)
-        for (unsigned i = tid; i < at; i += TH) sh.weight[i] = weigh(Key<T>::value(key_in(sh.list[i])));
+        for (unsigned i = tid; i < all; i += TH) sh.weight[i] = weigh(K::value(key_in(sh.list[i])));
       // the bin's places spread evenly over the first histogram
       const u64 span = z - a;
       const int shift = span < kBins ? 0 : 64 - __clzll(span) - 10;
-      return bk.select(mode, (int)at, target, [&](u64 c) { return (int)((z - c) >> shift); });
+      return bk.select(mode, (int)all, target, [&](u64 c) { return (int)((z - c) >> shift); });
     }
     // the range of the bin's places
     u64 a = ~0ull, z = 0;
-    sl.each([&](uint32_t k, u64 c) {
-      if (inside(k, c)) {
-        a = c < a ? c : a;
-        z = c > z ? c : z;
-      }
+    sl.between(lo, hi, [&](uint32_t, u64 c) {
+      a = c < a ? c : a;
+      z = c > z ? c : z;
     });
     a = bk.least(a);
     z = bk.most(z);
@@ -748,11 +889,8 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
       sh.word[1] = z;
     }
     cl.sync();
-    for (unsigned r = 0; r < ranks; ++r) {
-      const u64* w = cl.map_shared_rank(sh.word, r);
-      a = w[0] < a ? w[0] : a;
-      z = w[1] > z ? w[1] : z;
-    }
+    a = over_lanes(of_lane_rank<u64>(cl, &sh.word[0], ~0ull), [](u64 x, u64 y) { return x < y ? x : y; });
+    z = over_lanes(of_lane_rank<u64>(cl, &sh.word[1], 0), [](u64 x, u64 y) { return x > y ? x : y; });
     cl.sync();
     lo = a;
     hi = z;
@@ -812,19 +950,8 @@ template <typename T>
 __device__ __forceinline__ uint32_t min_p_key(float min_p, uint32_t top, float temp, const Weigh& weigh) {
   const double zmin = log((double)fminf(min_p, 1.0f));
   if (weigh.infinite) return top;
-  auto keeps = [&](uint32_t k) { return weigh.z(Key<T>::value(k)) >= zmin; };
-  // between a key that is not kept and one that is: mostly two keys around the
-  // nearest T of the value in f64
-  uint32_t lo = Key<T>::kNone, hi = top;
-  const uint32_t k = min(max(Key<T>::near((float)(weigh.top_d + zmin * (double)temp)), lo), hi);
-  if (k > lo + 2 && !keeps(k - 2)) lo = k - 2;
-  if (k + 2 < hi && keeps(k + 2)) hi = k + 2;
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (keeps(mid)) hi = mid;
-    else lo = mid;
-  }
-  return hi;
+  return lowest_key<T>(top, (float)(weigh.top_d + zmin * (double)temp),
+                       [&](uint32_t k) { return weigh.z(Key<T>::value(k)) >= zmin; });
 }
 
 template <typename T, int TH>
@@ -897,12 +1024,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
         sh.key_word[1] = bound;
       }
       cl.sync();
-      bound = ~0u;
-      for (unsigned r = 0; r < ranks; ++r) {
-        const unsigned* w = cl.map_shared_rank(sh.key_word, r);
-        top = max(top, w[0]);
-        bound = min(bound, w[1]);
-      }
+      top = __reduce_max_sync(kFull, of_lane_rank<unsigned>(cl, &sh.key_word[0], 0u));
+      bound = __reduce_min_sync(kFull, of_lane_rank<unsigned>(cl, &sh.key_word[1], ~0u));
     }
     if (top <= Key<T>::kInf || sl.nan) break;
     sl.nan = true;  // the same again without them
@@ -912,14 +1035,12 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     // the first column with the largest key
     unsigned at = 0xffffffffu;
     if (top > Key<T>::kNone)
-      sl.each([&](uint32_t k, u64 c) {
-        if (k == top) at = min(at, ~(uint32_t)c);
-      });
+      sl.between((u64)top << 32, ((u64)top << 32) | 0xffffffffu, [&](uint32_t, u64 c) { at = min(at, ~(uint32_t)c); });
     at = ~bk.most32(~at);
     if (ranks > 1) {
       if (tid == 0) sh.word[0] = at;
       cl.sync();
-      for (unsigned r = 0; r < ranks; ++r) at = min(at, (unsigned)cl.map_shared_rank(sh.word, r)[0]);
+      at = __reduce_min_sync(kFull, (unsigned)of_lane_rank<u64>(cl, &sh.word[0], ~0ull));
       cl.sync();  // no CTA leaves while its word is read
     }
     if (rank == 0 && tid == 0) answer(d, row, (int)at, at != 0xffffffffu, 0.0, 1ull << kFix);
@@ -972,11 +1093,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
       if (rank == 0) {
         if (tid < parts) sh.offset[tid] = ((unsigned)at << 12) | m;
         __syncthreads();
-        for (int p = warp; p < parts; p += kWarps) {
-          const unsigned o = sh.offset[p] >> 12, c = sh.offset[p] & 4095u;
-          const u64* from = (ranks > 1 ? cl.map_shared_rank(sh.weight, p / kWarps) : sh.weight) + (p % kWarps) * kPart;
-          for (unsigned i = lane; i < c; i += 32) sh.list[o + i] = from[i];
-        }
+        const int g = TH / parts, p = tid / g;  // threads of a part (powers of two)
+        const unsigned o = sh.offset[p] >> 12, c = sh.offset[p] & 4095u;
+        const u64* from = (ranks > 1 ? cl.map_shared_rank(sh.weight, p / kWarps) : sh.weight) + (p % kWarps) * kPart;
+#pragma unroll 4
+        for (unsigned i = tid % g; i < c; i += g) sh.list[o + i] = from[i];
       }
       if (ranks > 1) cl.sync();
       else __syncthreads();
@@ -1006,21 +1127,27 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   // ---- otherwise: the last kept place by histograms over the cluster ----------------
   u64 last = (u64)(Key<T>::kNone + 1) << 32;
   if (f.k > 0)
-    last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, weigh, f.bins_per_unit);
+    last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, top, weigh, f.bins_per_unit);
   if (f.use_p)
-    last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, weigh,
+    last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, top, weigh,
                           f.bins_per_unit);
 
   // ---- the draw: a warp's vectors, then the threads of the CTA over that warp's ----
   last = last > f.min_place ? last : f.min_place;
+  const auto floor = sl.floor_of(last, weigh);
   u64 sum = 0;
   unsigned cnt = 0;
-  sl.weighed(v0 + lane, v1, 32, last, weigh, [&](int, uint32_t, u64 w) {
-    sum += w;
-    ++cnt;
-  });
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+  static_assert(sizeof(sh.list) + sizeof(sh.weight) >= TH * 16 * sizeof(float), "a column of 16 a thread");
+  if (key_in(last) > Key<T>::kNone + 1) {
+    __syncthreads();
+    sl.gathered(v0, v1, floor, weigh, reinterpret_cast<float*>(sh.list), sum, cnt);
+  } else {
+    sl.weighed(v0 + lane, v1, 32, floor, weigh, [&](int, float, u64 w, int) {
+      sum += w;
+      ++cnt;
+    });
+  }
+  sum = lanes_sum(sum);
   cnt = bk.sum32(cnt);
   if (lane == 0) sh.scan[warp] = sum;
   __syncthreads();
@@ -1035,11 +1162,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   const int t0 = min(sl.nv, w * seg), t1 = min(sl.nv, t0 + seg), more = (t1 - t0 + TH - 1) / TH;
   const int a0 = min(t1, t0 + tid * more), a1 = min(t1, a0 + more);
   u64 own = 0, all;
-  sl.weighed(a0, a1, 1, last, weigh, [&](int, uint32_t, u64 w) { own += w; });
+  sl.weighed(a0, a1, 1, floor, weigh, [&](int, float, u64 w, int) { own += w; });
   u64 at = run + bk.prefix(own, &all);
   if (goal < at || goal >= at + own) return;
-  sl.weighed(a0, a1, 1, last, weigh, [&](int i, uint32_t k, u64 w) {
-    if (at <= goal && goal < at + w) answer(d, row, base + i, (int)count, weigh.z(Key<T>::value(k)), total);
+  sl.weighed(a0, a1, 1, floor, weigh, [&](int i, float l, u64 w, int) {
+    if (at <= goal && goal < at + w) answer(d, row, base + i, (int)count, weigh.z(l), total);
     at += w;
   });
 }
