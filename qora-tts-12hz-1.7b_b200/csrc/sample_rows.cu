@@ -169,7 +169,7 @@ struct Bins {
   __device__ __forceinline__ u64 weight(int b) const { return (u64)w[0][b] + ((u64)w[1][b] << 15) + ((u64)w[2][b] << 30); }
 };
 
-constexpr int kFew = 32;      // tokens that a search leaves to one warp
+constexpr int kFew = 128;     // tokens that a search leaves to a thread each
 constexpr int kSmall = 64;    // tokens whose filters and draw one warp does alone
 struct alignas(16) Shared {
   Bins bins;
@@ -182,7 +182,6 @@ struct alignas(16) Shared {
   double exp2_32[32];
   u64 scan[32];
   unsigned scan32[32];
-  unsigned tally[2][2][32];
   u64 word[2];            // what this CTA tells the cluster
   unsigned key_word[2];
   unsigned part[32];      // tokens in this CTA's part of the list, by warp
@@ -332,12 +331,12 @@ struct Block {
           }
         }
         __syncthreads();
-        if (warp == 0) {  // the weight at or above each lane's entry
-          const int m = sh.n;
-          const u64 c = lane < m ? sh.few[lane] : 0, w = lane < m ? sh.few_weight[lane] : 0;
+        if (const int m = sh.n; tid < m) {  // the weight at or above each thread's entry
+          const u64 c = sh.few[tid], w = sh.few_weight[tid];
           u64 incl = 0;
+#pragma unroll 4
           for (int i = 0; i < m; ++i) incl += sh.few[i] >= c ? sh.few_weight[i] : 0;
-          if (lane < m && incl >= target && incl - w < target) sh.found_at = c;
+          if (incl >= target && incl - w < target) sh.found_at = c;
         }
         __syncthreads();
         return sh.found_at;
@@ -604,6 +603,11 @@ struct Slice {
   __device__ __forceinline__ uint4 words(int v) const { return kept ? kept[v] : to_keys(raw(v)); }
   static __device__ __forceinline__ uint32_t largest_of(uint4 u) {
     return K::largest(K::larger(K::larger(u.x, u.y), K::larger(u.z, u.w)));
+  }
+  static __device__ __forceinline__ uint32_t pick(uint4 u, int j) {  // the j-th key
+    const int i = j * 4 / E;
+    const uint32_t w = i & 2 ? (i & 1 ? u.w : u.z) : (i & 1 ? u.y : u.x);
+    return E == 4 ? w : (w >> (16 * (j & 1))) & 0xffffu;
   }
   static __device__ __forceinline__ void apart(uint4 u, uint32_t (&k)[E]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -899,34 +903,35 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
   }
 }
 
-// The largest key, but for low bits of a 32-bit one left at 0, that at least
-// `each` of the CTA's keys v (N a thread) reach; 1 above kNone if there are
-// fewer.  Two bits a step, one barrier each.
+// A key that at least `each` of the CTA's keys v (N a thread, `top` the largest)
+// reach, and not many more; 1 above kNone if there are fewer.  Histograms over
+// the range of keys that holds the each-th, until its bin has few.  (Two bits
+// of the key a step, by counts: 11000 cycles a row for k = 1000, and 4000 so.)
 template <typename T, int TH, int N>
-__device__ __forceinline__ uint32_t bound_of(Block<TH>& bk, const uint32_t (&v)[N], unsigned each) {
-  constexpr int kTop = sizeof(T) == 4 ? 30 : 14, kLow = sizeof(T) == 4 ? 10 : 0;
-  uint32_t bound = 0;
-  int turn = 0;
-#pragma unroll 1
-  for (int b = kTop; b >= kLow; b -= 2, turn ^= 1) {
-    unsigned c[3] = {0, 0, 0};
+__device__ __forceinline__ uint32_t bound_of(Block<TH>& bk, const uint32_t (&v)[N], unsigned each, uint32_t top) {
+  Shared& sh = bk.sh;
+  uint32_t lo = ~0u, hi = top;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (v[j] > Key<T>::kNone) lo = min(lo, v[j]);
+  lo = ~bk.most32(~lo);
+  if (lo == ~0u) return Key<T>::kNone + 1;
+  unsigned want = each;
+  for (;;) {
+    const uint32_t span = hi - lo;
+    const int s = span < kBins ? 0 : 32 - __clz(span) - 10;
+    bk.clear(COUNT);
 #pragma unroll
     for (int j = 0; j < N; ++j)
-#pragma unroll
-      for (int q = 0; q < 3; ++q) c[q] += v[j] >= (bound | ((uint32_t)(q + 1) << b));
-    const unsigned ab = __reduce_add_sync(kFull, c[0] | c[1] << 16), cc = __reduce_add_sync(kFull, c[2]);
-    if (bk.lane == 0) {
-      bk.sh.tally[turn][0][bk.warp] = ab;
-      bk.sh.tally[turn][1][bk.warp] = cc;
-    }
+      if (v[j] >= lo && v[j] <= hi) atomicAdd(&sh.bins.count[(hi - v[j]) >> s], 1u);
     __syncthreads();
-    const bool in = bk.lane < Block<TH>::kWarps;
-    const unsigned all = __reduce_add_sync(kFull, in ? bk.sh.tally[turn][0][bk.lane] : 0u);
-    const unsigned third = __reduce_add_sync(kFull, in ? bk.sh.tally[turn][1][bk.lane] : 0u);
-    const uint32_t q = third >= each ? 3 : (all >> 16) >= each ? 2 : (all & 0xffffu) >= each ? 1 : 0;
-    bound |= q << b;
+    auto count = [&](int b) { return sh.bins.count[b]; };
+    if (bk.find([&](u64) { return (u64)want; }, [&](int b) { return (u64)count(b); }, count) < want) return Key<T>::kNone + 1;
+    want -= (unsigned)sh.found_before;
+    hi -= sh.found_bin << s;
+    if (hi - lo >= (1u << s)) lo = hi - ((1u << s) - 1);
+    if (s == 0 || sh.found_n <= 32 || sh.found_n * 4 <= each) return lo;
   }
-  return max(bound, Key<T>::kNone + 1);
 }
 
 // The same by one warp, without barriers, for its keys alone.
@@ -1016,7 +1021,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
         bound = sh.key_word[1];
       }
     } else if (bounded) {
-      bound = bound_of<T, TH>(bk, maxima, each);
+      bound = bound_of<T, TH>(bk, maxima, each, top);
     }
     if (ranks > 1) {
       if (tid == 0) {
@@ -1053,32 +1058,43 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   // ---- a list: what lies above the bound, or a short row ---------------------------
   if (bounded) {
     unsigned mine = 0;
-#pragma unroll 2
-    for (int w0 = v0; w0 < v1; w0 += 32) {  // in the order of the columns
-      const int v = w0 + lane;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (v < v1) u = sl.words(v);
-      if (!__any_sync(kFull, sl.largest_of(u) >= bound)) continue;
-      uint32_t k[E];
-      sl.apart(u, k);
-      unsigned hits = 0;
+    for (int w0 = v0; w0 < v1; w0 += 128) {  // in the order of the columns
+      uint4 u[4];
 #pragma unroll
-      for (int j = 0; j < E; ++j) hits |= k[j] >= bound ? 1u << j : 0u;
-      unsigned at = __popc(hits);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned y = __shfl_up_sync(kFull, at, o);
-        if (lane >= o) at += y;
+      for (int q = 0; q < 4; ++q) {
+        const int v = w0 + q * 32 + lane;
+        u[q] = make_uint4(0, 0, 0, 0);
+        if (v < v1) u[q] = sl.words(v);
       }
-      const unsigned all = __shfl_sync(kFull, at, 31);
-      at += mine - __popc(hits);
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if ((hits >> j) & 1) {
-          if (at < kPart) sh.weight[warp * kPart + at] = place_of(k[j], base + v * E + j);
-          ++at;
+      for (int q = 0; q < 4; ++q) {
+        const unsigned lanes = __ballot_sync(kFull, sl.largest_of(u[q]) >= bound);
+        if (!lanes) continue;
+        uint32_t k[E];
+        sl.apart(u[q], k);
+        unsigned hits = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) hits |= k[j] >= bound ? 1u << j : 0u;
+        // the hits of lower lanes: mostly one a lane
+        const unsigned own = __popc(hits);
+        unsigned at = __popc(lanes & ((1u << lane) - 1)), all = __popc(lanes);
+        if (__any_sync(kFull, own > 1)) {
+          at = own;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(kFull, at, o);
+            if (lane >= o) at += y;
+          }
+          all = __shfl_sync(kFull, at, 31);
+          at -= own;
         }
-      mine += all;
+        at += mine;
+        for (; hits; hits &= hits - 1, ++at) {
+          const int j = __ffs(hits) - 1;
+          if (at < kPart) sh.weight[warp * kPart + at] = place_of(sl.pick(u[q], j), base + (w0 + q * 32 + lane) * E + j);
+        }
+        mine += all;
+      }
     }
     if (lane == 0) sh.part[warp] = mine;
     if (ranks > 1) cl.sync();
