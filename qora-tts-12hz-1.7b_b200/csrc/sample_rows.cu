@@ -38,12 +38,14 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kFix = 45;     // fraction bits of a weight: 2^18 weights of 1 stay below 2^63
 constexpr int kList = 2048;  // tokens of a list
 constexpr int kBins = 1024;
+constexpr int kShortThreads = 256;  // of a CTA that has a row of at most kList logits; 512 otherwise
 typedef unsigned long long u64;
 
 struct SampleRowsDesc {
   const void* logits = nullptr;
   long ld = 0;
   int V = 0, per = 0;  // columns, columns of a CTA
+  bool keep = false;   // a CTA's columns stay in shared memory
   const float* temperature = nullptr;
   const int* top_k = nullptr;
   const float *top_p = nullptr, *min_p = nullptr, *u = nullptr;
@@ -111,8 +113,8 @@ struct Weigh {
   float light;            // about top - 36 T: what lies below weighs nothing
   double top_d, inv_t;
   bool infinite;          // top is: the infinite logits share, whatever the temperature
-  const double* exp2_32;  // 2^(i / 32)
-  __device__ __forceinline__ Weigh(float t, float temp, const double* table) : top(t), exp2_32(table) {
+  const uint32_t* exp2_32;  // the low words of 2^(i / 32), then the high ones: no two of them share a bank
+  __device__ __forceinline__ Weigh(float t, float temp, const uint32_t* table) : top(t), exp2_32(table) {
     light = top - 36.0f * temp;
     top_d = top;
     inv_t = 1.0 / (double)temp;
@@ -144,8 +146,8 @@ struct Weigh {
     p = __fma_rn(p, r, 0.5);
     p = __fma_rn(p, r, 1.0);
     p = __fma_rn(p, r, 1.0);
-    const double t = exp2_32[n & 31];
-    const double s = __hiloint2double(__double2hiint(t) + (((n >> 5) + kFix) << 20), __double2loint(t));
+    const uint32_t* t = exp2_32 + (n & 31);
+    const double s = __hiloint2double((int)t[32] + (((n >> 5) + kFix) << 20), (int)t[0]);
     const double w = __fma_rn(s, p, 0x1p52);  // the sum's mantissa is the integer
     return (u64)(__double_as_longlong(w) - __double_as_longlong(0x1p52));
   }
@@ -179,7 +181,7 @@ struct alignas(16) Shared {
   };
   u64 weight[kList];  // of the list; before it is made, this CTA's part of the list
   u64 few[kFew], few_weight[kFew];
-  double exp2_32[32];
+  uint32_t exp2_32[64];
   u64 scan[32];
   unsigned scan32[32];
   u64 word[2];            // what this CTA tells the cluster
@@ -383,15 +385,15 @@ __device__ __forceinline__ void answer(const SampleRowsDesc& d, int row, int tok
   if (d.logprob) d.logprob[row] = token < 0 ? -INFINITY : (float)(logw - log((double)total * (1.0 / (1ull << kFix))));
 }
 
-// The bin of a key in the histogram over (top - l) / T, 32 bins a unit.
+// The bin of a logit in the histogram over (top - l) / T, 32 bins a unit.
 template <typename T>
 struct FirstBin {
   float top, per_unit;
-  __device__ __forceinline__ int key(uint32_t k) const {
-    const float l = Key<T>::value(k), x = (top - l) * per_unit;
+  __device__ __forceinline__ int logit(float l) const {
+    const float x = (top - l) * per_unit;
     return l == top ? 0 : x < (float)(kBins - 1) ? (int)x : kBins - 1;
   }
-  __device__ __forceinline__ int operator()(u64 place) const { return key(key_in(place)); }
+  __device__ __forceinline__ int operator()(u64 place) const { return logit(Key<T>::value(key_in(place))); }
 };
 
 // All filters and the draw on a list of at most kSmall tokens that holds every
@@ -414,6 +416,7 @@ __device__ void draw_small(Shared& sh, const SampleRowsDesc& d, const Weigh& wei
   __syncwarp();
   u64 above[2] = {0, 0};
   int rank[2] = {0, 0};
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
     const u64 ci = sh.list[i], wi = sh.weight[i];
 #pragma unroll
@@ -524,8 +527,7 @@ __device__ __forceinline__ u64 lanes_sum(u64 v) {
   return over_lanes(v, [](u64 a, u64 b) { return a + b; });
 }
 // What the CTAs of a cluster (at most 16) tell each other is read by a lane a
-// CTA, as one read of another SM's shared memory takes hundreds of cycles.  (A
-// row of 151936 logits over 16 CTAs with top-p: CTA after CTA 37 us.)
+// CTA, as one read of another SM's shared memory takes hundreds of cycles.
 template <typename V>
 __device__ __forceinline__ V of_lane_rank(cg::cluster_group& cl, V* word, V none) {
   const unsigned r = threadIdx.x & 31;
@@ -546,7 +548,7 @@ __device__ __forceinline__ void cluster_sum(cg::cluster_group& cl, Shared& sh, u
 }
 
 // One CTA's columns [0, n) of the row, as vectors of E columns: 16 bytes a load
-// where the row starts on that boundary.  A short row's keys are kept.
+// where the row starts on that boundary.  Those of a short slice are kept.
 template <typename T, int TH>
 struct Slice {
   using K = Key<T>;
@@ -554,7 +556,7 @@ struct Slice {
   const T* src;
   int n, nv, base;  // columns, vectors, the first column's index
   bool aligned, nan;
-  uint4* kept;      // shared memory, or null
+  uint4* kept;      // the vectors in shared memory, or null
 
   __device__ __forceinline__ uint4 raw(int v) const {
     if (aligned && (v + 1) * E <= n) return reinterpret_cast<const uint4*>(src)[v];
@@ -590,8 +592,8 @@ struct Slice {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (v0 + j * TH < nv) {
-          u[j] = to_keys(u[j]);
           if (kept) kept[v0 + j * TH] = u[j];
+          u[j] = to_keys(u[j]);
           most[0] = K::larger(most[0], u[j].x);
           most[1] = K::larger(most[1], u[j].y);
           most[2] = K::larger(most[2], u[j].z);
@@ -599,8 +601,9 @@ struct Slice {
         }
     }
   }
-  // later passes: the keys of a vector, in words
-  __device__ __forceinline__ uint4 words(int v) const { return kept ? kept[v] : to_keys(raw(v)); }
+  // later passes: a vector, and its keys in words
+  __device__ __forceinline__ uint4 again(int v) const { return kept ? kept[v] : raw(v); }
+  __device__ __forceinline__ uint4 words(int v) const { return to_keys(again(v)); }
   static __device__ __forceinline__ uint32_t largest_of(uint4 u) {
     return K::largest(K::larger(K::larger(u.x, u.y), K::larger(u.z, u.w)));
   }
@@ -621,39 +624,8 @@ struct Slice {
       }
     }
   }
-  // f(key, place) of the columns whose places lie in [lo, hi] (lo above kNone), as
-  // long as go(); the loads of four vectors are on their way at once
-  template <typename F, typename Go>
-  __device__ __forceinline__ void between(u64 lo, u64 hi, F f, Go go) const {
-    const uint32_t k0 = key_in(lo), span = key_in(hi) - k0;
-#pragma unroll 1
-    for (int v0 = threadIdx.x; v0 < nv && go(); v0 += 4 * TH) {
-      uint4 u[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (v0 + j * TH < nv) u[j] = kept ? kept[v0 + j * TH] : raw(v0 + j * TH);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (v0 + j * TH >= nv) break;
-        uint32_t k[E];
-        apart(kept ? u[j] : to_keys(u[j]), k);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (k[e] - k0 <= span) {
-            const u64 c = place_of(k[e], base + (v0 + j * TH) * E + e);
-            if (c >= lo && c <= hi) f(k[e], c);
-          }
-      }
-    }
-  }
-  template <typename F>
-  __device__ __forceinline__ void between(u64 lo, u64 hi, F f) const {
-    between(lo, hi, f, [] { return true; });
-  }
-  // The logits of a vector of a long row, as they are: NaN compares like what
-  // is never drawn.
-  __device__ __forceinline__ void logits(int v, float (&l)[E]) const {
-    const uint4 u = raw(v);
+  // The logits of a vector as they are: NaN compares like what is never drawn.
+  static __device__ __forceinline__ void logits(uint4 u, float (&l)[E]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -667,6 +639,35 @@ struct Slice {
         l[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
       }
     }
+  }
+  // f(logit, place) of the columns whose places lie in [lo, hi] (lo above
+  // kNone), as long as go(); the loads of four vectors are on their way at once
+  template <typename F, typename Go>
+  __device__ __forceinline__ void between(u64 lo, u64 hi, F f, Go go) const {
+    const float from = K::value(key_in(lo)), to = K::value(key_in(hi));
+#pragma unroll 1
+    for (int v0 = threadIdx.x; v0 < nv && go(); v0 += 4 * TH) {
+      uint4 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v0 + j * TH < nv) u[j] = again(v0 + j * TH);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (v0 + j * TH >= nv) break;
+        float l[E];
+        logits(u[j], l);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (l[e] >= from && l[e] <= to) {
+            const u64 c = place_of(K::near(l[e]), base + (v0 + j * TH) * E + e);
+            if (c >= lo && c <= hi) f(l[e], c);
+          }
+      }
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void between(u64 lo, u64 hi, F f) const {
+    between(lo, hi, f, [] { return true; });
   }
   // A floor (a place) in terms of logits and columns of this slice
   struct Floor {
@@ -688,7 +689,7 @@ struct Slice {
 #pragma unroll 1
     for (int v = first; v < last; v += step) {
       float l[E];
-      logits(v, l);
+      logits(again(v), l);
 #pragma unroll
       for (int h = 0; h < E; h += 4) {
         const float* x = l + h;
@@ -742,7 +743,7 @@ struct Slice {
       const int v = v0 + lane;
       if (v < last) {
         float l[E];
-        logits(v, l);
+        logits(again(v), l);
 #pragma unroll
         for (int j = 0; j < E; ++j)
           if (floor(l[j], v * E + j)) {
@@ -787,8 +788,8 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
   // weights the steps of ln2 / 32 that their arithmetic has at hand
   auto bin_of_steps = [&](int steps) { return min(-steps, kBins - 1); };
   auto bin_of_key = [&](uint32_t k) {
-    if (mode == COUNT) return first_bin.key(k);
     const float l = K::value(k);
+    if (mode == COUNT) return first_bin.logit(l);
     if (weigh.infinite) return l == weigh.top ? 0 : kBins - 1;
     return l >= floor.heavy ? bin_of_steps(weigh.steps(l)) : kBins - 1;
   };
@@ -798,7 +799,7 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
   for (;;) {
     bk.clear(mode);
     if (mode == COUNT) {
-      sl.between(lo, hi, [&](uint32_t k, u64 c) { atomicAdd(&sh.bins.count[s < 0 ? first_bin.key(k) : (int)((hi - c) >> s)], 1u); });
+      sl.between(lo, hi, [&](float l, u64 c) { atomicAdd(&sh.bins.count[s < 0 ? first_bin.logit(l) : (int)((hi - c) >> s)], 1u); });
     } else {
       sl.weighed(tid, sl.nv, TH, floor, weigh, [&](int i, float l, u64 w, int steps) {
         int b = bin_of_steps(steps);
@@ -851,7 +852,7 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
     }
     // every CTA gathers the bin's tokens from all, each from its own part
     volatile unsigned* count = &sh.n;
-    sl.between(lo, hi, [&](uint32_t, u64 c) {
+    sl.between(lo, hi, [&](float, u64 c) {
       const unsigned at = atomicAdd(&sh.n, 1u);
       if (at < kList) sh.weight[at] = c;  // (the weights are filled in below)
     }, [&] { return *count <= kList; });
@@ -882,7 +883,7 @@ __device__ u64 cluster_select(cg::cluster_group& cl, Block<TH>& bk, const Slice<
     }
     // the range of the bin's places
     u64 a = ~0ull, z = 0;
-    sl.between(lo, hi, [&](uint32_t, u64 c) {
+    sl.between(lo, hi, [&](float, u64 c) {
       a = c < a ? c : a;
       z = c > z ? c : z;
     });
@@ -934,18 +935,22 @@ __device__ __forceinline__ uint32_t bound_of(Block<TH>& bk, const uint32_t (&v)[
   }
 }
 
-// The same by one warp, without barriers, for its keys alone.
+// The same by one warp, without barriers, for its keys alone, but for low bits
+// of a 32-bit key left at 0: two bits a step.
 template <typename T, int N>
 __device__ __forceinline__ uint32_t warp_bound_of(const uint32_t (&v)[N], unsigned each) {
-  constexpr int kTop = sizeof(T) == 4 ? 31 : 15, kLow = sizeof(T) == 4 ? 10 : 0;
+  constexpr int kTop = sizeof(T) == 4 ? 30 : 14, kLow = sizeof(T) == 4 ? 12 : 0;
   uint32_t bound = 0;
 #pragma unroll 1
-  for (int b = kTop; b >= kLow; --b) {
-    const uint32_t t = bound | (1u << b);
-    unsigned c = 0;
+  for (int b = kTop; b >= kLow; b -= 2) {
+    unsigned c[3] = {0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < N; ++j) c += v[j] >= t;
-    if (__reduce_add_sync(kFull, c) >= each) bound = t;
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) c[q] += v[j] >= (bound | ((uint32_t)(q + 1) << b));
+    const unsigned two = __reduce_add_sync(kFull, c[0] | c[1] << 16), three = __reduce_add_sync(kFull, c[2]);
+    const uint32_t q = three >= each ? 3 : (two >> 16) >= each ? 2 : (two & 0xffffu) >= each ? 1 : 0;
+    bound |= q << b;
   }
   return max(bound, Key<T>::kNone + 1);
 }
@@ -963,13 +968,18 @@ template <typename T, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid_constant__ SampleRowsDesc d) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
-  if (threadIdx.x < 32) sh.exp2_32[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
+  if (threadIdx.x < 32) {
+    const double e = exp2(threadIdx.x * (1.0 / 32.0));
+    sh.exp2_32[threadIdx.x] = __double2loint(e);
+    sh.exp2_32[threadIdx.x + 32] = __double2hiint(e);
+  }
   pdl_launch_dependents();
   pdl_wait();
   cg::cluster_group cl = cg::this_cluster();
   constexpr int kWarps = TH / 32, kPart = kList / kWarps;  // tokens of a warp's part of the list
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x;
-  const unsigned rank = cl.block_rank(), ranks = cl.num_blocks();
+  constexpr bool kShort = TH == kShortThreads;  // a row of at most kList logits, one CTA
+  const unsigned rank = kShort ? 0 : cl.block_rank(), ranks = kShort ? 1 : cl.num_blocks();
   const int base = (int)rank * d.per, n = max(0, min(d.per, d.V - base));
   constexpr int E = Slice<T, TH>::E;
   Slice<T, TH> sl;
@@ -978,7 +988,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   sl.nv = (n + E - 1) / E;
   sl.base = base;
   sl.aligned = (reinterpret_cast<uintptr_t>(sl.src) & 15) == 0;
-  sl.kept = d.V <= kList ? reinterpret_cast<uint4*>(smem + sizeof(Shared)) : nullptr;
+  sl.kept = d.keep ? reinterpret_cast<uint4*>(smem + sizeof(Shared)) : nullptr;
   Block<TH> bk(sh);
   Filters f;
   const float temp = d.temperature ? d.temperature[row] : 1.0f;
@@ -1004,10 +1014,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     uint32_t most[4], maxima[E];
     sl.largest(most);
     sl.apart(make_uint4(most[0], most[1], most[2], most[3]), maxima);
-    top = bk.most32(sl.largest_of(make_uint4(most[0], most[1], most[2], most[3])));
+    const uint32_t own_top = sl.largest_of(make_uint4(most[0], most[1], most[2], most[3]));
+    top = bk.most32(own_top);
     if (bounded && by_warp) {
       unsigned* own = reinterpret_cast<unsigned*>(sh.weight);
-      own[tid] = sl.largest_of(make_uint4(most[0], most[1], most[2], most[3]));
+      own[tid] = own_top;
       __syncthreads();
       if (warp == 0) {
         uint32_t v[kWarps];
@@ -1040,7 +1051,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     // the first column with the largest key
     unsigned at = 0xffffffffu;
     if (top > Key<T>::kNone)
-      sl.between((u64)top << 32, ((u64)top << 32) | 0xffffffffu, [&](uint32_t, u64 c) { at = min(at, ~(uint32_t)c); });
+      sl.between((u64)top << 32, ((u64)top << 32) | 0xffffffffu, [&](float, u64 c) { at = min(at, ~(uint32_t)c); });
     at = ~bk.most32(~at);
     if (ranks > 1) {
       if (tid == 0) sh.word[0] = at;
@@ -1058,16 +1069,17 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
   // ---- a list: what lies above the bound, or a short row ---------------------------
   if (bounded) {
     unsigned mine = 0;
-    for (int w0 = v0; w0 < v1; w0 += 128) {  // in the order of the columns
-      uint4 u[4];
+    for (int w0 = v0; w0 < v1; w0 += 64) {  // in the order of the columns
+      uint4 u[2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
         const int v = w0 + q * 32 + lane;
         u[q] = make_uint4(0, 0, 0, 0);
         if (v < v1) u[q] = sl.words(v);
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
+        if (w0 + q * 32 >= v1) break;
         const unsigned lanes = __ballot_sync(kFull, sl.largest_of(u[q]) >= bound);
         if (!lanes) continue;
         uint32_t k[E];
@@ -1127,7 +1139,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     }
     if (ranks > 1) cl.sync();
   }
-  if (d.V <= kList) {
+  if constexpr (kShort) {
     for (int v = tid; v < sl.nv; v += TH) {
       uint32_t k[E];
       sl.apart(sl.words(v), k);
@@ -1137,63 +1149,66 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_rows_kernel(const __grid
     }
     __syncthreads();
     draw_from_list<T>(bk, d, weigh, f, row, n);
-    return;
-  }
-
-  // ---- otherwise: the last kept place by histograms over the cluster ----------------
-  u64 last = (u64)(Key<T>::kNone + 1) << 32;
-  if (f.k > 0)
-    last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, top, weigh, f.bins_per_unit);
-  if (f.use_p)
-    last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, top, weigh,
-                          f.bins_per_unit);
-
-  // ---- the draw: a warp's vectors, then the threads of the CTA over that warp's ----
-  last = last > f.min_place ? last : f.min_place;
-  const auto floor = sl.floor_of(last, weigh);
-  u64 sum = 0;
-  unsigned cnt = 0;
-  static_assert(sizeof(sh.list) + sizeof(sh.weight) >= TH * 16 * sizeof(float), "a column of 16 a thread");
-  if (key_in(last) > Key<T>::kNone + 1) {
-    __syncthreads();
-    sl.gathered(v0, v1, floor, weigh, reinterpret_cast<float*>(sh.list), sum, cnt);
   } else {
-    sl.weighed(v0 + lane, v1, 32, floor, weigh, [&](int, float, u64 w, int) {
-      sum += w;
-      ++cnt;
+    // ---- otherwise: the last kept place by histograms over the cluster ----------------
+    u64 last = (u64)(Key<T>::kNone + 1) << 32;
+    if (f.k > 0)
+      last = cluster_select(cl, bk, sl, COUNT, [&](u64) { return (u64)f.k; }, last, top, weigh, f.bins_per_unit);
+    if (f.use_p)
+      last = cluster_select(cl, bk, sl, WEIGHT, [&](u64 total) { return nucleus(f.p, total); }, last, top, weigh,
+                            f.bins_per_unit);
+
+    // ---- the draw: a warp's vectors, then the threads of the CTA over that warp's ----
+    last = last > f.min_place ? last : f.min_place;
+    const auto floor = sl.floor_of(last, weigh);
+    u64 sum = 0;
+    unsigned cnt = 0;
+    static_assert(sizeof(sh.list) + sizeof(sh.weight) >= TH * 16 * sizeof(float), "a column of 16 a thread");
+    if (key_in(last) > Key<T>::kNone + 1) {
+      __syncthreads();
+      sl.gathered(v0, v1, floor, weigh, reinterpret_cast<float*>(sh.list), sum, cnt);
+    } else {
+      sl.weighed(v0 + lane, v1, 32, floor, weigh, [&](int, float, u64 w, int) {
+        sum += w;
+        ++cnt;
+      });
+    }
+    sum = lanes_sum(sum);
+    cnt = bk.sum32(cnt);
+    if (lane == 0) sh.scan[warp] = sum;
+    __syncthreads();
+    u64 mine = 0;
+    for (int w = 0; w < kWarps; ++w) mine += sh.scan[w];
+    u64 total, count, run;
+    cluster_sum(cl, sh, mine, cnt, &total, &count, &run);
+    const u64 goal = goal_of(f.u, total);
+    if (goal < run || goal >= run + mine) return;  // another CTA's
+    int w = 0;
+    while (goal >= run + sh.scan[w]) run += sh.scan[w++];
+    const int t0 = min(sl.nv, w * seg), t1 = min(sl.nv, t0 + seg), more = (t1 - t0 + TH - 1) / TH;
+    const int a0 = min(t1, t0 + tid * more), a1 = min(t1, a0 + more);
+    u64 own = 0, all;
+    sl.weighed(a0, a1, 1, floor, weigh, [&](int, float, u64 w, int) { own += w; });
+    u64 at = run + bk.prefix(own, &all);
+    if (goal < at || goal >= at + own) return;
+    sl.weighed(a0, a1, 1, floor, weigh, [&](int i, float l, u64 w, int) {
+      if (at <= goal && goal < at + w) answer(d, row, base + i, (int)count, weigh.z(l), total);
+      at += w;
     });
   }
-  sum = lanes_sum(sum);
-  cnt = bk.sum32(cnt);
-  if (lane == 0) sh.scan[warp] = sum;
-  __syncthreads();
-  u64 mine = 0;
-  for (int w = 0; w < kWarps; ++w) mine += sh.scan[w];
-  u64 total, count, run;
-  cluster_sum(cl, sh, mine, cnt, &total, &count, &run);
-  const u64 goal = goal_of(f.u, total);
-  if (goal < run || goal >= run + mine) return;  // another CTA's
-  int w = 0;
-  while (goal >= run + sh.scan[w]) run += sh.scan[w++];
-  const int t0 = min(sl.nv, w * seg), t1 = min(sl.nv, t0 + seg), more = (t1 - t0 + TH - 1) / TH;
-  const int a0 = min(t1, t0 + tid * more), a1 = min(t1, a0 + more);
-  u64 own = 0, all;
-  sl.weighed(a0, a1, 1, floor, weigh, [&](int, float, u64 w, int) { own += w; });
-  u64 at = run + bk.prefix(own, &all);
-  if (goal < at || goal >= at + own) return;
-  sl.weighed(a0, a1, 1, floor, weigh, [&](int i, float l, u64 w, int) {
-    if (at <= goal && goal < at + w) answer(d, row, base + i, (int)count, weigh.z(l), total);
-    at += w;
-  });
 }
 
+// Bytes of a CTA's columns up to which they stay in shared memory: two CTAs an
+// SM fit.  (One row of 151936 f32 logits, 38 KB a CTA, top-p: 30.3 us, and 31.4
+// us read through the L2 cache pass by pass.)
+constexpr int kKeep = 48 * 1024;
 template <typename T, int TH>
 cudaError_t launch_t(const SampleRowsDesc& d, int n_rows, int ranks, cudaStream_t st) {
-  const size_t smem = sizeof(Shared) + (d.V <= kList ? kList * sizeof(T) : 0);
+  const size_t smem = sizeof(Shared) + (d.keep ? d.per * sizeof(T) : 0);
   static std::atomic<int> ready[kMaxDevices];
   const cudaError_t set = once_per_device(ready, [] {
     const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)(sizeof(Shared) + kList * sizeof(T)));
+                                               (int)sizeof(Shared) + kKeep);
     if (e != cudaSuccess) return e;
     return cudaFuncSetAttribute(sample_rows_kernel<T, TH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   });
@@ -1210,7 +1225,8 @@ cudaError_t launch(SampleRowsDesc d, int n_rows, int sms, cudaStream_t st) {
   int ranks = 1;
   while (ranks < 16 && (d.V > ranks * kMaxSlice || (d.V > ranks * 4096 && (long)n_rows * ranks <= sms))) ranks *= 2;
   d.per = ((d.V + ranks - 1) / ranks + 31) / 32 * 32;
-  return d.V <= kList ? launch_t<T, 256>(d, n_rows, 1, st) : launch_t<T, 512>(d, n_rows, ranks, st);
+  d.keep = d.per * sizeof(T) <= kKeep;
+  return d.V <= kList ? launch_t<T, kShortThreads>(d, n_rows, 1, st) : launch_t<T, 512>(d, n_rows, ranks, st);
 }
 
 }  // namespace
