@@ -452,6 +452,20 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
     const int nslots = rows * nh;
     const bool on = g < nslots;
 
+    // the slot's query is on its way before the pages, which would hold it up
+    Raw4<T> raw[KJ][4];
+    {
+      const T* qp = static_cast<const T*>(d.q) + (size_t)(unit_row0 + slot_row) * d.ldq +
+                    (size_t)(h0 + (on ? g % nh : 0)) * HD;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          raw[j][i] = Raw4<T>{};
+          if (on) raw[j][i] = *reinterpret_cast<const Raw4<T>*>(qp + 16 * (t + 4 * j) + 4 * i);
+        }
+    }
+
     // this split's pages [pb, pe); the warp takes every NW-th of them
     const int p0 = hi > 0 ? lo / kKv8Page : 0, p1 = (hi + kKv8Page - 1) / kKv8Page;
     const int share = (p1 - p0 + nsplit - 1) / nsplit;
@@ -504,13 +518,11 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       float4 x[KJ][4];
       float big = 0.0f;
       bool finite = true;
-      const T* qp = static_cast<const T*>(d.q) + (size_t)(unit_row0 + slot_row) * d.ldq +
-                    (size_t)(h0 + (on ? g % nh : 0)) * HD;
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[j][i] = on ? load4(qp + 16 * (t + 4 * j) + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[j][i] = load4(reinterpret_cast<const T*>(&raw[j][i]));
           const float4 v = make_float4(fabsf(x[j][i].x), fabsf(x[j][i].y), fabsf(x[j][i].z), fabsf(x[j][i].w));
           finite &= v.x <= FLT_MAX && v.y <= FLT_MAX && v.z <= FLT_MAX && v.w <= FLT_MAX;
           big = fmaxf(big, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
