@@ -324,11 +324,13 @@ QTTS_API int qtts_kv8_append_dev(const qtts_kv8_cache* cache, const void* k, int
  * seq[r], or the last `window` of them (0: all); out = softmax(scale * q.k) v
  * and lse[n_rows][heads] (nullable, f32) its log-sum-exp.  pos < 0: nothing is
  * attended, out is 0 and lse -inf.  seq < 0: a padding row, left as it was.
- * Sums are held in f32; q and the softmax weights keep about 22 bits with f32
- * q, so that f32 results agree with f32 arithmetic to ~1e-6.  max_rows (the
- * rows that one sequence has next to each other; 0 = 1) and max_len (the
- * longest sequence; 0 = the whole table) choose how the work is split; results
- * are right whatever they say. */
+ * Sums are held in f32; q and the softmax weights keep about 22 bits, so that
+ * f32 results agree with f32 arithmetic to ~1e-6; with 16-bit q and max_rows
+ * above 1 the weights may be rounded to f16 (2^-11 each).  A page that a row
+ * does not see has no say in it, whatever its scale.  max_rows (the rows that
+ * one sequence has next to each other; 0 = 1) and max_len (the longest
+ * sequence; 0 = the whole table) choose how the work is split; results are
+ * right whatever they say. */
 QTTS_API int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t ldq, int heads, int dtype,
                                     float scale, int window, const int32_t* seq, const int32_t* pos, int n_rows,
                                     int max_rows, int max_len, void* out, int64_t ldo, float* lse, int32_t* flags,
@@ -339,7 +341,7 @@ QTTS_API int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, 
  * and uniform numbers that the caller gives.  Per row (stride ld elements):
  * tokens are ordered by logit, equal ones by index; NaN counts as -inf, and
  * -inf is never drawn.  temperature[r] (null: 1) divides the logits; not above
- * 0: the first token of the order is taken.  w = exp((logit - largest) /
+ * 0, or NaN: the first token of the order is taken.  w = exp((logit - largest) /
  * temperature).  Kept are the first top_k[r] (null or < 1: all); of these the
  * shortest beginning that holds top_p[r] of their weight (null or not below
  * 1: all; at least one token); of these w >= min_p[r] (null or not above 0:

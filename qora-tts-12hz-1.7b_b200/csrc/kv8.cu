@@ -300,9 +300,13 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
 
 // A warp takes the blocks that start in a chunk of rows, for one K or V head
 // (they are its alone: the block's scale needs all of its new tokens), or
-// kQHeads query heads of one row.  HBM-bound: every input is read from HBM once, every
+// kQHeads query heads of one row.  Every input is read from HBM once, every
 // output written once, and a block that grows has its earlier codes read and
-// written again.
+// written again.  16 chunks of 611 bf16 rows (16 query, 8 K/V heads of 128):
+// 54 us, 109 MB at 2.0 TB/s: 31 million warp instructions (norm, rotation and
+// codes with each rounding of its own), issued in 54% of the cycles by 19 warps
+// an SM, which wait for loads in between.  512 single f32 tokens: 8.0 us, 22 MB at
+// 2.8 TB/s, which is one warp's chain of loads and reductions; one token: 3.1 us.
 template <typename T, int HD, int KEEP>
 __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
   pdl_launch_dependents();
@@ -321,12 +325,24 @@ __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constan
 }
 
 // ---- attention -------------------------------------------------------------------
-// Scores and products run on the matrix units in f16 with f32 sums.  A code is
-// exact in f16; a query (scaled by a power of two to at most 2) and a weight
-// (at most 2) are split into f16 hi + lo, lo scaled by 2^11, about 22 bits.
-// One m16n8k16 product takes up to 8 slots (a slot is a query head of a row)
-// with hi in row s and lo in row s + 8 of its 16-row operand, so the split
-// costs nothing, and hi + lo of a slot meet in one thread.
+// Single tokens and few rows: a slot is a query head of a row, and a unit is up
+// to 8 slots that share a K/V head and its pages; a warp takes every n-th page
+// and keeps the running maximum and sum of each slot, and the output's sums.
+// Scores: a query, scaled by a power of two, is an integer of 22 bits in three
+// signed bytes, and the products with the 8-bit codes on the integer matrix
+// units are exact (f16 hi + lo took 13% longer).  A product of 16 rows takes
+// two of the bytes of 8 slots.  Output: a weight times the V scale is split
+// into f16 hi + lo, lo scaled by 2^11, about 22 bits, and V's codes are exact
+// in f16: hi in row s and lo in row s + 8 of the 16-row operand, so the split
+// costs nothing, and hi + lo of a slot meet in one thread; sums in f32.
+//
+// 256 sequences of up to 4099 positions (16 heads, 8 K/V heads of 128), one bf16
+// row each: 301 - 309 us, 1.61 GB at 5.2 - 5.4 TB/s: HBM bounds it.  With fewer
+// pages a warp, about 500 instructions a page and the start do (rows, then the
+// table, then the pages: three trips to HBM; at the end the warps' sums): 64
+// sequences of up to 530, f32: 20 us, 53 MB at 2.7 TB/s; one of 32003 in
+// clusters of 10 CTAs of 12 warps: 29 us, 49 MB at 1.7 TB/s, as clusters of a
+// K/V head each leave 68 SMs idle; one of 265: 7.5 us.
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -795,8 +811,9 @@ cudaError_t launch_attn_t(const Kv8AttnDesc& d, long units, int pages, int sms, 
   // warp, a cluster of n counting like 0.4 + 0.1 n steps and a warp like 0.05:
   // 512 units of 19 pages take 15.0 us with 3 warps, 17.4 with 2, 20.1 with 4
   // (two waves); 128 units of 63 pages 16.5 us with 12 warps, 21.2 as 6 x 2; 256
-  // of 63 pages 21.6 us as 2 x 3, 23.6 with 4; 8 of 2001 pages 29 us as 10 x 12.  Clusters of more than 8 have to fit the
-  // GPU's processing clusters (16 x 12 warps: two waves, 42 us).
+  // of 63 pages 21.6 us as 2 x 3, 23.6 with 4; 8 of 2001 pages 29 us as 10 x 12.
+  // Clusters of more than 8 have to fit the GPU's processing clusters (16 x 12
+  // warps: two waves, 42 us).
   int best_w = 0;
   unsigned best_n = 1;
   double best = 1e30;
@@ -849,10 +866,11 @@ cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max
   };
   // Units of 8 slots here, or tiles of 128 (kv8_tile.cu)?  Both as measured, in
   // us: a unit costs 0.0085 and 0.0009 a page (of 128 dims) over 7; a CTA of
-  // tiles 10 and 2.2 a tile over 4 (10 with splits), one an SM at a time.  One sequence's 100
-  // rows over 100 positions (16 heads, 8 K/V heads of 128): 10.3 here and 16 in
-  // tiles; 8 such sequences: 27 and 16; 4 of 64 rows over 4000: 102 and 45; 16
-  // rows over 1000: 12 and 20; 500 rows of 16 heads of 64, window 72: 13.5 and 20.
+  // tiles 10 and 2.2 a tile over 4 (10 with splits), one an SM at a time.  One
+  // sequence's 100 rows over 100 positions (16 heads, 8 K/V heads of 128): 10.3
+  // here and 16 in tiles; 8 such sequences: 27 and 16; 4 of 64 rows over 4000: 102
+  // and 45; 16 of 4 over 2000: 23 and 37; 16 rows over 1000: 12 and 20; 500 rows
+  // of 16 heads of 64, window 72: 13.5 and 20.
   if (max_rows > 1) {
     const double here = 7.0 + units * (0.0085 + 0.0009 * d.c.head_dim / 128 * ((seen(d.group_rows) + kKv8Page - 1) / kKv8Page));
     Kv8AttnDesc t = d;

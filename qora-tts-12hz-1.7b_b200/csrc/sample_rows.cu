@@ -9,15 +9,26 @@
 //
 // A row is cut down to a list of at most kList tokens in one CTA's shared memory:
 //   a short row is one;
-//   small top-k: the least of the CTAs' own (k / CTAs)-th largest thread
-//     maxima has k logits above it and few more; those are the list;
+//   small top-k: a key that (k / CTAs) of each CTA's thread maxima reach has k
+//     logits above it and few more; those are the list;
 //   otherwise a histogram over (largest - l) / T of counts (top-k) or weights
 //     (top-p) gives the bin in which the last kept token lies, and that bin's
 //     tokens are the list.
 // In a list the token at which the running count or weight reaches a target is
-// found by histograms over the range that still holds it, until one warp can
-// put the rest in order.  A long row is shared by a cluster of CTAs, which read
-// it from HBM once and from the L2 cache in the passes after the first.
+// found by histograms over the range that still holds it, until there is a
+// thread for each token.  A long row is shared by a cluster of CTAs, which keep
+// their columns in shared memory where they fit, and otherwise read them again
+// from the L2 cache.
+//
+// A row's bytes would take HBM a fraction of this; what bounds it:
+//   256 rows of 2048 f32 logits, top-k 50: 7.8 us (0.27 TB/s), a dozen block-wide
+//     steps one after the other;
+//   one row of 151936 f32, top-p: 29 us on 16 SMs, the same and the f64
+//     exponentials (a quarter of it);
+//   128 rows of 151936 bf16, top-k 1000, top-p, min-p: 40 us, 39 MB at 1.0 TB/s,
+//     half of it the two passes over the row;
+//   the same rows with top-p alone: 141 us, of which the weights' histogram takes
+//     55 (about 90 issue slots a logit, the f64 series the most of it).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
