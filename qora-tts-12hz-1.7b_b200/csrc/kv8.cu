@@ -261,40 +261,66 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
 }
 
 constexpr int kQHeads = 4;  // query heads of a warp
+// Rows of a warp of query heads: one where most rows are single tokens, which are
+// few, and 2 of a prompt, whose loads hide each other.  (16 chunks of 611 rows:
+// 55.2, 50.9, 51.9 and 56.2 us with 1, 2, 3 and 4.)
+template <int KEEP>
+constexpr int kQRows = KEEP == kAppendKeep ? 2 : 1;
 
-// kQHeads query heads of one row, from h0 on.
-template <typename T, int HD>
+// kQHeads query heads of rows [row, row + ROWS), from h0 on: the loads of all
+// rows are on their way before the first is worked on.
+template <typename T, int HD, int ROWS>
 __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
   constexpr int LPT = HD / 4, TPW = 32 / LPT, N = kQHeads / TPW;
   const int lane = threadIdx.x & 31, sub = lane / LPT, d0 = (lane % LPT) * 4;
   const bool upper = (lane % LPT) >= LPT / 2;
-  const int seq = d.seq[row], pos = d.pos[row], rp = d.rope_pos ? d.rope_pos[row] : pos;
-  const T* src = static_cast<const T*>(d.q) + (size_t)row * d.ldq;
-  T* dst = static_cast<T*>(d.q_out) + (size_t)row * d.ldqo;
-  float4 x[N];
+  Raw4<T> raw[ROWS][N];
+  int rp[ROWS];
+  bool ok[ROWS];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int h = h0 + i * TPW + sub;
-    x[i] = h < d.heads ? load4(src + (size_t)h * HD + d0) : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  if (seq < 0 || seq >= d.c.n_seqs || pos < 0 || pos >= d.c.pages_per_seq * kKv8Page) return;  // flagged with K and V
-  float4 cs, sn;
-  bool turn = d.rope_cos != nullptr;
-  if (turn) {
-    turn = rp >= 0 && rp < d.rope_rows;
-    if (turn) {
-      cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
-      sn = signed_sin(load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2)), upper);
-    } else {
-      raise(d.flags, QTTS_KV8_ROPE_RANGE);
+  for (int r = 0; r < ROWS; ++r) {
+    const int at = min(row + r, d.n_rows - 1);
+    const int seq = d.seq[at], pos = d.pos[at];
+    rp[r] = d.rope_pos ? d.rope_pos[at] : pos;
+    // (what is out of range is flagged with K and V)
+    ok[r] = row + r < d.n_rows && seq >= 0 && seq < d.c.n_seqs && pos >= 0 && pos < d.c.pages_per_seq * kKv8Page;
+    const T* src = static_cast<const T*>(d.q) + (size_t)at * d.ldq;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int h = h0 + i * TPW + sub;
+      raw[r][i] = Raw4<T>{};
+      if (h < d.heads) raw[r][i] = *reinterpret_cast<const Raw4<T>*>(src + (size_t)h * HD + d0);
     }
   }
-  if (d.q_norm) head_norm<HD, N>(x, norm_weight(d.q_norm, d0));
+  float4 cs[ROWS], sn[ROWS];
+  bool turn[ROWS];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int h = h0 + i * TPW + sub;
-    if (turn) x[i] = rotate<HD>(x[i], cs, sn);
-    if (h < d.heads) store4(dst + (size_t)h * HD + d0, x[i]);
+  for (int r = 0; r < ROWS; ++r) {
+    turn[r] = ok[r] && d.rope_cos != nullptr;
+    if (turn[r]) {
+      turn[r] = rp[r] >= 0 && rp[r] < d.rope_rows;
+      if (turn[r]) {
+        cs[r] = load4(d.rope_cos + (size_t)rp[r] * (HD / 2) + d0 % (HD / 2));
+        sn[r] = load4(d.rope_sin + (size_t)rp[r] * (HD / 2) + d0 % (HD / 2));
+      } else {
+        raise(d.flags, QTTS_KV8_ROPE_RANGE);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (!ok[r]) continue;
+    float4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = load4(reinterpret_cast<const T*>(&raw[r][i]));
+    if (d.q_norm) head_norm<HD, N>(x, norm_weight(d.q_norm, d0));
+    T* dst = static_cast<T*>(d.q_out) + (size_t)(row + r) * d.ldqo;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int h = h0 + i * TPW + sub;
+      if (turn[r]) x[i] = rotate<HD>(x[i], cs[r], signed_sin(sn[r], upper));
+      if (h < d.heads) store4(dst + (size_t)h * HD + d0, x[i]);
+    }
   }
 }
 
@@ -303,10 +329,10 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
 // kQHeads query heads of one row.  Every input is read from HBM once, every
 // output written once, and a block that grows has its earlier codes read and
 // written again.  16 chunks of 611 bf16 rows (16 query, 8 K/V heads of 128):
-// 54 us, 109 MB at 2.0 TB/s: 31 million warp instructions (norm, rotation and
+// 51 us, 109 MB at 2.1 TB/s: 31 million warp instructions (norm, rotation and
 // codes with each rounding of its own), issued in 54% of the cycles by 19 warps
-// an SM, which wait for loads in between.  512 single f32 tokens: 8.0 us, 22 MB at
-// 2.8 TB/s, which is one warp's chain of loads and reductions; one token: 3.1 us.
+// an SM, which wait for loads in between.  512 single f32 tokens: 8.2 us, 22 MB at
+// 2.7 TB/s, which is one warp's chain of loads and reductions; one token: 3.1 us.
 template <typename T, int HD, int KEEP>
 __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
   pdl_launch_dependents();
@@ -320,7 +346,8 @@ __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constan
   } else {
     const int per = (d.heads + kQHeads - 1) / kQHeads;
     const long i = w - d.kv_warps;
-    if (per > 0 && i < (long)d.n_rows * per) rotate_queries<T, HD>(d, (int)(i / per), (int)(i % per) * kQHeads);
+    const long row = per > 0 ? i / per * kQRows<KEEP> : d.n_rows;
+    if (row < d.n_rows) rotate_queries<T, HD, kQRows<KEEP>>(d, (int)row, (int)(i % per) * kQHeads);
   }
 }
 
@@ -767,7 +794,8 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
 
 template <typename T, int HD>
 cudaError_t launch_append_t(const Kv8AppendDesc& d, bool single, cudaStream_t st) {
-  const long warps = d.kv_warps + (d.q ? (long)d.n_rows * ((d.heads + kQHeads - 1) / kQHeads) : 0);
+  const int rows = single ? 1 : kQRows<kAppendKeep>;
+  const long warps = d.kv_warps + (d.q ? ((long)d.n_rows + rows - 1) / rows * ((d.heads + kQHeads - 1) / kQHeads) : 0);
   const auto kernel = single ? kv8_append_kernel<T, HD, 128 / HD> : kv8_append_kernel<T, HD, kAppendKeep>;
   return launch_k(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, st, LaunchOpts{true, 1}, d);
 }

@@ -178,6 +178,54 @@ def test_same_rows_same_tokens_whatever_the_batch(qtts):
         assert all(p[r] == q[0] for p, q in zip(a, b))
 
 
+def test_in_a_graph_and_on_two_streams_at_once(qtts):
+    # no workspace: calls of every path run side by side, and a captured call
+    # reads its logits and numbers anew at each replay
+    rng = np.random.default_rng(31)
+    cases = [(3, 151936, dict(top_p=0.9)), (40, 2048, dict(top_k=50)), (20, 30000, dict(top_k=300, top_p=0.95, min_p=0.01)),
+             (2, 151936, dict(temperature=0.0))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    made = []
+    for n, V, kw in cases:
+        t = {"x": torch.empty(n, V, device="cuda"), "u": torch.empty(n, device="cuda"),
+             "token": torch.zeros(n, dtype=torch.int32, device="cuda"), "kept": torch.zeros(n, dtype=torch.int32, device="cuda")}
+        t.update({k + "_ptr": torch.full((n,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device="cuda")
+                  for k, v in kw.items()})
+        made.append((n, V, kw, t))
+
+    def call(n, V, kw, t, stream):
+        qtts.sample_rows_dev(t["x"].data_ptr(), n, V, t["u"].data_ptr(), t["token"].data_ptr(), kept_ptr=t["kept"].data_ptr(),
+                             stream=stream.cuda_stream, **{k: v.data_ptr() for k, v in t.items() if k.endswith("_ptr")})
+
+    graphs = []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for c in made[i::2]:
+                call(*c, s)
+        graphs.append(g)
+    for turn in range(3):
+        for n, V, kw, t in made:
+            t["x"].copy_(torch.from_numpy((rng.standard_normal((n, V)) * 2.5).astype(np.float32)))
+            t["u"].copy_(torch.from_numpy(rng.random(n).astype(np.float32)))
+        torch.cuda.synchronize()
+        if turn < 2:
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        else:
+            for i, c in enumerate(made):
+                call(*c, streams[i % 2])
+        torch.cuda.synchronize()
+        for n, V, kw, t in made:
+            x, u = t["x"].cpu().numpy(), t["u"].cpu().numpy()
+            for r in range(n):
+                wt, wk, _, margin = R.sample(x[r], kw.get("temperature", 1.0), kw.get("top_k", 0),
+                                             np.float32(kw.get("top_p", 1.0)), np.float32(kw.get("min_p", 0.0)), u[r])
+                assert t["kept"][r].item() == wk
+                assert margin <= V * 2.0 ** -45 or t["token"][r].item() == wt
+
+
 def test_host_logits_are_refused(qtts):
     t = torch.zeros(64)
     d = torch.zeros(64, device="cuda")
