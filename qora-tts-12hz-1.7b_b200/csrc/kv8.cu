@@ -586,11 +586,17 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
         see_lo = d.window > 0 ? max(0, see_hi - d.window) : 0;
       }
     }
-    float o[NT][4];
+    // The matrix units' sums are cut off, not rounded, which adds up over a long
+    // cache (26000 positions: 1.3e-5).  With f32 rows they hold one step, and
+    // `sum` all of them, rounded; 16-bit results do not show the difference.
+    constexpr bool kRounded = sizeof(T) == 4;
+    float o[NT][4], sum[kRounded ? NT : 1][2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+      if constexpr (kRounded) sum[i][0] = sum[i][1] = 0.0f;
+    }
     float m = -INFINITY, mo = -INFINITY, l = 0.0f;
 
     // kStep pages at a time: independent chains of products and one running
@@ -656,11 +662,11 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       const float mz = mn == -INFINITY ? 0.0f : mn;
       l *= ex2(m - mz);
       const float beta = mo == mon ? 1.0f : ex2(mo - mon);
-      if (__any_sync(kFull, beta != 1.0f)) {
+      if (kRounded || __any_sync(kFull, beta != 1.0f)) {
 #pragma unroll
         for (int k = 0; k < NT; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[k][e] *= beta;
+          for (int e = 0; e < 4; ++e) o[k][e] = kRounded ? 0.0f : o[k][e] * beta;
       }
       m = mn;
       mo = mon;
@@ -707,6 +713,12 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       }
       __syncwarp();  // every lane has read these pages
       issue(i + kStages);
+      if constexpr (kRounded) {
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) sum[k][e] = fmaf(sum[k][e], beta, fmaf(o[k][e + 2], 1.0f / kSplitLoScale, o[k][e]));
+      }
     }
     // join the warps, then the splits of the cluster, in their order
     l += __shfl_xor_sync(kFull, l, 1);
@@ -720,11 +732,11 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int k = 0; k < NT; k += 4) {
-          float4 v;
-          v.x = (o[k][e] + o[k][e + 2] * (1.0f / kSplitLoScale)) * back;
-          v.y = (o[k + 1][e] + o[k + 1][e + 2] * (1.0f / kSplitLoScale)) * back;
-          v.z = (o[k + 2][e] + o[k + 2][e + 2] * (1.0f / kSplitLoScale)) * back;
-          v.w = (o[k + 3][e] + o[k + 3][e + 2] * (1.0f / kSplitLoScale)) * back;
+          auto all = [&](int i) {
+            if constexpr (kRounded) return sum[i][e] * back;
+            else return (o[i][e] + o[i][e + 2] * (1.0f / kSplitLoScale)) * back;
+          };
+          const float4 v = make_float4(all(k), all(k + 1), all(k + 2), all(k + 3));
           *reinterpret_cast<float4*>(&s_o[warp][g][NT * (2 * t + e) + k]) = v;
         }
       if (t == 0) {

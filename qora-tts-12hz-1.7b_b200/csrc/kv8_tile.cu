@@ -48,7 +48,9 @@ namespace {
 constexpr int kTileM = 128, kTilePos = 128, kTilePages = kTilePos / kKv8Page;
 constexpr int kSoft = 256, kConvert = 128;  // threads of the softmax (two halves) and of the conversion
 constexpr int kTileThreads = kSoft + kConvert + 32;  // and a warp that issues the products
-constexpr uint32_t kTmemCols = 512;  // half h: S and P at 256 h, O at 256 h + 128
+// Half h: S and P at 256 h, O at 256 h + 128.  With f32 rows, which have one
+// half: O of tile n at 128 + 256 (n & 1), the sums of all tiles at kSums.
+constexpr uint32_t kTmemCols = 512, kSums = 256;
 constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr float kNoPage = 4.0f;  // no fraction of a scale (split_scale)
 constexpr int kScales = 4;  // tiles of scales kept: a half may be two tiles behind the conversion
@@ -59,6 +61,7 @@ struct TileSegment {
 struct TileShared {
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2];  // by buffer
   uint64_t s_full[2], p_full[2], o_full[2];             // by half
+  uint64_t o_free[2];  // f32: by O's buffer
   uint64_t q_full, fin;
   uint32_t tmem;
   int abort;
@@ -69,6 +72,7 @@ struct TileShared {
   // V scale; NaN keeps a page from the short way (Softmax::tile_short)
   float4 scale[kScales][kTilePages];
   float m[2 * kTileM], l[2 * kTileM];
+  float mo[4][kTileM];  // f32: the exponent of O of the last tiles
 };
 
 template <typename T, int HD>
@@ -376,16 +380,22 @@ struct Products {
     constexpr uint32_t idesc = instruction(HD, true);
     if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
     ++done[h];
+    if (C::kSplit && done[h] > 2) {  // the buffer's tile before has been added up
+      const int n = done[h] - 3;
+      if (!warp_wait(&sh.o_free[n & 1], (n >> 1) & 1, &sh.abort)) return false;
+    }
     if (lane == 0) {
-      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h, o = s + kTilePos;
+      const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h;
+      const uint32_t o = s + kTilePos + (C::kSplit ? 256 * ((done[h] - 1) & 1) : 0);
       tc_fence_after();
 #pragma unroll
       for (int e = 0; e < kTilePos / 16; ++e) {
         const uint32_t p = s + 32 * (e >> 1) + 8 * (e & 1);
-        mma_ts(o, p, operand(v + e * 256, 2048), idesc, !first || e > 0);
+        mma_ts(o, p, operand(v + e * 256, 2048), idesc, (!first && !C::kSplit) || e > 0);
         if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
       }
       commit_to(&sh.o_full[h]);
+      if (C::kSplit) bar_arrive(&sh.o_full[h]);  // (passes on sh.mo, as above)
       if (last) commit_to(&sh.v_free[b]);
     }
     __syncwarp();
@@ -417,10 +427,10 @@ struct Running {
 
 // The running exponent of O follows max(score + exponent of the V scale); O is
 // rescaled when it has grown by 6.  (mo of -inf: nothing is in O yet.)
-template <int HD>
+template <int HD, bool SPLIT>
 __device__ __forceinline__ void grow_to(float mon, float& mo, uint32_t o) {
   const bool grow = mon > mo + 6.0f, rescale = grow && mo > -INFINITY;
-  if (__any_sync(kFull, rescale)) {
+  if (!SPLIT && __any_sync(kFull, rescale)) {
     const float beta = rescale ? ex2(mo - mon) : 1.0f;
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
@@ -462,7 +472,7 @@ __device__ __noinline__ Running tile_long(Running r, uint32_t s, unsigned from, 
       }
     }
   }
-  grow_to<HD>(mon, r.mo, s + kTilePos);
+  grow_to<HD, SPLIT>(mon, r.mo, s + kTilePos);
   const float mz = mn == -INFINITY ? 0.0f : mn;
   r.l *= ex2(r.m - mz);
   r.m = mn;
@@ -598,7 +608,7 @@ struct Softmax {
       tmem_wait(r[0], x);  // the load on its way
       return false;
     }
-    grow_to<HD>(mon, mo, s + kTilePos);
+    grow_to<HD, C::kSplit>(mon, mo, s + kTilePos);
     l *= ex2(m - mn);
     m = mn;
 #pragma unroll
@@ -655,12 +665,15 @@ struct Softmax {
         mo = r.mo;
         l = r.l;
       }
+      if (C::kSplit) sh.mo[done & 3][slot] = mo;
       tmem_store_wait();
       tc_fence_before();
       bar_arrive(&sh.p_full[half]);
     }
     if (t1 > t0) {
-      if (!warp_wait(&sh.o_full[half], (done - 1) & 1, &sh.abort)) return false;
+      const int n = done - 1;
+      if (C::kSplit ? !warp_wait(&sh.o_free[n & 1], (n >> 1) & 1, &sh.abort) : !warp_wait(&sh.o_full[half], n & 1, &sh.abort))
+        return false;
       tc_fence_after();
     }
     return true;
@@ -674,7 +687,7 @@ struct Softmax {
     for (int c = 0; c < HD / 32; ++c) {
       float x[32];
       if (any) {
-        tmem_load(columns() + kTilePos + 32 * c, x);
+        tmem_load(columns() + (C::kSplit ? kSums : kTilePos) + 32 * c, x);
 #pragma unroll
         for (int e = 0; e < 32; ++e) x[e] *= back;
       } else {
@@ -683,6 +696,55 @@ struct Softmax {
       }
       f(32 * c, x);
     }
+  }
+};
+
+// ---- sums of f32 rows --------------------------------------------------------------
+// The matrix units' sums are cut off, not rounded, which adds up over many tiles
+// (2700 positions: 7.6e-6 of the result).  With f32 rows O holds one tile, and
+// the warps of the second half, which these rows leave free, add it up in f32.
+template <typename T, int HD>
+struct Sums {
+  using J = TileJob<T, HD>;
+  const J& job;
+  const uint32_t columns;
+  int done = 0;
+
+  __device__ explicit Sums(const J& j) : job(j), columns(j.tmem + ((threadIdx.x & 96u) << 16)) {}
+  __device__ bool run(const TileSegment& g) {
+    TileShared& sh = job.sh;
+    int p0, p1, t0, t1;
+    job.tiles(g, p0, p1, t0, t1);
+    float last = -INFINITY;
+    for (int t = t0; t < t1; ++t, ++done) {
+      if (!warp_wait(&sh.o_full[0], done & 1, &sh.abort)) return false;
+      tc_fence_after();
+      const float mo = sh.mo[done & 3][threadIdx.x & (kTileM - 1)];
+      const float beta = last == mo ? 1.0f : ex2(last - mo);  // (0 after -inf)
+      last = mo;
+      const uint32_t o = columns + kTilePos + 256 * (done & 1), sums = columns + kSums;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        float x[32], y[32];
+        tmem_load(o + 32 * c, x);
+        if (t > t0) {
+          tmem_load(sums + 32 * c, y);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = fmaf(y[e], beta, x[e]);
+        }
+        uint32_t r[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(x[16 * h + e]);
+          tmem_store16(sums + 32 * c + 16 * h, r);
+        }
+      }
+      tmem_store_wait();
+      tc_fence_before();
+      bar_arrive(&sh.o_free[done & 1]);
+    }
+    return true;
   }
 };
 
@@ -752,7 +814,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bar_init(&sh.v_free[i], 1);
       bar_init(&sh.s_full[i], 2);
       bar_init(&sh.p_full[i], kTileM);
-      bar_init(&sh.o_full[i], 1);
+      bar_init(&sh.o_full[i], C::kSplit ? 2 : 1);
+      bar_init(&sh.o_free[i], kTileM);
     }
     bar_init(&sh.q_full, kTileM * d.halves);
     bar_init(&sh.fin, 1);
@@ -801,6 +864,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   Converter<T, HD> conv(job);
   Products<T, HD> products(job);
+  Sums<T, HD> sums_of(job);
   bool ok = true;
   int it = 0;
   if (softmax) {  // (while the first codes are on their way)
@@ -816,6 +880,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (softmax) ok = soft.run(seg, it);
       else if (warp == kLast) ok = products.run(seg, it);
       else if (tid >= kSoft) ok = conv.run(seg, it);
+      else if (C::kSplit) ok = sums_of.run(seg);
     }
     const bool mine = softmax && soft.row >= seg.row0 && soft.row < seg.row0 + seg.rows;
     int p0, p1, t0, t1;

@@ -397,6 +397,39 @@ def test_negative_scales(qtts, rows):
     check_attention(qtts, p, rng, seq, pos, 16, "f32", max_rows=rows)
 
 
+@pytest.mark.parametrize("rows,length,n_seqs,kvh,hd", [(1, 12000, 150, 1, 128), (1, 12000, 150, 1, 64), (256, 3000, 8, 8, 64),
+                                                         (256, 3000, 4, 8, 128)])
+def test_long_f32_sums_are_rounded(qtts, rows, length, n_seqs, kvh, hd):
+    # Sequences that share their pages, many pages a warp or tiles a CTA.  Scores
+    # of at most a few units: a weight is off by 2^-21 (exp2, the pair, the
+    # score's rounding), which for values of random sign is the result's relative
+    # error in the norm, and sums that are rounded at each step add
+    # sqrt(steps) 2^-24 and 2^-22 for the products within one: less than 2^-19.
+    # Sums cut off at each product would be off by 2^-24 times their number, here
+    # by 5e-6 and more.
+    rng = np.random.default_rng(length + hd)
+    p = Pool(qtts, rng, 1, (length + 15) // 16, kvh, hd)
+    table = p.d_table.expand(n_seqs, -1).contiguous()
+    cache = qtts.Kv8Cache(p.d_codes.data_ptr(), p.d_scales.data_ptr(), table.data_ptr(), p.codes.shape[0], n_seqs,
+                          table.shape[1], kvh, hd)
+    seq, pos = rows_of([(s, length - rows, rows) for s in range(n_seqs)])
+    q = dev((rng.standard_normal((len(seq), kvh * hd)) * 0.3).astype(np.float32))
+    out = torch.empty_like(q)
+    t = dev(seq), dev(pos)
+    qtts.kv8_attention_dev(cache, q.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), len(seq), kvh,
+                           scale=hd ** -0.5, max_rows=rows, max_len=length)
+    torch.cuda.synchronize()
+    at = dev(p.table[0].astype(np.int64))
+    kv = p.d_codes[at, 0].double() * p.d_scales[at, 0].double()[..., None, None]  # [page][2][kvh][16][hd]
+    kv = kv.permute(1, 2, 0, 3, 4).reshape(2, kvh, -1, hd)[:, :, :length]
+    for h in range(kvh):
+        a = q[:, h * hd:(h + 1) * hd].double() @ kv[0, h].T * hd ** -0.5
+        a.masked_fill_(torch.arange(length, device="cuda")[None] > t[1][:, None], -float("inf"))
+        want = torch.softmax(a, -1) @ kv[1, h]
+        err = (out[:, h * hd:(h + 1) * hd].double() - want).norm() / want.norm()
+        assert err.item() <= 2.0 ** -19, (h, err.item())
+
+
 # Enough rows that tiles of 128 slots take over (the choice weighs the units of
 # eight slots against them), with everything that can go wrong in a tile.
 MANY = [(0, 57, 100), (-1, 3, 4), (1, 0, 130), (2, 300, 99), (3, -5, 60), (3, 55, 40), (-1, 0, 33), (4, 399, 1), (5, 128, 128),
