@@ -367,9 +367,9 @@ __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constan
 // row each: 301 - 309 us, 1.61 GB at 5.2 - 5.4 TB/s: HBM bounds it.  With fewer
 // pages a warp, about 500 instructions a page and the start do (rows, then the
 // table, then the pages: three trips to HBM; at the end the warps' sums): 64
-// sequences of up to 530, f32: 20 us, 53 MB at 2.7 TB/s; one of 32003 in
+// sequences of up to 530, f32: 21 us, 53 MB at 2.5 TB/s; one of 32003 in
 // clusters of 10 CTAs of 12 warps: 29 us, 49 MB at 1.7 TB/s, as clusters of a
-// K/V head each leave 68 SMs idle; one of 265: 7.5 us.
+// K/V head each leave 68 SMs idle; one of 265: 7.0 us.
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -587,8 +587,9 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       }
     }
     // The matrix units' sums are cut off, not rounded, which adds up over a long
-    // cache (26000 positions: 1.3e-5).  With f32 rows they hold one step, and
-    // `sum` all of them, rounded; 16-bit results do not show the difference.
+    // cache (26177 positions, 4 warps: 1.3e-5).  With f32 rows they hold one step,
+    // and `sum` all of them, rounded (2.7e-6, and 8e-7 with l's roundings made up
+    // for); 16-bit results do not show the difference.
     constexpr bool kRounded = sizeof(T) == 4;
     float o[NT][4], sum[kRounded ? NT : 1][2];
 #pragma unroll
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
       if constexpr (kRounded) sum[i][0] = sum[i][1] = 0.0f;
     }
-    float m = -INFINITY, mo = -INFINITY, l = 0.0f;
+    float m = -INFINITY, mo = -INFINITY, l = 0.0f, lost = 0.0f;  // lost: what roundings added to l
 
     // kStep pages at a time: independent chains of products and one running
     // maximum for all of them
@@ -660,7 +661,8 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
         mon = fmaxf(mon, pm[k] + ev[k]);
       }
       const float mz = mn == -INFINITY ? 0.0f : mn;
-      l *= ex2(m - mz);
+      const float alpha = ex2(m - mz);
+      float part = 0.0f;  // of l
       const float beta = mo == mon ? 1.0f : ex2(mo - mon);
       if (kRounded || __any_sync(kFull, beta != 1.0f)) {
 #pragma unroll
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const float a = ex2(s[k][n][0] - mz), b = ex2(s[k][n][1] - mz);
-          l += a + b;
+          part += a + b;
           split_pair(a * fac, b * fac, pa[n * 2], pa[n * 2 + 1]);
         }
         const uint8_t* vb = base + k * 2 * R::kBlock + R::kBlock;
@@ -710,6 +712,11 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
           mma16816(o[q * 4 + 2], pa, half2_of(a23, 0x4140), half2_of(b23, 0x4140));
           mma16816(o[q * 4 + 3], pa, half2_of(a23, 0x4342), half2_of(b23, 0x4342));
         }
+      }
+      {
+        const float add = fmaf(lost, -alpha, part), before = l * alpha;
+        l = before + add;
+        lost = (l - before) - add;
       }
       __syncwarp();  // every lane has read these pages
       issue(i + kStages);
