@@ -21,13 +21,14 @@
 // split query take the room of two halves, so that f32 has one half.
 // The V scales are folded into P, relative to a running exponent of their own,
 // so that P stays within f16 whatever the scales are; O is rescaled only when
-// that exponent has grown by 6 (P then reaches 2^7).
+// that exponent has grown by 6 (P then reaches 2^13).
 //
 // Four chunks of 1000 bf16 rows over up to 3001 positions (16 heads, 8 K/V heads
 // of 128): 157 us, 49 GFLOP at 314 TFLOP/s.  A half's chain bounds it: a tile
 // takes 6000 cycles, 3700 for the softmax and the rest for the products before
-// and after it, while the exponentials' pipe is 27% and the tensor pipe 24% busy.  f32 has twice the products and one half
-// (four chunks of 64 rows over 4000: 44 us in bf16, 58 in f32).
+// and after it, while the exponentials' pipe is 27% and the tensor pipe 24% busy.
+// f32 has twice the products and one half (four chunks of 64 rows over 4000: 44
+// us in bf16, 58 in f32).
 //
 // A tile of rows may span sequences: its segments (runs of rows of one
 // sequence) are taken one after the other, with the other slots masked.
@@ -358,14 +359,17 @@ struct Products {
       const uint32_t q = smem_of(job.ops + C::kQ) + h * C::kHalf, k = smem_of(job.ops + C::kK) + b * C::kHalf;
       const uint32_t s = job.tmem + 256 * h;
       tc_fence_after();
-#pragma unroll
-      for (int e = 0; e < HD / 16; ++e)
-        mma_ss(s, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, e > 0);
+      // lo first: each product's sum is cut off, which is less while it is small
+      // (f32 rows over 2714 positions: 1.46e-6 of the result with lo last or
+      // between, 6.3e-7 so)
       if (C::kSplit) {
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e)
-          mma_ss(s, operand(q + C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, true);
+          mma_ss(s, operand(q + C::kHalf + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, e > 0);
       }
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e)
+        mma_ss(s, operand(q + e * 256, 16 * HD), operand(k + e * 256, 16 * HD), idesc, C::kSplit || e > 0);
       commit_to(&sh.s_full[h]);
       if (last) commit_to(&sh.k_free[b]);
       // a plain arrival besides the products' own: it passes on what the
@@ -389,12 +393,14 @@ struct Products {
       const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h;
       const uint32_t o = s + kTilePos + (C::kSplit ? 256 * ((done[h] - 1) & 1) : 0);
       tc_fence_after();
+      auto columns = [&](int e) { return s + 32 * (e >> 1) + 8 * (e & 1); };
+      if (C::kSplit) {
 #pragma unroll
-      for (int e = 0; e < kTilePos / 16; ++e) {
-        const uint32_t p = s + 32 * (e >> 1) + 8 * (e & 1);
-        mma_ts(o, p, operand(v + e * 256, 2048), idesc, (!first && !C::kSplit) || e > 0);
-        if (C::kSplit) mma_ts(o, p + 16, operand(v + e * 256, 2048), idesc, true);
+        for (int e = 0; e < kTilePos / 16; ++e) mma_ts(o, columns(e) + 16, operand(v + e * 256, 2048), idesc, e > 0);
       }
+#pragma unroll
+      for (int e = 0; e < kTilePos / 16; ++e)
+        mma_ts(o, columns(e), operand(v + e * 256, 2048), idesc, C::kSplit || !first || e > 0);
       commit_to(&sh.o_full[h]);
       if (C::kSplit) bar_arrive(&sh.o_full[h]);  // (passes on sh.mo, as above)
       if (last) commit_to(&sh.v_free[b]);
@@ -422,6 +428,10 @@ struct Products {
 };
 
 // ---- softmax -----------------------------------------------------------------------
+// P starts at up to 2^kAbove: the lo of a pair is rounded to 2^-25, which a
+// typical weight of a long row, 2^-6 of the largest, would show (f32 rows over
+// 2714 positions: 1.58e-6 of the result with P up to 1, 1.46e-6 so).
+constexpr float kAbove = 6.0f;
 struct Running {
   float m, mo, l;  // largest score, exponent of O, sum of exp2(score - m)
 };
@@ -430,9 +440,9 @@ struct Running {
 // rescaled when it has grown by 6.  (mo of -inf: nothing is in O yet.)
 template <int HD, bool SPLIT>
 __device__ __forceinline__ void grow_to(float mon, float& mo, uint32_t o) {
-  const bool grow = mon > mo + 6.0f, rescale = grow && mo > -INFINITY;
+  const bool grow = mon > mo + 2 * kAbove, rescale = grow && mo > -INFINITY;
   if (!SPLIT && __any_sync(kFull, rescale)) {
-    const float beta = rescale ? ex2(mo - mon) : 1.0f;
+    const float beta = rescale ? ex2(mo - (mon - kAbove)) : 1.0f;
 #pragma unroll 1
     for (int c = 0; c < HD / 32; ++c) {
       float x[32];
@@ -446,7 +456,7 @@ __device__ __forceinline__ void grow_to(float mon, float& mo, uint32_t o) {
       }
     }
   }
-  if (grow || mo == -INFINITY) mo = mon;
+  if (grow || mo == -INFINITY) mo = mon - kAbove;
 }
 
 // Any tile: S at columns s (this warp's lanes), of which this slot sees positions
@@ -601,7 +611,7 @@ struct Softmax {
       mn = fmaxf(mn, pm[k]);
       mon = fmaxf(mon, pm[k] + log_v[k]);
     }
-    const float mo_new = mon > mo + 6.0f || mo == -INFINITY ? mon : mo;
+    const float mo_new = mon > mo + 2 * kAbove || mo == -INFINITY ? mon - kAbove : mo;
 #pragma unroll
     for (int k = 0; k < kTilePages; ++k) near &= fabsf(mn + log_v[k] - mo_new) < 40.0f;  // (false for NaN)
     if (!__all_sync(kFull, near)) {
