@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constan
 // Single tokens and few rows: a slot is a query head of a row, and a unit is up
 // to 8 slots that share a K/V head and its pages; a warp takes every n-th page
 // and keeps the running maximum and sum of each slot, and the output's sums.
-// Scores: a query, scaled by a power of two, is an integer of 22 bits in three
-// signed bytes, and the products with the 8-bit codes on the integer matrix
+// Scores: a query, scaled, is an integer of at most 127 * 2^16 in three signed
+// bytes, and the products with the 8-bit codes on the integer matrix
 // units are exact (f16 hi + lo took 13% longer).  A product of 16 rows takes
 // two of the bytes of 8 slots.  Output: a weight times the V scale is split
 // into f16 hi + lo, lo scaled by 2^11, about 22 bits, and V's codes are exact
@@ -388,7 +388,7 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
 // 2^22 is read as a float by one subtraction.
 constexpr int kIntBias = 0x4B400000;
 constexpr float kFloatBias = 12582912.0f;
-// Four numbers of less than 2^22 as three signed bytes each (x = 65536 l0 +
+// Four numbers of at most 127 * 2^16 as three signed bytes each (x = 65536 l0 +
 // 256 l1 + l2): the words of their l0, l1 and l2.
 __device__ __forceinline__ void limbs4(float4 v, float up, uint32_t& w0, uint32_t& w1, uint32_t& w2) {
   const float x[4] = {v.x, v.y, v.z, v.w};
@@ -573,10 +573,9 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
       big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
       finite = ((__ballot_sync(kFull, finite) >> (lane & 28)) & 15u) == 15u;
-      // big in [2^ex, 2^(ex+1)) becomes an integer in [2^21, 2^22)
-      const int ex = min(127, max(-100, ((__float_as_int(big) >> 23) & 255) - 127));
-      const float up = ldexpf(1.0f, 21 - ex);
-      qscale = finite ? ldexpf(d.scale * 1.4426950408889634f, ex - 21) : NAN;  // scores in units of log 2
+      // the largest becomes the integer 127 * 2^16, which three signed bytes hold
+      const float top = fmaxf(big, 0x1p-100f), up = __fdiv_rn(8323072.0f, top);
+      qscale = finite ? d.scale * 1.4426950408889634f * (top * (1.0f / 8323072.0f)) : NAN;  // scores in units of log 2
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
