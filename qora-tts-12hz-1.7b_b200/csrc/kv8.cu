@@ -573,9 +573,9 @@ __global__ void __launch_bounds__(NW * 32, 12 / NW) kv8_attn_kernel(const __grid
       big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
       big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
       finite = ((__ballot_sync(kFull, finite) >> (lane & 28)) & 15u) == 15u;
-      // the largest becomes the integer 127 * 2^16, which three signed bytes hold
-      const float top = fmaxf(big, 0x1p-100f), up = __fdiv_rn(8323072.0f, top);
-      qscale = finite ? d.scale * 1.4426950408889634f * (top * (1.0f / 8323072.0f)) : NAN;  // scores in units of log 2
+      constexpr float kMost = 127.0f * 65536.0f;  // what the largest becomes: three signed bytes hold it
+      const float top = fmaxf(big, 0x1p-100f), up = __fdiv_rn(kMost, top);
+      qscale = finite ? d.scale * 1.4426950408889634f * (top * (1.0f / kMost)) : NAN;  // scores in units of log 2
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
