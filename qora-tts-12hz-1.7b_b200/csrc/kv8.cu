@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constan
 // costs nothing, and hi + lo of a slot meet in one thread; sums in f32.
 //
 // 256 sequences of up to 4099 positions (16 heads, 8 K/V heads of 128), one bf16
-// row each: 301 - 309 us, 1.61 GB at 5.2 - 5.4 TB/s: HBM bounds it.  With fewer
+// row each: 288 - 312 us, 1.61 GB at 5.2 - 5.6 TB/s: HBM bounds it.  With fewer
 // pages a warp, about 500 instructions a page and the start do (rows, then the
 // table, then the pages: three trips to HBM; at the end the warps' sums): 64
 // sequences of up to 530, f32: 21 us, 53 MB at 2.5 TB/s; one of 32003 in
