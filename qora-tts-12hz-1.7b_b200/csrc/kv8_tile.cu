@@ -40,6 +40,7 @@
 #include "common.cuh"
 #include "engine.h"
 #include "kv8.cuh"
+#include "kv8_order.h"
 
 namespace cg = cooperative_groups;
 
@@ -62,7 +63,8 @@ struct TileSegment {
 };
 struct TileShared {
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2];  // by buffer
-  uint64_t s_full[2], p_full[2], o_full[2];             // by half
+  uint64_t s_full[2], p_full[2];                        // by half
+  uint64_t o_full[2];  // by half; f32: by O's buffer (kv8_order.h)
   uint64_t o_free[2];  // f32: by O's buffer
   uint64_t q_full, fin;
   uint32_t tmem;
@@ -349,12 +351,15 @@ struct Products {
   int done[2] = {0, 0};  // tiles of each half
 
   __device__ explicit Products(const J& j) : job(j) {}
+  __device__ __forceinline__ bool wait_for(uint64_t (&bars)[2], TileTurn at) const {
+    return warp_wait(&bars[at.bar], at.parity, &job.sh.abort);
+  }
   // S = Q K^T of half h with K of buffer b; last: no other half reads this K
   __device__ __forceinline__ bool score(int h, int b, bool last) const {
     TileShared& sh = job.sh;
     constexpr uint32_t idesc = instruction(kTilePos, false);
     // P of the half's tile before lies where S goes
-    if (done[h] > 0 && !warp_wait(&sh.o_full[h], (done[h] - 1) & 1, &sh.abort)) return false;
+    if (done[h] > 0 && !wait_for(sh.o_full, o_full_turn(C::kSplit, h, done[h] - 1))) return false;
     if (lane == 0) {
       const uint32_t q = smem_of(job.ops + C::kQ) + h * C::kHalf, k = smem_of(job.ops + C::kK) + b * C::kHalf;
       const uint32_t s = job.tmem + 256 * h;
@@ -384,14 +389,13 @@ struct Products {
     TileShared& sh = job.sh;
     constexpr uint32_t idesc = instruction(HD, true);
     if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
-    ++done[h];
-    if (C::kSplit && done[h] > 2) {  // the buffer's tile before has been added up
-      const int n = done[h] - 3;
-      if (!warp_wait(&sh.o_free[n & 1], (n >> 1) & 1, &sh.abort)) return false;
-    }
+    const int n = done[h]++;
+    // the buffer's tile before has been added up
+    if (C::kSplit && n > 1 && !wait_for(sh.o_free, o_free_turn(n - 2))) return false;
     if (lane == 0) {
       const uint32_t v = smem_of(job.ops + C::kV) + b * C::kHalf, s = job.tmem + 256 * h;
-      const uint32_t o = s + kTilePos + (C::kSplit ? 256 * ((done[h] - 1) & 1) : 0);
+      const uint32_t o = s + kTilePos + (C::kSplit ? 256 * (n & 1) : 0);
+      uint64_t* full = &sh.o_full[o_full_turn(C::kSplit, h, n).bar];
       tc_fence_after();
       auto columns = [&](int e) { return s + 32 * (e >> 1) + 8 * (e & 1); };
       if (C::kSplit) {
@@ -401,8 +405,8 @@ struct Products {
 #pragma unroll
       for (int e = 0; e < kTilePos / 16; ++e)
         mma_ts(o, columns(e), operand(v + e * 256, 2048), idesc, C::kSplit || !first || e > 0);
-      commit_to(&sh.o_full[h]);
-      if (C::kSplit) bar_arrive(&sh.o_full[h]);  // (passes on sh.mo, as above)
+      commit_to(full);
+      if (C::kSplit) bar_arrive(full);  // (passes on sh.mo, as above)
       if (last) commit_to(&sh.v_free[b]);
     }
     __syncwarp();
@@ -683,8 +687,8 @@ struct Softmax {
     }
     if (t1 > t0) {
       const int n = done - 1;
-      if (C::kSplit ? !warp_wait(&sh.o_free[n & 1], (n >> 1) & 1, &sh.abort) : !warp_wait(&sh.o_full[half], n & 1, &sh.abort))
-        return false;
+      const TileTurn at = C::kSplit ? o_free_turn(n) : o_full_turn(false, half, n);
+      if (!warp_wait(C::kSplit ? &sh.o_free[at.bar] : &sh.o_full[at.bar], at.parity, &sh.abort)) return false;
       tc_fence_after();
     }
     return true;
@@ -728,7 +732,8 @@ struct Sums {
     job.tiles(g, p0, p1, t0, t1);
     float last = -INFINITY;
     for (int t = t0; t < t1; ++t, ++done) {
-      if (!warp_wait(&sh.o_full[0], done & 1, &sh.abort)) return false;
+      const TileTurn full = o_full_turn(true, 0, done);
+      if (!warp_wait(&sh.o_full[full.bar], full.parity, &sh.abort)) return false;
       tc_fence_after();
       const float mo = sh.mo[done & 3][threadIdx.x & (kTileM - 1)];
       const float beta = last == mo ? 1.0f : ex2(last - mo);  // (0 after -inf)
@@ -753,7 +758,7 @@ struct Sums {
       }
       tmem_store_wait();
       tc_fence_before();
-      bar_arrive(&sh.o_free[done & 1]);
+      bar_arrive(&sh.o_free[o_free_turn(done).bar]);
     }
     return true;
   }
