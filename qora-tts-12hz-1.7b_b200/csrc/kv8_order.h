@@ -31,4 +31,10 @@ QTTS_TILE_HD TileTurn o_full_turn(bool split, int half, int n) {
 // f32 rows: "the n-th tile has been added up, its buffer of O is free."
 QTTS_TILE_HD TileTurn o_free_turn(int n) { return TileTurn{n & 1, (unsigned)(n >> 1) & 1u}; }
 
+// f32 rows: "all tiles of the n-th segment that has any are added up", which the
+// softmax waits for before it reads the sums.  (o_free of the last tile would not
+// do: the tile of that buffer before may still be on its way then, and the wait
+// would take its parity for the one that is meant.)
+QTTS_TILE_HD unsigned summed_parity(int n) { return (unsigned)n & 1u; }
+
 }  // namespace qtts

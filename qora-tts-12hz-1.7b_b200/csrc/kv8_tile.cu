@@ -66,6 +66,7 @@ struct TileShared {
   uint64_t s_full[2], p_full[2];                        // by half
   uint64_t o_full[2];  // by half; f32: by O's buffer (kv8_order.h)
   uint64_t o_free[2];  // f32: by O's buffer
+  uint64_t summed;     // f32: once a segment
   uint64_t q_full, fin;
   uint32_t tmem;
   int abort;
@@ -532,6 +533,7 @@ struct Softmax {
   float m, mo, l;
   int see_lo, see_hi;
   int done = 0;  // tiles of this half
+  int segments = 0;  // of at least one tile
 
   __device__ explicit Softmax(const J& j) : job(j), row((int)threadIdx.x / j.nh), head((int)threadIdx.x % j.nh) {}
   __device__ __forceinline__ uint32_t columns() const {
@@ -686,9 +688,11 @@ struct Softmax {
       bar_arrive(&sh.p_full[half]);
     }
     if (t1 > t0) {
-      const int n = done - 1;
-      const TileTurn at = C::kSplit ? o_free_turn(n) : o_full_turn(false, half, n);
-      if (!warp_wait(C::kSplit ? &sh.o_free[at.bar] : &sh.o_full[at.bar], at.parity, &sh.abort)) return false;
+      const TileTurn at = o_full_turn(false, half, done - 1);
+      if (!(C::kSplit ? warp_wait(&sh.summed, summed_parity(segments), &sh.abort)
+                      : warp_wait(&sh.o_full[at.bar], at.parity, &sh.abort)))
+        return false;
+      ++segments;
       tc_fence_after();
     }
     return true;
@@ -760,6 +764,7 @@ struct Sums {
       tc_fence_before();
       bar_arrive(&sh.o_free[o_free_turn(done).bar]);
     }
+    if (t1 > t0) bar_arrive(&sh.summed);
     return true;
   }
 };
@@ -833,6 +838,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bar_init(&sh.o_full[i], C::kSplit ? 2 : 1);
       bar_init(&sh.o_free[i], kTileM);
     }
+    bar_init(&sh.summed, kTileM);
     bar_init(&sh.q_full, kTileM * d.halves);
     bar_init(&sh.fin, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

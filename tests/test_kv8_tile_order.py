@@ -24,6 +24,7 @@ extern "C" int o_free(int n) {
   const qtts::TileTurn t = qtts::o_free_turn(n);
   return t.bar * 2 + (int)t.parity;
 }
+extern "C" int summed(int n) { return (int)qtts::summed_parity(n); }
 """
 
 
@@ -83,16 +84,18 @@ def walk(agents, counts):
     return None
 
 
-S_FULL, P_FULL, O_FULL, O_FREE, BARS = 0, 1, 2, 4, 6
+S_FULL, P_FULL, O_FULL, O_FREE, SUMMED = 0, 1, 2, 4, 6
 
 
-def f32_rows(order, segments, who=2):
+def f32_rows(order, segments, who=2, end=None):
     """The parts of a CTA with f32 rows over `segments` of so many tiles each,
-    `who` threads standing for the 128 of the softmax and of the sums."""
+    `who` threads standing for the 128 of the softmax and of the sums.  end: the
+    softmax's step before it reads a segment's sums, of (segment, last tile)."""
     full = lambda n: (O_FULL + order.o_full(1, 0, n) // 2, order.o_full(1, 0, n) % 2)  # noqa: E731
     free = lambda n: (O_FREE + order.o_free(n) // 2, order.o_free(n) % 2)  # noqa: E731
     phase = lambda turn, n: sum(turn(i)[0] == turn(n)[0] for i in range(n))  # noqa: E731
     total = sum(segments)
+    last = [sum(segments[:i + 1]) - 1 for i in range(len(segments))]
     issue, cores, softmax, sums = [], [], [], []
     for n in range(total):
         if n:  # score(n): P of the tile before lies where S goes
@@ -106,15 +109,28 @@ def f32_rows(order, segments, who=2):
         cores += [("take", "o"), ("arrive", full(n)[0])]
         softmax += [("wait", S_FULL, n & 1, n), ("arrive", P_FULL)]
         sums += [("wait", *full(n), phase(full, n)), ("arrive", free(n)[0])]
-        if n + 1 in [sum(segments[:i + 1]) for i in range(len(segments))]:  # the segment's sums are read
-            softmax.append(("order", free(n)[0], phase(free, n)))
-    counts = [2, who, 2, 2, who, who]
+        if n in last:  # the segment's sums are read
+            sums.append(("arrive", SUMMED))
+            softmax.append(end(last.index(n), n) if end else ("order", free(n)[0], phase(free, n)))
+    counts = [2, who, 2, 2, who, who, who]
     return [issue, cores] + [softmax] * who + [sums] * who, counts
 
 
 @pytest.mark.parametrize("segments", [[1], [2], [5], [7], [1, 1, 1], [3, 1, 2], [2, 5]])
 def test_no_wait_of_products_and_sums_is_left_to_timing(order, segments):
     assert walk(*f32_rows(order, segments)) is None
+
+
+@pytest.mark.parametrize("segments", [[1], [2], [3], [6], [1, 1, 1], [3, 1, 2], [2, 5]])
+def test_the_sums_are_read_when_all_tiles_are_in_them(order, segments):
+    end = lambda i, n: ("wait", SUMMED, order.summed(i), i)  # noqa: E731
+    assert walk(*f32_rows(order, segments, end=end)) is None
+
+
+def test_the_walk_finds_sums_read_by_the_last_buffer_alone(order):
+    # the order that was there before: the wait for o_free of the last tile
+    end = lambda i, n: ("wait", O_FREE + (n & 1), (n >> 1) & 1, n >> 1)  # noqa: E731
+    assert "of barrier %d" % O_FREE in walk(*f32_rows(order, [3], end=end))
 
 
 def test_sixteen_bit_halves_have_a_barrier_each(order):
