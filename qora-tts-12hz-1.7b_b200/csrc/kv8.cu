@@ -163,18 +163,19 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
     const float had = slot0 ? *sp : 0.0f;
     float4 x[STEPS];
     uint32_t most = 0;  // the largest |value|'s bits, above those of FLT_MAX if one is not finite
-    // the angles of a step's token (none: 1 and 0)
+    // the angles of a step's token; false: there are none (a rotation by 1 and 0
+    // would not do, as 0 times an infinity half a head away is NaN)
     auto angles = [&](int t, float4& cs, float4& sn) {
       const int rp = __shfl_sync(kFull, rope, min(31, i + t));
-      cs = make_float4(1.f, 1.f, 1.f, 1.f);
-      sn = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (t >= n) return;
-      if (rp >= 0 && rp < d.rope_rows) {
-        cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
-        sn = signed_sin(load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2)), upper);
-      } else {
+      cs = sn = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (t >= n) return false;
+      if (rp < 0 || rp >= d.rope_rows) {
         raise(d.flags, QTTS_KV8_ROPE_RANGE);
+        return false;
       }
+      cs = load4(d.rope_cos + (size_t)rp * (HD / 2) + d0 % (HD / 2));
+      sn = signed_sin(load4(d.rope_sin + (size_t)rp * (HD / 2) + d0 % (HD / 2)), upper);
+      return true;
     };
     Raw4<T> raw[STEPS];  // the next tokens, on their way while the ones before are worked on
     const T* from = src + (size_t)(first + i + sub) * ld + (size_t)h * HD + d0;
@@ -191,7 +192,7 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
       for (int s = 0; s < STEPS; ++s) x[s] = load4(reinterpret_cast<const T*>(&raw[s]));
       if (t0 + KEEP < n) read(t0 + KEEP);
       float4 cs, sn;
-      if (turn) angles(t0 + sub, cs, sn);  // (of each step while the one before is worked on)
+      bool has = turn && angles(t0 + sub, cs, sn);  // (of each step while the one before is worked on)
       if (which == 0 && d.k_norm) {
         if (STEPS > 1 && n - t0 <= TPW) {  // one step
           float4 one[1] = {x[0]};
@@ -206,8 +207,10 @@ __device__ void append_blocks(const Kv8AppendDesc& d, int chunk, int which, int 
         if (t0 + s * TPW >= n) break;
         if (turn) {
           const float4 c0 = cs, s0 = sn;
-          if (s + 1 < STEPS && t0 + (s + 1) * TPW < n) angles(t0 + (s + 1) * TPW + sub, cs, sn);
-          x[s] = rotate<HD>(x[s], c0, s0);
+          const bool now = has;
+          if (s + 1 < STEPS && t0 + (s + 1) * TPW < n) has = angles(t0 + (s + 1) * TPW + sub, cs, sn);
+          const float4 y = rotate<HD>(x[s], c0, s0);
+          if (now) x[s] = y;
         }
         if (t0 + s * TPW + sub < n) most = max(most, abs_bits4(x[s]));
         if (n > KEEP) kept[(t0 / TPW + s) * 32] = x[s];
