@@ -44,3 +44,44 @@ def test_a_key_without_angles_keeps_its_infinities_and_their_partners(qtts, hd, 
     assert np.array_equal(scales, p.scales)
     assert np.array_equal(codes, p.codes)
     assert flags.item() == qtts.KV8_ROPE_RANGE
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("hd,length", [(128, 30000), (64, 32001)])
+def test_long_f32_tiles_sum_their_weights_in_full(qtts, hd, length, sign):
+    # So many units that no cluster shares the positions: a slot adds up the
+    # weights of the whole cache, page by page (a negative scale takes the path
+    # of any tile, otherwise used for masked ones).  The bound of
+    # test_long_f32_sums_are_rounded, here for every row and head, as an error of
+    # the weights' sum is common to all of a row: the weights are off by 2^-21
+    # with random sign, rounded sums of 250 tiles by 2^-20 at most, and the sum
+    # of the weights, compensated, by 2^-23.  Plain sums of n weights are off by
+    # about sqrt(n) 2^-25 and up to n 2^-24: 5e-6 for 30000.
+    rng = np.random.default_rng(length)
+    kvh, n_seqs, rows = 8, 10, 128
+    p = Pool(qtts, rng, 1, (length + 15) // 16, kvh, hd)
+    table = p.d_table.expand(n_seqs, -1).contiguous()
+    cache = qtts.Kv8Cache(p.d_codes.data_ptr(), p.d_scales.data_ptr(), table.data_ptr(), p.codes.shape[0], n_seqs,
+                          table.shape[1], kvh, hd)
+    seq, pos = rows_of([(s, length - rows, rows) for s in range(n_seqs)])
+    q = dev((rng.standard_normal((len(seq), kvh * hd)) * 0.3).astype(np.float32))
+    out, lse = torch.empty_like(q), torch.empty(len(seq), kvh, device="cuda")
+    t = dev(seq), dev(pos)
+    scale = sign * hd ** -0.5
+    qtts.kv8_attention_dev(cache, q.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), len(seq), kvh,
+                           scale=scale, max_rows=rows, max_len=length, lse_ptr=lse.data_ptr())
+    torch.cuda.synchronize()
+    at = dev(p.table[0].astype(np.int64))
+    kv = p.d_codes[at, 0].double() * p.d_scales[at, 0].double()[..., None, None]
+    kv = kv.permute(1, 2, 0, 3, 4).reshape(2, kvh, -1, hd)[:, :, :length]
+    worst = 0.0
+    for h in range(kvh):
+        a = q[:, h * hd:(h + 1) * hd].double() @ kv[0, h].T * scale
+        a.masked_fill_(torch.arange(length, device="cuda")[None] > t[1][:, None], -float("inf"))
+        want = torch.softmax(a, -1) @ kv[1, h]
+        err = (out[:, h * hd:(h + 1) * hd].double() - want).norm(dim=-1) / want.norm(dim=-1)
+        worst = max(worst, err.max().item())
+        # log2 of the sum, its product with ln 2 and the result, each rounded (values up to 16)
+        assert float((lse[:, h].double() - torch.logsumexp(a, -1)).abs().max()) <= 2.0 ** -19 + 16 * 3 * 2.0 ** -24
+    print("worst row", worst)
+    assert worst <= 2.0 ** -19
