@@ -289,7 +289,7 @@ QTTS_API int qtts_q4_quantize(const float* data, int k, int n, uint8_t* packed, 
 #define QTTS_KV8_BAD_ROW 1    /* seq past n_seqs, or a position outside the sequence's pages */
 #define QTTS_KV8_BAD_PAGE 2   /* a page table entry outside [0, n_pages) */
 #define QTTS_KV8_ROPE_RANGE 4 /* a position outside the rotation tables (left unrotated) */
-#define QTTS_KV8_TIMEOUT 8    /* a bounded device wait (1 s) ran out: outputs undefined */
+#define QTTS_KV8_TIMEOUT 8    /* a bounded device wait (1 s) ran out: the rows concerned are NaN, lse too */
 typedef struct {
   int8_t* codes;
   float* scales;
@@ -335,6 +335,11 @@ QTTS_API int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, 
                                     float scale, int window, const int32_t* seq, const int32_t* pos, int n_rows,
                                     int max_rows, int max_len, void* out, int64_t ldo, float* lse, int32_t* flags,
                                     void* stream);
+
+/* Limit in ns (at most 2e9, 1e9 unless set) of a device wait of the attention
+ * calls that this thread makes from now on; with 0 one is made to run out.  For
+ * validation of QTTS_KV8_TIMEOUT. */
+QTTS_API int qtts_kv8_wait_limit(int64_t ns);
 
 /* ---- sampling rows of logits on device pointers ----------------------------
  * qtts_sample with nucleus and min-p filters, for rows of up to 262144 logits

@@ -943,6 +943,10 @@ cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max
 
 // ---- host side of the entry points ----------------------------------------------
 
+namespace {
+thread_local unsigned g_wait_ns = kKv8WaitNs;
+}
+
 OnDeviceOf::OnDeviceOf(const void* p) {
   cudaPointerAttributes a;
   cudaError_t e = cudaPointerGetAttributes(&a, p);
@@ -1096,6 +1100,7 @@ int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t l
   d.pos = pos;
   d.n_rows = n_rows;
   d.flags = flags;
+  d.wait_ns = g_wait_ns;
   const int cap = cache->pages_per_seq * kKv8Page;
   int len = max_len == 0 ? cap : std::min(max_len, cap);
   max_rows = std::max(1, std::min(max_rows, n_rows));
@@ -1103,6 +1108,12 @@ int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t l
   return launched(launch_kv8_attention(d, dtype, max_rows, len, on.sm_count, (cudaStream_t)stream));
 } catch (...) {
   return QTTS_ERR_OOM;
+}
+
+int qtts_kv8_wait_limit(int64_t ns) {
+  if (ns < 0 || ns > 2000000000ll) return refuse("kv8 wait limit", "not 0 .. 2e9 ns");
+  g_wait_ns = (unsigned)ns;
+  return QTTS_OK;
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 namespace qtts {
 
 constexpr int kKv8Page = 16;  // positions per page, the block a scale belongs to
+constexpr unsigned kKv8WaitNs = 1000000000u;  // limit of a device wait
 
 enum DType : int { DT_F32 = QTTS_F32, DT_F16 = QTTS_F16, DT_BF16 = QTTS_BF16 };
 inline int dtype_bytes(int t) { return t == DT_F32 ? 4 : 2; }
@@ -76,6 +77,7 @@ struct Kv8AttnDesc {
   int unit_heads = 1;   // query heads of a unit
   int halves = 1;       // tile kernel: halves of 128 slots of a unit
   int seq_units = 1;    // tile kernel: units of a sequence of max_rows rows
+  unsigned wait_ns = kKv8WaitNs;  // tile kernel: limit of a wait; 0: one is made to run out
 };
 cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max_len, int sms, cudaStream_t st);
 // The same for many rows: tiles of 128 slots on the tensor cores (kv8_tile.cu).

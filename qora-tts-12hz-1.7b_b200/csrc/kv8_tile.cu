@@ -54,7 +54,6 @@ constexpr int kTileThreads = kSoft + kConvert + 32;  // and a warp that issues t
 // Half h: S and P at 256 h, O at 256 h + 128.  With f32 rows, which have one
 // half: O of tile n at 128 + 256 (n & 1), the sums of all tiles at kSums.
 constexpr uint32_t kTmemCols = 512, kSums = 256;
-constexpr unsigned long long kWaitNs = 1000000000ull;
 constexpr float kNoPage = 4.0f;  // no fraction of a scale (split_scale)
 constexpr int kScales = 4;  // tiles of scales kept: a half may be two tiles behind the conversion
 
@@ -69,7 +68,8 @@ struct TileShared {
   uint64_t summed;     // f32: once a segment
   uint64_t q_full, fin;
   uint32_t tmem;
-  int abort;
+  int over;  // a wait of the CTA has run out: nobody waits any longer
+  int row0, rows, h0, nh;  // the unit, for mark_rows
   int n_segments;
   int seq[2 * kTileM], pos[2 * kTileM];
   TileSegment segment[2 * kTileM];
@@ -131,10 +131,11 @@ __device__ __forceinline__ void bar_init(uint64_t* bar, unsigned count) {
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(bar)) : "memory");
 }
-// Waits for the phase, at most kWaitNs or until another thread has given up.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity, int* abort) {
+// Waits for the phase, at most `ns` (less than the 4.3 s of the clock's low word)
+// or until another thread has given up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity, int* over, unsigned ns) {
   const uint32_t a = smem_of(bar);
-  unsigned long long t0 = 0;
+  unsigned t0 = 0;
   for (unsigned it = 0;; ++it) {
     uint32_t done;
     asm volatile(
@@ -146,20 +147,16 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, unsigned parity, int* ab
         : "memory");
     if (done) return true;
     if ((it & 255u) == 255u) {
-      if (*reinterpret_cast<volatile int*>(abort)) return false;
-      unsigned long long t;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > kWaitNs) {
-        *reinterpret_cast<volatile int*>(abort) = 1;
+      if (*reinterpret_cast<volatile int*>(over)) return false;
+      unsigned t;
+      asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+      if (it == 255u) t0 = t;
+      else if (t - t0 > ns) {
+        *reinterpret_cast<volatile int*>(over) = 1;
         return false;
       }
     }
   }
-}
-// The same for a warp as one, so that it stays together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, int* abort) {
-  return __all_sync(kFull, bar_wait(bar, parity, abort));
 }
 // 32 columns on their way into r, which may be read after tmem_wait(r).
 __device__ __forceinline__ void tmem_start(uint32_t addr, uint32_t (&r)[32]) {
@@ -228,6 +225,10 @@ struct TileJob {
     const int share = (nt + nsplit - 1) / nsplit;
     t0 = min(nt, split * share);
     t1 = min(nt, t0 + share);
+  }
+  // for a warp as one, so that it stays together
+  __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity) const {
+    return __all_sync(kFull, bar_wait(bar, parity, &sh.over, d.wait_ns));
   }
   // whether half h holds rows of the segment
   __device__ __forceinline__ bool takes(const TileSegment& g, int h) const {
@@ -316,7 +317,7 @@ struct Converter {
       const int b = it & 1;
       const unsigned before = (unsigned)((it >> 1) - 1) & 1u;  // the buffers' last use
       const int after = pages(table, p0, p1, t + 2);
-      if (it > 1 && !warp_wait(&sh.k_free[b], before, &sh.abort)) return false;
+      if (it > 1 && !job.wait(&sh.k_free[b], before)) return false;
       if (warp == 0 && lane < kTilePages) {
         float ev, fr;
         split_scale(sv, ev, fr);
@@ -329,7 +330,7 @@ struct Converter {
       bar_arrive(&sh.k_full[b]);
       fetch(1, ids);
       fetch_scales(next);
-      if (it > 1 && !warp_wait(&sh.v_free[b], before, &sh.abort)) return false;
+      if (it > 1 && !job.wait(&sh.v_free[b], before)) return false;
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       put_v(b);
       smem_to_async();
@@ -353,7 +354,7 @@ struct Products {
 
   __device__ explicit Products(const J& j) : job(j) {}
   __device__ __forceinline__ bool wait_for(uint64_t (&bars)[2], TileTurn at) const {
-    return warp_wait(&bars[at.bar], at.parity, &job.sh.abort);
+    return job.wait(&bars[at.bar], at.parity);
   }
   // S = Q K^T of half h with K of buffer b; last: no other half reads this K
   __device__ __forceinline__ bool score(int h, int b, bool last) const {
@@ -389,7 +390,7 @@ struct Products {
   __device__ __forceinline__ bool weigh(int h, int b, bool first, bool last) {
     TileShared& sh = job.sh;
     constexpr uint32_t idesc = instruction(HD, true);
-    if (!warp_wait(&sh.p_full[h], done[h] & 1, &sh.abort)) return false;
+    if (!job.wait(&sh.p_full[h], done[h] & 1)) return false;
     const int n = done[h]++;
     // the buffer's tile before has been added up
     if (C::kSplit && n > 1 && !wait_for(sh.o_free, o_free_turn(n - 2))) return false;
@@ -421,11 +422,11 @@ struct Products {
     for (int t = t0; t < t1; ++t, ++it) {
       const int b = it & 1;
       const unsigned use = (unsigned)(it >> 1) & 1u;
-      if (!warp_wait(&sh.k_full[b], use, &sh.abort)) return false;
+      if (!job.wait(&sh.k_full[b], use)) return false;
       if (one && !score(0, b, !two)) return false;
       if (two && t > t0 && !weigh(1, b ^ 1, t - 1 == t0, true)) return false;
       if (two && !score(1, b, true)) return false;
-      if (!warp_wait(&sh.v_full[b], use, &sh.abort)) return false;
+      if (!job.wait(&sh.v_full[b], use)) return false;
       if (one && !weigh(0, b, t == t0, !two)) return false;
     }
     return !two || t0 == t1 || weigh(1, (it - 1) & 1, t1 - 1 == t0, true);
@@ -691,7 +692,7 @@ struct Softmax {
     }
     for (int t = t0; t < t1; ++t, ++it, ++done) {
       const int at = (p0 + t * kTilePages) * kKv8Page;
-      if (!warp_wait(&sh.s_full[half], done & 1, &sh.abort)) return false;
+      if (!job.wait(&sh.s_full[half], done & 1)) return false;
       tc_fence_after();
       const float4* sc = sh.scale[it % kScales];
       // a slot of another segment has no say: its row is never read
@@ -711,8 +712,8 @@ struct Softmax {
     }
     if (t1 > t0) {
       const TileTurn at = o_full_turn(false, half, done - 1);
-      if (!(C::kSplit ? warp_wait(&sh.summed, summed_parity(segments), &sh.abort)
-                      : warp_wait(&sh.o_full[at.bar], at.parity, &sh.abort)))
+      if (!(C::kSplit ? job.wait(&sh.summed, summed_parity(segments))
+                      : job.wait(&sh.o_full[at.bar], at.parity)))
         return false;
       ++segments;
       tc_fence_after();
@@ -759,7 +760,7 @@ struct Sums {
     float last = -INFINITY;
     for (int t = t0; t < t1; ++t, ++done) {
       const TileTurn full = o_full_turn(true, 0, done);
-      if (!warp_wait(&sh.o_full[full.bar], full.parity, &sh.abort)) return false;
+      if (!job.wait(&sh.o_full[full.bar], full.parity)) return false;
       tc_fence_after();
       const float mo = sh.mo[done & 3][threadIdx.x & (kTileM - 1)];
       const float beta = last == mo ? 1.0f : ex2(last - mo);  // (0 after -inf)
@@ -802,6 +803,20 @@ __device__ __forceinline__ void store_row(T* p, const float (&x)[32], float mul)
 template <int HD>
 __device__ __forceinline__ int sum_at(int s, int e) {
   return s * HD + (e ^ ((s & 7) << 2));
+}
+
+// A wait ran out: the unit's rows say so.  (A call of its own, so that its
+// registers are not taken from the loops.)
+template <typename T, int HD>
+__device__ __noinline__ void mark_rows(const Kv8AttnDesc& d, const TileShared& sh) {
+  for (int i = threadIdx.x; i < sh.rows * sh.nh * (HD / 4); i += kTileThreads) {
+    const int s = i / (HD / 4), e = i % (HD / 4) * 4, row = s / sh.nh, head = sh.h0 + s % sh.nh;
+    if (sh.seq[row] < 0) continue;
+    const size_t at = sh.row0 + row;
+    store4(static_cast<T*>(d.out) + at * d.ldo + (size_t)head * HD + e, make_float4(NAN, NAN, NAN, NAN));
+    if (e == 0 && d.lse) d.lse[at * d.heads + head] = NAN;
+  }
+  if (threadIdx.x == 0) raise(d.flags, QTTS_KV8_TIMEOUT);
 }
 
 template <typename T, int HD>
@@ -864,7 +879,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     bar_init(&sh.q_full, kTileM * d.halves);
     bar_init(&sh.fin, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    sh.abort = 0;
+    sh.over = 0;
+    sh.row0 = job.row0;
+    sh.rows = job.rows;
+    sh.h0 = job.h0;
+    sh.nh = job.nh;
   }
   constexpr int kLast = kTileThreads / 32 - 1;  // the warp of the products
   if (warp == kLast) {
@@ -914,9 +933,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (softmax) {  // (while the first codes are on their way)
     soft.put_query();
     smem_to_async();
-    bar_arrive(&sh.q_full);
+    if (d.wait_ns > 0) bar_arrive(&sh.q_full);  // (0: the wait for it is to run out)
   }
-  if (warp == kLast) ok = warp_wait(&sh.q_full, 0, &sh.abort);
+  if (warp == kLast) ok = job.wait(&sh.q_full, 0);
   for (int g = 0; g < sh.n_segments; ++g) {
     const TileSegment seg = sh.segment[g];
     if (seg.seq < 0) continue;  // padding
@@ -984,19 +1003,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     cluster.sync();  // no CTA goes on while its sums are read
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // (none is left unless a wait ran out)
   // A dependent kernel may start now: it could take TMEM that a CTA of this one
   // still had to get, had it started before the allocation.
   pdl_launch_dependents();
-  // every product is done (a wait that ran out leaves some in flight) before TMEM goes
   __syncthreads();
+  if (sh.over) mark_rows<T, HD>(d, sh);  // (after what other CTAs of the cluster have written)
+  // every product is done (a wait that ran out leaves some in flight) before TMEM goes
   if (tid == kLast * 32) commit_to(&sh.fin);
   if (warp == kLast) {
-    int plain = 0;
-    bar_wait(&sh.fin, 0, &plain);
+    int over = 0;  // (of this wait alone)
+    bar_wait(&sh.fin, 0, &over, kKv8WaitNs);
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(job.tmem), "r"(kTmemCols));
   }
-  if (tid == 0 && sh.abort) raise(d.flags, QTTS_KV8_TIMEOUT);
 }
 
 template <typename T, int HD>

@@ -126,6 +126,7 @@ def _load():
                                           C.c_int64, C.c_int, C.c_int, P, P, P, P, C.c_int, P, P, P, C.c_int, P, P]),
         "qtts_kv8_attention_dev": (C.c_int, [C.POINTER(Kv8CacheDesc), P, C.c_int64, C.c_int, C.c_int, C.c_float,
                                              C.c_int, P, P, C.c_int, C.c_int, C.c_int, P, C.c_int64, P, P, P]),
+        "qtts_kv8_wait_limit": (C.c_int, [C.c_int64]),
         "qtts_sample_rows_dev": (C.c_int, [P, C.c_int64, C.c_int, C.c_int, C.c_int, P, P, P, P, P, P, P, P, P]),
         "qtts_q4_quantize": (C.c_int, [fp, C.c_int, C.c_int, C.POINTER(C.c_uint8), C.POINTER(C.c_uint16)]),
     }
@@ -549,6 +550,12 @@ def kv8_attention_dev(cache: Kv8Cache, q_ptr, out_ptr, seq_ptr, pos_ptr, n_rows,
                                       cache.head_dim ** -0.5 if scale is None else scale, window, seq_ptr or None,
                                       pos_ptr or None, n_rows, max_rows, max_len, out_ptr or None, ldo or cols,
                                       lse_ptr or None, flags_ptr or None, stream or None))
+
+
+def kv8_wait_limit(ns=1_000_000_000):
+    """Limit in ns of a device wait of this thread's later kv8_attention_dev
+    calls (qtts.h qtts_kv8_wait_limit), for validation of KV8_TIMEOUT."""
+    _check(lib.qtts_kv8_wait_limit(ns))
 
 
 def sample_rows_dev(logits_ptr, n_rows, V, u_ptr, token_ptr, dtype="f32", temperature_ptr=0, top_k_ptr=0, top_p_ptr=0,

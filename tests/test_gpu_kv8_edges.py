@@ -85,3 +85,46 @@ def test_long_f32_tiles_sum_their_weights_in_full(qtts, hd, length, sign):
         assert float((lse[:, h].double() - torch.logsumexp(a, -1)).abs().max()) <= 2.0 ** -19 + 16 * 3 * 2.0 ** -24
     print("worst row", worst)
     assert worst <= 2.0 ** -19
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", ["whole", "split"])
+def test_a_wait_that_runs_out_marks_its_rows(qtts, dtype, shape):
+    # A wait that nothing ends, with no time given: every CTA gives up, the call
+    # ends, the rows are NaN (padding rows stay), the flag says why, and the next
+    # call is right.
+    rng = np.random.default_rng(31)
+    # (shapes that tiles take; single tokens and few rows have nothing to wait for)
+    n_seqs, rows, length, kvh, hd = (8, 100, 200, 8, 64) if shape == "whole" else (1, 400, 3000, 2, 128)
+    heads = 2 * kvh
+    p = Pool(qtts, rng, n_seqs, (length + 15) // 16, kvh, hd)
+    seq, pos = rows_of([(s, length - rows, rows) for s in range(n_seqs)] + [(-1, 0, 3)])
+    n = len(seq)
+    q = dev(rng.standard_normal((n, heads * hd)).astype(np.float32), dtype)
+    t = dev(seq), dev(pos)
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call(out, lse):
+        qtts.kv8_attention_dev(p.cache, q.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), n, heads,
+                               dtype=dtype, max_rows=rows, lse_ptr=lse.data_ptr(), flags_ptr=flags.data_ptr())
+
+    want, wlse = torch.full_like(q, 5.0), torch.full((n, heads), 5.0, device="cuda")
+    call(want, wlse)
+    torch.cuda.synchronize()
+    assert flags.item() == 0 and bool(torch.isfinite(want).all())
+    for again in range(2):
+        out, lse = torch.full_like(q, 5.0), torch.full((n, heads), 5.0, device="cuda")
+        qtts.kv8_wait_limit(0)
+        try:
+            call(out, lse)
+        finally:
+            qtts.kv8_wait_limit()
+        torch.cuda.synchronize()
+        assert flags.item() == qtts.KV8_TIMEOUT
+        assert bool(out[:n - 3].isnan().all()) and bool(lse[:n - 3].isnan().all())
+        assert bool((out[n - 3:] == 5.0).all()) and bool((lse[n - 3:] == 5.0).all())
+        flags.zero_()
+        out, lse = torch.full_like(q, 5.0), torch.full((n, heads), 5.0, device="cuda")
+        call(out, lse)
+        torch.cuda.synchronize()
+        assert flags.item() == 0 and torch.equal(out, want) and torch.equal(lse, wlse)
