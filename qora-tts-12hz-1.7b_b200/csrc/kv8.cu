@@ -983,8 +983,6 @@ OnDeviceOf::~OnDeviceOf() {
 
 namespace {
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
 // nullptr, or what is wrong with the cache description
 const char* cache_fault(const qtts_kv8_cache* c) {
   if (!c || !c->codes || !c->scales || !c->page_table) return "the cache has a null pointer";
@@ -1039,6 +1037,7 @@ int qtts_kv8_append_dev(const qtts_kv8_cache* cache, const void* k, int64_t ldk,
     }
   }
   if (!rope_cos != !rope_sin || (rope_cos && rope_rows <= 0)) return refuse("kv8 append", "bad rotation tables");
+  if (!words_aligned({seq, pos, rope_pos, flags})) return refuse("kv8 append", "misaligned seq, pos, rope_pos or flags");
   if (!aligned(rope_cos, 16) || !aligned(rope_sin, 16) || !aligned(q_norm, 8) || !aligned(k_norm, 8))
     return refuse("kv8 append", "misaligned rotation tables or norm weights");
   if (n_rows == 0) return QTTS_OK;
@@ -1080,6 +1079,7 @@ int qtts_kv8_attention_dev(const qtts_kv8_cache* cache, const void* q, int64_t l
     return refuse("kv8 attention", "heads is not a multiple of the cache's kv_heads (up to 16384)");
   if (window < 0 || max_rows < 0 || max_len < 0) return refuse("kv8 attention", "negative window, max_rows or max_len");
   if (n_rows < 0 || (n_rows > 0 && (!seq || !pos))) return refuse("kv8 attention", "bad rows");
+  if (!words_aligned({seq, pos, lse, flags})) return refuse("kv8 attention", "misaligned seq, pos, lse or flags");
   if (n_rows == 0) return QTTS_OK;
   const int64_t cols = (int64_t)heads * cache->head_dim;
   if ((f = rows_fault(q, ldq, cols, dtype)) || (f = rows_fault(out, ldo, cols, dtype))) return refuse("kv8 attention, q or out", f);

@@ -2,6 +2,8 @@
 // and attention kernels, and what the entry points on device pointers share.
 #pragma once
 #include <atomic>
+#include <cstdint>
+#include <initializer_list>
 
 #include "../../include/qtts.h"
 #include "kernels.h"
@@ -13,6 +15,14 @@ constexpr unsigned kKv8WaitNs = 1000000000u;  // limit of a device wait
 
 enum DType : int { DT_F32 = QTTS_F32, DT_F16 = QTTS_F16, DT_BF16 = QTTS_BF16 };
 inline int dtype_bytes(int t) { return t == DT_F32 ? 4 : 2; }
+
+// what an entry point asks of a pointer before a kernel follows it
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline bool words_aligned(std::initializer_list<const void*> all) {  // of 4 bytes; null is
+  for (const void* p : all)
+    if (!aligned(p, 4)) return false;
+  return true;
+}
 
 // Makes the device that holds `p` current while it lives, so that a caller's
 // buffers may lie on another device than its current one.  `err` says why not

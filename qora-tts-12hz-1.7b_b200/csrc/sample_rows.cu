@@ -1257,6 +1257,8 @@ extern "C" int qtts_sample_rows_dev(const void* logits, int64_t ld, int dtype, i
   if (!logits || !u || !token) return fail(QTTS_ERR_BADARG, "sample rows: a null pointer");
   if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dtype))
     return fail(QTTS_ERR_BADARG, "sample rows: misaligned logits");
+  if (!words_aligned({temperature, top_k, top_p, min_p, u, token, kept, logprob}))
+    return fail(QTTS_ERR_BADARG, "sample rows: a misaligned array of a value a row");
   OnDeviceOf on(logits);
   if (on.err) return fail(on.code, std::string("sample rows, the logits: ") + on.err);
   SampleRowsDesc d;
