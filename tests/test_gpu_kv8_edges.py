@@ -128,3 +128,83 @@ def test_a_wait_that_runs_out_marks_its_rows(qtts, dtype, shape):
         call(out, lse)
         torch.cuda.synchronize()
         assert flags.item() == 0 and torch.equal(out, want) and torch.equal(lse, wlse)
+
+
+def by_row_and_head(p, q, heads, seq, pos, scale, window):
+    """64-bit attention [n][heads][hd] and, for its error, of every row and head:
+    the sums of weight * |v|, the largest weight * V scale, the largest
+    scale * sum |q k|, and the number of positions seen."""
+    kvh, hd, cap = p.codes.shape[2], p.hd, p.table.shape[1] * 16
+    n = len(seq)
+    want, mass = np.zeros((2, n, heads, hd))
+    heavy, most = np.zeros((2, n, heads))
+    seen = np.zeros(n)
+    for r in range(n):
+        if pos[r] < 0:
+            continue
+        lo = max(0, pos[r] + 1 - window) if window else 0
+        at = np.arange(lo, min(int(pos[r]), cap - 1) + 1)
+        page = p.table[seq[r], at // 16]
+        seen[r] = len(at)
+        for h in range(heads):
+            k, v = (p.codes[page, i, h * kvh // heads, at % 16].astype(np.float64) *
+                    p.scales[page, i, h * kvh // heads, None].astype(np.float64) for i in (0, 1))
+            x = q[r, h * hd:(h + 1) * hd].astype(np.float64)
+            a = k @ x * scale
+            w = np.exp(a - a.max())
+            w /= w.sum()
+            want[r, h], mass[r, h] = w @ v, w @ np.abs(v)
+            heavy[r, h] = (w * np.abs(p.scales[page, 1, h * kvh // heads].astype(np.float64))).max()
+            most[r, h] = abs(scale) * (np.abs(k) @ np.abs(x)).max()
+    return want, mass, heavy, most, seen
+
+
+@pytest.mark.parametrize("rows,max_rows,n_seqs,kvh,hd", [(1, 1, 8, 8, 64), (3, 3, 8, 2, 128), (100, 100, 8, 8, 64),
+                                                        (100, 1, 2, 2, 64), (60, 60, 12, 8, 128)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window", [0, 60])
+def test_scales_far_apart_row_by_row(qtts, rows, max_rows, n_seqs, kvh, hd, dtype, window):
+    # V scales of 1e-9 .. 1e9 in an order that grows, falls or jumps, so that the
+    # running exponent moves both ways; each row and head against its own bound
+    rng = np.random.default_rng(rows + hd + window)
+    per = 20
+    p = Pool(qtts, rng, n_seqs, per, kvh, hd)
+    power = rng.integers(-9, 10, (len(p.scales), kvh)).astype(np.float64)
+    for s in range(n_seqs):
+        if s % 4 == 1:
+            power[p.table[s]] = np.linspace(-9, 9, per)[:, None]
+        elif s % 4 == 2:
+            power[p.table[s]] = np.linspace(9, -9, per)[:, None]
+    p.scales[:, 1] *= (10.0 ** power).astype(np.float32)
+    p.scales[p.table[0, 2], 1] = 0.0
+    p.scales[p.table[0, 3], 0] = 0.0
+    p.scales[p.table[1, :5], 1] = 0.0
+    p.d_scales[:, 0] = dev(p.scales)
+    heads = 2 * kvh
+    top = 203 if dtype != "f16" else 150
+    seq, pos = rows_of([(s, top - 11 * s if rows == 1 else top, rows) for s in range(n_seqs)])
+    if dtype == "f16":  # results that f16 holds
+        p.scales[:, 1] = np.clip(p.scales[:, 1], 0, 1)
+        p.d_scales[:, 0] = dev(p.scales)
+    n = len(seq)
+    q = dev(rng.standard_normal((n, heads * hd)).astype(np.float32), dtype)
+    out = torch.full_like(q, 5.0)
+    t = dev(seq), dev(pos)
+    qtts.kv8_attention_dev(p.cache, q.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), n, heads, dtype=dtype,
+                           window=window, scale=hd ** -0.5, max_rows=max_rows)
+    torch.cuda.synchronize()
+    want, mass, heavy, most, seen = by_row_and_head(p, host(q), heads, seq, pos, hd ** -0.5, window)
+    # As in check_attention: scores off by d, weights by twice that, 2^-20 for exp2
+    # and the pair, 2^-11 where they are f16; sums by 2^-23 a step of 16 positions
+    # and 32 for joins; all of weight * |v|.  A pair's lo part is rounded to 2^-25
+    # of the row's largest weight * V scale, for a code of up to 127 at every position.
+    d = most * (hd / 16 + 8) * 2.0 ** -23
+    weights = 2.0 ** -11 if dtype != "f32" and max_rows > 1 else 0.0
+    rel = 2 * d + weights + 2.0 ** -20 + ((seen[:, None] + 128) / 16 + 32) * 2.0 ** -23
+    half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
+    tol = mass * rel[..., None] + (heavy * seen[:, None] * 127 * 2.0 ** -25)[..., None] + half * np.abs(want)
+    if dtype == "f16":
+        tol = tol + 2.0 ** -25  # its subnormals
+    got = host(out).reshape(n, heads, hd).astype(np.float64)
+    bad = np.abs(got - want) > tol
+    assert not bad.any(), (np.argwhere(bad)[:3], (np.abs(got - want) / np.maximum(tol, 1e-300)).max())
