@@ -5,7 +5,7 @@ import pytest
 
 import serving_ref as R
 from conftest import has_gpu
-from test_gpu_kv8 import Pool, dev, host, rows_of, run_append, tables
+from test_gpu_kv8 import Pool, check_attention, dev, host, rows_of, run_append, tables
 
 pytestmark = pytest.mark.gpu
 if has_gpu():
@@ -208,3 +208,69 @@ def test_scales_far_apart_row_by_row(qtts, rows, max_rows, n_seqs, kvh, hd, dtyp
     got = host(out).reshape(n, heads, hd).astype(np.float64)
     bad = np.abs(got - want) > tol
     assert not bad.any(), (np.argwhere(bad)[:3], (np.abs(got - want) / np.maximum(tol, 1e-300)).max())
+
+
+@pytest.mark.parametrize("heads,kvh", [(300, 1), (39, 3)])
+@pytest.mark.parametrize("max_rows", [1, 90])
+def test_many_heads_a_cache_head(qtts, heads, kvh, max_rows):
+    # more query heads than a tile has slots, and counts that its chunks do not divide
+    rng = np.random.default_rng(heads)
+    p = Pool(qtts, rng, 2, 8, kvh, 64)
+    seq, pos = rows_of([(0, 5, 90), (-1, 0, 1), (1, 100, 20)])
+    for dtype in ("f32", "bf16"):
+        check_attention(qtts, p, rng, seq, pos, heads, dtype, max_rows=max_rows)
+
+
+@pytest.mark.parametrize("rows", [1, 150])
+def test_hints_and_windows_at_their_ends(qtts, rows):
+    # results do not depend on max_rows and max_len, and a window may be any size;
+    # positions and sequences far outside are flagged, far below nothing
+    rng = np.random.default_rng(rows)
+    p = Pool(qtts, rng, 4, 30, 4, 128)
+    seq, pos = rows_of([(s, 479 - rows, rows) for s in range(4)])
+    q = rng.standard_normal((len(seq), 8 * 128))
+    for max_rows in (0, 1, 7, 2 ** 31 - 1):
+        for max_len in (0, 1, 2 ** 31 - 1):
+            for window in (0, 33, 2 ** 31 - 1):
+                check_attention(qtts, p, rng, seq, pos, 8, "f32", q=q, max_rows=max_rows, max_len=max_len, window=window)
+    pos[0] = -2 ** 31
+    flags = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for max_rows in (1, 150):
+        check_attention(qtts, p, rng, seq, pos, 8, "f32", q=q, max_rows=max_rows, window=20, flags=flags)
+        assert flags.item() == 0
+        far = pos.copy()
+        far[-1] = 2 ** 31 - 1
+        check_attention(qtts, p, rng, seq, far, 8, "f32", q=q, max_rows=max_rows, flags=flags)
+        assert flags.item() == qtts.KV8_BAD_ROW
+        flags.zero_()
+
+
+@pytest.mark.parametrize("n_seqs", [1, 700])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_queries_turned_in_place(qtts, dtype, n_seqs):
+    # q_out may be q; an odd number of rows, as a prompt's warps take two each, and
+    # the same rows in a pool of many sequences
+    rng = np.random.default_rng(n_seqs)
+    hd, kvh, heads = 64, 2, 6
+    p = Pool(qtts, rng, n_seqs, 4, kvh, hd)
+    seq, pos = rows_of([(0, 1, 61), (-1, 0, 2)])
+    n = len(seq)
+    cos, sin = tables(64, hd)
+    gq = (1 + 0.1 * rng.standard_normal(hd)).astype(np.float16)
+    dc, ds, dgq, dseq, dpos = dev(cos), dev(sin), dev(gq), dev(seq), dev(pos)
+    x = dev(rng.standard_normal((n, (heads + 2 * kvh) * hd)).astype(np.float32), dtype)
+    before = host(x)
+    ld, b, size = x.stride(0), x.data_ptr(), x.element_size()
+    qtts.kv8_append_dev(p.cache, b + heads * hd * size, b + (heads + kvh) * hd * size, dseq.data_ptr(), dpos.data_ptr(), n,
+                        dtype=dtype, q_ptr=b, q_out_ptr=b, heads=heads, q_norm_ptr=dgq.data_ptr(), cos_ptr=dc.data_ptr(),
+                        sin_ptr=ds.data_ptr(), rope_rows=64, ldk=ld, ldv=ld, ldq=ld, ldqo=ld)
+    torch.cuda.synchronize()
+    want = before.copy()
+    for r in range(n):
+        if seq[r] >= 0:
+            want[r, :heads * hd] = R.norm_rotate(before[r, :heads * hd].reshape(heads, hd), gq, cos[pos[r]], sin[pos[r]]).reshape(-1)
+    assert torch.equal(x, dev(want, dtype))
+    k, v = before[:, heads * hd:(heads + kvh) * hd], before[:, (heads + kvh) * hd:]
+    R.append(p.codes, p.scales, p.table, k, v, seq, pos, None, cos, sin)
+    codes, scales = p.got()
+    assert np.array_equal(codes, p.codes) and np.array_equal(scales, p.scales)
