@@ -149,3 +149,67 @@ def test_the_walk_finds_one_barrier_for_both_buffers(order):
             return n & 1
 
     assert "of barrier %d" % O_FULL in walk(*f32_rows(One, [5]))
+
+
+def halves(order, segments, who):
+    """The parts of a CTA with 16-bit rows: `segments` of (tiles, whether the
+    first half holds rows of it, whether the second does); `who` threads of each
+    group that arrives together."""
+    k_full, v_full, k_free, v_free, s_full, p_full, o_full = (2 * i for i in range(7))
+    full = lambda h, n: (o_full + order.o_full(0, h, n) // 2, order.o_full(0, h, n) % 2)  # noqa: E731
+    convert, issue, cores, softmax = [], [], [], ([], [])
+    done = [0, 0]
+
+    def buffer(bar, it):  # the use of a pair of buffers by tile `it`
+        return ("wait", bar + (it & 1), (it >> 1) & 1, it >> 1)
+
+    def score(h, b, last):
+        if done[h]:
+            issue.append(("wait", *full(h, done[h] - 1), done[h] - 1))
+        issue.extend([("give", "m"), ("arrive", s_full + h)])
+        cores.extend([("take", "m"), ("arrive", s_full + h)] + ([("arrive", k_free + b)] if last else []))
+
+    def weigh(h, b, last):
+        n = done[h]
+        done[h] += 1
+        issue.extend([("wait", p_full + h, n & 1, n), ("give", "m")])
+        cores.extend([("take", "m"), ("arrive", full(h, n)[0])] + ([("arrive", v_free + b)] if last else []))
+
+    it = 0
+    for tiles, one, two in segments:
+        first, begin = it, list(done)
+        for t in range(tiles):
+            b = it & 1
+            if it > 1:
+                convert.append(buffer(k_free, it - 2))
+            convert.append(("arrive", k_full + b))
+            if it > 1:
+                convert.append(buffer(v_free, it - 2))
+            convert.append(("arrive", v_full + b))
+            issue.append(buffer(k_full, it))
+            if one:
+                score(0, b, not two)
+            if two and t:
+                weigh(1, b ^ 1, True)
+            if two:
+                score(1, b, True)
+            issue.append(buffer(v_full, it))
+            if one:
+                weigh(0, b, not two)
+            it += 1
+        if two and it > first:
+            weigh(1, (it - 1) & 1, True)
+        for h, here in ((0, one), (1, two)):
+            for n in range(begin[h], done[h]):
+                softmax[h].extend([("wait", s_full + h, n & 1, n), ("arrive", p_full + h)])
+            if here and done[h] > begin[h]:
+                softmax[h].append(("wait", *full(h, done[h] - 1), done[h] - 1))
+    counts = [who] * 4 + [1] * 4 + [2] * 2 + [who] * 2 + [1] * 2
+    return [issue, cores] + [convert] * who + [softmax[0]] * who + [softmax[1]] * who, counts
+
+
+@pytest.mark.parametrize("who,segments", [(1, [(5, True, True)]), (1, [(3, True, False), (2, True, True), (3, False, True)]),
+                                          (1, [(1, True, True)] * 3), (1, [(2, False, True), (1, True, False), (2, True, True)]),
+                                          (2, [(3, True, True)]), (2, [(4, True, False)]), (2, [(2, True, False), (1, False, True)])])
+def test_no_wait_of_two_halves_is_left_to_timing(order, who, segments):
+    assert walk(*halves(order, segments, who)) is None
