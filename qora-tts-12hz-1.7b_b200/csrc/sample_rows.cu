@@ -168,8 +168,11 @@ struct Weigh {
   }
 };
 
-// Histogram bins: counts, and weights as three words of 15 bits, whose sums of
-// up to 2^17 tokens stay in 32 bits (64-bit shared atomics are retry loops).
+// Histogram bins: counts, and weights as three words of 15 bits (64-bit shared
+// atomics are retry loops).  The high word of a weight of 1 is 2^15, so a sum of
+// fewer than 2^17 tokens stays in 32 bits; kMaxSlice sees to it.
+constexpr int kMaxSlice = 98304;  // columns of a CTA
+static_assert(((u64)kMaxSlice << (kFix - 30)) <= 0xffffffffull && kFix <= 45, "a bin's words hold a slice's weights");
 struct Bins {
   unsigned count[kBins];
   unsigned w[3][kBins];
@@ -1230,9 +1233,7 @@ cudaError_t launch_t(const SampleRowsDesc& d, int n_rows, int ranks, cudaStream_
 template <typename T>
 cudaError_t launch(SampleRowsDesc d, int n_rows, int sms, cudaStream_t st) {
   // Rows that do not fill the device (two CTAs an SM) are spread over more
-  // CTAs, down to 4096 logits each; kMaxSlice keeps the histograms' words in
-  // 32 bits.
-  constexpr int kMaxSlice = 98304;
+  // CTAs, down to 4096 logits each.
   int ranks = 1;
   while (ranks < 16 && (d.V > ranks * kMaxSlice || (d.V > ranks * 4096 && (long)n_rows * ranks <= sms))) ranks *= 2;
   d.per = ((d.V + ranks - 1) / ranks + 31) / 32 * 32;
