@@ -274,3 +274,32 @@ def test_queries_turned_in_place(qtts, dtype, n_seqs):
     R.append(p.codes, p.scales, p.table, k, v, seq, pos, None, cos, sin)
     codes, scales = p.got()
     assert np.array_equal(codes, p.codes) and np.array_equal(scales, p.scales)
+
+
+@pytest.mark.parametrize("n_seqs", [1, 160])
+def test_long_f32_tokens_row_by_row(qtts, n_seqs):
+    # the bound of test_long_f32_tiles_sum_their_weights_in_full for single tokens:
+    # one sequence whose pages a cluster shares, and so many that a CTA has them alone
+    rng = np.random.default_rng(n_seqs)
+    kvh, hd, length = 8, 128, 32003
+    p = Pool(qtts, rng, 1, (length + 15) // 16, kvh, hd)
+    table = p.d_table.expand(n_seqs, -1).contiguous()
+    cache = qtts.Kv8Cache(p.d_codes.data_ptr(), p.d_scales.data_ptr(), table.data_ptr(), p.codes.shape[0], n_seqs,
+                          table.shape[1], kvh, hd)
+    seq, pos = np.arange(n_seqs, dtype=np.int32), (length - 1 - np.arange(n_seqs)).astype(np.int32)
+    q = dev((rng.standard_normal((n_seqs, 2 * kvh * hd)) * 0.3).astype(np.float32))
+    out, lse = torch.empty_like(q), torch.empty(n_seqs, 2 * kvh, device="cuda")
+    t = dev(seq), dev(pos)
+    qtts.kv8_attention_dev(cache, q.data_ptr(), out.data_ptr(), t[0].data_ptr(), t[1].data_ptr(), n_seqs, 2 * kvh,
+                           max_len=length, lse_ptr=lse.data_ptr())
+    torch.cuda.synchronize()
+    at = dev(p.table[0].astype(np.int64))
+    kv = p.d_codes[at, 0].double() * p.d_scales[at, 0].double()[..., None, None]
+    kv = kv.permute(1, 2, 0, 3, 4).reshape(2, kvh, -1, hd)[:, :, :length]
+    for h in range(2 * kvh):
+        a = q[:, h * hd:(h + 1) * hd].double() @ kv[0, h // 2].T * hd ** -0.5
+        a.masked_fill_(torch.arange(length, device="cuda")[None] > t[1][:, None], -float("inf"))
+        want = torch.softmax(a, -1) @ kv[1, h // 2]
+        err = (out[:, h * hd:(h + 1) * hd].double() - want).norm(dim=-1) / want.norm(dim=-1)
+        assert err.max().item() <= 2.0 ** -19, h
+        assert float((lse[:, h].double() - torch.logsumexp(a, -1)).abs().max()) <= 2.0 ** -19 + 16 * 3 * 2.0 ** -24
