@@ -325,8 +325,8 @@ QTTS_API int qtts_kv8_append_dev(const qtts_kv8_cache* cache, const void* k, int
  * and lse[n_rows][heads] (nullable, f32) its log-sum-exp.  pos < 0: nothing is
  * attended, out is 0 and lse -inf.  seq < 0: a padding row, left as it was.
  * Sums are held in f32; q and the softmax weights keep about 22 bits, so that
- * f32 results agree with f32 arithmetic to ~1e-6; with 16-bit q and max_rows
- * above 1 the weights may be rounded to f16 (2^-11 each).  A page that a row
+ * f32 results agree with f32 arithmetic to ~1e-6 (2e-6 over 30000 positions); with
+ * 16-bit q and max_rows above 1 the weights may be rounded to f16 (2^-11 each).  A page that a row
  * does not see has no say in it, whatever its scale.  max_rows (the rows that
  * one sequence has next to each other; 0 = 1) and max_len (the longest
  * sequence; 0 = the whole table) choose how the work is split; results are

@@ -332,10 +332,11 @@ __device__ void rotate_queries(const Kv8AppendDesc& d, int row, int h0) {
 // kQHeads query heads of one row.  Every input is read from HBM once, every
 // output written once, and a block that grows has its earlier codes read and
 // written again.  16 chunks of 611 bf16 rows (16 query, 8 K/V heads of 128):
-// 51 us, 109 MB at 2.1 TB/s: 31 million warp instructions (norm, rotation and
-// codes with each rounding of its own), issued in 54% of the cycles by 19 warps
+// 51 us, 109 MB at 2.1 TB/s: 32 million warp instructions (norm, rotation and
+// codes with each rounding of its own), issued in 57% of the cycles by 19 warps
 // an SM, which wait for loads in between.  512 single f32 tokens: 8.2 us, 22 MB at
-// 2.7 TB/s, which is one warp's chain of loads and reductions; one token: 3.1 us.
+// 2.7 TB/s, which is 2.9 rounds of one warp's chain of loads and reductions; one
+// token: 3.1 us.
 template <typename T, int HD, int KEEP>
 __global__ void __launch_bounds__(128, 6) kv8_append_kernel(const __grid_constant__ Kv8AppendDesc d) {
   pdl_launch_dependents();

@@ -24,10 +24,11 @@
 //   256 rows of 2048 f32 logits, top-k 50: 7.8 us (0.27 TB/s), a dozen block-wide
 //     steps one after the other;
 //   one row of 151936 f32, top-p: 29 us on 16 SMs, the same and the f64
-//     exponentials (a quarter of it);
+//     exponentials (a quarter of it); 55 us between other kernels, which put its
+//     code out of the instruction caches;
 //   128 rows of 151936 bf16, top-k 1000, top-p, min-p: 40 us, 39 MB at 1.0 TB/s,
 //     half of it the two passes over the row;
-//   the same rows with top-p alone: 141 us, of which the weights' histogram takes
+//   the same rows with top-p alone: 146 us, of which the weights' histogram takes
 //     55 (about 90 issue slots a logit, the f64 series the most of it).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -47,7 +48,10 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kFix = 45;     // fraction bits of a weight: 2^18 weights of 1 stay below 2^63
-constexpr int kList = 2048;  // tokens of a list
+// Tokens of a list, and logits of a row that is one.  Rows past that go through
+// the larger kernel (256 rows, f32, top-k 50: 2048 logits 8.0 us, 2049 9.6, 4096
+// 9.8).
+constexpr int kList = 2048;
 constexpr int kBins = 1024;
 constexpr int kShortThreads = 256;  // of a CTA that has a row of at most kList logits; 512 otherwise
 typedef unsigned long long u64;
