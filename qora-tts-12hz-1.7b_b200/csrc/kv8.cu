@@ -924,11 +924,14 @@ cudaError_t launch_kv8_attention(Kv8AttnDesc d, int dtype, int max_rows, int max
   };
   // Units of 8 slots here, or tiles of 128 (kv8_tile.cu)?  Both as measured, in
   // us: a unit costs 0.0085 and 0.0009 a page (of 128 dims) over 7; a CTA of
-  // tiles 10 and 2.2 a tile over 4 (10 with splits), one an SM at a time.  One
-  // sequence's 100 rows over 100 positions (16 heads, 8 K/V heads of 128): 10.3
-  // here and 16 in tiles; 8 such sequences: 27 and 16; 4 of 64 rows over 4000: 102
-  // and 45; 16 of 4 over 2000: 23 and 37; 16 rows over 1000: 12 and 20; 500 rows
-  // of 16 heads of 64, window 72: 13.5 and 20.
+  // tiles 10 and 2.2 a tile over 4 (10 with splits), one an SM at a time.  Here and
+  // in tiles, bf16 (f32), 16 heads, 8 K/V heads of 128: one sequence's 100 rows over
+  // 100 positions 10.4 and 15.0 (10.6 and 16.5); 8 such 25.7 and 15.5 (26 and 17);
+  // 2 of 300 over 300 30 and 22 (31 and 26); 4 of 64 rows over 4000 104 and 45
+  // (112 and 58); 200 rows over 8000 147 and 64 (163 and 92); 16 of 4 over 2000 22
+  // and 51 (23 and 74); 64 of 8 over 500 46 and 75 (49 and 94); 16 rows over 1000
+  // 11.6 and 17.6 (11.2 and 20.4); 500 rows of 16 heads of 64, window 72: 14.9 and
+  // 15.7 (14.8 and 17.6).
   if (max_rows > 1) {
     const double here = 7.0 + units * (0.0085 + 0.0009 * d.c.head_dim / 128 * ((seen(d.group_rows) + kKv8Page - 1) / kKv8Page));
     Kv8AttnDesc t = d;
